@@ -318,6 +318,84 @@ SKMETAL_API int skmetal_hip_lloyd_get_labels(skmetal_hip_lloyd* h, int32_t* labe
 /* Inertia of the current labels against the current centres (fp64). */
 SKMETAL_API int skmetal_hip_lloyd_inertia(skmetal_hip_lloyd* h, double* out);
 
+/* ---- routing and low-rank adapters (no counterpart in the reference) ----
+ *
+ * A router's choice of experts with its balance loss, and the experts' products
+ * as low-rank adapters, for callers whose tensors are in device memory.  Unlike
+ * the calls above these are ASYNCHRONOUS: every pointer is a device pointer of
+ * the library's device, the work is enqueued on `stream` (a hipStream_t of the
+ * HIP runtime this library is linked to; NULL: the default stream) and the call
+ * returns.  They allocate nothing, take no lock, keep no pointer and may be
+ * captured into a HIP graph; two calls may run at once on different streams if
+ * their workspaces and outputs differ.  Scratch comes from the caller:
+ * `workspace` holds at least the bytes that the *_workspace function gives for
+ * the same sizes (16-byte aligned).  skmetal_init must have succeeded, and the
+ * calling thread's current device must be the library's.  A bad argument
+ * returns an error and enqueues nothing.
+ *
+ * dtype: the type of scores, rows and adapters.  Sums, softmax statistics and
+ * the low-rank products are fp32, each result rounded once to its type.  Rows
+ * are ld_* elements apart (the elements of a row side by side). */
+#define SKMETAL_F32 0
+#define SKMETAL_BF16 1
+#define SKMETAL_F16 2
+
+/* Top-k routing with the balance loss.  logits [n x E]; mask (nullable, one
+ * byte a row, mask_stride bytes apart): rows that count.  E <= 2048, 1 <= k <=
+ * min(E, 16), n < 2^31.  A score of -inf or NaN is excluded.
+ *   weights, experts [n x k]: per row the experts of the k largest scores,
+ *     largest first, equal scores by the lowest index, and their softmax
+ *     probabilities (normalize != 0: divided by their sum).  A row that is
+ *     masked or has fewer than k scores left takes -1 with weight 0 in the
+ *     places that remain.
+ *   counts [E]: rows that take each expert; prob_sums [E]: the sum of its
+ *     probabilities over the rows that count; rows [1]: their number N (not
+ *     masked, a score left);
+ *   loss [1] = E / (k N^2) sum_e counts[e] prob_sums[e]: 1 when rows and
+ *     probability are spread evenly (0 when N = 0).
+ * The same inputs give the same bits on every call. */
+SKMETAL_API size_t skmetal_hip_route_workspace(size_t n, size_t E);
+SKMETAL_API int skmetal_hip_route(int dtype, const void* logits, size_t ld_logits, const uint8_t* mask, size_t mask_stride,
+                                  size_t n, size_t E, size_t k, int normalize, float* weights, int32_t* experts,
+                                  int32_t* counts, float* prob_sums, int32_t* rows, float* loss, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+/* grad_logits [n x E] from grad_weights [n x k] and grad_loss [1] (each
+ * nullable: no gradient), with weights, experts, counts and rows as
+ * skmetal_hip_route gave them (counts are held constant, as they have no
+ * gradient).  Excluded scores and masked rows get 0. */
+SKMETAL_API int skmetal_hip_route_backward(int dtype, const void* logits, size_t ld_logits, const uint8_t* mask,
+                                           size_t mask_stride, size_t n, size_t E, size_t k, int normalize,
+                                           const float* weights, const int32_t* experts, const int32_t* counts,
+                                           const int32_t* rows, const float* grad_weights, const float* grad_loss,
+                                           void* grad_logits, size_t ld_grad, void* stream);
+
+/* Low-rank adapters beside a shared projection: with q = ids[i],
+ *   out_i = base_i + gates_i scales_q up_q^T (down_q x_i)
+ * x [n x d], base [n x o] (nullable: 0), out [n x o] (may be base itself);
+ * down [a][r][d] and up [a][r][o], adapters *_stride and ranks *_ld elements
+ * apart; ids [n] int32 (ids_stride elements apart), outside [0, a): the row has
+ * no adapter; gates [n] (nullable: 1, gates_stride elements apart) and scales
+ * [a] (nullable: 1) fp32.  low (nullable): [n x r] fp32, receives down_q x_i,
+ * which the backward call takes.  1 <= r <= 128, n < 2^31, a <= 65535. */
+SKMETAL_API size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int backward);
+SKMETAL_API int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const void* down, size_t down_stride,
+                                  size_t down_ld, const void* up, size_t up_stride, size_t up_ld, const int32_t* ids,
+                                  size_t ids_stride, const float* gates, size_t gates_stride, const float* scales,
+                                  const void* base, size_t ld_base, void* out, size_t ld_out, float* low, size_t n,
+                                  size_t d, size_t o, size_t r, size_t a, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+/* Gradients from grad [n x o], that of out: grad_x_i = base_i + the adapters'
+ * part (base [n x d] nullable: 0; may be grad_x itself), grad_down [a][r][d]
+ * and grad_up [a][r][o] (dense; 0 for an adapter without rows), grad_gates [n]
+ * fp32 (nullable).  base's own gradient is grad. */
+SKMETAL_API int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t ld_grad, const void* x, size_t ld_x,
+                                           const void* down, size_t down_stride, size_t down_ld, const void* up,
+                                           size_t up_stride, size_t up_ld, const int32_t* ids, size_t ids_stride,
+                                           const float* gates, size_t gates_stride, const float* scales, const float* low,
+                                           const void* base, size_t ld_base, void* grad_x, size_t ld_grad_x,
+                                           void* grad_down, void* grad_up, float* grad_gates, size_t n, size_t d, size_t o,
+                                           size_t r, size_t a, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,7 +11,9 @@ never compute anything on the CPU.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
+import sys
 import warnings
 from pathlib import Path
 
@@ -31,7 +33,31 @@ def _find_library() -> str:
     raise RuntimeError(f"{LIB_NAME} not found; build it with `python -m skmetal_amd._build`")
 
 
+def _share_torch_runtime() -> None:
+    """A process has one HIP runtime that its tensors and streams belong to.  A ROCm build
+    of PyTorch brings its own libamdhip64; loading that one first (torch itself is not
+    imported) makes this library bind to it whichever of the two is imported first."""
+    if "torch" in sys.modules:
+        return
+    try:
+        spec = importlib.util.find_spec("torch")
+        path = Path(spec.origin).parent / "lib" / "libamdhip64.so" if spec is not None and spec.origin else None
+        if path is not None and path.exists():
+            ctypes.CDLL(str(path))
+    except Exception:  # noqa: BLE001 -- the library then uses ROCm's own runtime
+        pass
+
+
+def require_torch_runtime() -> None:
+    """Raises when torch and this library are on different HIP runtimes."""
+    with open("/proc/self/maps") as f:
+        runtimes = sorted({line.split()[-1] for line in f if "/libamdhip64.so" in line})
+    if len(runtimes) > 1:
+        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(runtimes)}): import torch before skmetal_amd")
+
+
 _c_size = ctypes.c_size_t
+_int = ctypes.c_int
 _vp = ctypes.c_void_p
 
 # (c_name, restype, argtypes...) -- the KMeans subset of the reference's registry
@@ -77,6 +103,17 @@ _REGISTRY = [
      ctypes.POINTER(ctypes.c_int)),
     ("skmetal_hip_kmeans_batch_fused_noalloc", ctypes.c_int, _vp, _vp, _vp, _c_size, _c_size, _c_size, _c_size,
      ctypes.c_float, ctypes.POINTER(ctypes.c_int32)),
+    ("skmetal_hip_route_workspace", _c_size, _c_size, _c_size),
+    ("skmetal_hip_route", _int, _int, _vp, _c_size, _vp, _c_size, _c_size, _c_size, _c_size, _int, _vp, _vp, _vp, _vp,
+     _vp, _vp, _vp, _c_size, _vp),
+    ("skmetal_hip_route_backward", _int, _int, _vp, _c_size, _vp, _c_size, _c_size, _c_size, _c_size, _int, _vp, _vp,
+     _vp, _vp, _vp, _vp, _vp, _c_size, _vp),
+    ("skmetal_hip_adapt_workspace", _c_size, _int, _c_size, _c_size, _c_size, _c_size, _c_size, _int),
+    ("skmetal_hip_adapt", _int, _int, _vp, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _vp,
+     _c_size, _vp, _vp, _c_size, _vp, _c_size, _vp, _c_size, _c_size, _c_size, _c_size, _c_size, _vp, _c_size, _vp),
+    ("skmetal_hip_adapt_backward", _int, _int, _vp, _c_size, _vp, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _c_size,
+     _vp, _c_size, _vp, _c_size, _vp, _vp, _vp, _c_size, _vp, _c_size, _vp, _vp, _vp, _c_size, _c_size, _c_size, _c_size,
+     _c_size, _vp, _c_size, _vp),
 ]
 
 SKMETAL_FIT_STRICT = 1
@@ -85,6 +122,7 @@ _lib = None
 _load_error = None
 HIP_AVAILABLE = False
 try:
+    _share_torch_runtime()
     _lib = ctypes.CDLL(_find_library())
     for _name, _restype, *_argtypes in _REGISTRY:
         _f = getattr(_lib, _name)

@@ -41,6 +41,8 @@ SOURCES = [
     ("plusplus_kernels.hip", []),
     ("transform_kernels.hip", []),
     ("sample_kernels.hip", []),
+    ("route_kernels.hip", []),
+    ("adapt_kernels.hip", []),
     ("skmetal_hip.hip", VGPR_FORM),
 ]
 

@@ -12,6 +12,7 @@
 //     and return at once after the loop has stopped, so the host synchronises
 //     once per batch, not once per iteration.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -29,6 +30,7 @@
 
 #include "skmetal_hip.h"
 #include "internal.h"
+#include "experts.h"
 
 using namespace skm;
 
@@ -108,7 +110,7 @@ constexpr size_t kMaxTimedSteps = 4096;  // steps skmetal_hip_lloyd_iterate can 
 // ---------------------------------------------------------------------------
 struct Context {
     std::recursive_mutex mu;
-    bool ready = false;
+    std::atomic<bool> ready{false};  // read without the lock by the entry points that take a stream
     int dev = 0;
     int num_cu = 0;
     int max_threads = 0;
@@ -2120,6 +2122,186 @@ int skmetal_hip_lloyd_inertia(skmetal_hip_lloyd* h, double* out)
     Guard g(c);
     if (!h || !out) return fail(SKMETAL_EINVAL, "null pointer argument");
     return h->L.inertia(out);
+}
+
+// ---- routing and low-rank adapters: device pointers, the caller's stream, no lock ----
+
+}  // extern "C"
+
+namespace {
+
+// What every entry point that takes a stream needs of the library: set up, and
+// the calling thread on its device (the launches go to that device's stream).
+int on_device()
+{
+    const Context& c = ctx();
+    if (!c.ready) return fail(SKMETAL_ENODEV, "skmetal_init must run first: this entry point does not set the library up");
+    int dev = -1;
+    HIP_TRY(hipGetDevice(&dev), "hipGetDevice");
+    if (dev != c.dev)
+        return fail(SKMETAL_EINVAL, "the current device is %d, this library was set up on device %d", dev, c.dev);
+    return 0;
+}
+
+int check_dtype(int dtype)
+{
+    if (dtype != SKMETAL_F32 && dtype != SKMETAL_BF16 && dtype != SKMETAL_F16)
+        return fail(SKMETAL_EINVAL, "dtype=%d is not SKMETAL_F32, SKMETAL_BF16 or SKMETAL_F16", dtype);
+    return 0;
+}
+
+constexpr size_t kMaxRows = (size_t(1) << 31) - 1;
+constexpr size_t kMaxStride = size_t(1) << 40;  // elements: byte offsets stay far inside 64 bits
+
+int check_aligned(const void* p, size_t bytes, const char* what)
+{
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return fail(SKMETAL_EINVAL, "%s is not aligned to %zu bytes", what, bytes);
+    return 0;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need)
+{
+    if (need == 0) return 0;
+    if (ws == nullptr || have < need) return fail(SKMETAL_EINVAL, "the workspace has %zu bytes, this call needs %zu", ws ? have : 0, need);
+    return check_aligned(ws, 16, "the workspace");
+}
+
+int check_route(int dtype, size_t n, size_t E, size_t k, size_t ld, size_t mask_stride)
+{
+    TRY(check_dtype(dtype));
+    if (E == 0 || k == 0 || k > E) return fail(SKMETAL_EINVAL, "k=%zu must be in [1, E], E=%zu positive", k, E);
+    if (E > size_t(kRouteMaxE) || k > size_t(kRouteMaxK))
+        return fail(SKMETAL_ERANGE, "E=%zu, k=%zu: at most %d experts, of which a row takes at most %d", E, k, kRouteMaxE, kRouteMaxK);
+    if (n > kMaxRows || ld > kMaxStride || mask_stride > kMaxStride) return fail(SKMETAL_ERANGE, "n=%zu or a stride exceeds the supported range", n);
+    return 0;
+}
+
+struct AdaptSizes {
+    size_t n, d, o, r, a;
+};
+
+int check_adapt(int dtype, const AdaptSizes& z, std::initializer_list<size_t> strides)
+{
+    TRY(check_dtype(dtype));
+    if (z.d == 0 || z.o == 0 || z.r == 0) return fail(SKMETAL_EINVAL, "d, o and r must be positive (d=%zu o=%zu r=%zu)", z.d, z.o, z.r);
+    if (z.r > size_t(kAdaptMaxR)) return fail(SKMETAL_ERANGE, "r=%zu: a rank of at most %d", z.r, kAdaptMaxR);
+    if (z.n > kMaxRows || z.a > 65535 || z.d > kMaxDim || z.o > kMaxDim)
+        return fail(SKMETAL_ERANGE, "n=%zu, a=%zu, d=%zu or o=%zu exceeds the supported range", z.n, z.a, z.d, z.o);
+    for (const size_t s : strides)
+        if (s > kMaxStride) return fail(SKMETAL_ERANGE, "a stride of %zu elements exceeds the supported range", s);
+    return 0;
+}
+
+int launched(hipError_t e, const char* what)
+{
+    if (e == hipSuccess) return 0;
+    (void)hipGetLastError();  // else the next launch reports it
+    return hip_fail(e, what);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t skmetal_hip_route_workspace(size_t n, size_t E)
+{
+    return n > kMaxRows || E > size_t(kRouteMaxE) ? 0 : route_workspace((long)n, (int)E);
+}
+
+int skmetal_hip_route(int dtype, const void* logits, size_t ld_logits, const uint8_t* mask, size_t mask_stride, size_t n,
+                      size_t E, size_t k, int normalize, float* weights, int32_t* experts, int32_t* counts,
+                      float* prob_sums, int32_t* rows, float* loss, void* workspace, size_t workspace_bytes, void* stream)
+{
+    g_err.clear();
+    TRY(check_route(dtype, n, E, k, ld_logits, mask_stride));
+    if (!counts || !prob_sums || !rows || !loss || (n > 0 && (!logits || !weights || !experts)))
+        return fail(SKMETAL_EINVAL, "null pointer argument");
+    TRY(check_aligned(logits, elem_size(dtype), "logits"));
+    TRY(check_workspace(workspace, workspace_bytes, route_workspace((long)n, (int)E)));
+    TRY(on_device());
+    RouteArgs a{logits, dtype, (long)n, (int)E, (long)ld_logits, mask, (long)mask_stride, (int)k, normalize, weights,
+                experts, counts, prob_sums, rows, loss, static_cast<char*>(workspace)};
+    return launched(launch_route(a, static_cast<hipStream_t>(stream)), "route");
+}
+
+int skmetal_hip_route_backward(int dtype, const void* logits, size_t ld_logits, const uint8_t* mask, size_t mask_stride,
+                               size_t n, size_t E, size_t k, int normalize, const float* weights, const int32_t* experts,
+                               const int32_t* counts, const int32_t* rows, const float* grad_weights,
+                               const float* grad_loss, void* grad_logits, size_t ld_grad, void* stream)
+{
+    g_err.clear();
+    TRY(check_route(dtype, n, E, k, ld_logits, mask_stride));
+    if (ld_grad > kMaxStride) return fail(SKMETAL_ERANGE, "ld_grad=%zu exceeds the supported range", ld_grad);
+    if (ld_grad < E && n > 1) return fail(SKMETAL_EINVAL, "ld_grad=%zu: the rows of grad_logits overlap", ld_grad);
+    if (!counts || !rows || (n > 0 && (!logits || !weights || !experts || !grad_logits)))
+        return fail(SKMETAL_EINVAL, "null pointer argument");
+    TRY(check_aligned(logits, elem_size(dtype), "logits"));
+    TRY(check_aligned(grad_logits, elem_size(dtype), "grad_logits"));
+    TRY(on_device());
+    RouteBackArgs a{logits, dtype, (long)n, (int)E, (long)ld_logits, mask, (long)mask_stride, (int)k, normalize, weights,
+                    experts, counts, rows, grad_weights, grad_loss, grad_logits, (long)ld_grad};
+    return launched(launch_route_back(a, static_cast<hipStream_t>(stream)), "route_backward");
+}
+
+size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int backward)
+{
+    if (check_adapt(dtype, {n, d, o, r, a}, {}) != 0) return 0;
+    return adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, backward);
+}
+
+int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const void* down, size_t down_stride, size_t down_ld,
+                      const void* up, size_t up_stride, size_t up_ld, const int32_t* ids, size_t ids_stride,
+                      const float* gates, size_t gates_stride, const float* scales, const void* base, size_t ld_base,
+                      void* out, size_t ld_out, float* low, size_t n, size_t d, size_t o, size_t r, size_t a,
+                      void* workspace, size_t workspace_bytes, void* stream)
+{
+    g_err.clear();
+    TRY(check_adapt(dtype, {n, d, o, r, a}, {ld_x, down_stride, down_ld, up_stride, up_ld, ids_stride, gates_stride, ld_base, ld_out}));
+    if ((n > 0 && (!x || !ids || !out)) || (a > 0 && (!down || !up))) return fail(SKMETAL_EINVAL, "null pointer argument");
+    if (ld_out < o && n > 1) return fail(SKMETAL_EINVAL, "ld_out=%zu: the rows of out overlap", ld_out);
+    const size_t es = elem_size(dtype);
+    TRY(check_aligned(x, es, "x"));
+    TRY(check_aligned(down, es, "down"));
+    TRY(check_aligned(up, es, "up"));
+    TRY(check_aligned(base, es, "base"));
+    TRY(check_aligned(out, es, "out"));
+    TRY(check_workspace(workspace, workspace_bytes, adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, 0)));
+    TRY(on_device());
+    AdaptArgs A{dtype, (long)n, (int)d, (int)o, (int)r, (int)a, x, (long)ld_x, down, (long)down_stride, (long)down_ld,
+                up, (long)up_stride, (long)up_ld, ids, (long)ids_stride, gates, (long)gates_stride, scales, base,
+                (long)ld_base, out, (long)ld_out, low, static_cast<char*>(workspace)};
+    return launched(launch_adapt(A, static_cast<hipStream_t>(stream)), "adapt");
+}
+
+int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t ld_grad, const void* x, size_t ld_x, const void* down,
+                               size_t down_stride, size_t down_ld, const void* up, size_t up_stride, size_t up_ld,
+                               const int32_t* ids, size_t ids_stride, const float* gates, size_t gates_stride,
+                               const float* scales, const float* low, const void* base, size_t ld_base, void* grad_x,
+                               size_t ld_grad_x, void* grad_down, void* grad_up, float* grad_gates, size_t n, size_t d,
+                               size_t o, size_t r, size_t a, void* workspace, size_t workspace_bytes, void* stream)
+{
+    g_err.clear();
+    TRY(check_adapt(dtype, {n, d, o, r, a},
+                    {ld_grad, ld_x, down_stride, down_ld, up_stride, up_ld, ids_stride, gates_stride, ld_base, ld_grad_x}));
+    if ((n > 0 && (!grad || !x || !ids || !low || !grad_x)) || (a > 0 && (!down || !up || !grad_down || !grad_up)))
+        return fail(SKMETAL_EINVAL, "null pointer argument");
+    if (ld_grad_x < d && n > 1) return fail(SKMETAL_EINVAL, "ld_grad_x=%zu: the rows of grad_x overlap", ld_grad_x);
+    const size_t es = elem_size(dtype);
+    TRY(check_aligned(grad, es, "grad"));
+    TRY(check_aligned(x, es, "x"));
+    TRY(check_aligned(down, es, "down"));
+    TRY(check_aligned(up, es, "up"));
+    TRY(check_aligned(base, es, "base"));
+    TRY(check_aligned(grad_x, es, "grad_x"));
+    TRY(check_aligned(grad_down, es, "grad_down"));
+    TRY(check_aligned(grad_up, es, "grad_up"));
+    TRY(check_workspace(workspace, workspace_bytes, adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, 1)));
+    TRY(on_device());
+    AdaptBackArgs A{dtype, (long)n, (int)d, (int)o, (int)r, (int)a, grad, (long)ld_grad, x, (long)ld_x, down,
+                    (long)down_stride, (long)down_ld, up, (long)up_stride, (long)up_ld, ids, (long)ids_stride, gates,
+                    (long)gates_stride, scales, low, base, (long)ld_base, grad_x, (long)ld_grad_x, grad_down, grad_up,
+                    grad_gates, static_cast<char*>(workspace)};
+    return launched(launch_adapt_back(A, static_cast<hipStream_t>(stream)), "adapt_backward");
 }
 
 }  // extern "C"
