@@ -43,7 +43,8 @@ hipError_t launch_route_back(const RouteBackArgs& a, hipStream_t s);
 
 // ---- adapt_kernels.hip ----
 
-constexpr int kAdaptMaxR = 128;  // rank
+constexpr int kAdaptMaxR = 128;   // rank
+constexpr int kAdaptMaxA = 2048;  // adapters
 
 struct AdaptArgs {
     int type; long n; int d, o, r, a;
