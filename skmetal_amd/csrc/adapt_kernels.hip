@@ -19,8 +19,10 @@
 namespace skm {
 namespace {
 
-constexpr int kTile = 64;        // rows of a k_shrink / k_expand tile
-constexpr int kPlanRows = 4096;  // rows of a k_plan block, 1024 a wave
+constexpr int kTile = 64;          // rows of a k_shrink / k_expand tile
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanLoads = 16;     // rows a k_plan lane holds
+constexpr int kPlanRows = kPlanThreads * kPlanLoads;
 
 struct Tile {
     int q;      // adapter; a: rows without one; -1: an unused entry
@@ -31,7 +33,7 @@ struct Tile {
 
 struct PlanArgs {
     const int* ids; long ids_stride; int n, a;
-    int* hist;           // [chunks x (a + 1)], more than one chunk only
+    int* hist;           // [blocks x (a + 1)], more than one block only
     int* perm;           // [n] rows in the order of their adapters
     Tile* tiles; int ntiles;    // kTile rows each
     Tile* chunks; int nchunks;  // nullable; `chunk` rows each, one at least per adapter
@@ -57,10 +59,11 @@ __device__ __forceinline__ unsigned long long same_key(int key, bool on, int bit
     return m;
 }
 
-// Exclusive sum of v[0 .. count) in place (256 threads), v[count] = the total.
+// Exclusive sum of v[0 .. count) in place, v[count] = the total; tmp holds a value a wave.
 __device__ void block_scan(int* v, int count, int* tmp)
 {
-    const int per = (count + 255) / 256, lo = min(count, (int)threadIdx.x * per), hi = min(count, lo + per);
+    const int per = (count + kPlanThreads - 1) / kPlanThreads;
+    const int lo = min(count, (int)threadIdx.x * per), hi = min(count, lo + per);
     int s = 0;
     for (int i = lo; i < hi; ++i) s += v[i];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -78,49 +81,62 @@ __device__ void block_scan(int* v, int count, int* tmp)
         v[i] = base;
         base += x;
     }
-    if (threadIdx.x == 255) v[count] = base;
+    if (threadIdx.x == kPlanThreads - 1) v[count] = base;
     __syncthreads();
 }
 
-// Per wave of this block's rows, how many have each key (the leaders of equal keys add
-// them up, so no two lanes write one place).
-__device__ void count_keys(const PlanArgs& p, unsigned short* wh, int K, int bits)
+// The keys of this block's rows, a wave's 64 * kPlanLoads rows side by side, and per wave how many
+// have each key (the first lane of equal keys adds them up, so no two lanes write one
+// place).  rank: lanes before this one with its key, and 256 times all lanes with it.
+__device__ __forceinline__ void count_keys(const PlanArgs& p, unsigned short* wh, int K, int bits, int* key, int* rank)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int j = threadIdx.x; j < 4 * K; j += 256) wh[j] = 0;
+    const long first = (long)blockIdx.x * kPlanRows + wave * (64 * kPlanLoads) + lane;
+#pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it) {
+        const long i = first + it * 64;
+        key[it] = p.n > 0 ? p.ids[min(i, (long)p.n - 1) * p.ids_stride] : 0;
+        key[it] = i >= p.n ? -1 : key[it] >= 0 && key[it] < p.a ? key[it] : p.a;
+    }
+    for (int j = threadIdx.x; j < kPlanThreads / 64 * K; j += kPlanThreads) wh[j] = 0;
     __syncthreads();
-    for (int it = 0; it < kPlanRows / 256; ++it) {
-        const long i = (long)blockIdx.x * kPlanRows + wave * (kPlanRows / 4) + it * 64 + lane;
-        const bool on = i < p.n;
-        const int key = on ? adapter_of(p.ids, p.ids_stride, i, p.a) : 0;
-        const unsigned long long m = same_key(key, on, bits);
-        if (on && (m & ((1ull << lane) - 1)) == 0) wh[wave * K + key] += (unsigned short)__popcll(m);
+    volatile unsigned short* mine = wh + wave * K;
+#pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it) {
+        const unsigned long long m = same_key(key[it], key[it] >= 0, bits);
+        const int before = __popcll(m & ((1ull << lane) - 1)), all = __popcll(m);
+        rank[it] = before + 256 * all;
+        if (key[it] >= 0 && before == 0) mine[key[it]] = (unsigned short)(mine[key[it]] + all);
     }
     __syncthreads();
 }
 
-__global__ __launch_bounds__(256) void k_plan_count(PlanArgs p, int bits)
+__global__ __launch_bounds__(kPlanThreads) void k_plan_count(PlanArgs p, int bits)
 {
     extern __shared__ char lds[];
     unsigned short* wh = reinterpret_cast<unsigned short*>(lds);
     const int K = p.a + 1;
-    count_keys(p, wh, K, bits);
-    for (int k = threadIdx.x; k < K; k += 256)
-        p.hist[(long)blockIdx.x * K + k] = wh[k] + wh[K + k] + wh[2 * K + k] + wh[3 * K + k];
+    int key[kPlanLoads], rank[kPlanLoads];
+    count_keys(p, wh, K, bits, key, rank);
+    for (int k = threadIdx.x; k < K; k += kPlanThreads) {
+        int c = 0;
+        for (int w = 0; w < kPlanThreads / 64; ++w) c += wh[w * K + k];
+        p.hist[(long)blockIdx.x * K + k] = c;
+    }
 }
 
-// `size` = rows per key, consumed: the tiles of `len` rows of every key.
+// The tiles of `len` rows of every key (off[k] .. off[k + 1] are its places); `whole`: one
+// at least per adapter and none for the rows without one.
 __device__ void write_tiles(const int* off, int* first, int K, int a, int len, bool whole, Tile* out, int bound, int* tmp, int2* merge)
 {
-    // whole: one tile at least per adapter and none for the rows without one
-    for (int k = threadIdx.x; k < K; k += 256) {
+    for (int k = threadIdx.x; k < K; k += kPlanThreads) {
         const int c = off[k + 1] - off[k], t = (c + len - 1) / len;
         first[k] = !whole ? t : k == a ? 0 : max(1, t);
     }
     __syncthreads();
     block_scan(first, K, tmp);
     const int total = first[K];
-    for (int t = threadIdx.x; t < bound; t += 256) {
+    for (int t = threadIdx.x; t < bound; t += kPlanThreads) {
         Tile e{-1, 0, 0, -1};
         if (t < total) {
             int lo = 0, hi = K;  // the last key whose tiles start at t or before
@@ -136,9 +152,8 @@ __device__ void write_tiles(const int* off, int* first, int K, int a, int len, b
         }
         out[t] = e;
     }
-    __syncthreads();
     if (merge != nullptr)
-        for (int k = threadIdx.x; k < a; k += 256) {
+        for (int k = threadIdx.x; k < a; k += kPlanThreads) {
             const int t = first[k + 1] - first[k];
             merge[k] = make_int2(first[k], t > 1 ? t : 0);
         }
@@ -147,18 +162,19 @@ __device__ void write_tiles(const int* off, int* first, int K, int a, int len, b
 
 // Places of the rows, and (block 0) the tiles.  Without a histogram this block holds all
 // the rows.
-__global__ __launch_bounds__(256) void k_plan_place(PlanArgs p, int bits)
+__global__ __launch_bounds__(kPlanThreads) void k_plan_place(PlanArgs p, int bits)
 {
     extern __shared__ char lds[];
     const int K = p.a + 1;
     int* off = reinterpret_cast<int*>(lds);        // [K + 1] first place of each key, over all rows
     int* at = off + K + 1;                         // [K + 1] first place of this block's
-    int* tmp = at + K + 1;                         // [4]
-    unsigned short* wh = reinterpret_cast<unsigned short*>(tmp + 4);  // [4 x K]
-    count_keys(p, wh, K, bits);
-    for (int k = threadIdx.x; k < K; k += 256) {
+    int* tmp = at + K + 1;                         // [16]
+    unsigned short* wh = reinterpret_cast<unsigned short*>(tmp + 16);  // [16 x K]
+    int key[kPlanLoads], rank[kPlanLoads];
+    count_keys(p, wh, K, bits, key, rank);
+    for (int k = threadIdx.x; k < K; k += kPlanThreads) {
         int c = 0;
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < kPlanThreads / 64; ++w) {
             const int x = wh[w * K + k];
             wh[w * K + k] = (unsigned short)c;
             c += x;
@@ -177,21 +193,18 @@ __global__ __launch_bounds__(256) void k_plan_place(PlanArgs p, int bits)
     }
     __syncthreads();
     block_scan(off, K, tmp);
-    for (int k = threadIdx.x; k < K; k += 256) at[k] += off[k];
+    for (int k = threadIdx.x; k < K; k += kPlanThreads) at[k] += off[k];
     __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6;
+    const long first = (long)blockIdx.x * kPlanRows + wave * (64 * kPlanLoads) + (threadIdx.x & 63);
     volatile unsigned short* mine = wh + wave * K;
-    for (int it = 0; it < kPlanRows / 256; ++it) {
-        const long i = (long)blockIdx.x * kPlanRows + wave * (kPlanRows / 4) + it * 64 + lane;
-        const bool on = i < p.n;
-        const int key = on ? adapter_of(p.ids, p.ids_stride, i, p.a) : 0;
-        const unsigned long long m = same_key(key, on, bits), lower = m & ((1ull << lane) - 1);
-        if (on) {
-            const int seen = mine[key];
-            p.perm[at[key] + seen + __popcll(lower)] = (int)i;
-            if (lower == 0) mine[key] = (unsigned short)(seen + __popcll(m));
+#pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it)
+        if (key[it] >= 0) {
+            const int seen = mine[key[it]], before = rank[it] & 255;
+            p.perm[at[key[it]] + seen + before] = (int)(first + it * 64);
+            if (before == 0) mine[key[it]] = (unsigned short)(seen + (rank[it] >> 8));
         }
-    }
     if (blockIdx.x != 0) return;
     __syncthreads();
     write_tiles(off, at, K, p.a, kTile, false, p.tiles, p.ntiles, tmp, nullptr);
@@ -350,6 +363,30 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
 
 // ---- ranks to rows ----
 
+// v = hi + lo + (at most 2^-17 |v|): a low-rank value enters products of bf16 matrix cores
+// as two bf16, so that its rounding stays far under that of a bf16 result.
+__device__ __forceinline__ void split2(float v, bf16& hi, bf16& lo)
+{
+    hi = (bf16)v;
+    const float rest = v - (float)hi;
+    lo = (bf16)(__builtin_isfinite((float)hi) ? rest : 0.f);  // an infinity stays one
+}
+
+// b[j] = element j of the eight vectors a[0 .. 7]: an 8 x 8 transposition in registers.
+__device__ __forceinline__ void transpose8(const Vec<bf16>* a, Vec<bf16>* b)
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned x = __builtin_bit_cast(u32x4, a[2 * e])[j / 2], y = __builtin_bit_cast(u32x4, a[2 * e + 1])[j / 2];
+            w[e] = __builtin_amdgcn_perm(y, x, j % 2 ? 0x07060302u : 0x05040100u);
+        }
+        b[j] = __builtin_bit_cast(Vec<bf16>, w);
+    }
+}
+
 template <typename T>
 struct ExpandArgs {
     Rows rows;
@@ -360,96 +397,216 @@ struct ExpandArgs {
     T* out; long ld_out;
     int w, r;
     float* low;                              // nullable: [n x r], the splits' sum (0 for a row without an adapter)
-    const float* dot; float* dgates;         // nullable: dgates[i] = s_q <low_i, dot_i>
+    // backward (else null): the forward call's low, and its products with the splits' sum
+    const float* dot; float* dgates;         // dgates[i] = s_q <low_i, dot_i>, nullable
+    bf16* low_t; bf16* dot_t; long ld_t;     // f low and f dot for k_outer_split, nullable: [2][r][ld_t], by place
 };
 
+// What k_expand keeps of a tile's low-rank rows: f low as two bf16 (bf16 rows) or as it is.
+template <typename T, int RT, int KP>
+struct LowTile {
+    static constexpr bool kSplit = false;
+    float v[RT * 16][KP + 4];
+    __device__ void set(int i, int k, float x) { v[i][k] = x; }
+};
+template <int RT, int KP>
+struct LowTile<bf16, RT, KP> {
+    static constexpr bool kSplit = true;
+    bf16 v[RT * 16][2 * KP + 8];
+    __device__ void set(int i, int k, float x) { split2(x, v[i][k], v[i][KP + k]); }
+};
+
+// Sums the splits of a tile's low-rank rows (a row's ranks by neighbouring lanes) into L,
+// times f; store: the sums themselves to low; dot: their products with dot to dgates.
+template <typename T, int RT, int KP>
+__device__ __forceinline__ void stage_low(const ExpandArgs<T>& p, const Tile& t, bool has, float sc, const float* part, int splits, LowTile<T, RT, KP>& L,
+                                          float* store, float* dgates)
+{
+    constexpr int KW = KP < 64 ? KP : 64;
+#pragma unroll 1
+    for (int idx = threadIdx.x; idx < RT * 16 * KW; idx += 256) {
+        const int i = idx / KW, k0 = idx % KW;
+        const bool on = i < t.cnt;
+        const long row = row_at(p.rows, t.start + (on ? i : 0));
+        const float f = has ? (p.gates ? p.gates[row * p.gates_stride] : 1.f) * sc : 0.f;
+        float d = 0.f;
+#pragma unroll
+        for (int k = k0; k < KP; k += KW) {
+            float s = 0.f;
+            if (has && on && k < p.r)
+                for (int c = 0; c < splits; c += 4) {  // four loads at once; the sum stays in order
+                    float x[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) x[u] = part[(min(c + u, splits - 1) * p.n + row) * p.r + k];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) s += c + u < splits ? x[u] : 0.f;
+                }
+            L.set(i, k, has && on && k < p.r ? f * s : 0.f);
+            if (store != nullptr && on && k < p.r) store[row * p.r + k] = s;
+            if (dgates != nullptr && has && on && k < p.r) d += s * p.dot[row * p.r + k];
+        }
+        if (dgates != nullptr) {
+#pragma unroll
+            for (int off = 1; off < KW; off <<= 1) d += __shfl_xor(d, off, 64);
+            if (k0 == 0 && on) dgates[row] = has ? d * sc : 0.f;
+        }
+    }
+}
+
+// A tile's rows of L by rank, for k_outer_split.
+template <typename T, int RT, int KP>
+__device__ __forceinline__ void store_by_rank(const ExpandArgs<T>& p, const Tile& t, const LowTile<T, RT, KP>& L, bf16* out)
+{
+    if constexpr (LowTile<T, RT, KP>::kSplit)
+        for (int idx = threadIdx.x; idx < 2 * p.r * RT * 16; idx += 256) {
+            const int i = idx % (RT * 16), k = idx / (RT * 16);  // k: a rank's hi, and from r on its lo
+            if (i < t.cnt) out[k * p.ld_t + t.start + i] = L.v[i][k < p.r ? k : KP + k - p.r];
+        }
+}
+
+// The wave's rows and columns of a tile: out = base + L M.  The product is taken as
+// (M^T)(L^T), so that a lane ends up with 16 bytes of a row, four times.
+//
+// bf16: lanes hold eight ranks of eight columns each, transposed in registers, so M goes
+// to the matrix cores without a detour; L enters as two bf16 (one product of 32 where the
+// ranks fill half of it: hi and lo side by side, M twice).  Other types: fp32 matrix
+// cores, four ranks at a time, which need M by columns as it lies and L unrounded.
+// FULL: all the columns exist.
+//
+// The sums start from the base where its type rounds at 2^-8 or 2^-11 anyway; in fp32 they
+// would then round at the base's size once for every four ranks, so it is added last.
+template <typename T, int RT, int KP, bool FULL>
+__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, int c0, bool has)
+{
+    constexpr int V = kVec<T>;
+    constexpr bool kBaseFirst = sizeof(T) == 2;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    long row[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) row[i] = row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1));
+    Vec<T> y[2][4];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = c0 + (e * 4 + g) * V;
+            y[i & 1][e] = FULL ? load16(p.base + row[i] * p.ld_base + c) : load_part(p.base + row[i] * p.ld_base + c, p.w - c);
+        }
+    };
+    if (p.base == nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e & 1][e >> 1] = Vec<T>{};
+    } else {
+        fetch(0);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        if (i * 16 >= t.cnt) break;
+        if (i + 1 < RT && p.base != nullptr) fetch(i + 1);
+        f32x4 acc[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = kBaseFirst ? to_f(y[i & 1][e][j]) : 0.f;
+        if (has) {
+            if constexpr (LowTile<T, RT, KP>::kSplit) {
+#pragma unroll
+                for (int b = 0; b < (KP + 31) / 32; ++b) {
+                    const Vec<T> hi = *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][b * 32 + g * 8]);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[j] = mfma16(m[b][j], hi, acc[j]);
+                    if constexpr (KP >= 32) {
+                        const Vec<T> lo = *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][KP + b * 32 + g * 8]);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) acc[j] = mfma16(m[b][j], lo, acc[j]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < KP / 16; ++b) {
+                    const f32x4 lo = *reinterpret_cast<const f32x4*>(&L.v[i * 16 + l16][b * 16 + g * 4]);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f(m[b / 2][b % 2 * 4 + s][j]), lo[s], acc[j], 0, 0, 0);
+                }
+            }
+        }
+        if (i * 16 + l16 < t.cnt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = c0 + (e * 4 + g) * V, left = p.w - c;
+                Vec<T> z;
+#pragma unroll
+                for (int j = 0; j < V; ++j) z[j] = from_f<T>(kBaseFirst ? acc[j][e] : to_f(y[i & 1][e][j]) + acc[j][e]);
+                T* o = p.out + row[i] * p.ld_out + c;
+                if (FULL || left >= V)
+                    __builtin_memcpy(o, &z, 16);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (j < left) o[j] = z[j];
+            }
+    }
+}
+
 // out_row = base_row + f_row low_row M_q.  A block takes RT * 16 rows of one adapter and
-// four waves' columns, 16 * kVec each, of which a wave keeps M_q in registers.  The product is taken
-// as (M_q^T)(low^T) on the fp32 matrix cores, four ranks at a time: M_q then needs no
-// transposition, low no rounding, and a lane ends up with 16 bytes of a row, four times.
-template <typename T, int RT, int NB>
+// four waves' columns, 16 * kVec each, of which a wave keeps M_q in registers.  KP: the
+// ranks, rounded up.
+template <typename T, int RT, int KP, bool BACK>
 __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
 {
     constexpr int V = kVec<T>;
+    using Low = LowTile<T, RT, KP>;
+    __shared__ __align__(16) Low L;
     const Tile t = tile_at(p.rows, blockIdx.x);
     if (t.q < 0) return;
     const bool has = t.q < p.rows.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-    if (blockIdx.y == 0 && (p.low != nullptr || p.dgates != nullptr)) {
-        for (int at = wave; at < t.cnt; at += 4) {
-            const long row = row_at(p.rows, t.start + at);
-            float d = 0.f;
-            for (int k = lane; k < p.r; k += 64) {
-                float s = 0.f;
-                if (has)
-                    for (int c = 0; c < p.splits; ++c) s += p.part[(c * p.n + row) * p.r + k];
-                if (p.low != nullptr) p.low[row * p.r + k] = s;
-                if (p.dgates != nullptr && has) d += s * p.dot[row * p.r + k];
-            }
-            if (p.dgates != nullptr) {
-                for (int off = 1; off < 64; off <<= 1) d += __shfl_xor(d, off, 64);
-                if (lane == 0) p.dgates[row] = has ? d * (p.scales ? p.scales[t.q] : 1.f) : 0.f;
+    const float sc = has && p.scales ? p.scales[t.q] : 1.f;
+    const int c0 = (blockIdx.y * 4 + wave) * 16 * V;
+    const bool full = c0 + 16 * V <= p.w;
+    // eight ranks of kVec columns: bf16: g * 8 .. + 7 of every 32 (of 16, for half as many
+    // ranks); else g * 4 .. + 3 of every 16, two such
+    constexpr int NM = Low::kSplit ? (KP + 31) / 32 : (KP + 31) / 32;
+    Vec<T> m[NM][8];
+    if (has && c0 < p.w) {
+        const int cm = c0 + ((l16 & 3) * 4 + (l16 >> 2)) * V;  // the columns this lane brings
+#pragma unroll
+        for (int b = 0; b < NM; ++b) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int rank = Low::kSplit ? (KP == 16 ? (g & 1) * 8 + e : b * 32 + g * 8 + e) : b * 32 + e / 4 * 16 + g * 4 + e % 4;
+                const T* at = p.M + t.q * p.sa + (long)min(rank, p.r - 1) * p.ld + cm;
+                m[b][e] = full ? load16(at) : load_part(at, p.w - cm);
+                if (rank >= p.r) m[b][e] = Vec<T>{};
             }
         }
     }
-    const int c0 = (blockIdx.y * 4 + wave) * 16 * V;
-    if (c0 >= p.w) return;
-    Vec<T> m[NB][4];
-    const int cm = c0 + ((l16 & 3) * 4 + (l16 >> 2)) * V;  // the columns of M this lane brings
+    const bool first = blockIdx.y == 0;
+    if (has || first)
+        stage_low<T, RT, KP>(p, t, has, sc, p.part, p.splits, L, first ? p.low : nullptr, BACK && first ? p.dgates : nullptr);
+    __syncthreads();
+    if (BACK && Low::kSplit && first && has && p.low_t != nullptr) store_by_rank<T, RT, KP>(p, t, L, p.low_t);
+    if (c0 < p.w) {
+        if constexpr (Low::kSplit) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NM; ++b) {
+                Vec<T> x[8];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int rank = b * 16 + g * 4 + s;
-            m[b][s] = load_part(p.M + (has ? t.q * p.sa + (long)rank * p.ld + cm : 0), has && rank < p.r ? p.w - cm : 0);
-        }
-    const float sc = has && p.scales ? p.scales[t.q] : 1.f;
-#pragma unroll 1
-    for (int i = 0; i < RT; ++i) {
-        if (i * 16 >= t.cnt) break;
-        const bool on = i * 16 + l16 < t.cnt;
-        const long row = row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1));
-        Vec<T> y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int c = c0 + (e * 4 + g) * V;
-            y[e] = load_part(p.base + (p.base ? row * p.ld_base + c : 0), p.base && on ? p.w - c : 0);
-        }
-        f32x4 acc[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float f = 0.f;
-        if (has) {
-            f = (p.gates ? p.gates[row * p.gates_stride] : 1.f) * sc;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float lo[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int c = 0; c < p.splits; ++c)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const int rank = b * 16 + g * 4 + s;
-                        if (rank < p.r) lo[s] += p.part[(c * p.n + row) * p.r + rank];
-                    }
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f(m[b][s][j]), lo[s], acc[j], 0, 0, 0);
+                for (int e = 0; e < 8; ++e) x[e] = m[b][e];
+                transpose8(x, m[b]);
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int c = c0 + (e * 4 + g) * V, left = on ? p.w - c : 0;
-            Vec<T> z;
-#pragma unroll
-            for (int j = 0; j < V; ++j) z[j] = from_f<T>(has ? to_f(y[e][j]) + f * acc[j][e] : to_f(y[e][j]));
-            T* o = p.out + row * p.ld_out + c;
-            if (left >= V)
-                __builtin_memcpy(o, &z, 16);
-            else
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (j < left) o[j] = z[j];
-        }
+        if (full)
+            expand_columns<T, RT, KP, true>(p, t, m, L, c0, has);
+        else
+            expand_columns<T, RT, KP, false>(p, t, m, L, c0, has);
+    }
+    if (BACK && Low::kSplit && has && p.dot_t != nullptr && blockIdx.y == gridDim.y - 1) {
+        __syncthreads();
+        stage_low<T, RT, KP>(p, t, has, sc, p.dot, 1, L, nullptr, nullptr);
+        __syncthreads();
+        store_by_rank<T, RT, KP>(p, t, L, p.dot_t);
     }
 }
 
@@ -559,6 +716,101 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
         }
 }
 
+// The same for bf16 rows on the bf16 matrix cores: f low comes by rank as two bf16 (k_expand's
+// low_t, dot_t), 32 rows at a time; a lane's eight rows of eight columns are transposed
+// in registers.  A block takes a chunk and 512 columns, a wave 128 of them.
+struct SplitSide {
+    const bf16* low;                         // [2][r][ld_t]: hi, lo
+    const bf16* v; long ld_v; int w;
+    bf16* dM; float* part;
+};
+struct OuterSplitArgs {
+    const Tile* chunks; const int* perm; int r; long ld_t;
+    SplitSide side[2]; int split;
+};
+
+template <int NB>
+__global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
+{
+    __shared__ __align__(16) int rows[kMaxChunk + 32];
+    const Tile t = p.chunks[blockIdx.x];
+    if (t.q < 0) return;
+    const bool second = (int)blockIdx.y >= p.split;
+    const SplitSide s = second ? p.side[1] : p.side[0];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int c0 = (((int)blockIdx.y - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * (NB * 16);
+    for (int i = threadIdx.x; i < ((t.cnt + 31) & ~31); i += 256) rows[i] = p.perm[t.start + min(i, t.cnt - 1)];
+    __syncthreads();
+    if (c0 >= s.w) return;
+    const bool full = c0 + 128 <= s.w;
+    const int c = c0 + l16 * 8, left = s.w - c;
+    f32x4 acc[NB][8];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const bf16* lo0 = s.low + (long)p.r * p.ld_t;
+#pragma unroll 1
+    for (int i = g * 8; i < ((t.cnt + 31) & ~31); i += 32) {
+        Vec<bf16> v[8], x[8], hi[NB], lo[NB];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bf16* at = s.v + (long)rows[i + e] * s.ld_v + c;
+            v[e] = full ? load16(at) : load_part(at, left);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const long at = (long)min(rank0 + b * 16 + l16, p.r - 1) * p.ld_t + t.start + i;
+            hi[b] = load16(s.low + at);
+            lo[b] = load16(lo0 + at);
+        }
+        if (i - g * 8 + 32 > t.cnt) {  // the places past the chunk belong to other adapters
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e >= t.cnt) {
+                    v[e] = Vec<bf16>{};
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) hi[b][e] = lo[b][e] = (bf16)0.f;
+                }
+        }
+        transpose8(v, x);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[b][j] = mfma16(lo[b], x[j], mfma16(hi[b], x[j], acc[b][j]));
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int rank = rank0 + b * 16 + g * 4 + e;
+            if (rank >= p.r) continue;
+            if (t.slot >= 0) {
+                float* o = s.part + ((long)t.slot * p.r + rank) * s.w + c;
+                float z[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = acc[b][j][e];
+                if (full)
+                    __builtin_memcpy(o, z, 32);
+                else
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < left) o[j] = z[j];
+            } else {
+                bf16* o = s.dM + ((long)t.q * p.r + rank) * s.w + c;
+                Vec<bf16> z;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = (bf16)acc[b][j][e];
+                if (full)
+                    __builtin_memcpy(o, &z, 16);
+                else
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < left) o[j] = z[j];
+            }
+        }
+}
+
 // The chunks' sums of the adapters that have several, added in chunk order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_outer_merge(OuterArgs<T> p)
@@ -584,21 +836,23 @@ size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 
 struct Layout {
     long n; int a, r;
-    bool direct;
+    bool direct, split;                   // split: k_outer_split
     int blocks, ntiles, nchunks, chunk;
     int down_splits, up_splits;           // of d (t = D x) and of o (u = U dy)
-    size_t hist, perm, tiles, chunks, merge, part, low, dpart, upart, bytes;
+    long ld_t;
+    size_t hist, perm, tiles, chunks, merge, part, low, low_t, dot_t, dpart, upart, bytes;
 };
 
-// Parts of the columns, so that enough blocks read at once; each wave still has a step.
+// Parts of the columns, so that enough blocks read at once while a wave still has two
+// steps of its own.
 int split_count(long tiles, int w, int type, int zs)
 {
     if (tiles < 1) tiles = 1;
     const long steps = (w + 128 / (int)elem_size(type) - 1) / (128 / (int)elem_size(type));
-    long s = (1024 + tiles * zs - 1) / (tiles * zs);
-    const long most = (steps + 3) / 4;
+    long s = (512 + tiles * zs - 1) / (tiles * zs);
+    const long most = steps / 8;
     if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+    return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
 Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
@@ -606,11 +860,13 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     Layout L{};
     L.n = n; L.a = a; L.r = r;
     L.direct = n <= kDirectRows && !backward;
+    L.split = type == kBF16;
     L.blocks = (int)((n + kPlanRows - 1) / kPlanRows);
     if (L.blocks < 1) L.blocks = 1;
     L.ntiles = L.direct ? (int)n : (int)((n + kTile - 1) / kTile) + a + 1;
     L.chunk = kMaxChunk / 2;
     L.nchunks = (int)(n / L.chunk) + a;
+    L.ld_t = ((n + 31) & ~31l) + 32;
     const int zs = (r + 63) / 64;
     L.down_splits = split_count(L.direct ? n : (n + kTile - 1) / kTile, d, type, zs);
     L.up_splits = split_count(L.direct ? n : (n + kTile - 1) / kTile, o, type, zs);
@@ -625,7 +881,9 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     if (backward) {
         take(L.chunks, (size_t)L.nchunks * sizeof(Tile));
         take(L.merge, (size_t)a * sizeof(int2));
-        take(L.low, (size_t)n * r * 4);
+        take(L.low, L.split ? 0 : (size_t)n * r * 4);
+        take(L.low_t, L.split ? (size_t)2 * r * L.ld_t * 2 : 0);
+        take(L.dot_t, L.split ? (size_t)2 * r * L.ld_t * 2 : 0);
         take(L.dpart, (size_t)L.nchunks * r * d * 4);
         take(L.upart, (size_t)L.nchunks * r * o * 4);
     }
@@ -633,8 +891,21 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     return L;
 }
 
+// k_plan's dynamic LDS may pass 64 KB; set once a process.
+hipError_t plan_ready()
+{
+    static const hipError_t e = [] {
+        const int most = 8 * (kAdaptMaxA + 2) + 64 + kPlanThreads / 64 * 2 * (kAdaptMaxA + 1);
+        const hipError_t c = hipFuncSetAttribute(reinterpret_cast<const void*>(k_plan_count), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+        return c != hipSuccess ? c : hipFuncSetAttribute(reinterpret_cast<const void*>(k_plan_place), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    }();
+    return e;
+}
+
 hipError_t launch_plan(const Layout& L, const int* ids, long ids_stride, char* ws, bool backward, hipStream_t s)
 {
+    const hipError_t ready = plan_ready();
+    if (ready != hipSuccess) return ready;
     PlanArgs p{ids, ids_stride, (int)L.n, L.a, L.blocks > 1 ? reinterpret_cast<int*>(ws + L.hist) : nullptr,
                reinterpret_cast<int*>(ws + L.perm), reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles,
                backward ? reinterpret_cast<Tile*>(ws + L.chunks) : nullptr, L.nchunks,
@@ -642,8 +913,9 @@ hipError_t launch_plan(const Layout& L, const int* ids, long ids_stride, char* w
     const int K = L.a + 1;
     int bits = 0;
     while ((1 << bits) < K) ++bits;
-    if (L.blocks > 1) SKM_TRY_LAUNCH(k_plan_count, L.blocks, 256, 8 * (size_t)K, s, p, bits);
-    return launch(k_plan_place, L.blocks, 256, 8 * (size_t)(K + 1) + 16 + 8 * (size_t)K, s, p, bits);
+    const size_t hist = kPlanThreads / 64 * 2 * (size_t)K;
+    if (L.blocks > 1) SKM_TRY_LAUNCH(k_plan_count, L.blocks, kPlanThreads, hist, s, p, bits);
+    return launch(k_plan_place, L.blocks, kPlanThreads, 8 * (size_t)(K + 1) + 64 + hist, s, p, bits);
 }
 
 template <typename T, int RT>
@@ -655,25 +927,14 @@ hipError_t launch_shrink(const ShrinkArgs<T>& p, int ntiles, hipStream_t s)
     return launch(k_shrink<T, RT, 4>, grid, 256, 0, s, p);
 }
 
-template <typename T, int RT>
+template <typename T, int RT, bool BACK>
 hipError_t launch_expand(const ExpandArgs<T>& p, int ntiles, hipStream_t s)
 {
     const dim3 grid(ntiles, (p.w + 64 * kVec<T> - 1) / (64 * kVec<T>));
-    if (p.r <= 16) return launch(k_expand<T, RT, 1>, grid, 256, 0, s, p);
-    if (p.r <= 32) return launch(k_expand<T, RT, 2>, grid, 256, 0, s, p);
-    if (p.r <= 64) return launch(k_expand<T, RT, 4>, grid, 256, 0, s, p);
-    return launch(k_expand<T, RT, 8>, grid, 256, 0, s, p);
-}
-
-template <typename T>
-hipError_t shrink_expand(const Layout& L, const Rows& rows, const ShrinkArgs<T>& sh, const ExpandArgs<T>& ex, hipStream_t s)
-{
-    if (L.direct) {
-        const hipError_t e = L.a > 0 ? launch_shrink<T, 1>(sh, L.ntiles, s) : hipSuccess;
-        return e != hipSuccess ? e : launch_expand<T, 1>(ex, L.ntiles, s);
-    }
-    const hipError_t e = L.a > 0 ? launch_shrink<T, kTile / 16>(sh, L.ntiles, s) : hipSuccess;
-    return e != hipSuccess ? e : launch_expand<T, kTile / 16>(ex, L.ntiles, s);
+    if (p.r <= 16) return launch(k_expand<T, RT, 16, BACK>, grid, 256, 0, s, p);
+    if (p.r <= 32) return launch(k_expand<T, RT, 32, BACK>, grid, 256, 0, s, p);
+    if (p.r <= 64) return launch(k_expand<T, RT, 64, BACK>, grid, 256, 0, s, p);
+    return launch(k_expand<T, RT, 128, BACK>, grid, 256, 0, s, p);
 }
 
 }  // namespace
@@ -694,8 +955,12 @@ hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
         using T = decltype(tag);
         const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.down_splits, part};
         const ExpandArgs<T> ex{rows, part, L.down_splits, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
-                               (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, a.o, a.r, a.low, nullptr, nullptr};
-        return shrink_expand<T>(L, rows, sh, ex, s);
+                               (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, a.o, a.r, a.low, nullptr, nullptr, nullptr, nullptr, 0};
+        if (a.a > 0) {
+            const hipError_t e = L.direct ? launch_shrink<T, 1>(sh, L.ntiles, s) : launch_shrink<T, kTile / 16>(sh, L.ntiles, s);
+            if (e != hipSuccess) return e;
+        }
+        return L.direct ? launch_expand<T, 1, false>(ex, L.ntiles, s) : launch_expand<T, kTile / 16, false>(ex, L.ntiles, s);
     });
 }
 
@@ -706,29 +971,49 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
     const hipError_t planned = launch_plan(L, a.ids, a.ids_stride, a.ws, true, s);
     if (planned != hipSuccess) return planned;
     const Rows rows{reinterpret_cast<const Tile*>(a.ws + L.tiles), reinterpret_cast<const int*>(a.ws + L.perm), a.ids, a.ids_stride, a.a};
+    const Tile* chunks = reinterpret_cast<const Tile*>(a.ws + L.chunks);
     float* part = reinterpret_cast<float*>(a.ws + L.part);
-    float* u = reinterpret_cast<float*>(a.ws + L.low);
+    float* u = L.split ? nullptr : reinterpret_cast<float*>(a.ws + L.low);
+    bf16* u_t = L.split ? reinterpret_cast<bf16*>(a.ws + L.low_t) : nullptr;
+    bf16* t_t = L.split ? reinterpret_cast<bf16*>(a.ws + L.dot_t) : nullptr;
+    float* dpart = reinterpret_cast<float*>(a.ws + L.dpart);
+    float* upart = reinterpret_cast<float*>(a.ws + L.upart);
     return with_type(a.type, [&](auto tag) {
         using T = decltype(tag);
         if (a.n > 0) {
             const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.up_splits, part};
             const ExpandArgs<T> ex{rows, part, L.up_splits, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
-                                   (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates};
-            const hipError_t e = shrink_expand<T>(L, rows, sh, ex, s);
+                                   (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t, L.ld_t};
+            if (a.a > 0) {
+                const hipError_t e = launch_shrink<T, kTile / 16>(sh, L.ntiles, s);
+                if (e != hipSuccess) return e;
+            }
+            const hipError_t e = launch_expand<T, kTile / 16, true>(ex, L.ntiles, s);
             if (e != hipSuccess) return e;
         }
         if (a.a == 0) return hipSuccess;
         constexpr int W = 16 * kVec<T>;
-        const OuterArgs<T> ou{reinterpret_cast<const Tile*>(a.ws + L.chunks), reinterpret_cast<const int2*>(a.ws + L.merge), rows.perm, a.a, a.r,
-                              a.gates, a.gates_stride, a.scales,
-                              {{u, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, reinterpret_cast<float*>(a.ws + L.dpart)},
-                               {a.low, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, reinterpret_cast<float*>(a.ws + L.upart)}},
+        const OuterArgs<T> ou{chunks, reinterpret_cast<const int2*>(a.ws + L.merge), rows.perm, a.a, a.r, a.gates, a.gates_stride, a.scales,
+                              {{u, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {a.low, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
                               (a.d + W - 1) / W};
-        const int cols = ou.split + (a.o + W - 1) / W;
-        if (a.r <= 16)
-            SKM_TRY_LAUNCH(k_outer<T, 1>, dim3(L.nchunks, cols, 1), 256, 2 * 16 * W * 4, s, ou);
-        else
-            SKM_TRY_LAUNCH(k_outer<T, 2>, dim3(L.nchunks, cols, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
+        if constexpr (std::is_same_v<T, bf16>) {
+            const OuterSplitArgs os{chunks, rows.perm, a.r, L.ld_t,
+                                    {{u_t, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {t_t, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
+                                    (a.d + 511) / 512};
+            const int cols = os.split + (a.o + 511) / 512;
+            if (a.r <= 16)
+                SKM_TRY_LAUNCH(k_outer_split<1>, dim3(L.nchunks, cols, 1), 256, 0, s, os);
+            else if (a.r <= 32)
+                SKM_TRY_LAUNCH(k_outer_split<2>, dim3(L.nchunks, cols, 1), 256, 0, s, os);
+            else
+                SKM_TRY_LAUNCH(k_outer_split<4>, dim3(L.nchunks, cols, (a.r + 63) / 64), 256, 0, s, os);
+        } else {
+            const int cols = ou.split + (a.o + W - 1) / W;
+            if (a.r <= 16)
+                SKM_TRY_LAUNCH((k_outer<T, 1>), dim3(L.nchunks, cols, 1), 256, 2 * 16 * W * 4, s, ou);
+            else
+                SKM_TRY_LAUNCH((k_outer<T, 2>), dim3(L.nchunks, cols, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
+        }
         const long most = (long)a.r * (a.d > a.o ? a.d : a.o);
         return launch(k_outer_merge<T>, dim3((unsigned)((most + 1023) / 1024), a.a, 2), 256, 0, s, ou);
     });
