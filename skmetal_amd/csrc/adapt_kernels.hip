@@ -11,7 +11,7 @@
 //   dD_q = sum_i f_i u_i x_i^T        dU_q = sum_i f_i t_i dy_i^T
 //
 // Three products in all: rows to ranks (k_shrink: t, u), ranks to rows (k_expand: out, dx)
-// and rows by rows (k_outer: dD, dU).  k_plan_place first puts the rows of each adapter side by
+// and rows by rows (k_outer: dD, dU).  k_plan first puts the rows of each adapter side by
 // side (a stable counting sort) and cuts them into tiles of one adapter; with few rows
 // every row is its own tile and there is no sort.
 #include "experts_common.h"
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kTile = 64;          // rows of a k_shrink / k_expand tile
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanLoads = 16;     // rows a k_plan lane holds
+constexpr int kPlanLoads = 16;     // ids a k_plan lane holds
 constexpr int kPlanRows = kPlanThreads * kPlanLoads;
 
 struct Tile {
@@ -33,7 +33,6 @@ struct Tile {
 
 struct PlanArgs {
     const int* ids; long ids_stride; int n, a;
-    int* hist;           // [blocks x (a + 1)], more than one block only
     int* perm;           // [n] rows in the order of their adapters
     Tile* tiles; int ntiles;    // kTile rows each
     Tile* chunks; int nchunks;  // nullable; `chunk` rows each, one at least per adapter
@@ -47,168 +46,89 @@ __device__ __forceinline__ int adapter_of(const int* ids, long stride, long i, i
     return q >= 0 && q < a ? q : a;
 }
 
-// Lanes that hold the same key (of `bits` bits) as this one, among those with `on`.
-__device__ __forceinline__ unsigned long long same_key(int key, bool on, int bits)
+// The rows of adapter blockIdx.x (a: of none) in their order, and its tiles: every block
+// reads all the ids, counts those below its own and writes its own rows' places.  Tile j
+// of adapter q has the entry start_q / len + q + j: start_(q+1) / len + q + 1 is at least
+// that many entries on, so no block needs another's count; the entries between stay
+// unused.  (At 16,384 rows and 64 adapters 5 us; one block that sorts all rows took 18.)
+__device__ void write_tiles(int q, int a, int start, int cnt, int len, bool whole, Tile* out, int bound, int2* merge)
 {
-    unsigned long long m = __ballot(on);
-    for (int b = 0; b < bits; ++b) {
-        const bool one = (key >> b) & 1;
-        const unsigned long long v = __ballot(one);
-        m &= one ? v : ~v;
-    }
-    return m;
+    const int first = start / len + q;
+    const int tiles = !whole ? (cnt + len - 1) / len : q == a ? 0 : max(1, (cnt + len - 1) / len);
+    const int next = q == a ? bound : (start + cnt) / len + q + 1;
+    for (int j = threadIdx.x; first + j < next; j += kPlanThreads)
+        out[first + j] = j < tiles ? Tile{q, start + j * len, min(len, cnt - j * len), whole && tiles > 1 ? first + j : -1} : Tile{-1, 0, 0, -1};
+    if (merge != nullptr && q < a && threadIdx.x == 0) merge[q] = make_int2(first, tiles > 1 ? tiles : 0);
 }
 
-// Exclusive sum of v[0 .. count) in place, v[count] = the total; tmp holds a value a wave.
-__device__ void block_scan(int* v, int count, int* tmp)
+__global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs p)
 {
-    const int per = (count + kPlanThreads - 1) / kPlanThreads;
-    const int lo = min(count, (int)threadIdx.x * per), hi = min(count, lo + per);
-    int s = 0;
-    for (int i = lo; i < hi; ++i) s += v[i];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int inc = s;
-    for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(inc, off, 64);
-        if (lane >= off) inc += o;
-    }
-    if (lane == 63) tmp[wave] = inc;
-    __syncthreads();
-    int base = inc - s;
-    for (int w = 0; w < wave; ++w) base += tmp[w];
-    for (int i = lo; i < hi; ++i) {
-        const int x = v[i];
-        v[i] = base;
-        base += x;
-    }
-    if (threadIdx.x == kPlanThreads - 1) v[count] = base;
-    __syncthreads();
-}
-
-// The keys of this block's rows, a wave's 64 * kPlanLoads rows side by side, and per wave how many
-// have each key (the first lane of equal keys adds them up, so no two lanes write one
-// place).  rank: lanes before this one with its key, and 256 times all lanes with it.
-__device__ __forceinline__ void count_keys(const PlanArgs& p, unsigned short* wh, int K, int bits, int* key, int* rank)
-{
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long first = (long)blockIdx.x * kPlanRows + wave * (64 * kPlanLoads) + lane;
+    __shared__ int below[kPlanThreads / 64], equal[kPlanThreads / 64];
+    const int q = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int key[kPlanLoads];
 #pragma unroll
-    for (int it = 0; it < kPlanLoads; ++it) {
-        const long i = first + it * 64;
-        key[it] = p.n > 0 ? p.ids[min(i, (long)p.n - 1) * p.ids_stride] : 0;
-        key[it] = i >= p.n ? -1 : key[it] >= 0 && key[it] < p.a ? key[it] : p.a;
-    }
-    for (int j = threadIdx.x; j < kPlanThreads / 64 * K; j += kPlanThreads) wh[j] = 0;
-    __syncthreads();
-    volatile unsigned short* mine = wh + wave * K;
+    for (int it = 0; it < kPlanLoads; ++it) key[it] = p.a + 1;  // of no row
+    auto fetch = [&](long from) {
+        const long first = from + wave * (64 * kPlanLoads) + lane;
 #pragma unroll
-    for (int it = 0; it < kPlanLoads; ++it) {
-        const unsigned long long m = same_key(key[it], key[it] >= 0, bits);
-        const int before = __popcll(m & ((1ull << lane) - 1)), all = __popcll(m);
-        rank[it] = before + 256 * all;
-        if (key[it] >= 0 && before == 0) mine[key[it]] = (unsigned short)(mine[key[it]] + all);
+        for (int it = 0; it < kPlanLoads; ++it) {
+            const long i = first + it * 64;
+            const int k = p.ids[min(i, (long)p.n - 1) * p.ids_stride];
+            key[it] = i >= p.n ? p.a + 1 : k >= 0 && k < p.a ? k : p.a;
+        }
+    };
+    int lo = 0, eq = 0;
+    for (long from = 0; from < p.n; from += kPlanRows) {
+        fetch(from);
+#pragma unroll
+        for (int it = 0; it < kPlanLoads; ++it) {
+            lo += __popcll(__ballot(key[it] < q));
+            eq += __popcll(__ballot(key[it] == q));
+        }
     }
+    if (lane == 0) { below[wave] = lo; equal[wave] = eq; }
     __syncthreads();
-}
-
-__global__ __launch_bounds__(kPlanThreads) void k_plan_count(PlanArgs p, int bits)
-{
-    extern __shared__ char lds[];
-    unsigned short* wh = reinterpret_cast<unsigned short*>(lds);
-    const int K = p.a + 1;
-    int key[kPlanLoads], rank[kPlanLoads];
-    count_keys(p, wh, K, bits, key, rank);
-    for (int k = threadIdx.x; k < K; k += kPlanThreads) {
-        int c = 0;
-        for (int w = 0; w < kPlanThreads / 64; ++w) c += wh[w * K + k];
-        p.hist[(long)blockIdx.x * K + k] = c;
+    int start = 0, cnt = 0, place = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        start += below[w];
+        if (w < wave) place += equal[w];
+        cnt += equal[w];
     }
-}
-
-// The tiles of `len` rows of every key (off[k] .. off[k + 1] are its places); `whole`: one
-// at least per adapter and none for the rows without one.
-__device__ void write_tiles(const int* off, int* first, int K, int a, int len, bool whole, Tile* out, int bound, int* tmp, int2* merge)
-{
-    for (int k = threadIdx.x; k < K; k += kPlanThreads) {
-        const int c = off[k + 1] - off[k], t = (c + len - 1) / len;
-        first[k] = !whole ? t : k == a ? 0 : max(1, t);
-    }
-    __syncthreads();
-    block_scan(first, K, tmp);
-    const int total = first[K];
-    for (int t = threadIdx.x; t < bound; t += kPlanThreads) {
-        Tile e{-1, 0, 0, -1};
-        if (t < total) {
-            int lo = 0, hi = K;  // the last key whose tiles start at t or before
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (first[mid] <= t) lo = mid; else hi = mid;
+    if (p.n <= kPlanRows) {  // the keys are still here, each wave's rows follow those of the one before
+        place += start;
+#pragma unroll
+        for (int it = 0; it < kPlanLoads; ++it) {
+            const unsigned long long m = __ballot(key[it] == q);
+            if (key[it] == q) p.perm[place + __popcll(m & ((1ull << lane) - 1))] = wave * (64 * kPlanLoads) + it * 64 + lane;
+            place += __popcll(m);
+        }
+    } else {
+        int done = start;
+        for (long from = 0; from < p.n; from += kPlanRows) {
+            fetch(from);
+            eq = 0;
+#pragma unroll
+            for (int it = 0; it < kPlanLoads; ++it) eq += __popcll(__ballot(key[it] == q));
+            __syncthreads();
+            if (lane == 0) equal[wave] = eq;
+            __syncthreads();
+            place = done;
+#pragma unroll
+            for (int w = 0; w < kPlanThreads / 64; ++w) {
+                if (w < wave) place += equal[w];
+                done += equal[w];
             }
-            const int c = off[lo + 1] - off[lo], at = (t - first[lo]) * len;
-            e.q = lo;
-            e.start = off[lo] + at;
-            e.cnt = min(len, c - at);
-            if (whole && c > len) e.slot = t;
-        }
-        out[t] = e;
-    }
-    if (merge != nullptr)
-        for (int k = threadIdx.x; k < a; k += kPlanThreads) {
-            const int t = first[k + 1] - first[k];
-            merge[k] = make_int2(first[k], t > 1 ? t : 0);
-        }
-    __syncthreads();
-}
-
-// Places of the rows, and (block 0) the tiles.  Without a histogram this block holds all
-// the rows.
-__global__ __launch_bounds__(kPlanThreads) void k_plan_place(PlanArgs p, int bits)
-{
-    extern __shared__ char lds[];
-    const int K = p.a + 1;
-    int* off = reinterpret_cast<int*>(lds);        // [K + 1] first place of each key, over all rows
-    int* at = off + K + 1;                         // [K + 1] first place of this block's
-    int* tmp = at + K + 1;                         // [16]
-    unsigned short* wh = reinterpret_cast<unsigned short*>(tmp + 16);  // [16 x K]
-    int key[kPlanLoads], rank[kPlanLoads];
-    count_keys(p, wh, K, bits, key, rank);
-    for (int k = threadIdx.x; k < K; k += kPlanThreads) {
-        int c = 0;
-        for (int w = 0; w < kPlanThreads / 64; ++w) {
-            const int x = wh[w * K + k];
-            wh[w * K + k] = (unsigned short)c;
-            c += x;
-        }
-        int before = 0;
-        if (p.hist != nullptr) {
-            c = 0;
-            for (int b = 0; b < (int)gridDim.x; ++b) {
-                const int x = p.hist[(long)b * K + k];
-                if (b < (int)blockIdx.x) before += x;
-                c += x;
+#pragma unroll
+            for (int it = 0; it < kPlanLoads; ++it) {
+                const unsigned long long m = __ballot(key[it] == q);
+                if (key[it] == q) p.perm[place + __popcll(m & ((1ull << lane) - 1))] = (int)(from + wave * (64 * kPlanLoads) + it * 64 + lane);
+                place += __popcll(m);
             }
         }
-        off[k] = c;
-        at[k] = before;
     }
-    __syncthreads();
-    block_scan(off, K, tmp);
-    for (int k = threadIdx.x; k < K; k += kPlanThreads) at[k] += off[k];
-    __syncthreads();
-    const int wave = threadIdx.x >> 6;
-    const long first = (long)blockIdx.x * kPlanRows + wave * (64 * kPlanLoads) + (threadIdx.x & 63);
-    volatile unsigned short* mine = wh + wave * K;
-#pragma unroll
-    for (int it = 0; it < kPlanLoads; ++it)
-        if (key[it] >= 0) {
-            const int seen = mine[key[it]], before = rank[it] & 255;
-            p.perm[at[key[it]] + seen + before] = (int)(first + it * 64);
-            if (before == 0) mine[key[it]] = (unsigned short)(seen + (rank[it] >> 8));
-        }
-    if (blockIdx.x != 0) return;
-    __syncthreads();
-    write_tiles(off, at, K, p.a, kTile, false, p.tiles, p.ntiles, tmp, nullptr);
-    if (p.chunks != nullptr) write_tiles(off, at, K, p.a, p.chunk, true, p.chunks, p.nchunks, tmp, p.merge);
+    write_tiles(q, p.a, start, cnt, kTile, false, p.tiles, p.ntiles, nullptr);
+    if (p.chunks != nullptr) write_tiles(q, p.a, start, cnt, p.chunk, true, p.chunks, p.nchunks, p.merge);
 }
 
 // ---- loads of 16 bytes of a row, the elements past `left` as 0 ----
@@ -251,10 +171,13 @@ struct Rows {  // where the rows of a tile come from
     const int* ids; long ids_stride; int a;
 };
 
-__device__ __forceinline__ Tile tile_at(const Rows& w, int t)
+// The tile of block x.  Blocks go to the 8 XCDs in turn, so neighbouring tiles, which
+// share adapters, are given to blocks 8 apart: an XCD's L2 then serves an adapter to all
+// its tiles (gridDim.x is a multiple of 8).
+__device__ __forceinline__ Tile tile_at(const Rows& w, int x)
 {
-    if (w.tiles != nullptr) return w.tiles[t];
-    return Tile{adapter_of(w.ids, w.ids_stride, t, w.a), t, 1, -1};
+    if (w.tiles != nullptr) return w.tiles[(x & 7) * (gridDim.x >> 3) + (x >> 3)];
+    return Tile{adapter_of(w.ids, w.ids_stride, x, w.a), x, 1, -1};
 }
 
 __device__ __forceinline__ int row_at(const Rows& w, int place) { return w.tiles != nullptr ? w.perm[place] : place; }
@@ -268,10 +191,10 @@ struct ShrinkArgs {
     const T* M; long sa, ld;     // [a][r][w]
     int w, r; long n;
     int splits;                  // of w, one a blockIdx.y
-    float* part;                 // [splits][n][r]
+    float* part; int rp;         // [splits][n places][rp], rp = the ranks in whole 16s
 };
 
-// part[s][row][t] = sum over the s-th part of the columns of M_q[t] v_row.  A block takes
+// part[s][place][t] = sum over the s-th part of the columns of M_q[t] v_row, 0 from r on.  A block takes
 // RT * 16 rows of one adapter and NB * 16 ranks; its four waves take the columns in turn,
 // 128 bytes of each row at a time, and add up their sums at the end, so that rows and
 // adapter are read once and go to the matrix cores straight from memory.
@@ -345,18 +268,17 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
         __syncthreads();
     }
     if (wave != 0) return;
-    float* out = p.part + (long)blockIdx.y * p.n * p.r;
+    float* out = p.part + ((long)blockIdx.y * p.n + t.start) * p.rp;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int at = i * 16 + g * 4 + e;
             if (at >= t.cnt) continue;
-            const long row = row_at(p.rows, t.start + at);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int rank = rank0 + b * 16 + l16;
-                if (rank < p.r) out[row * p.r + rank] = acc[i][b][e];
+                if (rank < p.rp) out[at * p.rp + rank] = rank < p.r ? acc[i][b][e] : 0.f;
             }
         }
 }
@@ -390,7 +312,7 @@ __device__ __forceinline__ void transpose8(const Vec<bf16>* a, Vec<bf16>* b)
 template <typename T>
 struct ExpandArgs {
     Rows rows;
-    const float* part; int splits; long n;   // k_shrink's
+    const float* part; int splits, rp; long n;   // k_shrink's
     const T* M; long sa, ld;                 // [a][r][w]
     const float* gates; long gates_stride; const float* scales;
     const T* base; long ld_base;             // nullable
@@ -407,49 +329,100 @@ template <typename T, int RT, int KP>
 struct LowTile {
     static constexpr bool kSplit = false;
     float v[RT * 16][KP + 4];
-    __device__ void set(int i, int k, float x) { v[i][k] = x; }
+    __device__ void set(int i, int k, f32x4 x) { *reinterpret_cast<f32x4*>(&v[i][k]) = x; }
 };
 template <int RT, int KP>
 struct LowTile<bf16, RT, KP> {
     static constexpr bool kSplit = true;
     bf16 v[RT * 16][2 * KP + 8];
-    __device__ void set(int i, int k, float x) { split2(x, v[i][k], v[i][KP + k]); }
+    __device__ void set(int i, int k, f32x4 x)
+    {
+        bf16 __attribute__((ext_vector_type(4))) hi, lo;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            bf16 a, b;
+            split2(x[u], a, b);
+            hi[u] = a;
+            lo[u] = b;
+        }
+        __builtin_memcpy(&v[i][k], &hi, 8);
+        __builtin_memcpy(&v[i][KP + k], &lo, 8);
+    }
 };
 
-// Sums the splits of a tile's low-rank rows (a row's ranks by neighbouring lanes) into L,
-// times f; store: the sums themselves to low; dot: their products with dot to dgates.
+// A row's own numbers in a tile, which its first threads look up.
+template <int RT>
+struct TileRows {
+    int row[RT * 16];
+    float f[RT * 16];
+};
+
+template <typename T, int RT>
+__device__ __forceinline__ void stage_rows(const ExpandArgs<T>& p, const Tile& t, bool has, float sc, TileRows<RT>& R)
+{
+    if (threadIdx.x < RT * 16) {
+        const int row = row_at(p.rows, t.start + min((int)threadIdx.x, t.cnt - 1));
+        R.row[threadIdx.x] = row;
+        R.f[threadIdx.x] = has ? (p.gates ? p.gates[row * p.gates_stride] : 1.f) * sc : 0.f;
+    }
+}
+
+// The splits' sums of a tile's low-rank rows, four ranks a thread at a time, times f into L.
+// store: the sums themselves, by row; dgates: s_q times their products with dot.
+// Barriers: one before this writes L and reads R, the caller's one after it.
 template <typename T, int RT, int KP>
-__device__ __forceinline__ void stage_low(const ExpandArgs<T>& p, const Tile& t, bool has, float sc, const float* part, int splits, LowTile<T, RT, KP>& L,
+__device__ __forceinline__ void stage_low(const ExpandArgs<T>& p, const Tile& t, bool has, float sc, LowTile<T, RT, KP>& L, const TileRows<RT>& R,
                                           float* store, float* dgates)
 {
-    constexpr int KW = KP < 64 ? KP : 64;
-#pragma unroll 1
-    for (int idx = threadIdx.x; idx < RT * 16 * KW; idx += 256) {
-        const int i = idx / KW, k0 = idx % KW;
-        const bool on = i < t.cnt;
-        const long row = row_at(p.rows, t.start + (on ? i : 0));
-        const float f = has ? (p.gates ? p.gates[row * p.gates_stride] : 1.f) * sc : 0.f;
+    constexpr int Q = KP / 4, ALL = RT * 16 * Q, PER = (ALL + 255) / 256;
+    f32x4 s[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (has)
+        for (int c = 0; c < p.splits; ++c) {
+            const float* part = p.part + ((long)c * p.n + t.start) * p.rp;
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const int idx = threadIdx.x + u * 256, i = idx / Q, k = idx % Q * 4;
+                if (idx < ALL && i < t.cnt && k < p.rp) s[u] += *reinterpret_cast<const f32x4*>(part + i * p.rp + k);
+            }
+        }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        const int idx = threadIdx.x + u * 256, i = idx / Q, k = idx % Q * 4;
+        if (idx >= ALL) break;
+        L.set(i, k, s[u] * R.f[i]);
+        if (store == nullptr && dgates == nullptr) continue;
+        const long row = R.row[i];
         float d = 0.f;
 #pragma unroll
-        for (int k = k0; k < KP; k += KW) {
-            float s = 0.f;
-            if (has && on && k < p.r)
-                for (int c = 0; c < splits; c += 4) {  // four loads at once; the sum stays in order
-                    float x[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) x[u] = part[(min(c + u, splits - 1) * p.n + row) * p.r + k];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) s += c + u < splits ? x[u] : 0.f;
-                }
-            L.set(i, k, has && on && k < p.r ? f * s : 0.f);
-            if (store != nullptr && on && k < p.r) store[row * p.r + k] = s;
-            if (dgates != nullptr && has && on && k < p.r) d += s * p.dot[row * p.r + k];
-        }
+        for (int v = 0; v < 4; ++v)
+            if (i < t.cnt && k + v < p.r) {
+                if (store != nullptr) store[row * p.r + k + v] = s[u][v];
+                if (dgates != nullptr && has) d += s[u][v] * p.dot[row * p.r + k + v];
+            }
         if (dgates != nullptr) {
 #pragma unroll
-            for (int off = 1; off < KW; off <<= 1) d += __shfl_xor(d, off, 64);
-            if (k0 == 0 && on) dgates[row] = has ? d * sc : 0.f;
+            for (int off = 1; off < Q; off <<= 1) d += __shfl_xor(d, off, 64);
+            if (k == 0 && i < t.cnt) dgates[row] = has ? d * sc : 0.f;
         }
+    }
+}
+
+// f dot into L, dot [n x r] by row (R is there).
+template <typename T, int RT, int KP>
+__device__ __forceinline__ void stage_dot(const ExpandArgs<T>& p, const Tile& t, LowTile<T, RT, KP>& L, const TileRows<RT>& R)
+{
+    constexpr int Q = KP / 4, ALL = RT * 16 * Q;
+#pragma unroll 4
+    for (int idx = threadIdx.x; idx < ALL; idx += 256) {
+        const int i = idx / Q, k = idx % Q * 4;
+        const float* at = p.dot + (long)R.row[i] * p.r + k;
+        f32x4 s;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[v] = i < t.cnt && k + v < p.r ? at[v] : 0.f;
+        L.set(i, k, s * R.f[i]);
     }
 }
 
@@ -476,14 +449,14 @@ __device__ __forceinline__ void store_by_rank(const ExpandArgs<T>& p, const Tile
 // The sums start from the base where its type rounds at 2^-8 or 2^-11 anyway; in fp32 they
 // would then round at the base's size once for every four ranks, so it is added last.
 template <typename T, int RT, int KP, bool FULL>
-__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, int c0, bool has)
+__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, const TileRows<RT>& R, int c0, bool has)
 {
     constexpr int V = kVec<T>;
     constexpr bool kBaseFirst = sizeof(T) == 2;
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
     long row[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) row[i] = row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1));
+    for (int i = 0; i < RT; ++i) row[i] = R.row[i * 16 + l16];
     Vec<T> y[2][4];
     auto fetch = [&](int i) {
 #pragma unroll
@@ -558,6 +531,7 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
     constexpr int V = kVec<T>;
     using Low = LowTile<T, RT, KP>;
     __shared__ __align__(16) Low L;
+    __shared__ TileRows<RT> R;
     const Tile t = tile_at(p.rows, blockIdx.x);
     if (t.q < 0) return;
     const bool has = t.q < p.rows.a;
@@ -567,7 +541,7 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
     const bool full = c0 + 16 * V <= p.w;
     // eight ranks of kVec columns: bf16: g * 8 .. + 7 of every 32 (of 16, for half as many
     // ranks); else g * 4 .. + 3 of every 16, two such
-    constexpr int NM = Low::kSplit ? (KP + 31) / 32 : (KP + 31) / 32;
+    constexpr int NM = (KP + 31) / 32;
     Vec<T> m[NM][8];
     if (has && c0 < p.w) {
         const int cm = c0 + ((l16 & 3) * 4 + (l16 >> 2)) * V;  // the columns this lane brings
@@ -583,8 +557,8 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
         }
     }
     const bool first = blockIdx.y == 0;
-    if (has || first)
-        stage_low<T, RT, KP>(p, t, has, sc, p.part, p.splits, L, first ? p.low : nullptr, BACK && first ? p.dgates : nullptr);
+    stage_rows<T, RT>(p, t, has, sc, R);
+    stage_low<T, RT, KP>(p, t, has, sc, L, R, first ? p.low : nullptr, BACK && first ? p.dgates : nullptr);
     __syncthreads();
     if (BACK && Low::kSplit && first && has && p.low_t != nullptr) store_by_rank<T, RT, KP>(p, t, L, p.low_t);
     if (c0 < p.w) {
@@ -598,13 +572,13 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
             }
         }
         if (full)
-            expand_columns<T, RT, KP, true>(p, t, m, L, c0, has);
+            expand_columns<T, RT, KP, true>(p, t, m, L, R, c0, has);
         else
-            expand_columns<T, RT, KP, false>(p, t, m, L, c0, has);
+            expand_columns<T, RT, KP, false>(p, t, m, L, R, c0, has);
     }
     if (BACK && Low::kSplit && has && p.dot_t != nullptr && blockIdx.y == gridDim.y - 1) {
         __syncthreads();
-        stage_low<T, RT, KP>(p, t, has, sc, p.dot, 1, L, nullptr, nullptr);
+        stage_dot<T, RT, KP>(p, t, L, R);
         __syncthreads();
         store_by_rank<T, RT, KP>(p, t, L, p.dot_t);
     }
@@ -730,7 +704,7 @@ struct OuterSplitArgs {
 };
 
 template <int NB>
-__global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
+__global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
 {
     __shared__ __align__(16) int rows[kMaxChunk + 32];
     const Tile t = p.chunks[blockIdx.x];
@@ -811,18 +785,37 @@ __global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
         }
 }
 
-// The chunks' sums of the adapters that have several, added in chunk order.
+// The chunks' sums of the adapters that have several, added in chunk order; every block a
+// part of each such adapter's matrix.
 template <typename T>
 __global__ __launch_bounds__(256) void k_outer_merge(OuterArgs<T> p)
 {
-    const int2 m = p.merge[blockIdx.y];
-    if (m.y == 0) return;
-    const OuterSide<T>& s = p.side[blockIdx.z];
+    const OuterSide<T>& s = p.side[blockIdx.y];
     const long size = (long)p.r * s.w;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long)gridDim.x * 256) {
-        float v = 0.f;
-        for (int k = 0; k < m.y; ++k) v += s.part[(m.x + k) * size + i];
-        s.dM[blockIdx.y * size + i] = from_f<T>(v);
+    for (int q0 = 0; q0 < p.a; q0 += 256) {
+        __shared__ int2 some[256];
+        __shared__ int who[256], count;
+        __syncthreads();
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        const int q = q0 + threadIdx.x;
+        if (q < p.a) {
+            const int2 m = p.merge[q];
+            if (m.y != 0) {
+                const int at = atomicAdd(&count, 1);  // in any order: each is summed by itself
+                some[at] = m;
+                who[at] = q;
+            }
+        }
+        __syncthreads();
+        for (int j = 0; j < count; ++j) {
+            const int2 m = some[j];
+            for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long)gridDim.x * 256) {
+                float v = 0.f;
+                for (int k = 0; k < m.y; ++k) v += s.part[(m.x + k) * size + i];
+                s.dM[who[j] * size + i] = from_f<T>(v);
+            }
+        }
     }
 }
 
@@ -837,10 +830,11 @@ size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 struct Layout {
     long n; int a, r;
     bool direct, split;                   // split: k_outer_split
-    int blocks, ntiles, nchunks, chunk;
+    int ntiles, nchunks, chunk;           // ntiles: in whole 8s unless direct
+    int rp;
     int down_splits, up_splits;           // of d (t = D x) and of o (u = U dy)
     long ld_t;
-    size_t hist, perm, tiles, chunks, merge, part, low, low_t, dot_t, dpart, upart, bytes;
+    size_t perm, tiles, chunks, merge, part, low, low_t, dot_t, dpart, upart, bytes;
 };
 
 // Parts of the columns, so that enough blocks read at once while a wave still has two
@@ -855,16 +849,25 @@ int split_count(long tiles, int w, int type, int zs)
     return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
+// Rows a k_outer block sums up: as many as leave about two blocks a CU, for every cut
+// costs a partial matrix written and read.
+int chunk_rows(long n, int w, int a, int type)
+{
+    const int cols = type == kBF16 ? 512 : 16 * (16 / (int)elem_size(type));
+    int c = kMaxChunk;
+    while (c > 64 && (n / c + (a < n / c ? a : n / c)) * 2 * ((w + cols - 1) / cols) < 512) c /= 2;
+    return c;
+}
+
 Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
 {
     Layout L{};
     L.n = n; L.a = a; L.r = r;
     L.direct = n <= kDirectRows && !backward;
     L.split = type == kBF16;
-    L.blocks = (int)((n + kPlanRows - 1) / kPlanRows);
-    if (L.blocks < 1) L.blocks = 1;
-    L.ntiles = L.direct ? (int)n : (int)((n + kTile - 1) / kTile) + a + 1;
-    L.chunk = kMaxChunk / 2;
+    L.ntiles = L.direct ? (int)n : (int)((n / kTile + a + 1 + 7) & ~7l);
+    L.rp = (r + 15) & ~15;
+    L.chunk = chunk_rows(n, d < o ? d : o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
     L.ld_t = ((n + 31) & ~31l) + 32;
     const int zs = (r + 63) / 64;
@@ -873,11 +876,10 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     size_t at = 0;
     auto take = [&](size_t& where, size_t bytes) { where = at; at += up16(bytes); };
     if (!L.direct) {
-        take(L.hist, L.blocks > 1 ? (size_t)L.blocks * (a + 1) * 4 : 0);
         take(L.perm, (size_t)n * 4);
         take(L.tiles, (size_t)L.ntiles * sizeof(Tile));
     }
-    take(L.part, (size_t)(backward ? L.up_splits : L.down_splits) * n * r * 4);
+    take(L.part, (size_t)(backward ? L.up_splits : L.down_splits) * n * L.rp * 4);
     if (backward) {
         take(L.chunks, (size_t)L.nchunks * sizeof(Tile));
         take(L.merge, (size_t)a * sizeof(int2));
@@ -891,31 +893,12 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     return L;
 }
 
-// k_plan's dynamic LDS may pass 64 KB; set once a process.
-hipError_t plan_ready()
-{
-    static const hipError_t e = [] {
-        const int most = 8 * (kAdaptMaxA + 2) + 64 + kPlanThreads / 64 * 2 * (kAdaptMaxA + 1);
-        const hipError_t c = hipFuncSetAttribute(reinterpret_cast<const void*>(k_plan_count), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-        return c != hipSuccess ? c : hipFuncSetAttribute(reinterpret_cast<const void*>(k_plan_place), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    }();
-    return e;
-}
-
 hipError_t launch_plan(const Layout& L, const int* ids, long ids_stride, char* ws, bool backward, hipStream_t s)
 {
-    const hipError_t ready = plan_ready();
-    if (ready != hipSuccess) return ready;
-    PlanArgs p{ids, ids_stride, (int)L.n, L.a, L.blocks > 1 ? reinterpret_cast<int*>(ws + L.hist) : nullptr,
-               reinterpret_cast<int*>(ws + L.perm), reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles,
-               backward ? reinterpret_cast<Tile*>(ws + L.chunks) : nullptr, L.nchunks,
-               backward ? reinterpret_cast<int2*>(ws + L.merge) : nullptr, L.chunk};
-    const int K = L.a + 1;
-    int bits = 0;
-    while ((1 << bits) < K) ++bits;
-    const size_t hist = kPlanThreads / 64 * 2 * (size_t)K;
-    if (L.blocks > 1) SKM_TRY_LAUNCH(k_plan_count, L.blocks, kPlanThreads, hist, s, p, bits);
-    return launch(k_plan_place, L.blocks, kPlanThreads, 8 * (size_t)(K + 1) + 64 + hist, s, p, bits);
+    const PlanArgs p{ids, ids_stride, (int)L.n, L.a, reinterpret_cast<int*>(ws + L.perm), reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles,
+                     backward ? reinterpret_cast<Tile*>(ws + L.chunks) : nullptr, L.nchunks,
+                     backward ? reinterpret_cast<int2*>(ws + L.merge) : nullptr, L.chunk};
+    return launch(k_plan, L.a + 1, kPlanThreads, 0, s, p);
 }
 
 template <typename T, int RT>
@@ -953,8 +936,8 @@ hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
     float* part = reinterpret_cast<float*>(a.ws + L.part);
     return with_type(a.type, [&](auto tag) {
         using T = decltype(tag);
-        const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.down_splits, part};
-        const ExpandArgs<T> ex{rows, part, L.down_splits, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
+        const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.down_splits, part, L.rp};
+        const ExpandArgs<T> ex{rows, part, L.down_splits, L.rp, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
                                (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, a.o, a.r, a.low, nullptr, nullptr, nullptr, nullptr, 0};
         if (a.a > 0) {
             const hipError_t e = L.direct ? launch_shrink<T, 1>(sh, L.ntiles, s) : launch_shrink<T, kTile / 16>(sh, L.ntiles, s);
@@ -981,8 +964,8 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
     return with_type(a.type, [&](auto tag) {
         using T = decltype(tag);
         if (a.n > 0) {
-            const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.up_splits, part};
-            const ExpandArgs<T> ex{rows, part, L.up_splits, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
+            const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.up_splits, part, L.rp};
+            const ExpandArgs<T> ex{rows, part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
                                    (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t, L.ld_t};
             if (a.a > 0) {
                 const hipError_t e = launch_shrink<T, kTile / 16>(sh, L.ntiles, s);
@@ -1015,7 +998,7 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
                 SKM_TRY_LAUNCH((k_outer<T, 2>), dim3(L.nchunks, cols, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
         }
         const long most = (long)a.r * (a.d > a.o ? a.d : a.o);
-        return launch(k_outer_merge<T>, dim3((unsigned)((most + 1023) / 1024), a.a, 2), 256, 0, s, ou);
+        return launch(k_outer_merge<T>, dim3((unsigned)(most + 255 < 1024 * 256 ? (most + 255) / 256 : 1024), 2), 256, 0, s, ou);
     });
 }
 
