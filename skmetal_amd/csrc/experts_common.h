@@ -2,6 +2,7 @@
 #pragma once
 
 #include <tuple>
+#include <type_traits>
 #include <utility>
 
 #include "experts.h"
@@ -17,6 +18,9 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
 // Rounded to nearest, ties to even: the one rounding of a result to its type.
 template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
+
+// exp(x) by the hardware's base-2 exponential.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 
 // Launches `kernel` and returns that launch's own status (an error that other code left
 // on the thread is not taken for it).

@@ -8,194 +8,588 @@
 //   loss = E / (k N^2) sum_j c_j S_j
 // A score of -inf or NaN is excluded: probability 0, never taken.  A row that is masked
 // or has no score left takes no expert (-1, weight 0) and counts nowhere.
+//
+// One pass over the scores each way.  A row lies on L lanes, NC times eight columns a
+// lane (column = (c L + lane) 8 + e), so a wave takes 64 / L rows at once and a row's sums
+// and its choice need log2(L) exchanges.
 #include "experts_common.h"
 
 namespace skm {
 namespace {
 
-// One wave per row, each lane the columns lane, lane + 64, ...; k passes over the row for
-// the next largest (value, lowest index).
+constexpr int kThreads = 256;
+constexpr int kMaxBlocks = 1024;  // partial sums that k_route_total adds
+constexpr int kOneBlock = 16;     // groups of 64 / L rows up to which one block takes all and no second launch is needed
+
+// A score as a whole number whose order is that of (score, lowest index first): the key of
+// a taken score, 0 of an excluded one.  16-bit scores and the index share 32 bits.
+template <typename T> struct Order;
+template <> struct Order<bf16> {
+    using Key = unsigned;
+    static constexpr unsigned kInf = 0x7f80;
+    static __device__ __forceinline__ float value(Key k) { const unsigned o = k >> 16; return __uint_as_float((o & 0x8000 ? o & 0x7fff : o ^ 0xffff) << 16); }
+};
+template <> struct Order<f16> {
+    using Key = unsigned;
+    static constexpr unsigned kInf = 0x7c00;
+    static __device__ __forceinline__ float value(Key k)
+    {
+        const unsigned o = k >> 16;
+        return (float)__builtin_bit_cast(f16, (unsigned short)(o & 0x8000 ? o & 0x7fff : o ^ 0xffff));
+    }
+};
+template <> struct Order<float> {
+    using Key = unsigned long long;
+    static __device__ __forceinline__ float value(Key k)
+    {
+        const unsigned o = (unsigned)(k >> 32);
+        return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+    }
+};
+
+// Eight scores of a row: their values (-inf where excluded) and keys from column j on.
 template <typename T>
-__global__ __launch_bounds__(256) void k_route(RouteArgs a, int nb, float* psum, int* pcnt, int* prow)
+__device__ __forceinline__ void decode8(const T* raw, int j, float* x, typename Order<T>::Key* key)
 {
-    extern __shared__ char lds[];
-    float* bs = reinterpret_cast<float*>(lds);       // [E] sums of this block's rows, wave by wave
-    int* bc = reinterpret_cast<int*>(bs + a.E);      // [E]
-    __shared__ int brow;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int j = threadIdx.x; j < a.E; j += 256) { bs[j] = 0.f; bc[j] = 0; }
-    if (threadIdx.x == 0) brow = 0;
-    __syncthreads();
-    constexpr int V = kRouteMaxE / 64;
-    float acc[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.f;
-    int mine = 0;
-    for (long i = (long)blockIdx.x * 4 + wave; i < a.n; i += (long)nb * 4) {
-        const T* z = static_cast<const T*>(a.z) + i * a.ld;
-        const bool on = a.mask == nullptr || a.mask[i * a.mask_stride] != 0;
-        float x[V];
-        float m = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = v * 64 + lane;
-            x[v] = on && j < a.E ? to_f(z[j]) : -INFINITY;
-            if (x[v] != x[v]) x[v] = -INFINITY;
-            m = fmaxf(m, x[v]);
-        }
-        for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-        const bool live = m > -INFINITY;
-        float s = 0.f;
-        float p[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) { p[v] = live && x[v] > -INFINITY ? __expf(x[v] - m) : 0.f; s += p[v]; }
-        for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
-        const float inv = live ? 1.f / s : 0.f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { p[v] *= inv; acc[v] += p[v]; }
-        mine += live;
-        float total = 0.f, wt = 0.f;
-        int et = -1;
-        for (int t = 0; t < a.k; ++t) {
-            float best = -INFINITY, pb = 0.f;
-            int at = 0x7fffffff;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (x[v] > best) { best = x[v]; at = v * 64 + lane; pb = p[v]; }
-            for (int off = 1; off < 64; off <<= 1) {
-                const float ob = __shfl_xor(best, off, 64), op = __shfl_xor(pb, off, 64);
-                const int oa = __shfl_xor(at, off, 64);
-                if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; pb = op; }
-            }
-            if (!(best > -INFINITY)) break;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v * 64 + lane == at) x[v] = -INFINITY;
-            total += pb;
-            if (lane == t) { wt = pb; et = at; }
-        }
-        if (lane < a.k) {
-            a.w[i * a.k + lane] = a.normalize && et >= 0 ? wt / total : wt;
-            a.ex[i * a.k + lane] = et;
-            if (et >= 0) atomicAdd(&bc[et], 1);
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(T) == 2) {
+            unsigned u = __builtin_bit_cast(unsigned short, raw[e]);
+            const bool out = (u & 0x7fff) > Order<T>::kInf || u == (Order<T>::kInf | 0x8000);
+            if (u == 0x8000) u = 0;  // -0 and 0 are equal scores
+            key[e] = out ? 0u : ((u & 0x8000 ? u ^ 0xffff : u | 0x8000) << 16) | (0xffffu - (j + e));
+            x[e] = out ? -INFINITY : to_f(raw[e]);
+        } else {
+            const bool out = !(raw[e] > -INFINITY);
+            const unsigned u = __float_as_uint(raw[e] + 0.f);  // -0 becomes 0
+            key[e] = out ? 0ull : ((unsigned long long)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32) | (0xffffffffu - (unsigned)(j + e));
+            x[e] = out ? -INFINITY : raw[e];
         }
     }
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
+}
+
+template <typename K> __device__ __forceinline__ int index_of(K k);
+template <> __device__ __forceinline__ int index_of(unsigned k) { return 0xffff - (k & 0xffff); }
+template <> __device__ __forceinline__ int index_of(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
+
+template <typename K>
+__device__ __forceinline__ void order(K& hi, K& lo)  // the larger to hi
+{
+    const K a = hi > lo ? hi : lo, b = hi > lo ? lo : hi;
+    hi = a;
+    lo = b;
+}
+
+// a[0 .. N) falls and then rises (or the other way round): in falling order.
+template <int N, typename K>
+__device__ __forceinline__ void merge_bitonic(K* a)
+{
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v * 64 + lane < a.E) bs[v * 64 + lane] += acc[v];
-            if (lane == 0) brow += mine;
+    for (int half = N / 2; half >= 1; half /= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((i & half) == 0) order(a[i], a[i + half]);
+}
+
+// a[0 .. N) in falling order.
+template <int N, typename K>
+__device__ __forceinline__ void sort_falling(K* a)
+{
+#pragma unroll
+    for (int size = 2; size <= N; size *= 2)
+#pragma unroll
+        for (int half = size / 2; half >= 1; half /= 2)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if ((i & half) == 0) {
+                    if ((i & size) == 0) order(a[i], a[i + half]); else order(a[i + half], a[i]);
+                }
+}
+
+// top, in falling order, takes in b, in falling order: of the two lists' N largest, one is
+// in each pair of top's i-th and b's i-th from the end.
+template <int N, typename K>
+__device__ __forceinline__ void merge_top(K* top, const K* b)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) top[i] = top[i] > b[N - 1 - i] ? top[i] : b[N - 1 - i];
+    merge_bitonic<N>(top);
+}
+
+// The value of the lane `off` away (xor).
+template <typename V>
+__device__ __forceinline__ V across(V v, int off) { return __shfl_xor(v, off, 64); }
+
+// Sum over a row's lanes, on all of them.
+template <int L>
+__device__ __forceinline__ float row_sum(float v)
+{
+#pragma unroll
+    for (int off = 1; off < L; off <<= 1) v += across(v, off);
+    return v;
+}
+
+// The eight scores at p, those past `left` as NaN (excluded).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, T* raw)
+{
+    if (left >= 8) {
+        __builtin_memcpy(raw, p, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = e < left ? p[e] : (T)__builtin_nanf("");
+    }
+}
+
+template <typename T, int L, int NC>
+__device__ __forceinline__ void load_row(const void* z, long ld, const uint8_t* mask, long mask_stride, long n, int E, long row, T (*raw)[8], bool& on)
+{
+    const int j = (threadIdx.x & (L - 1)) * 8;
+    on = row < n;
+    const long r = on ? row : n - 1;
+    const T* p = static_cast<const T*>(z) + r * ld;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+        if (c * L * 8 < E) load8(p + c * L * 8 + j, E - c * L * 8 - j, raw[c]);
+    if (mask != nullptr) on = on && mask[r * mask_stride] != 0;
+}
+
+// The blocks' sums and counts (or the only block's) become the results.
+__device__ __forceinline__ float balance_loss(double dot, int E, int k, int rows) { return rows > 0 ? (float)(dot * E / ((double)k * rows * rows)) : 0.f; }
+
+template <typename T, int L, int NC, int KP>
+__global__ __launch_bounds__(kThreads) void k_route(RouteArgs a, int nb, float* psum, int* pcnt, int* prow, unsigned* ticket)
+{
+    using O = Order<T>;
+    using Key = typename O::Key;
+    constexpr int RW = 64 / L, W = kThreads / 64, SPAN = L * 8 * NC;
+    __shared__ float sums[W][SPAN];
+    __shared__ int counts[SPAN];
+    __shared__ int rows[W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & (L - 1);
+    for (int i = threadIdx.x; i < SPAN; i += kThreads) counts[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && ticket != nullptr) *ticket = 0;
+    __syncthreads();
+    float acc[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[c][e] = 0.f;
+    int mine = 0;
+    const long groups = (a.n + RW - 1) / RW;
+    T next[NC][8];
+    bool next_on = false;
+    long grp = (long)blockIdx.x * W + wave;
+    if (grp < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, grp * RW + lane / L, next, next_on);
+    for (; grp < groups; grp += (long)nb * W) {
+        const long row = grp * RW + lane / L;
+        T raw[NC][8];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) raw[c][e] = next[c][e];
+        const bool on = next_on;
+        const long after = grp + (long)nb * W;
+        if (after < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, after * RW + lane / L, next, next_on);
+
+        float x[NC][8];
+        Key top[KP];
+#pragma unroll
+        for (int t = 0; t < KP; ++t) top[t] = 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (c * L * 8 >= a.E) break;
+            Key key[8];
+            decode8<T>(raw[c], (c * L + j) * 8, x[c], key);
+            if constexpr (KP >= 8) {
+                // the eight in falling order, and as many zeros
+                Key some[KP];
+#pragma unroll
+                for (int t = 0; t < KP; ++t) some[t] = t < 8 ? key[t] : 0;
+                sort_falling<8>(some);
+                if (c == 0)
+#pragma unroll
+                    for (int t = 0; t < KP; ++t) top[t] = some[t];
+                else
+                    merge_top<KP>(top, some);
+            } else {
+                // KP at a time; for one or two this is a plain insertion
+#pragma unroll
+                for (int b = 0; b < 8; b += KP) {
+                    sort_falling<KP>(key + b);
+                    if (c == 0 && b == 0)
+#pragma unroll
+                        for (int t = 0; t < KP; ++t) top[t] = key[t];
+                    else
+                        merge_top<KP>(top, key + b);
+                }
+            }
+        }
+#pragma unroll
+        for (int off = 1; off < L; off <<= 1) {
+            Key other[KP];
+#pragma unroll
+            for (int t = 0; t < KP; ++t) other[t] = across(top[t], off);
+            merge_top<KP>(top, other);
+        }
+        const bool live = on && top[0] != 0;
+        const float m = O::value(top[0]);
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (c * L * 8 >= a.E) break;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[c][e] = live ? exp_of(x[c][e] - m) : 0.f;
+                s += x[c][e];
+            }
+        }
+        s = row_sum<L>(s);
+        const float inv = live ? 1.f / s : 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (c * L * 8 >= a.E) break;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[c][e] += x[c][e] * inv;
+        }
+        mine += live && j == 0;
+
+        // slots j, j + L, ... of the row on this lane
+        constexpr int SL = (KP + L - 1) / L;
+        float w[SL];
+        int ex[SL];
+        float total = 0.f;
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            Key key = 0;
+#pragma unroll
+            for (int t = 0; t < KP; ++t)
+                if (t % L == j && t / L == i) key = top[t];
+            const bool taken = live && key != 0 && i * L + j < a.k;
+            w[i] = taken ? exp_of(O::value(key) - m) : 0.f;
+            ex[i] = taken ? index_of(key) : -1;
+            total += w[i];
+        }
+        const float scale = a.normalize ? (live ? 1.f / row_sum<L>(total) : 0.f) : inv;
+        if (row < a.n)
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                const int t = i * L + j;
+                if (t >= a.k) continue;
+                a.w[row * a.k + t] = w[i] * scale;
+                a.ex[row * a.k + t] = ex[i];
+                if (ex[i] >= 0) atomicAdd(&counts[ex[i]], 1);
+            }
+    }
+    // the wave's rows' sums, then the waves', in order
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if (c * L * 8 >= a.E) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+#pragma unroll
+            for (int off = L; off < 64; off <<= 1) acc[c][e] += across(acc[c][e], off);
+            if (lane < L) sums[wave][(c * L + j) * 8 + e] = acc[c][e];
+        }
+    }
+    for (int off = 1; off < 64; off <<= 1) mine += across(mine, off);
+    if (lane == 0) rows[wave] = mine;
+    __syncthreads();
+    if (nb > 1) {
+        for (int i = threadIdx.x; i < a.E; i += kThreads) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s += sums[w][i];
+            psum[(long)blockIdx.x * a.E + i] = s;
+            pcnt[(long)blockIdx.x * a.E + i] = counts[i];
+        }
+        if (threadIdx.x == 0) prow[blockIdx.x] = rows[0] + rows[1] + rows[2] + rows[3];
+        return;
+    }
+    double dot = 0.0;
+    for (int i = threadIdx.x; i < a.E; i += kThreads) {
+        double s = 0.0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += sums[w][i];
+        a.sums[i] = (float)s;
+        a.counts[i] = counts[i];
+        dot += s * counts[i];
+    }
+    __shared__ double dots[W];
+    for (int off = 1; off < 64; off <<= 1) dot += across(dot, off);
+    if (lane == 0) dots[wave] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int all = rows[0] + rows[1] + rows[2] + rows[3];
+        a.rows[0] = all;
+        a.loss[0] = balance_loss(dots[0] + dots[1] + dots[2] + dots[3], a.E, a.k, all);
+    }
+}
+
+// The blocks' sums and counts added, 16 columns a block, always in the same order; the last
+// block to finish adds up the loss.
+constexpr int kTotalThreads = 1024;
+__global__ __launch_bounds__(kTotalThreads) void k_route_total(RouteArgs a, int nb, const float* psum, const int* pcnt, const int* prow, double* dots,
+                                                               unsigned* ticket)
+{
+    __shared__ double s16[64][17];
+    __shared__ int c16[64][17];
+    __shared__ double dot16[16];
+    __shared__ bool last;
+    const int col = threadIdx.x & 15, part = threadIdx.x >> 4, j = blockIdx.x * 16 + col;
+    double s = 0.0;
+    int c = 0;
+    if (j < a.E) {
+#pragma unroll 4
+        for (int b = part; b < nb; b += 64) {
+            s += psum[(long)b * a.E + j];
+            c += pcnt[(long)b * a.E + j];
+        }
+    }
+    s16[part][col] = s;
+    c16[part][col] = c;
+    __syncthreads();
+    for (int half = 32; half >= 1; half /= 2) {
+        if (part < half) {
+            s16[part][col] += s16[part + half][col];
+            c16[part][col] += c16[part + half][col];
         }
         __syncthreads();
     }
-    for (int j = threadIdx.x; j < a.E; j += 256) {
-        psum[(long)blockIdx.x * a.E + j] = bs[j];
-        pcnt[(long)blockIdx.x * a.E + j] = bc[j];
+    if (threadIdx.x < 16) {
+        dot16[col] = 0.0;
+        if (j < a.E) {
+            a.sums[j] = (float)s16[0][col];
+            a.counts[j] = c16[0][col];
+            dot16[col] = s16[0][col] * c16[0][col];
+        }
     }
-    if (threadIdx.x == 0) prow[blockIdx.x] = brow;
-}
-
-// The blocks' sums and counts added in block order, and the loss.
-__global__ __launch_bounds__(256) void k_route_total(RouteArgs a, int nb, const float* psum, const int* pcnt, const int* prow)
-{
-    __shared__ double part[256];
-    double dot = 0.0;
-    for (int j = threadIdx.x; j < a.E; j += 256) {
-        double s = 0.0;
-        int c = 0;
-        for (int b = 0; b < nb; ++b) { s += psum[(long)b * a.E + j]; c += pcnt[(long)b * a.E + j]; }
-        a.sums[j] = (float)s;
-        a.counts[j] = c;
-        dot += s * c;
-    }
-    part[threadIdx.x] = dot;
     __syncthreads();
     if (threadIdx.x == 0) {
-        int rows = 0;
-        for (int b = 0; b < nb; ++b) rows += prow[b];
-        double t = 0.0;
-        for (int i = 0; i < 256; ++i) t += part[i];
-        a.rows[0] = rows;
-        a.loss[0] = rows > 0 ? (float)(t * a.E / ((double)a.k * rows * rows)) : 0.f;
+        double d = 0.0;
+        for (int i = 0; i < 16; ++i) d += dot16[i];
+        __hip_atomic_store(dots + blockIdx.x, d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __threadfence();
+        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    int rows = 0;
+    for (int b = threadIdx.x; b < nb; b += kTotalThreads) rows += prow[b];
+    for (int off = 1; off < 64; off <<= 1) rows += across(rows, off);
+    if ((threadIdx.x & 63) == 0) c16[threadIdx.x >> 6][0] = rows;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int all = 0;
+        for (int w = 0; w < kTotalThreads / 64; ++w) all += c16[w][0];
+        double d = 0.0;
+        for (unsigned b = 0; b < gridDim.x; ++b) d += __hip_atomic_load(dots + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        a.rows[0] = all;
+        a.loss[0] = balance_loss(d, a.E, a.k, all);
     }
 }
 
-// dz_ij = p_ij (G_j - sum_j p_ij G_j) + the chosen ones' gate part.
-template <typename T>
-__global__ __launch_bounds__(256) void k_route_back(RouteBackArgs a, int nb)
+// dz_ij = p_ij (G_j - sum_j p_ij G_j) + the chosen ones' gate part, with G_j = dloss E c_j / (k N^2).
+// The gate part of a chosen score is w (dw - sum w dw) for normalized weights; otherwise w dw,
+// and sum w dw joins the sum over the row.  It reaches its column through LDS.
+template <typename T, int L, int NC>
+__global__ __launch_bounds__(kThreads) void k_route_back(RouteBackArgs a, int nb)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int V = kRouteMaxE / 64;
+    constexpr int RW = 64 / L, W = kThreads / 64, SPAN = L * 8 * NC;
+    constexpr int kSlots = (kRouteMaxK + L - 1) / L;
+    __shared__ __align__(16) float gate[W][RW][SPAN + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & (L - 1);
+    float* mine = &gate[wave][lane / L][0];
+    for (int i = lane; i < RW * (SPAN + 4); i += 64) (&gate[wave][0][0])[i] = 0.f;
     const int N = a.rows[0];
     const float each = a.dloss != nullptr && N > 0 ? (float)((double)a.dloss[0] * a.E / ((double)a.k * N * N)) : 0.f;
-    for (long i = (long)blockIdx.x * 4 + wave; i < a.n; i += (long)nb * 4) {
-        const T* z = static_cast<const T*>(a.z) + i * a.ld;
-        T* dz = static_cast<T*>(a.dz) + i * a.ld_dz;
-        const bool on = a.mask == nullptr || a.mask[i * a.mask_stride] != 0;
-        float x[V], m = -INFINITY;
+    float G[NC][8];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = v * 64 + lane;
-            x[v] = on && j < a.E ? to_f(z[j]) : -INFINITY;
-            if (x[v] != x[v]) x[v] = -INFINITY;
-            m = fmaxf(m, x[v]);
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int col = (c * L + j) * 8 + e;
+            G[c][e] = a.dloss != nullptr && col < a.E ? each * a.counts[col] : 0.f;
         }
-        for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-        const bool live = m > -INFINITY;
+    const long groups = (a.n + RW - 1) / RW;
+    T next[NC][8];
+    bool next_on = false;
+    long grp = (long)blockIdx.x * W + wave;
+    if (grp < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, grp * RW + lane / L, next, next_on);
+    for (; grp < groups; grp += (long)nb * W) {
+        const long row = grp * RW + lane / L;
+        // the row's slots
+        float w[kSlots], dw[kSlots];
+        int ex[kSlots];
+        if (a.dw != nullptr)
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) {
+                const int t = i * L + j;
+                const bool there = row < a.n && t < a.k;
+                ex[i] = there ? a.ex[row * a.k + t] : -1;
+                w[i] = there ? a.w[row * a.k + t] : 0.f;
+                dw[i] = there ? a.dw[row * a.k + t] : 0.f;
+            }
+        float x[NC][8];
+        float m = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (c * L * 8 >= a.E) break;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = to_f(next[c][e]);
+                x[c][e] = v > -INFINITY ? v : -INFINITY;  // NaN too
+                m = fmaxf(m, x[c][e]);
+            }
+        }
+        const bool on = next_on;
+        const long after = grp + (long)nb * W;
+        if (after < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, after * RW + lane / L, next, next_on);
+#pragma unroll
+        for (int off = 1; off < L; off <<= 1) m = fmaxf(m, across(m, off));
+        const bool live = on && m > -INFINITY;
         float s = 0.f, g = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = v * 64 + lane;
-            x[v] = live && x[v] > -INFINITY ? __expf(x[v] - m) : 0.f;
-            s += x[v];
-            g += x[v] * (j < a.E ? each * a.counts[j] : 0.f);
-        }
-        for (int off = 1; off < 64; off <<= 1) { s += __shfl_xor(s, off, 64); g += __shfl_xor(g, off, 64); }
-        const float inv = live ? 1.f / s : 0.f;
-        g *= inv;
-        float wd = 0.f;
-        if (a.dw != nullptr)
-            for (int t = 0; t < a.k; ++t)
-                if (a.ex[i * a.k + t] >= 0) wd += a.w[i * a.k + t] * a.dw[i * a.k + t];
-        if (!a.normalize) g += wd;
+        for (int c = 0; c < NC; ++c) {
+            if (c * L * 8 >= a.E) break;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = v * 64 + lane;
-            if (j >= a.E) continue;
-            float r = x[v] * inv * (each * a.counts[j] - g);
-            if (a.dw != nullptr)
-                for (int t = 0; t < a.k; ++t)
-                    if (a.ex[i * a.k + t] == j) r += a.w[i * a.k + t] * (a.dw[i * a.k + t] - (a.normalize ? wd : 0.f));
-            dz[j] = from_f<T>(r);
+            for (int e = 0; e < 8; ++e) {
+                x[c][e] = live ? exp_of(x[c][e] - m) : 0.f;
+                s += x[c][e];
+                g += x[c][e] * G[c][e];
+            }
+        }
+        s = row_sum<L>(s);
+        const float inv = live ? 1.f / s : 0.f;
+        g = row_sum<L>(g) * inv;
+        if (a.dw != nullptr) {
+            float wd = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) wd += live && ex[i] >= 0 ? w[i] * dw[i] : 0.f;
+            wd = row_sum<L>(wd);
+            if (!a.normalize) g += wd;
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i)
+                if (live && ex[i] >= 0 && ex[i] < a.E) mine[ex[i]] = w[i] * (a.normalize ? dw[i] - wd : dw[i]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        T* dz = static_cast<T*>(a.dz) + row * a.ld_dz;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (c * L * 8 >= a.E) break;
+            const int col = (c * L + j) * 8;
+            float gt[8] = {};
+            if (a.dw != nullptr) __builtin_memcpy(gt, __builtin_assume_aligned(mine + col, 16), 32);
+            T out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = from_f<T>(x[c][e] * inv * (G[c][e] - g) + gt[e]);
+            if (row < a.n) {
+                if (col + 8 <= a.E)
+                    __builtin_memcpy(dz + col, out, 8 * sizeof(T));
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e < a.E) dz[col + e] = out[e];
+            }
+        }
+        if (a.dw != nullptr) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i)
+                if (live && ex[i] >= 0 && ex[i] < a.E) mine[ex[i]] = 0.f;
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
 
-int route_blocks(long n) { return (int)(n < 4 * 512 ? (n + 3) / 4 > 0 ? (n + 3) / 4 : 1 : 512); }
+// Lanes a row takes: one up to 32 experts (no exchanges at all), eight up to 256, a wave
+// beyond.
+int row_lanes(int E) { return E <= 32 ? 1 : E <= 256 ? 8 : 64; }
+
+int route_blocks(long n, int E)
+{
+    const long rw = 64 / row_lanes(E), groups = (n + rw - 1) / rw;
+    if (groups <= kOneBlock) return 1;
+    const long b = (groups + kThreads / 64 - 1) / (kThreads / 64);
+    return (int)(b < kMaxBlocks ? b : kMaxBlocks);
+}
+
+struct RouteSpace {
+    size_t dots, ticket, sum, cnt, row, bytes;
+};
+RouteSpace route_space(long n, int E)
+{
+    const size_t nb = (size_t)route_blocks(n, E);
+    RouteSpace s{};
+    s.dots = 0;
+    s.ticket = s.dots + 8 * (size_t)(kRouteMaxE / 16);
+    s.sum = s.ticket + 16;
+    s.cnt = s.sum + nb * E * 4;
+    s.row = s.cnt + nb * E * 4;
+    s.bytes = s.row + nb * 4;
+    return s;
+}
+
+// f(lanes a row, times eight columns a lane)
+template <typename F>
+hipError_t with_shape(int E, F&& f)
+{
+    using std::integral_constant;
+    switch (row_lanes(E)) {
+    case 1: return f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    case 8:
+        if (E <= 64) return f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+        return f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    default:
+        if (E <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+        return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    }
+}
+
+template <typename F>
+hipError_t with_slots(int k, F&& f)
+{
+    using std::integral_constant;
+    if (k <= 1) return f(integral_constant<int, 1>{});
+    if (k <= 2) return f(integral_constant<int, 2>{});
+    if (k <= 4) return f(integral_constant<int, 4>{});
+    if (k <= 8) return f(integral_constant<int, 8>{});
+    return f(integral_constant<int, 16>{});
+}
 
 }  // namespace
 
-size_t route_workspace(long n, int E) { return (size_t)route_blocks(n) * (8 * (size_t)E + 4); }
+size_t route_workspace(long n, int E) { return route_space(n, E).bytes; }
 
 hipError_t launch_route(const RouteArgs& a, hipStream_t s)
 {
-    const int nb = route_blocks(a.n);
-    float* psum = reinterpret_cast<float*>(a.ws);
-    int* pcnt = reinterpret_cast<int*>(psum + (size_t)nb * a.E);
-    int* prow = pcnt + (size_t)nb * a.E;
-    return with_type(a.type, [&](auto t) {
-        SKM_TRY_LAUNCH(k_route<decltype(t)>, nb, 256, 8 * (size_t)a.E, s, a, nb, psum, pcnt, prow);
-        return launch(k_route_total, 1, 256, 0, s, a, nb, psum, pcnt, prow);
+    const int nb = route_blocks(a.n, a.E);
+    const RouteSpace at = route_space(a.n, a.E);
+    double* dots = reinterpret_cast<double*>(a.ws + at.dots);
+    unsigned* ticket = reinterpret_cast<unsigned*>(a.ws + at.ticket);
+    float* psum = reinterpret_cast<float*>(a.ws + at.sum);
+    int* pcnt = reinterpret_cast<int*>(a.ws + at.cnt);
+    int* prow = reinterpret_cast<int*>(a.ws + at.row);
+    const hipError_t e = with_type(a.type, [&](auto t) {
+        return with_shape(a.E, [&](auto lanes, auto times) {
+            return with_slots(a.k, [&](auto slots) {
+                return launch(k_route<decltype(t), lanes.value, times.value, slots.value>, nb, kThreads, 0, s, a, nb, psum, pcnt, prow, ticket);
+            });
+        });
     });
+    if (e != hipSuccess || nb == 1) return e;
+    return launch(k_route_total, (a.E + 15) / 16, kTotalThreads, 0, s, a, nb, psum, pcnt, prow, dots, ticket);
 }
 
 hipError_t launch_route_back(const RouteBackArgs& a, hipStream_t s)
 {
     if (a.n == 0) return hipSuccess;
-    const int nb = (int)((a.n + 3) / 4 < 4096 ? (a.n + 3) / 4 : 4096);
+    const long rw = 64 / row_lanes(a.E), b = ((a.n + rw - 1) / rw + kThreads / 64 - 1) / (kThreads / 64);
+    const int nb = (int)(b < 2 * kMaxBlocks ? b : 2 * kMaxBlocks);
     return with_type(a.type, [&](auto t) {
-        return launch(k_route_back<decltype(t)>, nb, 256, 0, s, a, nb);
+        return with_shape(a.E, [&](auto lanes, auto times) { return launch(k_route_back<decltype(t), lanes.value, times.value>, nb, kThreads, 0, s, a, nb); });
     });
 }
 
