@@ -18,8 +18,9 @@ namespace skm {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kOneThreads = 1024;
 constexpr int kMaxBlocks = 1024;  // partial sums that k_route_total adds
-constexpr int kOneBlock = 16;     // groups of 64 / L rows up to which one block takes all and no second launch is needed
+constexpr int kOneBlock = kOneThreads / 64;  // groups of 64 / L rows that one block takes at once: no second launch then
 
 // A score as a whole number whose order is that of (score, lowest index first): the key of
 // a taken score, 0 of an excluded one.  16-bit scores and the index share 32 bits.
@@ -116,9 +117,27 @@ __device__ __forceinline__ void merge_top(K* top, const K* b)
     merge_bitonic<N>(top);
 }
 
-// The value of the lane `off` away (xor).
-template <typename V>
-__device__ __forceinline__ V across(V v, int off) { return __shfl_xor(v, off, 64); }
+// The value of the lane `off` away (xor), within a butterfly that takes off = 1, 2, 4, ... or starts
+// at 8: at 4 the four lanes of a quad hold one value, so the lane opposite within eight
+// (7 - lane) serves as well.
+__device__ __forceinline__ unsigned across_bits(unsigned v, int off)
+{
+    switch (off) {
+    case 1: return __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);    // quad_perm [1, 0, 3, 2]
+    case 2: return __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);    // quad_perm [2, 3, 0, 1]
+    case 4: return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);   // row_half_mirror
+    case 8: return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);   // row_ror:8
+    case 16: return __builtin_amdgcn_ds_swizzle(v, 0x401f);                    // xor 16
+    default: return __shfl_xor(v, off, 64);
+    }
+}
+__device__ __forceinline__ unsigned across(unsigned v, int off) { return across_bits(v, off); }
+__device__ __forceinline__ int across(int v, int off) { return (int)across_bits((unsigned)v, off); }
+__device__ __forceinline__ float across(float v, int off) { return __uint_as_float(across_bits(__float_as_uint(v), off)); }
+__device__ __forceinline__ unsigned long long across(unsigned long long v, int off)
+{
+    return (unsigned long long)across_bits((unsigned)(v >> 32), off) << 32 | across_bits((unsigned)v, off);
+}
 
 // Sum over a row's lanes, on all of them.
 template <int L>
@@ -157,20 +176,21 @@ __device__ __forceinline__ void load_row(const void* z, long ld, const uint8_t* 
 // The blocks' sums and counts (or the only block's) become the results.
 __device__ __forceinline__ float balance_loss(double dot, int E, int k, int rows) { return rows > 0 ? (float)(dot * E / ((double)k * rows * rows)) : 0.f; }
 
-template <typename T, int L, int NC, int KP>
-__global__ __launch_bounds__(kThreads) void k_route(RouteArgs a, int nb, float* psum, int* pcnt, int* prow, unsigned* ticket)
+// ONE: a single block, a wave a group of rows.
+template <typename T, int L, int NC, int KP, bool ONE>
+__global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArgs a, int nb, float* psum, int* pcnt, int* prow, unsigned* ticket)
 {
     using O = Order<T>;
     using Key = typename O::Key;
-    constexpr int RW = 64 / L, W = kThreads / 64, SPAN = L * 8 * NC;
+    constexpr int NT = ONE ? kOneThreads : kThreads, RW = 64 / L, W = NT / 64, SPAN = L * 8 * NC;
     __shared__ float sums[W][SPAN];
     __shared__ int counts[SPAN];
     __shared__ int rows[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & (L - 1);
-    for (int i = threadIdx.x; i < SPAN; i += kThreads) counts[i] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0 && ticket != nullptr) *ticket = 0;
+    for (int i = threadIdx.x; i < SPAN; i += NT) counts[i] = 0;
+    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
     __syncthreads();
-    float acc[NC][8];
+    float acc[NC][8];  // a wave without rows adds zeros
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -181,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a, int nb, float* 
     bool next_on = false;
     long grp = (long)blockIdx.x * W + wave;
     if (grp < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, grp * RW + lane / L, next, next_on);
-    for (; grp < groups; grp += (long)nb * W) {
+    for (; grp < groups; grp += ONE ? groups : (long)nb * W) {
         const long row = grp * RW + lane / L;
         T raw[NC][8];
 #pragma unroll
@@ -190,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a, int nb, float* 
             for (int e = 0; e < 8; ++e) raw[c][e] = next[c][e];
         const bool on = next_on;
         const long after = grp + (long)nb * W;
-        if (after < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, after * RW + lane / L, next, next_on);
+        if (!ONE && after < groups) load_row<T, L, NC>(a.z, a.ld, a.mask, a.mask_stride, a.n, a.E, after * RW + lane / L, next, next_on);
 
         float x[NC][8];
         Key top[KP];
@@ -292,37 +312,42 @@ __global__ __launch_bounds__(kThreads) void k_route(RouteArgs a, int nb, float* 
             if (lane < L) sums[wave][(c * L + j) * 8 + e] = acc[c][e];
         }
     }
+#pragma unroll
     for (int off = 1; off < 64; off <<= 1) mine += across(mine, off);
     if (lane == 0) rows[wave] = mine;
     __syncthreads();
-    if (nb > 1) {
-        for (int i = threadIdx.x; i < a.E; i += kThreads) {
+    if (!ONE) {
+        for (int i = threadIdx.x; i < a.E; i += NT) {
             float s = 0.f;
 #pragma unroll
             for (int w = 0; w < W; ++w) s += sums[w][i];
             psum[(long)blockIdx.x * a.E + i] = s;
             pcnt[(long)blockIdx.x * a.E + i] = counts[i];
         }
-        if (threadIdx.x == 0) prow[blockIdx.x] = rows[0] + rows[1] + rows[2] + rows[3];
+        if (threadIdx.x == 0) prow[blockIdx.x] = rows[0] + rows[1] + rows[2] + rows[3];  // W = 4
         return;
     }
     double dot = 0.0;
-    for (int i = threadIdx.x; i < a.E; i += kThreads) {
+    for (int i = threadIdx.x; i < a.E; i += NT) {
         double s = 0.0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) s += sums[w][i];
+        for (int w = 0; w < W && w < groups; ++w) s += sums[w][i];
         a.sums[i] = (float)s;
         a.counts[i] = counts[i];
         dot += s * counts[i];
     }
     __shared__ double dots[W];
-    for (int off = 1; off < 64; off <<= 1) dot += across(dot, off);
+    for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off, 64);
     if (lane == 0) dots[wave] = dot;
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int all = rows[0] + rows[1] + rows[2] + rows[3];
+        int all = 0;
+        double d = 0.0;
+        for (int w = 0; w < W; ++w) {
+            all += rows[w];
+            d += dots[w];
+        }
         a.rows[0] = all;
-        a.loss[0] = balance_loss(dots[0] + dots[1] + dots[2] + dots[3], a.E, a.k, all);
+        a.loss[0] = balance_loss(d, a.E, a.k, all);
     }
 }
 
@@ -376,6 +401,7 @@ __global__ __launch_bounds__(kTotalThreads) void k_route_total(RouteArgs a, int 
     if (!last) return;
     int rows = 0;
     for (int b = threadIdx.x; b < nb; b += kTotalThreads) rows += prow[b];
+#pragma unroll
     for (int off = 1; off < 64; off <<= 1) rows += across(rows, off);
     if ((threadIdx.x & 63) == 0) c16[threadIdx.x >> 6][0] = rows;
     __syncthreads();
@@ -561,7 +587,7 @@ hipError_t with_slots(int k, F&& f)
 
 }  // namespace
 
-size_t route_workspace(long n, int E) { return route_space(n, E).bytes; }
+size_t route_workspace(long n, int E) { return route_blocks(n, E) == 1 ? 0 : route_space(n, E).bytes; }
 
 hipError_t launch_route(const RouteArgs& a, hipStream_t s)
 {
@@ -575,7 +601,9 @@ hipError_t launch_route(const RouteArgs& a, hipStream_t s)
     const hipError_t e = with_type(a.type, [&](auto t) {
         return with_shape(a.E, [&](auto lanes, auto times) {
             return with_slots(a.k, [&](auto slots) {
-                return launch(k_route<decltype(t), lanes.value, times.value, slots.value>, nb, kThreads, 0, s, a, nb, psum, pcnt, prow, ticket);
+                if (nb == 1)
+                    return launch(k_route<decltype(t), lanes.value, times.value, slots.value, true>, 1, kOneThreads, 0, s, a, nb, psum, pcnt, prow, ticket);
+                return launch(k_route<decltype(t), lanes.value, times.value, slots.value, false>, nb, kThreads, 0, s, a, nb, psum, pcnt, prow, ticket);
             });
         });
     });

@@ -67,15 +67,19 @@ def _fail(name):
     raise RuntimeError(f"{name} failed: {_bridge.last_error()}")
 
 
-def _rows(t, name, dtype, shape, device):
-    """`t` as a matrix of `shape` (None: any) whose rows' elements lie side by side;
-    returns its row stride."""
+def _refuse(t, name, dtype, shape, device):
+    """Says what is wrong with a tensor of another type, device or shape."""
     if t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _rows(t, name, dtype, shape, device):
+    """The row stride of the matrix `t`, whose rows' elements lie side by side."""
+    if t.dtype != dtype or t.shape != shape or t.device != device:
+        _refuse(t, name, dtype, shape, device)
     ld, one = t.stride()
     if one != 1 and shape[1] > 1:
         raise ValueError(f"{name}'s rows must have their elements side by side (stride(1) is {one})")
@@ -83,22 +87,14 @@ def _rows(t, name, dtype, shape, device):
 
 
 def _vector(t, name, dtype, n, device):
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
+    if t.dtype != dtype or t.shape != (n,) or t.device != device:
+        _refuse(t, name, dtype, (n,), device)
     return t.stride(0)
 
 
 def _dense(t, name, dtype, shape, device):
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype or t.shape != shape or t.device != device:
+        _refuse(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
@@ -141,8 +137,12 @@ def _adapt_workspace(code, n, d, o, r, a, backward):
     return _lib().skmetal_hip_adapt_workspace(code, n, d, o, r, a, backward)
 
 
+# the current stream's handle, without an object around it where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
 
 
 def _check_route(logits, top_k):
@@ -174,15 +174,15 @@ def route(logits, top_k, *, mask=None, normalize=False) -> Routing:
     lib = _lib()
     weights = torch.empty((n, k), dtype=torch.float32, device=device)
     experts = torch.empty((n, k), dtype=torch.int32, device=device)
-    whole = torch.empty(e + 1, dtype=torch.int32, device=device)
-    real = torch.empty(e + 1, dtype=torch.float32, device=device)
+    whole = torch.empty(2 * e + 2, dtype=torch.int32, device=device)
     size = _route_workspace(n, e)
     ws, ws_ptr = _workspace(size, device)
-    at, to = whole.data_ptr(), real.data_ptr()
+    at = whole.data_ptr()
     if lib.skmetal_hip_route(code, logits.data_ptr(), ld, mask_ptr, mask_stride, n, e, k, 1 if normalize else 0, weights.data_ptr(), experts.data_ptr(),
-                             at, to, at + 4 * e, to + 4 * e, ws_ptr, size, _stream(device)):
+                             at, at + 4 * e, at + 8 * e, at + 8 * e + 4, ws_ptr, size, _stream(device)):
         _fail("route")
-    return Routing(weights, experts, whole[:e], real[:e], whole[e:], real[e])
+    counts, sums, rows, loss = whole.split_with_sizes((e, e, 1, 1))
+    return Routing(weights, experts, counts, sums.view(torch.float32), rows, loss.view(torch.float32)[0])
 
 
 def route_backward(logits, routing: Routing, *, grad_weights=None, grad_loss=None, mask=None, normalize=False):
@@ -207,28 +207,24 @@ def route_backward(logits, routing: Routing, *, grad_weights=None, grad_loss=Non
     return grad
 
 
-def _adapters(t, name, dtype, width, device):
-    """The adapter and rank strides of `t` [a, r, width]."""
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.dim() != 3 or (width is not None and t.shape[2] != width):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected (adapters, rank, {'width' if width is None else width})")
+def _adapters(t, name, dtype, device):
+    """The sizes and the adapter and rank strides of `t` [a, r, width]."""
+    if t.dtype != dtype or t.device != device or t.dim() != 3:
+        _refuse(t, name, dtype, ("adapters", "rank", "width"), device)
     sa, ld, one = t.stride()
-    if one != 1 and t.shape[2] > 1:
+    a, r, width = t.shape
+    if one != 1 and width > 1:
         raise ValueError(f"{name}'s ranks must have their elements side by side (stride(2) is {one})")
-    return sa, ld
+    return a, r, width, sa, ld
 
 
 def _check_adapt(x, first, down, up, ids, gates, scales):
     code, device = _first(x, first)
-    n, d = x.shape
+    n = x.shape[0]
     dtype = x.dtype
-    down_sa, down_ld = _adapters(down, "down", dtype, None, device)
-    up_sa, up_ld = _adapters(up, "up", dtype, None, device)
-    a, r = down.shape[:2]
-    if up.shape[:2] != (a, r):
+    a, r, d, down_sa, down_ld = _adapters(down, "down", dtype, device)
+    a2, r2, o, up_sa, up_ld = _adapters(up, "up", dtype, device)
+    if a2 != a or r2 != r:
         raise ValueError(f"down has shape {tuple(down.shape)} and up {tuple(up.shape)}: their adapters and ranks must agree")
     if not 1 <= r <= MAX_RANK:
         raise ValueError(f"a rank of {r} is not in [1, {MAX_RANK}]")
@@ -236,7 +232,7 @@ def _check_adapt(x, first, down, up, ids, gates, scales):
     gate_ptr, gate_stride = (None, 0) if gates is None else (gates.data_ptr(), _vector(gates, "gates", torch.float32, n, device))
     scale_ptr = None if scales is None else _dense(scales, "scales", torch.float32, (a,), device)
     shared = (down.data_ptr(), down_sa, down_ld, up.data_ptr(), up_sa, up_ld, ids.data_ptr(), ids_stride, gate_ptr, gate_stride, scale_ptr)
-    return code, device, n, down.shape[2], up.shape[2], r, a, shared
+    return code, device, n, d, o, r, a, shared
 
 
 def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, return_low=False):
@@ -257,8 +253,9 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
     base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, o), device))
     lib = _lib()
     if out is None:
-        out = torch.empty((n, o), dtype=dtype, device=device)
-    out_ld = _rows(out, "out", dtype, (n, o), device)
+        out, out_ld = torch.empty((n, o), dtype=dtype, device=device), o
+    else:
+        out_ld = _rows(out, "out", dtype, (n, o), device)
     low = torch.empty((n, r), dtype=torch.float32, device=device) if return_low else None
     size = _adapt_workspace(code, n, d, o, r, a, 0)
     ws, ws_ptr = _workspace(size, device)
