@@ -19,34 +19,39 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kOneThreads = 1024;
-constexpr int kMaxBlocks = 1024;  // partial sums that k_route_total adds
+constexpr int kMaxBlocks = 768;  // three a CU at once: what the registers of the widest rows allow
 constexpr int kOneBlock = kOneThreads / 64;  // groups of 64 / L rows that one block takes at once: no second launch then
 
-// A score as a whole number whose order is that of (score, lowest index first): the key of
-// a taken score, 0 of an excluded one.  16-bit scores and the index share 32 bits.
-template <typename T> struct Order;
-template <> struct Order<bf16> {
+// A score as a whole number whose order is that of (score, lowest index first).  The value is
+// ordered as its fp32 bits; those of a 16-bit type leave the low 16 (bf16) or 13 bits (fp16) to
+// the index, and fp32 scores take 64.  -0 counts as 0; -inf and NaN, the excluded ones, lie
+// under every other score's key.
+template <typename T>
+struct Order {
     using Key = unsigned;
-    static constexpr unsigned kInf = 0x7f80;
-    static __device__ __forceinline__ float value(Key k) { const unsigned o = k >> 16; return __uint_as_float((o & 0x8000 ? o & 0x7fff : o ^ 0xffff) << 16); }
+    static constexpr unsigned kIndex = sizeof(T) == 2 && std::is_same_v<T, f16> ? 0x1fff : 0xffff;
+    static __device__ __forceinline__ Key of(unsigned ordered, int j) { return (ordered & ~kIndex) | (kIndex - j); }
+    static __device__ __forceinline__ unsigned ordered(Key k) { return k & ~kIndex; }
+    static __device__ __forceinline__ int index(Key k) { return kIndex - (k & kIndex); }
 };
-template <> struct Order<f16> {
-    using Key = unsigned;
-    static constexpr unsigned kInf = 0x7c00;
-    static __device__ __forceinline__ float value(Key k)
-    {
-        const unsigned o = k >> 16;
-        return (float)__builtin_bit_cast(f16, (unsigned short)(o & 0x8000 ? o & 0x7fff : o ^ 0xffff));
-    }
-};
-template <> struct Order<float> {
+template <>
+struct Order<float> {
     using Key = unsigned long long;
-    static __device__ __forceinline__ float value(Key k)
-    {
-        const unsigned o = (unsigned)(k >> 32);
-        return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
-    }
+    static __device__ __forceinline__ Key of(unsigned ordered, int j) { return (Key)ordered << 32 | (0xffffffffu - (unsigned)j); }
+    static __device__ __forceinline__ unsigned ordered(Key k) { return (unsigned)(k >> 32); }
+    static __device__ __forceinline__ int index(Key k) { return (int)(0xffffffffu - (unsigned)k); }
 };
+static_assert(kRouteMaxE <= 0x2000, "the index of an fp16 score has 13 bits");
+
+template <typename T>
+__device__ __forceinline__ bool takable(typename Order<T>::Key k) { return Order<T>::ordered(k) >= 0x00800000u; }
+
+template <typename T>
+__device__ __forceinline__ float value_of(typename Order<T>::Key k)
+{
+    const unsigned o = Order<T>::ordered(k), mask = std::is_same_v<T, float> ? 0xffffffffu : ~(std::is_same_v<T, f16> ? 0x1fffu : 0xffffu);
+    return __uint_as_float((o & 0x80000000u ? o ^ 0x80000000u : ~o) & mask);
+}
 
 // Eight scores of a row: their values (-inf where excluded) and keys from column j on.
 template <typename T>
@@ -54,24 +59,11 @@ __device__ __forceinline__ void decode8(const T* raw, int j, float* x, typename 
 {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        if constexpr (sizeof(T) == 2) {
-            unsigned u = __builtin_bit_cast(unsigned short, raw[e]);
-            const bool out = (u & 0x7fff) > Order<T>::kInf || u == (Order<T>::kInf | 0x8000);
-            if (u == 0x8000) u = 0;  // -0 and 0 are equal scores
-            key[e] = out ? 0u : ((u & 0x8000 ? u ^ 0xffff : u | 0x8000) << 16) | (0xffffu - (j + e));
-            x[e] = out ? -INFINITY : to_f(raw[e]);
-        } else {
-            const bool out = !(raw[e] > -INFINITY);
-            const unsigned u = __float_as_uint(raw[e] + 0.f);  // -0 becomes 0
-            key[e] = out ? 0ull : ((unsigned long long)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32) | (0xffffffffu - (unsigned)(j + e));
-            x[e] = out ? -INFINITY : raw[e];
-        }
+        x[e] = fmaxf(to_f(raw[e]) + 0.f, -INFINITY);  // -0 becomes 0, NaN -inf
+        const int u = __float_as_int(x[e]);
+        key[e] = Order<T>::of((unsigned)(u ^ ((u >> 31) | (int)0x80000000)), j + e);
     }
 }
-
-template <typename K> __device__ __forceinline__ int index_of(K k);
-template <> __device__ __forceinline__ int index_of(unsigned k) { return 0xffff - (k & 0xffff); }
-template <> __device__ __forceinline__ int index_of(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
 
 template <typename K>
 __device__ __forceinline__ void order(K& hi, K& lo)  // the larger to hi
@@ -148,28 +140,23 @@ __device__ __forceinline__ float row_sum(float v)
     return v;
 }
 
-// The eight scores at p, those past `left` as NaN (excluded).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, T* raw)
-{
-    if (left >= 8) {
-        __builtin_memcpy(raw, p, 8 * sizeof(T));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) raw[e] = e < left ? p[e] : (T)__builtin_nanf("");
-    }
-}
-
 template <typename T, int L, int NC>
 __device__ __forceinline__ void load_row(const void* z, long ld, const uint8_t* mask, long mask_stride, long n, int E, long row, T (*raw)[8], bool& on)
 {
     const int j = (threadIdx.x & (L - 1)) * 8;
     on = row < n;
     const long r = on ? row : n - 1;
-    const T* p = static_cast<const T*>(z) + r * ld;
+    const T* p = static_cast<const T*>(z) + r * ld + j;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-        if (c * L * 8 < E) load8(p + c * L * 8 + j, E - c * L * 8 - j, raw[c]);
+    for (int c = 0; c < NC; ++c) {
+        const int col = c * L * 8;
+        if (col + L * 8 <= E) {
+            __builtin_memcpy(raw[c], p + col, 8 * sizeof(T));
+        } else if (col < E) {  // the columns past the row as NaN (excluded)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) raw[c][e] = col + j + e < E ? p[col + e] : (T)__builtin_nanf("");
+        }
+    }
     if (mask != nullptr) on = on && mask[r * mask_stride] != 0;
 }
 
@@ -252,8 +239,8 @@ __global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArg
             for (int t = 0; t < KP; ++t) other[t] = across(top[t], off);
             merge_top<KP>(top, other);
         }
-        const bool live = on && top[0] != 0;
-        const float m = O::value(top[0]);
+        const bool live = on && takable<T>(top[0]);
+        const float m = value_of<T>(top[0]);
         float s = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -285,9 +272,9 @@ __global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArg
 #pragma unroll
             for (int t = 0; t < KP; ++t)
                 if (t % L == j && t / L == i) key = top[t];
-            const bool taken = live && key != 0 && i * L + j < a.k;
-            w[i] = taken ? exp_of(O::value(key) - m) : 0.f;
-            ex[i] = taken ? index_of(key) : -1;
+            const bool taken = live && takable<T>(key) && i * L + j < a.k;
+            w[i] = taken ? exp_of(value_of<T>(key) - m) : 0.f;
+            ex[i] = taken ? O::index(key) : -1;
             total += w[i];
         }
         const float scale = a.normalize ? (live ? 1.f / row_sum<L>(total) : 0.f) : inv;
@@ -365,7 +352,7 @@ __global__ __launch_bounds__(kTotalThreads) void k_route_total(RouteArgs a, int 
     double s = 0.0;
     int c = 0;
     if (j < a.E) {
-#pragma unroll 4
+#pragma unroll 12
         for (int b = part; b < nb; b += 64) {
             s += psum[(long)b * a.E + j];
             c += pcnt[(long)b * a.E + j];
@@ -463,8 +450,7 @@ __global__ __launch_bounds__(kThreads) void k_route_back(RouteBackArgs a, int nb
             if (c * L * 8 >= a.E) break;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = to_f(next[c][e]);
-                x[c][e] = v > -INFINITY ? v : -INFINITY;  // NaN too
+                x[c][e] = fmaxf(to_f(next[c][e]), -INFINITY);  // NaN too
                 m = fmaxf(m, x[c][e]);
             }
         }
@@ -511,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void k_route_back(RouteBackArgs a, int nb
 #pragma unroll
             for (int e = 0; e < 8; ++e) out[e] = from_f<T>(x[c][e] * inv * (G[c][e] - g) + gt[e]);
             if (row < a.n) {
-                if (col + 8 <= a.E)
+                if ((c + 1) * L * 8 <= a.E)
                     __builtin_memcpy(dz + col, out, 8 * sizeof(T));
                 else
 #pragma unroll
@@ -615,7 +601,8 @@ hipError_t launch_route_back(const RouteBackArgs& a, hipStream_t s)
 {
     if (a.n == 0) return hipSuccess;
     const long rw = 64 / row_lanes(a.E), b = ((a.n + rw - 1) / rw + kThreads / 64 - 1) / (kThreads / 64);
-    const int nb = (int)(b < 2 * kMaxBlocks ? b : 2 * kMaxBlocks);
+    const long most = a.E <= 64 && a.E > 32 ? 2 * kMaxBlocks : kMaxBlocks;
+    const int nb = (int)(b < most ? b : most);
     return with_type(a.type, [&](auto t) {
         return with_shape(a.E, [&](auto lanes, auto times) { return launch(k_route_back<decltype(t), lanes.value, times.value>, nb, kThreads, 0, s, a, nb); });
     });
