@@ -171,14 +171,26 @@ struct Rows {  // where the rows of a tile come from
     const int* ids; long ids_stride; int a;
 };
 
-// The tile of block x.  Blocks go to the 8 XCDs in turn, so neighbouring tiles, which
-// share adapters, are given to blocks 8 apart: an XCD's L2 then serves an adapter to all
-// its tiles (gridDim.x is a multiple of 8).
-__device__ __forceinline__ Tile tile_at(const Rows& w, int x)
+__device__ __forceinline__ Tile tile_at(const Rows& w, int i)
 {
-    if (w.tiles != nullptr) return w.tiles[(x & 7) * (gridDim.x >> 3) + (x >> 3)];
-    return Tile{adapter_of(w.ids, w.ids_stride, x, w.a), x, 1, -1};
+    if (w.tiles != nullptr) return w.tiles[i];
+    return Tile{adapter_of(w.ids, w.ids_stride, i, w.a), i, 1, -1};
 }
+
+// Which of `count` tiles (or chunks) and of `parts` parts of its work block x takes.  Blocks go to the
+// 8 XCDs in turn, so an XCD gets an eighth of the tiles side by side, each with all its
+// parts one after the other.  Neighbouring tiles share adapters, which that XCD's L2
+// then holds.  And the parts are stretches of the rows' columns: were the blocks that run
+// together all at one stretch, rows a multiple of 4 KB apart would put them on a quarter of
+// the memory channels (k_outer_split at 16,384 x 4,096, rank 64: 298 us that way).
+// The grid has ceil(count / 8) * 8 * parts blocks.
+struct Place { int tile, part; };
+__device__ __forceinline__ Place place_of(unsigned x, int count, int parts)
+{
+    const int per = (count + 7) / 8, i = x >> 3;
+    return Place{(int)(x & 7) * per + i / parts, i % parts};
+}
+inline unsigned place_grid(int count, int parts) { return (unsigned)((count + 7) / 8) * 8u * (unsigned)parts; }
 
 __device__ __forceinline__ int row_at(const Rows& w, int place) { return w.tiles != nullptr ? w.perm[place] : place; }
 
@@ -190,7 +202,7 @@ struct ShrinkArgs {
     const T* v; long ld_v;       // [n x w]
     const T* M; long sa, ld;     // [a][r][w]
     int w, r; long n;
-    int splits;                  // of w, one a blockIdx.y
+    int ntiles, splits;          // splits of w
     float* part; int rp;         // [splits][n places][rp], rp = the ranks in whole 16s
 };
 
@@ -203,7 +215,9 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
 {
     constexpr int KS = 128 / sizeof(T);
     __shared__ float sum[2][RT * 16][NB * 16 + 1];
-    const Tile t = tile_at(p.rows, blockIdx.x);
+    const Place at = place_of(blockIdx.x, p.ntiles, p.splits);
+    if (at.tile >= p.ntiles) return;
+    const Tile t = tile_at(p.rows, at.tile);
     if (t.q < 0 || t.q >= p.rows.a) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const int rank0 = blockIdx.z * (NB * 16);
@@ -219,9 +233,11 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[i][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int steps = (p.w + KS - 1) / KS;
-    const int s0 = (int)((long)steps * blockIdx.y / p.splits), s1 = (int)((long)steps * (blockIdx.y + 1) / p.splits);
+    const int s0 = (int)((long)steps * at.part / p.splits), count = (int)((long)steps * (at.part + 1) / p.splits) - s0;
     const int full = p.w / KS;
-    for (int s = s0 + wave; s < s1; s += 4) {
+    const int turn = count > 0 ? at.tile * 4 % count : 0;  // tiles start at different columns (the memory channels)
+    for (int k = wave; k < count; k += 4) {
+        const int s = s0 + (k + turn < count ? k + turn : k + turn - count);
         Vec<T> x[RT][2], y[NB][2];
         if (s < full) {
 #pragma unroll
@@ -268,17 +284,17 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
         __syncthreads();
     }
     if (wave != 0) return;
-    float* out = p.part + ((long)blockIdx.y * p.n + t.start) * p.rp;
+    float* out = p.part + ((long)at.part * p.n + t.start) * p.rp;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int at = i * 16 + g * 4 + e;
-            if (at >= t.cnt) continue;
+            const int row = i * 16 + g * 4 + e;
+            if (row >= t.cnt) continue;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int rank = rank0 + b * 16 + l16;
-                if (rank < p.rp) out[at * p.rp + rank] = rank < p.r ? acc[i][b][e] : 0.f;
+                if (rank < p.rp) out[row * p.rp + rank] = rank < p.r ? acc[i][b][e] : 0.f;
             }
         }
 }
@@ -311,7 +327,7 @@ __device__ __forceinline__ void transpose8(const Vec<bf16>* a, Vec<bf16>* b)
 
 template <typename T>
 struct ExpandArgs {
-    Rows rows;
+    Rows rows; int ntiles, parts;            // parts: blocks a tile, of 64 kVec columns
     const float* part; int splits, rp; long n;   // k_shrink's
     const T* M; long sa, ld;                 // [a][r][w]
     const float* gates; long gates_stride; const float* scales;
@@ -532,12 +548,14 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
     using Low = LowTile<T, RT, KP>;
     __shared__ __align__(16) Low L;
     __shared__ TileRows<RT> R;
-    const Tile t = tile_at(p.rows, blockIdx.x);
+    const Place at = place_of(blockIdx.x, p.ntiles, p.parts);
+    if (at.tile >= p.ntiles) return;
+    const Tile t = tile_at(p.rows, at.tile);
     if (t.q < 0) return;
     const bool has = t.q < p.rows.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const float sc = has && p.scales ? p.scales[t.q] : 1.f;
-    const int c0 = (blockIdx.y * 4 + wave) * 16 * V;
+    const int c0 = (at.part * 4 + wave) * 16 * V;
     const bool full = c0 + 16 * V <= p.w;
     // eight ranks of kVec columns: bf16: g * 8 .. + 7 of every 32 (of 16, for half as many
     // ranks); else g * 4 .. + 3 of every 16, two such
@@ -550,13 +568,13 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int rank = Low::kSplit ? (KP == 16 ? (g & 1) * 8 + e : b * 32 + g * 8 + e) : b * 32 + e / 4 * 16 + g * 4 + e % 4;
-                const T* at = p.M + t.q * p.sa + (long)min(rank, p.r - 1) * p.ld + cm;
-                m[b][e] = full ? load16(at) : load_part(at, p.w - cm);
+                const T* from = p.M + t.q * p.sa + (long)min(rank, p.r - 1) * p.ld + cm;
+                m[b][e] = full ? load16(from) : load_part(from, p.w - cm);
                 if (rank >= p.r) m[b][e] = Vec<T>{};
             }
         }
     }
-    const bool first = blockIdx.y == 0;
+    const bool first = at.part == 0;
     stage_rows<T, RT>(p, t, has, sc, R);
     stage_low<T, RT, KP>(p, t, has, sc, L, R, first ? p.low : nullptr, BACK && first ? p.dgates : nullptr);
     __syncthreads();
@@ -576,7 +594,7 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
         else
             expand_columns<T, RT, KP, false>(p, t, m, L, R, c0, has);
     }
-    if (BACK && Low::kSplit && has && p.dot_t != nullptr && blockIdx.y == gridDim.y - 1) {
+    if (BACK && Low::kSplit && has && p.dot_t != nullptr && at.part == p.parts - 1) {
         __syncthreads();
         stage_dot<T, RT, KP>(p, t, L, R);
         __syncthreads();
@@ -597,8 +615,8 @@ template <typename T>
 struct OuterArgs {
     const Tile* chunks; const int2* merge; const int* perm; int a, r;
     const float* gates; long gates_stride; const float* scales;
-    OuterSide<T> side[2];                    // blockIdx.y < split: side 0
-    int split;                               // blocks of side 0's columns
+    OuterSide<T> side[2];                    // parts below `split`: side 0
+    int split, nchunks, parts;               // parts: of both sides' columns
 };
 
 constexpr int kMaxChunk = 512;
@@ -614,11 +632,13 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
     __shared__ float fac[kMaxChunk];
     extern __shared__ char lds[];
     float* sum = reinterpret_cast<float*>(lds);  // [2][NB * 16][W]
-    const Tile t = p.chunks[blockIdx.x];
+    const Place at = place_of(blockIdx.x, p.nchunks, p.parts);
+    if (at.tile >= p.nchunks) return;
+    const Tile t = p.chunks[at.tile];
     if (t.q < 0) return;
-    const bool second = (int)blockIdx.y >= p.split;
+    const bool second = at.part >= p.split;
     const OuterSide<T>& s = p.side[second];
-    const int c0 = ((int)blockIdx.y - (second ? p.split : 0)) * W, rank0 = blockIdx.z * (NB * 16);
+    const int c0 = (at.part - (second ? p.split : 0)) * W, rank0 = blockIdx.z * (NB * 16);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const float sc = p.scales ? p.scales[t.q] : 1.f;
     for (int i = threadIdx.x; i < t.cnt; i += 256) {
@@ -700,19 +720,21 @@ struct SplitSide {
 };
 struct OuterSplitArgs {
     const Tile* chunks; const int* perm; int r; long ld_t;
-    SplitSide side[2]; int split;
+    SplitSide side[2]; int split, nchunks, parts;
 };
 
 template <int NB>
-__global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
+__global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
 {
     __shared__ __align__(16) int rows[kMaxChunk + 32];
-    const Tile t = p.chunks[blockIdx.x];
+    const Place at = place_of(blockIdx.x, p.nchunks, p.parts);
+    if (at.tile >= p.nchunks) return;
+    const Tile t = p.chunks[at.tile];
     if (t.q < 0) return;
-    const bool second = (int)blockIdx.y >= p.split;
+    const bool second = at.part >= p.split;
     const SplitSide s = second ? p.side[1] : p.side[0];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-    const int c0 = (((int)blockIdx.y - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * (NB * 16);
+    const int c0 = ((at.part - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * (NB * 16);
     for (int i = threadIdx.x; i < ((t.cnt + 31) & ~31); i += 256) rows[i] = p.perm[t.start + min(i, t.cnt - 1)];
     __syncthreads();
     if (c0 >= s.w) return;
@@ -723,35 +745,50 @@ __global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const bf16* lo0 = s.low + (long)p.r * p.ld_t;
-#pragma unroll 1
-    for (int i = g * 8; i < ((t.cnt + 31) & ~31); i += 32) {
-        Vec<bf16> v[8], x[8], hi[NB], lo[NB];
+    const bf16* low[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) low[b] = s.low + (long)min(rank0 + b * 16 + l16, p.r - 1) * p.ld_t + t.start + g * 8;
+    const long to_lo = (long)p.r * p.ld_t;
+    struct Step {
+        Vec<bf16> v[8], hi[NB], lo[NB];
+    };
+    // The operands of rows i .. i + 31 (those past the chunk belong to other adapters: zeros).
+    auto fetch = [&](Step& f, int i) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bf16* at = s.v + (long)rows[i + e] * s.ld_v + c;
-            v[e] = full ? load16(at) : load_part(at, left);
+            const bf16* from = s.v + (long)rows[i + g * 8 + e] * s.ld_v + c;
+            f.v[e] = full ? load16(from) : load_part(from, left);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const long at = (long)min(rank0 + b * 16 + l16, p.r - 1) * p.ld_t + t.start + i;
-            hi[b] = load16(s.low + at);
-            lo[b] = load16(lo0 + at);
+            f.hi[b] = load16(low[b] + i);
+            f.lo[b] = load16(low[b] + to_lo + i);
         }
-        if (i - g * 8 + 32 > t.cnt) {  // the places past the chunk belong to other adapters
+    };
+    auto use = [&](Step& f, int i) {
+        if (i + 32 > t.cnt) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (i + e >= t.cnt) {
-                    v[e] = Vec<bf16>{};
+                if (i + g * 8 + e >= t.cnt) {
+                    f.v[e] = Vec<bf16>{};
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) hi[b][e] = lo[b][e] = (bf16)0.f;
+                    for (int b = 0; b < NB; ++b) f.hi[b][e] = f.lo[b][e] = (bf16)0.f;
                 }
         }
-        transpose8(v, x);
+        Vec<bf16> x[8];
+        transpose8(f.v, x);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[b][j] = mfma16(lo[b], x[j], mfma16(hi[b], x[j], acc[b][j]));
+            for (int j = 0; j < 8; ++j) acc[b][j] = mfma16(f.lo[b], x[j], mfma16(f.hi[b], x[j], acc[b][j]));
+    };
+    Step f0, f1;
+    if (t.cnt > 0) fetch(f0, 0);
+    for (int i = 0; i < t.cnt; i += 64) {  // the next 32 rows are on their way while 32 are multiplied
+        if (i + 32 < t.cnt) fetch(f1, i + 32);
+        use(f0, i);
+        if (i + 64 < t.cnt) fetch(f0, i + 64);
+        if (i + 32 < t.cnt) use(f1, i + 32);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -830,7 +867,7 @@ size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 struct Layout {
     long n; int a, r;
     bool direct, split;                   // split: k_outer_split
-    int ntiles, nchunks, chunk;           // ntiles: in whole 8s unless direct
+    int ntiles, nchunks, chunk;
     int rp;
     int down_splits, up_splits;           // of d (t = D x) and of o (u = U dy)
     long ld_t;
@@ -865,7 +902,7 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     L.n = n; L.a = a; L.r = r;
     L.direct = n <= kDirectRows && !backward;
     L.split = type == kBF16;
-    L.ntiles = L.direct ? (int)n : (int)((n / kTile + a + 1 + 7) & ~7l);
+    L.ntiles = L.direct ? (int)n : (int)(n / kTile + a + 1);
     L.rp = (r + 15) & ~15;
     L.chunk = chunk_rows(n, d < o ? d : o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
@@ -902,18 +939,18 @@ hipError_t launch_plan(const Layout& L, const int* ids, long ids_stride, char* w
 }
 
 template <typename T, int RT>
-hipError_t launch_shrink(const ShrinkArgs<T>& p, int ntiles, hipStream_t s)
+hipError_t launch_shrink(const ShrinkArgs<T>& p, hipStream_t s)
 {
-    const dim3 grid(ntiles, p.splits, (p.r + 63) / 64);
+    const dim3 grid(place_grid(p.ntiles, p.splits), 1, (p.r + 63) / 64);
     if (p.r <= 16) return launch(k_shrink<T, RT, 1>, grid, 256, 0, s, p);
     if (p.r <= 32) return launch(k_shrink<T, RT, 2>, grid, 256, 0, s, p);
     return launch(k_shrink<T, RT, 4>, grid, 256, 0, s, p);
 }
 
 template <typename T, int RT, bool BACK>
-hipError_t launch_expand(const ExpandArgs<T>& p, int ntiles, hipStream_t s)
+hipError_t launch_expand(const ExpandArgs<T>& p, hipStream_t s)
 {
-    const dim3 grid(ntiles, (p.w + 64 * kVec<T> - 1) / (64 * kVec<T>));
+    const dim3 grid(place_grid(p.ntiles, p.parts));
     if (p.r <= 16) return launch(k_expand<T, RT, 16, BACK>, grid, 256, 0, s, p);
     if (p.r <= 32) return launch(k_expand<T, RT, 32, BACK>, grid, 256, 0, s, p);
     if (p.r <= 64) return launch(k_expand<T, RT, 64, BACK>, grid, 256, 0, s, p);
@@ -936,14 +973,14 @@ hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
     float* part = reinterpret_cast<float*>(a.ws + L.part);
     return with_type(a.type, [&](auto tag) {
         using T = decltype(tag);
-        const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.down_splits, part, L.rp};
-        const ExpandArgs<T> ex{rows, part, L.down_splits, L.rp, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
+        const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.ntiles, L.down_splits, part, L.rp};
+        const ExpandArgs<T> ex{rows, L.ntiles, (a.o + 64 * kVec<T> - 1) / (64 * kVec<T>), part, L.down_splits, L.rp, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
                                (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, a.o, a.r, a.low, nullptr, nullptr, nullptr, nullptr, 0};
         if (a.a > 0) {
-            const hipError_t e = L.direct ? launch_shrink<T, 1>(sh, L.ntiles, s) : launch_shrink<T, kTile / 16>(sh, L.ntiles, s);
+            const hipError_t e = L.direct ? launch_shrink<T, 1>(sh, s) : launch_shrink<T, kTile / 16>(sh, s);
             if (e != hipSuccess) return e;
         }
-        return L.direct ? launch_expand<T, 1, false>(ex, L.ntiles, s) : launch_expand<T, kTile / 16, false>(ex, L.ntiles, s);
+        return L.direct ? launch_expand<T, 1, false>(ex, s) : launch_expand<T, kTile / 16, false>(ex, s);
     });
 }
 
@@ -964,38 +1001,38 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
     return with_type(a.type, [&](auto tag) {
         using T = decltype(tag);
         if (a.n > 0) {
-            const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.up_splits, part, L.rp};
-            const ExpandArgs<T> ex{rows, part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
+            const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.ntiles, L.up_splits, part, L.rp};
+            const ExpandArgs<T> ex{rows, L.ntiles, (a.d + 64 * kVec<T> - 1) / (64 * kVec<T>), part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
                                    (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t, L.ld_t};
             if (a.a > 0) {
-                const hipError_t e = launch_shrink<T, kTile / 16>(sh, L.ntiles, s);
+                const hipError_t e = launch_shrink<T, kTile / 16>(sh, s);
                 if (e != hipSuccess) return e;
             }
-            const hipError_t e = launch_expand<T, kTile / 16, true>(ex, L.ntiles, s);
+            const hipError_t e = launch_expand<T, kTile / 16, true>(ex, s);
             if (e != hipSuccess) return e;
         }
         if (a.a == 0) return hipSuccess;
         constexpr int W = 16 * kVec<T>;
         const OuterArgs<T> ou{chunks, reinterpret_cast<const int2*>(a.ws + L.merge), rows.perm, a.a, a.r, a.gates, a.gates_stride, a.scales,
                               {{u, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {a.low, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
-                              (a.d + W - 1) / W};
+                              (a.d + W - 1) / W, L.nchunks, (a.d + W - 1) / W + (a.o + W - 1) / W};
         if constexpr (std::is_same_v<T, bf16>) {
             const OuterSplitArgs os{chunks, rows.perm, a.r, L.ld_t,
                                     {{u_t, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {t_t, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
-                                    (a.d + 511) / 512};
-            const int cols = os.split + (a.o + 511) / 512;
+                                    (a.d + 511) / 512, L.nchunks, (a.d + 511) / 512 + (a.o + 511) / 512};
+            const unsigned grid = place_grid(os.nchunks, os.parts);
             if (a.r <= 16)
-                SKM_TRY_LAUNCH(k_outer_split<1>, dim3(L.nchunks, cols, 1), 256, 0, s, os);
+                SKM_TRY_LAUNCH(k_outer_split<1>, dim3(grid), 256, 0, s, os);
             else if (a.r <= 32)
-                SKM_TRY_LAUNCH(k_outer_split<2>, dim3(L.nchunks, cols, 1), 256, 0, s, os);
+                SKM_TRY_LAUNCH(k_outer_split<2>, dim3(grid), 256, 0, s, os);
             else
-                SKM_TRY_LAUNCH(k_outer_split<4>, dim3(L.nchunks, cols, (a.r + 63) / 64), 256, 0, s, os);
+                SKM_TRY_LAUNCH(k_outer_split<4>, dim3(grid, 1, (a.r + 63) / 64), 256, 0, s, os);
         } else {
-            const int cols = ou.split + (a.o + W - 1) / W;
+            const unsigned grid = place_grid(ou.nchunks, ou.parts);
             if (a.r <= 16)
-                SKM_TRY_LAUNCH((k_outer<T, 1>), dim3(L.nchunks, cols, 1), 256, 2 * 16 * W * 4, s, ou);
+                SKM_TRY_LAUNCH((k_outer<T, 1>), dim3(grid), 256, 2 * 16 * W * 4, s, ou);
             else
-                SKM_TRY_LAUNCH((k_outer<T, 2>), dim3(L.nchunks, cols, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
+                SKM_TRY_LAUNCH((k_outer<T, 2>), dim3(grid, 1, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
         }
         const long most = (long)a.r * (a.d > a.o ? a.d : a.o);
         return launch(k_outer_merge<T>, dim3((unsigned)(most + 255 < 1024 * 256 ? (most + 255) / 256 : 1024), 2), 256, 0, s, ou);
