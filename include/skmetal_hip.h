@@ -376,7 +376,7 @@ SKMETAL_API int skmetal_hip_route_backward(int dtype, const void* logits, size_t
  * apart; ids [n] int32 (ids_stride elements apart), outside [0, a): the row has
  * no adapter; gates [n] (nullable: 1, gates_stride elements apart) and scales
  * [a] (nullable: 1) fp32.  low (nullable): [n x r] fp32, receives down_q x_i,
- * which the backward call takes.  1 <= r <= 128, n < 2^31, a <= 2048. */
+ * which the backward call takes.  1 <= r <= 128, n < 2^30, a <= 2048. */
 SKMETAL_API size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int backward);
 SKMETAL_API int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const void* down, size_t down_stride,
                                   size_t down_ld, const void* up, size_t up_stride, size_t up_ld, const int32_t* ids,

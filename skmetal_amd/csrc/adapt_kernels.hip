@@ -19,7 +19,6 @@
 namespace skm {
 namespace {
 
-constexpr int kTile = 64;          // rows of a k_shrink / k_expand tile
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanLoads = 16;     // ids a k_plan lane holds
 constexpr int kPlanRows = kPlanThreads * kPlanLoads;
@@ -33,8 +32,9 @@ struct Tile {
 
 struct PlanArgs {
     const int* ids; long ids_stride; int n, a;
+    int2* seen;          // [a + 1][segments] rows below and of each adapter, more than one segment only
     int* perm;           // [n] rows in the order of their adapters
-    Tile* tiles; int ntiles;    // kTile rows each
+    Tile* tiles; int ntiles, tile;    // `tile` rows each
     Tile* chunks; int nchunks;  // nullable; `chunk` rows each, one at least per adapter
     int2* merge;         // [a] first slot and number of an adapter's chunks where there are several
     int chunk;
@@ -46,11 +46,10 @@ __device__ __forceinline__ int adapter_of(const int* ids, long stride, long i, i
     return q >= 0 && q < a ? q : a;
 }
 
-// The rows of adapter blockIdx.x (a: of none) in their order, and its tiles: every block
-// reads all the ids, counts those below its own and writes its own rows' places.  Tile j
-// of adapter q has the entry start_q / len + q + j: start_(q+1) / len + q + 1 is at least
-// that many entries on, so no block needs another's count; the entries between stay
-// unused.  (At 16,384 rows and 64 adapters 5 us; one block that sorts all rows took 18.)
+// The tiles of adapter q, of `len` rows each (`whole`: one at least, and none for the rows
+// without an adapter).  Tile j of q has the entry start_q / len + q + j: start_(q+1) / len + q + 1
+// is at least that many entries on, so q's block needs no other's count; the entries
+// between stay unused.
 __device__ void write_tiles(int q, int a, int start, int cnt, int len, bool whole, Tile* out, int bound, int2* merge)
 {
     const int first = start / len + q;
@@ -61,33 +60,64 @@ __device__ void write_tiles(int q, int a, int start, int cnt, int len, bool whol
     if (merge != nullptr && q < a && threadIdx.x == 0) merge[q] = make_int2(first, tiles > 1 ? tiles : 0);
 }
 
-__global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs p)
+// The keys of a segment of kPlanRows rows, a wave's side by side (a + 1: no row).
+__device__ __forceinline__ void plan_keys(const PlanArgs& p, int* key)
 {
-    __shared__ int below[kPlanThreads / 64], equal[kPlanThreads / 64];
-    const int q = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int key[kPlanLoads];
+    const long first = (long)blockIdx.y * kPlanRows + (threadIdx.x >> 6) * (64 * kPlanLoads) + (threadIdx.x & 63);
 #pragma unroll
-    for (int it = 0; it < kPlanLoads; ++it) key[it] = p.a + 1;  // of no row
-    auto fetch = [&](long from) {
-        const long first = from + wave * (64 * kPlanLoads) + lane;
-#pragma unroll
-        for (int it = 0; it < kPlanLoads; ++it) {
-            const long i = first + it * 64;
-            const int k = p.ids[min(i, (long)p.n - 1) * p.ids_stride];
-            key[it] = i >= p.n ? p.a + 1 : k >= 0 && k < p.a ? k : p.a;
-        }
-    };
-    int lo = 0, eq = 0;
-    for (long from = 0; from < p.n; from += kPlanRows) {
-        fetch(from);
-#pragma unroll
-        for (int it = 0; it < kPlanLoads; ++it) {
-            lo += __popcll(__ballot(key[it] < q));
-            eq += __popcll(__ballot(key[it] == q));
+    for (int it = 0; it < kPlanLoads; ++it) {
+        const long i = first + it * 64;
+        key[it] = p.a + 1;
+        if (i < p.n) {
+            const int k = p.ids[i * p.ids_stride];
+            key[it] = k >= 0 && k < p.a ? k : p.a;
         }
     }
-    if (lane == 0) { below[wave] = lo; equal[wave] = eq; }
+}
+
+// Rows of the segment with keys below q, and with q, per wave.
+__device__ __forceinline__ void plan_count(const int* key, int q, int* below, int* equal)
+{
+    int lo = 0, eq = 0;
+#pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it) {
+        lo += __popcll(__ballot(key[it] < q));
+        eq += __popcll(__ballot(key[it] == q));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        below[threadIdx.x >> 6] = lo;
+        equal[threadIdx.x >> 6] = eq;
+    }
     __syncthreads();
+}
+
+__global__ __launch_bounds__(kPlanThreads) void k_plan_count(PlanArgs p)
+{
+    __shared__ int below[kPlanThreads / 64], equal[kPlanThreads / 64];
+    int key[kPlanLoads];
+    plan_keys(p, key);
+    plan_count(key, blockIdx.x, below, equal);
+    if (threadIdx.x != 0) return;
+    int2 s = make_int2(0, 0);
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        s.x += below[w];
+        s.y += equal[w];
+    }
+    p.seen[(long)blockIdx.x * gridDim.y + blockIdx.y] = s;
+}
+
+// The places of adapter blockIdx.x's rows (a: of the rows without one) among the rows of
+// segment blockIdx.y, in their order, and its tiles.  Every block reads the ids anew and counts
+// those below its own adapter: at 16,384 rows and 64 adapters 7 us against the 18 of one
+// block that sorts all the rows.
+__global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs p)
+{
+    __shared__ int below[kPlanThreads / 64], equal[kPlanThreads / 64], all[3];
+    const int q = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segments = gridDim.y;
+    int key[kPlanLoads];
+    plan_keys(p, key);
+    if (threadIdx.x < 3) all[threadIdx.x] = 0;
+    plan_count(key, q, below, equal);
     int start = 0, cnt = 0, place = 0;
 #pragma unroll
     for (int w = 0; w < kPlanThreads / 64; ++w) {
@@ -95,39 +125,28 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs p)
         if (w < wave) place += equal[w];
         cnt += equal[w];
     }
-    if (p.n <= kPlanRows) {  // the keys are still here, each wave's rows follow those of the one before
-        place += start;
-#pragma unroll
-        for (int it = 0; it < kPlanLoads; ++it) {
-            const unsigned long long m = __ballot(key[it] == q);
-            if (key[it] == q) p.perm[place + __popcll(m & ((1ull << lane) - 1))] = wave * (64 * kPlanLoads) + it * 64 + lane;
-            place += __popcll(m);
+    if (segments > 1) {  // k_plan_count's numbers of the other segments
+        for (int s = threadIdx.x; s < segments; s += kPlanThreads) {
+            const int2 v = p.seen[(long)q * segments + s];
+            atomicAdd(&all[0], v.x);
+            atomicAdd(&all[1], v.y);
+            if (s < (int)blockIdx.y) atomicAdd(&all[2], v.y);
         }
-    } else {
-        int done = start;
-        for (long from = 0; from < p.n; from += kPlanRows) {
-            fetch(from);
-            eq = 0;
-#pragma unroll
-            for (int it = 0; it < kPlanLoads; ++it) eq += __popcll(__ballot(key[it] == q));
-            __syncthreads();
-            if (lane == 0) equal[wave] = eq;
-            __syncthreads();
-            place = done;
-#pragma unroll
-            for (int w = 0; w < kPlanThreads / 64; ++w) {
-                if (w < wave) place += equal[w];
-                done += equal[w];
-            }
-#pragma unroll
-            for (int it = 0; it < kPlanLoads; ++it) {
-                const unsigned long long m = __ballot(key[it] == q);
-                if (key[it] == q) p.perm[place + __popcll(m & ((1ull << lane) - 1))] = (int)(from + wave * (64 * kPlanLoads) + it * 64 + lane);
-                place += __popcll(m);
-            }
-        }
+        __syncthreads();
+        start = all[0];
+        cnt = all[1];
+        place += all[2];
     }
-    write_tiles(q, p.a, start, cnt, kTile, false, p.tiles, p.ntiles, nullptr);
+    place += start;
+    const long first = (long)blockIdx.y * kPlanRows + wave * (64 * kPlanLoads) + lane;
+#pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it) {
+        const unsigned long long m = __ballot(key[it] == q);
+        if (key[it] == q) p.perm[place + __popcll(m & ((1ull << lane) - 1))] = (int)(first + it * 64);
+        place += __popcll(m);
+    }
+    if (blockIdx.y != 0) return;
+    write_tiles(q, p.a, start, cnt, p.tile, false, p.tiles, p.ntiles, nullptr);
     if (p.chunks != nullptr) write_tiles(q, p.a, start, cnt, p.chunk, true, p.chunks, p.nchunks, p.merge);
 }
 
@@ -164,6 +183,9 @@ __device__ __forceinline__ f32x4 mfma16(Vec<float> a, Vec<float> b, f32x4 acc)
     for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
     return acc;
 }
+
+// threadIdx.x / 64, which the compiler then knows to be the same on all lanes.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 struct Rows {  // where the rows of a tile come from
     const Tile* tiles;   // nullable: tile i is row i
@@ -219,14 +241,14 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
     if (at.tile >= p.ntiles) return;
     const Tile t = tile_at(p.rows, at.tile);
     if (t.q < 0 || t.q >= p.rows.a) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const int rank0 = blockIdx.z * (NB * 16);
     const T* v[RT];
     const T* m[NB];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) v[i] = p.v + (long)row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1)) * p.ld_v + g * (KS / 4);
+    for (int i = 0; i < RT; ++i) v[i] = p.v + (long)row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1)) * p.ld_v + g * kVec<T>;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) m[b] = p.M + t.q * p.sa + (long)min(rank0 + b * 16 + l16, p.r - 1) * p.ld + g * (KS / 4);
+    for (int b = 0; b < NB; ++b) m[b] = p.M + t.q * p.sa + (long)min(rank0 + b * 16 + l16, p.r - 1) * p.ld + g * kVec<T>;
     f32x4 acc[RT][NB];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -243,18 +265,18 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int i = 0; i < RT; ++i) x[i][h] = load16(v[i] + (long)s * KS + h * kVec<T>);
+                for (int i = 0; i < RT; ++i) x[i][h] = load16(v[i] + (long)s * KS + h * (KS / 2));
 #pragma unroll
-                for (int b = 0; b < NB; ++b) y[b][h] = load16(m[b] + (long)s * KS + h * kVec<T>);
+                for (int b = 0; b < NB; ++b) y[b][h] = load16(m[b] + (long)s * KS + h * (KS / 2));
             }
         } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int left = p.w - (s * KS + g * (KS / 4) + h * kVec<T>);
+                const int left = p.w - (s * KS + h * (KS / 2) + g * kVec<T>);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) x[i][h] = load_part(v[i] + (long)s * KS + h * kVec<T>, left);
+                for (int i = 0; i < RT; ++i) x[i][h] = load_part(v[i] + (long)s * KS + h * (KS / 2), left);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) y[b][h] = load_part(m[b] + (long)s * KS + h * kVec<T>, left);
+                for (int b = 0; b < NB; ++b) y[b][h] = load_part(m[b] + (long)s * KS + h * (KS / 2), left);
             }
         }
 #pragma unroll
@@ -327,7 +349,7 @@ __device__ __forceinline__ void transpose8(const Vec<bf16>* a, Vec<bf16>* b)
 
 template <typename T>
 struct ExpandArgs {
-    Rows rows; int ntiles, parts;            // parts: blocks a tile, of 64 kVec columns
+    Rows rows; int ntiles, parts;            // parts: blocks a tile
     const float* part; int splits, rp; long n;   // k_shrink's
     const T* M; long sa, ld;                 // [a][r][w]
     const float* gates; long gates_stride; const float* scales;
@@ -453,7 +475,21 @@ __device__ __forceinline__ void store_by_rank(const ExpandArgs<T>& p, const Tile
         }
 }
 
-// The wave's rows and columns of a tile: out = base + L M.  The product is taken as
+// A row tile's base: 16 bytes of a row a lane, four times.
+template <typename T, bool FULL>
+__device__ __forceinline__ void fetch_base(const ExpandArgs<T>& p, long row, int c0, Vec<T>* y)
+{
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int c = c0 + (e * 4 + g) * kVec<T>;
+        const T* from = p.base + row * p.ld_base + c;
+        y[e] = p.base == nullptr ? Vec<T>{} : FULL ? load16(from) : load_part(from, p.w - c);
+    }
+}
+
+// The wave's rows and columns of a tile: out = base + L M, with the first row tile's base in
+// y[0].  The product is taken as
 // (M^T)(L^T), so that a lane ends up with 16 bytes of a row, four times.
 //
 // bf16: lanes hold eight ranks of eight columns each, transposed in registers, so M goes
@@ -465,32 +501,15 @@ __device__ __forceinline__ void store_by_rank(const ExpandArgs<T>& p, const Tile
 // The sums start from the base where its type rounds at 2^-8 or 2^-11 anyway; in fp32 they
 // would then round at the base's size once for every four ranks, so it is added last.
 template <typename T, int RT, int KP, bool FULL>
-__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, const TileRows<RT>& R, int c0, bool has)
+__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, const long* row, Vec<T> (*y)[4], int c0, bool has)
 {
     constexpr int V = kVec<T>;
     constexpr bool kBaseFirst = sizeof(T) == 2;
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    long row[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) row[i] = R.row[i * 16 + l16];
-    Vec<T> y[2][4];
-    auto fetch = [&](int i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int c = c0 + (e * 4 + g) * V;
-            y[i & 1][e] = FULL ? load16(p.base + row[i] * p.ld_base + c) : load_part(p.base + row[i] * p.ld_base + c, p.w - c);
-        }
-    };
-    if (p.base == nullptr) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e & 1][e >> 1] = Vec<T>{};
-    } else {
-        fetch(0);
-    }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         if (i * 16 >= t.cnt) break;
-        if (i + 1 < RT && p.base != nullptr) fetch(i + 1);
+        if (i + 1 < RT) fetch_base<T, FULL>(p, row[i + 1], c0, y[(i + 1) & 1]);
         f32x4 acc[V];
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -539,10 +558,10 @@ __device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Til
 }
 
 // out_row = base_row + f_row low_row M_q.  A block takes RT * 16 rows of one adapter and
-// four waves' columns, 16 * kVec each, of which a wave keeps M_q in registers.  KP: the
-// ranks, rounded up.
+// every parts-th stretch of 64 * kVec columns, 16 * kVec a wave, which keeps M_q for them in
+// registers.  KP: the ranks, rounded up.
 template <typename T, int RT, int KP, bool BACK>
-__global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
+__global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand(ExpandArgs<T> p)
 {
     constexpr int V = kVec<T>;
     using Low = LowTile<T, RT, KP>;
@@ -553,46 +572,61 @@ __global__ __launch_bounds__(256) void k_expand(ExpandArgs<T> p)
     const Tile t = tile_at(p.rows, at.tile);
     if (t.q < 0) return;
     const bool has = t.q < p.rows.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const float sc = has && p.scales ? p.scales[t.q] : 1.f;
-    const int c0 = (at.part * 4 + wave) * 16 * V;
-    const bool full = c0 + 16 * V <= p.w;
+    long row[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) row[i] = row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1));
     // eight ranks of kVec columns: bf16: g * 8 .. + 7 of every 32 (of 16, for half as many
     // ranks); else g * 4 .. + 3 of every 16, two such
     constexpr int NM = (KP + 31) / 32;
-    Vec<T> m[NM][8];
-    if (has && c0 < p.w) {
-        const int cm = c0 + ((l16 & 3) * 4 + (l16 >> 2)) * V;  // the columns this lane brings
+    Vec<T> m[NM][8], y[2][4];
+    auto fetch = [&](int c0) {  // M and the first base of a stretch
+        if (c0 >= p.w) return;
+        const bool full = c0 + 16 * V <= p.w;
+        if (has) {
+            const int cm = c0 + ((l16 & 3) * 4 + (l16 >> 2)) * V;  // the columns this lane brings
 #pragma unroll
-        for (int b = 0; b < NM; ++b) {
+            for (int b = 0; b < NM; ++b) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int rank = Low::kSplit ? (KP == 16 ? (g & 1) * 8 + e : b * 32 + g * 8 + e) : b * 32 + e / 4 * 16 + g * 4 + e % 4;
-                const T* from = p.M + t.q * p.sa + (long)min(rank, p.r - 1) * p.ld + cm;
-                m[b][e] = full ? load16(from) : load_part(from, p.w - cm);
-                if (rank >= p.r) m[b][e] = Vec<T>{};
+                for (int e = 0; e < 8; ++e) {
+                    const int rank = Low::kSplit ? (KP == 16 ? (g & 1) * 8 + e : b * 32 + g * 8 + e) : b * 32 + e / 4 * 16 + g * 4 + e % 4;
+                    const T* from = p.M + t.q * p.sa + (long)min(rank, p.r - 1) * p.ld + cm;
+                    m[b][e] = full ? load16(from) : load_part(from, p.w - cm);
+                    if (rank >= p.r) m[b][e] = Vec<T>{};
+                }
             }
         }
-    }
+        if (full)
+            fetch_base<T, true>(p, row[0], c0, y[0]);
+        else
+            fetch_base<T, false>(p, row[0], c0, y[0]);
+    };
+    int c0 = (at.part * 4 + wave) * 16 * V;
+    fetch(c0);
     const bool first = at.part == 0;
     stage_rows<T, RT>(p, t, has, sc, R);
     stage_low<T, RT, KP>(p, t, has, sc, L, R, first ? p.low : nullptr, BACK && first ? p.dgates : nullptr);
     __syncthreads();
     if (BACK && Low::kSplit && first && has && p.low_t != nullptr) store_by_rank<T, RT, KP>(p, t, L, p.low_t);
-    if (c0 < p.w) {
+    while (c0 < p.w) {
         if constexpr (Low::kSplit) {
+            if (has) {
 #pragma unroll
-            for (int b = 0; b < NM; ++b) {
-                Vec<T> x[8];
+                for (int b = 0; b < NM; ++b) {
+                    Vec<T> x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = m[b][e];
-                transpose8(x, m[b]);
+                    for (int e = 0; e < 8; ++e) x[e] = m[b][e];
+                    transpose8(x, m[b]);
+                }
             }
         }
-        if (full)
-            expand_columns<T, RT, KP, true>(p, t, m, L, R, c0, has);
+        if (c0 + 16 * V <= p.w)
+            expand_columns<T, RT, KP, true>(p, t, m, L, row, y, c0, has);
         else
-            expand_columns<T, RT, KP, false>(p, t, m, L, R, c0, has);
+            expand_columns<T, RT, KP, false>(p, t, m, L, row, y, c0, has);
+        c0 += p.parts * 64 * V;
+        fetch(c0);
     }
     if (BACK && Low::kSplit && has && p.dot_t != nullptr && at.part == p.parts - 1) {
         __syncthreads();
@@ -639,7 +673,7 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
     const bool second = at.part >= p.split;
     const OuterSide<T>& s = p.side[second];
     const int c0 = (at.part - (second ? p.split : 0)) * W, rank0 = blockIdx.z * (NB * 16);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const float sc = p.scales ? p.scales[t.q] : 1.f;
     for (int i = threadIdx.x; i < t.cnt; i += 256) {
         const int row = p.perm[t.start + i];
@@ -733,7 +767,7 @@ __global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
     if (t.q < 0) return;
     const bool second = at.part >= p.split;
     const SplitSide s = second ? p.side[1] : p.side[0];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const int c0 = ((at.part - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * (NB * 16);
     for (int i = threadIdx.x; i < ((t.cnt + 31) & ~31); i += 256) rows[i] = p.perm[t.start + min(i, t.cnt - 1)];
     __syncthreads();
@@ -822,36 +856,33 @@ __global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
         }
 }
 
-// The chunks' sums of the adapters that have several, added in chunk order; every block a
-// part of each such adapter's matrix.
-template <typename T>
+// The chunks' sums of the adapters that have several, added in chunk order: blockIdx.z and
+// every gridDim.z-th such adapter.  Four values a thread (VEC), eight chunks in flight.
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_outer_merge(OuterArgs<T> p)
 {
+    constexpr int N = VEC ? 4 : 1;
     const OuterSide<T>& s = p.side[blockIdx.y];
     const long size = (long)p.r * s.w;
-    for (int q0 = 0; q0 < p.a; q0 += 256) {
-        __shared__ int2 some[256];
-        __shared__ int who[256], count;
-        __syncthreads();
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
-        const int q = q0 + threadIdx.x;
-        if (q < p.a) {
-            const int2 m = p.merge[q];
-            if (m.y != 0) {
-                const int at = atomicAdd(&count, 1);  // in any order: each is summed by itself
-                some[at] = m;
-                who[at] = q;
+    int nth = 0;
+    for (int q = 0; q < p.a; ++q) {
+        const int2 m = p.merge[q];
+        if (m.y == 0 || nth++ % (int)gridDim.z != (int)blockIdx.z) continue;
+        const float* part = s.part + m.x * size;
+        for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * N; i < size; i += (long)gridDim.x * 256 * N) {
+            float v[N] = {};
+            for (int k = 0; k < m.y; k += 8) {
+                float x[8][N];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) __builtin_memcpy(x[u], part + min(k + u, m.y - 1) * size + i, 4 * N);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[e] += k + u < m.y ? x[u][e] : 0.f;
             }
-        }
-        __syncthreads();
-        for (int j = 0; j < count; ++j) {
-            const int2 m = some[j];
-            for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long)gridDim.x * 256) {
-                float v = 0.f;
-                for (int k = 0; k < m.y; ++k) v += s.part[(m.x + k) * size + i];
-                s.dM[who[j] * size + i] = from_f<T>(v);
-            }
+            T* o = s.dM + q * size + i;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = from_f<T>(v[e]);
         }
     }
 }
@@ -867,11 +898,12 @@ size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 struct Layout {
     long n; int a, r;
     bool direct, split;                   // split: k_outer_split
-    int ntiles, nchunks, chunk;
+    int tile, ntiles, nchunks, chunk, segments;
+    long full_tiles;                      // of n rows, were they all of one adapter
     int rp;
     int down_splits, up_splits;           // of d (t = D x) and of o (u = U dy)
     long ld_t;
-    size_t perm, tiles, chunks, merge, part, low, low_t, dot_t, dpart, upart, bytes;
+    size_t seen, perm, tiles, chunks, merge, part, low, low_t, dot_t, dpart, upart, bytes;
 };
 
 // Parts of the columns, so that enough blocks read at once while a wave still has two
@@ -884,6 +916,29 @@ int split_count(long tiles, int w, int type, int zs)
     const long most = steps / 8;
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+
+// Columns in k_expand's stretches.
+int stretches(int w, int type)
+{
+    const int columns = 64 * (16 / (int)elem_size(type));
+    return (w + columns - 1) / columns;
+}
+
+// Rows a tile: as many as leave about three blocks a CU, for each reads its adapter anew.
+int tile_rows(long n, int w, int type)
+{
+    int t = 64;
+    while (t > 16 && (n + t - 1) / t * stretches(w, type) < 768) t /= 2;
+    return t;
+}
+
+// Blocks a k_expand tile: each stages the tile's low-rank rows again, so no more than
+// about 1,024 blocks in all.
+int part_count(long tiles, int w, int type)
+{
+    const long most = stretches(w, type), want = tiles > 0 ? (1024 + tiles - 1) / tiles : most;
+    return (int)(want < 1 ? 1 : want > most ? most : want);
 }
 
 // Rows a k_outer block sums up: as many as leave about two blocks a CU, for every cut
@@ -902,17 +957,22 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     L.n = n; L.a = a; L.r = r;
     L.direct = n <= kDirectRows && !backward;
     L.split = type == kBF16;
-    L.ntiles = L.direct ? (int)n : (int)(n / kTile + a + 1);
+    L.tile = L.direct ? 1 : tile_rows(n, d < o ? d : o, type);
+    L.full_tiles = (n + L.tile - 1) / L.tile;
+    L.ntiles = L.direct ? (int)n : (int)(n / L.tile + a + 1);
+    L.segments = (int)((n + kPlanRows - 1) / kPlanRows);
+    if (L.segments < 1) L.segments = 1;
     L.rp = (r + 15) & ~15;
     L.chunk = chunk_rows(n, d < o ? d : o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
     L.ld_t = ((n + 31) & ~31l) + 32;
     const int zs = (r + 63) / 64;
-    L.down_splits = split_count(L.direct ? n : (n + kTile - 1) / kTile, d, type, zs);
-    L.up_splits = split_count(L.direct ? n : (n + kTile - 1) / kTile, o, type, zs);
+    L.down_splits = split_count(L.full_tiles, d, type, zs);
+    L.up_splits = split_count(L.full_tiles, o, type, zs);
     size_t at = 0;
     auto take = [&](size_t& where, size_t bytes) { where = at; at += up16(bytes); };
     if (!L.direct) {
+        take(L.seen, L.segments > 1 ? (size_t)L.segments * (a + 1) * sizeof(int2) : 0);
         take(L.perm, (size_t)n * 4);
         take(L.tiles, (size_t)L.ntiles * sizeof(Tile));
     }
@@ -932,10 +992,13 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
 
 hipError_t launch_plan(const Layout& L, const int* ids, long ids_stride, char* ws, bool backward, hipStream_t s)
 {
-    const PlanArgs p{ids, ids_stride, (int)L.n, L.a, reinterpret_cast<int*>(ws + L.perm), reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles,
+    const PlanArgs p{ids, ids_stride, (int)L.n, L.a, reinterpret_cast<int2*>(ws + L.seen), reinterpret_cast<int*>(ws + L.perm),
+                     reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles, L.tile,
                      backward ? reinterpret_cast<Tile*>(ws + L.chunks) : nullptr, L.nchunks,
                      backward ? reinterpret_cast<int2*>(ws + L.merge) : nullptr, L.chunk};
-    return launch(k_plan, L.a + 1, kPlanThreads, 0, s, p);
+    const dim3 grid(L.a + 1, L.segments);
+    if (L.segments > 1) SKM_TRY_LAUNCH(k_plan_count, grid, kPlanThreads, 0, s, p);
+    return launch(k_plan, grid, kPlanThreads, 0, s, p);
 }
 
 template <typename T, int RT>
@@ -957,6 +1020,15 @@ hipError_t launch_expand(const ExpandArgs<T>& p, hipStream_t s)
     return launch(k_expand<T, RT, 128, BACK>, grid, 256, 0, s, p);
 }
 
+// f(row tiles of 16 a tile)
+template <typename F>
+hipError_t with_tile(int tile, F&& f)
+{
+    if (tile == 64) return f(std::integral_constant<int, 4>{});
+    if (tile == 32) return f(std::integral_constant<int, 2>{});
+    return f(std::integral_constant<int, 1>{});
+}
+
 }  // namespace
 
 size_t adapt_workspace(int type, long n, int d, int o, int r, int a, int backward) { return layout(type, n, d, o, r, a, backward != 0).bytes; }
@@ -974,13 +1046,12 @@ hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
     return with_type(a.type, [&](auto tag) {
         using T = decltype(tag);
         const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.ntiles, L.down_splits, part, L.rp};
-        const ExpandArgs<T> ex{rows, L.ntiles, (a.o + 64 * kVec<T> - 1) / (64 * kVec<T>), part, L.down_splits, L.rp, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
+        const ExpandArgs<T> ex{rows, L.ntiles, part_count(L.full_tiles, a.o, a.type), part, L.down_splits, L.rp, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
                                (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, a.o, a.r, a.low, nullptr, nullptr, nullptr, nullptr, 0};
-        if (a.a > 0) {
-            const hipError_t e = L.direct ? launch_shrink<T, 1>(sh, s) : launch_shrink<T, kTile / 16>(sh, s);
-            if (e != hipSuccess) return e;
-        }
-        return L.direct ? launch_expand<T, 1, false>(ex, s) : launch_expand<T, kTile / 16, false>(ex, s);
+        return with_tile(L.tile, [&](auto rt) {
+            const hipError_t e = a.a > 0 ? launch_shrink<T, rt.value>(sh, s) : hipSuccess;
+            return e != hipSuccess ? e : launch_expand<T, rt.value, false>(ex, s);
+        });
     });
 }
 
@@ -1002,13 +1073,12 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
         using T = decltype(tag);
         if (a.n > 0) {
             const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.ntiles, L.up_splits, part, L.rp};
-            const ExpandArgs<T> ex{rows, L.ntiles, (a.d + 64 * kVec<T> - 1) / (64 * kVec<T>), part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
+            const ExpandArgs<T> ex{rows, L.ntiles, part_count(L.full_tiles, a.d, a.type), part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
                                    (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t, L.ld_t};
-            if (a.a > 0) {
-                const hipError_t e = launch_shrink<T, kTile / 16>(sh, s);
-                if (e != hipSuccess) return e;
-            }
-            const hipError_t e = launch_expand<T, kTile / 16, true>(ex, s);
+            const hipError_t e = with_tile(L.tile, [&](auto rt) {
+                const hipError_t e = a.a > 0 ? launch_shrink<T, rt.value>(sh, s) : hipSuccess;
+                return e != hipSuccess ? e : launch_expand<T, rt.value, true>(ex, s);
+            });
             if (e != hipSuccess) return e;
         }
         if (a.a == 0) return hipSuccess;
@@ -1035,7 +1105,11 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
                 SKM_TRY_LAUNCH((k_outer<T, 2>), dim3(grid, 1, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
         }
         const long most = (long)a.r * (a.d > a.o ? a.d : a.o);
-        return launch(k_outer_merge<T>, dim3((unsigned)(most + 255 < 1024 * 256 ? (most + 255) / 256 : 1024), 2), 256, 0, s, ou);
+        if (L.n <= L.chunk) return hipSuccess;  // one chunk an adapter
+        const bool vec = ((long)a.r * a.d % 4 == 0) && ((long)a.r * a.o % 4 == 0);
+        const long blocks = (most / (vec ? 4 : 1) + 255) / 256;
+        const dim3 grid((unsigned)(blocks < 64 ? blocks : 64), 2, a.a < 8 ? a.a : 8);
+        return vec ? launch(k_outer_merge<T, true>, grid, 256, 0, s, ou) : launch(k_outer_merge<T, false>, grid, 256, 0, s, ou);
     });
 }
 

@@ -2185,7 +2185,7 @@ int check_adapt(int dtype, const AdaptSizes& z, std::initializer_list<size_t> st
     TRY(check_dtype(dtype));
     if (z.d == 0 || z.o == 0 || z.r == 0) return fail(SKMETAL_EINVAL, "d, o and r must be positive (d=%zu o=%zu r=%zu)", z.d, z.o, z.r);
     if (z.r > size_t(kAdaptMaxR)) return fail(SKMETAL_ERANGE, "r=%zu: a rank of at most %d", z.r, kAdaptMaxR);
-    if (z.n > kMaxRows || z.a > size_t(kAdaptMaxA) || z.d > kMaxDim || z.o > kMaxDim)
+    if (z.n > kMaxRows / 2 || z.a > size_t(kAdaptMaxA) || z.d > kMaxDim || z.o > kMaxDim)
         return fail(SKMETAL_ERANGE, "n=%zu, a=%zu, d=%zu or o=%zu exceeds the supported range", z.n, z.a, z.d, z.o);
     for (const size_t s : strides)
         if (s > kMaxStride) return fail(SKMETAL_ERANGE, "a stride of %zu elements exceeds the supported range", s);
