@@ -212,6 +212,12 @@ __device__ __forceinline__ Place place_of(unsigned x, int count, int parts)
     const int per = (count + 7) / 8, i = x >> 3;
     return Place{(int)(x & 7) * per + i / parts, i % parts};
 }
+// For k_outer, whose chunks share nothing and differ in length: a chunk's parts on all XCDs.
+__device__ __forceinline__ Place place_spread(unsigned x, int parts)
+{
+    const int chunk = x / parts;
+    return Place{chunk, (int)(x + chunk) % parts};
+}
 inline unsigned place_grid(int count, int parts) { return (unsigned)((count + 7) / 8) * 8u * (unsigned)parts; }
 
 __device__ __forceinline__ int row_at(const Rows& w, int place) { return w.tiles != nullptr ? w.perm[place] : place; }
@@ -257,9 +263,8 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
     const int steps = (p.w + KS - 1) / KS;
     const int s0 = (int)((long)steps * at.part / p.splits), count = (int)((long)steps * (at.part + 1) / p.splits) - s0;
     const int full = p.w / KS;
-    const int turn = count > 0 ? at.tile * 4 % count : 0;  // tiles start at different columns (the memory channels)
     for (int k = wave; k < count; k += 4) {
-        const int s = s0 + (k + turn < count ? k + turn : k + turn - count);
+        const int s = s0 + k;
         Vec<T> x[RT][2], y[NB][2];
         if (s < full) {
 #pragma unroll
@@ -390,7 +395,7 @@ struct LowTile<bf16, RT, KP> {
 
 // A row's own numbers in a tile, which its first threads look up.
 template <int RT>
-struct TileRows {
+struct __align__(16) TileRows {
     int row[RT * 16];
     float f[RT * 16];
 };
@@ -475,22 +480,22 @@ __device__ __forceinline__ void store_by_rank(const ExpandArgs<T>& p, const Tile
         }
 }
 
-// A row tile's base: 16 bytes of a row a lane, four times.
+// The rows of a 16-row tile that a lane brings and takes: g * 4 .. + 3 of it.
+struct Quad { int row[4]; };
+
+// Their base: 16 bytes of each row a lane, 256 bytes of a row side by side.
 template <typename T, bool FULL>
-__device__ __forceinline__ void fetch_base(const ExpandArgs<T>& p, long row, int c0, Vec<T>* y)
+__device__ __forceinline__ void fetch_base(const ExpandArgs<T>& p, const Quad& q, int c, Vec<T>* y)
 {
-    const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int c = c0 + (e * 4 + g) * kVec<T>;
-        const T* from = p.base + row * p.ld_base + c;
+        const T* from = p.base + q.row[e] * p.ld_base + c;
         y[e] = p.base == nullptr ? Vec<T>{} : FULL ? load16(from) : load_part(from, p.w - c);
     }
 }
 
-// The wave's rows and columns of a tile: out = base + L M, with the first row tile's base in
-// y[0].  The product is taken as
-// (M^T)(L^T), so that a lane ends up with 16 bytes of a row, four times.
+// The wave's rows and columns of a tile: out = base + L M, with the first 16 rows' base in
+// y[0].  A lane ends up with kVec columns (from c on) of four rows.
 //
 // bf16: lanes hold eight ranks of eight columns each, transposed in registers, so M goes
 // to the matrix cores without a detour; L enters as two bf16 (one product of 32 where the
@@ -501,15 +506,22 @@ __device__ __forceinline__ void fetch_base(const ExpandArgs<T>& p, long row, int
 // The sums start from the base where its type rounds at 2^-8 or 2^-11 anyway; in fp32 they
 // would then round at the base's size once for every four ranks, so it is added last.
 template <typename T, int RT, int KP, bool FULL>
-__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, const long* row, Vec<T> (*y)[4], int c0, bool has)
+__device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Tile& t, const Vec<T> (*m)[8], const LowTile<T, RT, KP>& L, const TileRows<RT>& R,
+                                               Vec<T> (*y)[4], int c, bool has)
 {
     constexpr int V = kVec<T>;
     constexpr bool kBaseFirst = sizeof(T) == 2;
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, left = p.w - c;
+    auto quad = [&](int i) { return *reinterpret_cast<const Quad*>(&R.row[i * 16 + g * 4]); };
+    Quad now = quad(0);
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         if (i * 16 >= t.cnt) break;
-        if (i + 1 < RT) fetch_base<T, FULL>(p, row[i + 1], c0, y[(i + 1) & 1]);
+        Quad next = now;
+        if (i + 1 < RT) {
+            next = quad(i + 1);
+            fetch_base<T, FULL>(p, next, c, y[(i + 1) & 1]);
+        }
         f32x4 acc[V];
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -521,11 +533,11 @@ __device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Til
                 for (int b = 0; b < (KP + 31) / 32; ++b) {
                     const Vec<T> hi = *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][b * 32 + g * 8]);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) acc[j] = mfma16(m[b][j], hi, acc[j]);
+                    for (int j = 0; j < V; ++j) acc[j] = mfma16(hi, m[b][j], acc[j]);
                     if constexpr (KP >= 32) {
                         const Vec<T> lo = *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][KP + b * 32 + g * 8]);
 #pragma unroll
-                        for (int j = 0; j < V; ++j) acc[j] = mfma16(m[b][j], lo, acc[j]);
+                        for (int j = 0; j < V; ++j) acc[j] = mfma16(lo, m[b][j], acc[j]);
                     }
                 }
             } else {
@@ -535,25 +547,25 @@ __device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Til
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
 #pragma unroll
-                        for (int j = 0; j < V; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f(m[b / 2][b % 2 * 4 + s][j]), lo[s], acc[j], 0, 0, 0);
+                        for (int j = 0; j < V; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(lo[s], to_f(m[b / 2][b % 2 * 4 + s][j]), acc[j], 0, 0, 0);
                 }
             }
         }
-        if (i * 16 + l16 < t.cnt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c = c0 + (e * 4 + g) * V, left = p.w - c;
-                Vec<T> z;
+        for (int e = 0; e < 4; ++e) {
+            if (i * 16 + g * 4 + e >= t.cnt) continue;
+            Vec<T> z;
 #pragma unroll
-                for (int j = 0; j < V; ++j) z[j] = from_f<T>(kBaseFirst ? acc[j][e] : to_f(y[i & 1][e][j]) + acc[j][e]);
-                T* o = p.out + row[i] * p.ld_out + c;
-                if (FULL || left >= V)
-                    __builtin_memcpy(o, &z, 16);
-                else
+            for (int j = 0; j < V; ++j) z[j] = from_f<T>(kBaseFirst ? acc[j][e] : to_f(y[i & 1][e][j]) + acc[j][e]);
+            T* o = p.out + now.row[e] * p.ld_out + c;
+            if (FULL || left >= V)
+                __builtin_memcpy(o, &z, 16);
+            else
 #pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (j < left) o[j] = z[j];
-            }
+                for (int j = 0; j < V; ++j)
+                    if (j < left) o[j] = z[j];
+        }
+        now = next;
     }
 }
 
@@ -574,9 +586,9 @@ __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand
     const bool has = t.q < p.rows.a;
     const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const float sc = has && p.scales ? p.scales[t.q] : 1.f;
-    long row[RT];
+    Quad row0;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) row[i] = row_at(p.rows, t.start + min(i * 16 + l16, t.cnt - 1));
+    for (int e = 0; e < 4; ++e) row0.row[e] = row_at(p.rows, t.start + min(g * 4 + e, t.cnt - 1));
     // eight ranks of kVec columns: bf16: g * 8 .. + 7 of every 32 (of 16, for half as many
     // ranks); else g * 4 .. + 3 of every 16, two such
     constexpr int NM = (KP + 31) / 32;
@@ -585,7 +597,7 @@ __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand
         if (c0 >= p.w) return;
         const bool full = c0 + 16 * V <= p.w;
         if (has) {
-            const int cm = c0 + ((l16 & 3) * 4 + (l16 >> 2)) * V;  // the columns this lane brings
+            const int cm = c0 + l16 * V;
 #pragma unroll
             for (int b = 0; b < NM; ++b) {
 #pragma unroll
@@ -598,9 +610,9 @@ __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand
             }
         }
         if (full)
-            fetch_base<T, true>(p, row[0], c0, y[0]);
+            fetch_base<T, true>(p, row0, c0 + l16 * V, y[0]);
         else
-            fetch_base<T, false>(p, row[0], c0, y[0]);
+            fetch_base<T, false>(p, row0, c0 + l16 * V, y[0]);
     };
     int c0 = (at.part * 4 + wave) * 16 * V;
     fetch(c0);
@@ -622,9 +634,9 @@ __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand
             }
         }
         if (c0 + 16 * V <= p.w)
-            expand_columns<T, RT, KP, true>(p, t, m, L, row, y, c0, has);
+            expand_columns<T, RT, KP, true>(p, t, m, L, R, y, c0 + l16 * V, has);
         else
-            expand_columns<T, RT, KP, false>(p, t, m, L, row, y, c0, has);
+            expand_columns<T, RT, KP, false>(p, t, m, L, R, y, c0 + l16 * V, has);
         c0 += p.parts * 64 * V;
         fetch(c0);
     }
@@ -650,7 +662,7 @@ struct OuterArgs {
     const Tile* chunks; const int2* merge; const int* perm; int a, r;
     const float* gates; long gates_stride; const float* scales;
     OuterSide<T> side[2];                    // parts below `split`: side 0
-    int split, nchunks, parts;               // parts: of both sides' columns
+    int split, parts;                        // parts: of both sides' columns
 };
 
 constexpr int kMaxChunk = 512;
@@ -666,8 +678,7 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
     __shared__ float fac[kMaxChunk];
     extern __shared__ char lds[];
     float* sum = reinterpret_cast<float*>(lds);  // [2][NB * 16][W]
-    const Place at = place_of(blockIdx.x, p.nchunks, p.parts);
-    if (at.tile >= p.nchunks) return;
+    const Place at = place_spread(blockIdx.x, p.parts);
     const Tile t = p.chunks[at.tile];
     if (t.q < 0) return;
     const bool second = at.part >= p.split;
@@ -754,15 +765,14 @@ struct SplitSide {
 };
 struct OuterSplitArgs {
     const Tile* chunks; const int* perm; int r; long ld_t;
-    SplitSide side[2]; int split, nchunks, parts;
+    SplitSide side[2]; int split, parts;
 };
 
 template <int NB>
 __global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
 {
     __shared__ __align__(16) int rows[kMaxChunk + 32];
-    const Place at = place_of(blockIdx.x, p.nchunks, p.parts);
-    if (at.tile >= p.nchunks) return;
+    const Place at = place_spread(blockIdx.x, p.parts);
     const Tile t = p.chunks[at.tile];
     if (t.q < 0) return;
     const bool second = at.part >= p.split;
@@ -1085,12 +1095,12 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
         constexpr int W = 16 * kVec<T>;
         const OuterArgs<T> ou{chunks, reinterpret_cast<const int2*>(a.ws + L.merge), rows.perm, a.a, a.r, a.gates, a.gates_stride, a.scales,
                               {{u, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {a.low, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
-                              (a.d + W - 1) / W, L.nchunks, (a.d + W - 1) / W + (a.o + W - 1) / W};
+                              (a.d + W - 1) / W, (a.d + W - 1) / W + (a.o + W - 1) / W};
         if constexpr (std::is_same_v<T, bf16>) {
             const OuterSplitArgs os{chunks, rows.perm, a.r, L.ld_t,
                                     {{u_t, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {t_t, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
-                                    (a.d + 511) / 512, L.nchunks, (a.d + 511) / 512 + (a.o + 511) / 512};
-            const unsigned grid = place_grid(os.nchunks, os.parts);
+                                    (a.d + 511) / 512, (a.d + 511) / 512 + (a.o + 511) / 512};
+            const unsigned grid = (unsigned)(L.nchunks * os.parts);
             if (a.r <= 16)
                 SKM_TRY_LAUNCH(k_outer_split<1>, dim3(grid), 256, 0, s, os);
             else if (a.r <= 32)
@@ -1098,7 +1108,7 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
             else
                 SKM_TRY_LAUNCH(k_outer_split<4>, dim3(grid, 1, (a.r + 63) / 64), 256, 0, s, os);
         } else {
-            const unsigned grid = place_grid(ou.nchunks, ou.parts);
+            const unsigned grid = (unsigned)(L.nchunks * ou.parts);
             if (a.r <= 16)
                 SKM_TRY_LAUNCH((k_outer<T, 1>), dim3(grid), 256, 2 * 16 * W * 4, s, ou);
             else
@@ -1108,7 +1118,7 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
         if (L.n <= L.chunk) return hipSuccess;  // one chunk an adapter
         const bool vec = ((long)a.r * a.d % 4 == 0) && ((long)a.r * a.o % 4 == 0);
         const long blocks = (most / (vec ? 4 : 1) + 255) / 256;
-        const dim3 grid((unsigned)(blocks < 64 ? blocks : 64), 2, a.a < 8 ? a.a : 8);
+        const dim3 grid((unsigned)(blocks < 256 ? blocks : 256), 2, a.a < 8 ? a.a : 8);
         return vec ? launch(k_outer_merge<T, true>, grid, 256, 0, s, ou) : launch(k_outer_merge<T, false>, grid, 256, 0, s, ou);
     });
 }
