@@ -765,9 +765,11 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
         }
 }
 
-// The same for bf16 rows on the bf16 matrix cores: f low comes by rank as two bf16 (k_expand's
-// low_t, dot_t), 32 rows at a time; a lane's eight rows of eight columns are transposed
-// in registers.  A block takes a chunk and 512 columns, a wave 128 of them.
+// The same for bf16 rows on the bf16 matrix cores, 32 rows at a time: a lane's eight rows of
+// eight columns are transposed in registers, and f low comes by rank as two bf16 (k_expand's
+// low_t, dot_t) through LDS, 64 rows at a time, for the block's four waves.  A block takes a
+// chunk and 512 columns, a wave 128 of them.  (16,384 rows x 4,096 twice, rank 64: 82 us
+// so; 120 with each wave's own loads of f low, 16 lines of 64 bytes apiece.)
 struct SplitSide {
     const bf16* low;                         // [2][r][ld_t]: hi, lo
     const bf16* v; long ld_v; int w;
@@ -779,71 +781,85 @@ struct OuterSplitArgs {
 };
 
 template <int NB>
-__global__ __launch_bounds__(256) void k_outer_split(OuterSplitArgs p)
+__global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
 {
+    constexpr int R = NB * 16;
+    constexpr int S = NB == 4 ? 32 : 64, NM = 2 * R * S / 8 / 256;  // rows staged at once, a thread's 16 bytes of them
     __shared__ __align__(16) int rows[kMaxChunk + 32];
+    __shared__ __align__(16) bf16 low[2][2][R][S + 8];  // twice: hi and lo of S rows by rank
     const Place at = place_spread(blockIdx.x, p.parts);
     const Tile t = p.chunks[at.tile];
     if (t.q < 0) return;
     const bool second = at.part >= p.split;
     const SplitSide s = second ? p.side[1] : p.side[0];
     const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
-    const int c0 = ((at.part - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * (NB * 16);
+    const int c0 = ((at.part - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * R;
+    const bool active = c0 < s.w, full = c0 + 128 <= s.w;
+    const int c = c0 + l16 * 8, left = s.w - c;
+    Vec<bf16> mine[NM];
+    auto fetch_low = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < NM; ++u) {
+            const int idx = threadIdx.x + u * 256, seg = idx % (S / 8), rank = idx / (S / 8) % R, half = idx / (S / 8 * R);
+            mine[u] = load16(s.low + (half * p.r + min(rank0 + rank, p.r - 1)) * p.ld_t + t.start + i + seg * 8);
+            if (i + S > t.cnt)  // the places past the chunk belong to other adapters
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (i + seg * 8 + e >= t.cnt) mine[u][e] = (bf16)0.f;
+        }
+    };
+    auto stage_low = [&](int turn) {
+#pragma unroll
+        for (int u = 0; u < NM; ++u) {
+            const int idx = threadIdx.x + u * 256, seg = idx % (S / 8), rank = idx / (S / 8) % R, half = idx / (S / 8 * R);
+            *reinterpret_cast<Vec<bf16>*>(&low[turn][half][rank][seg * 8]) = mine[u];
+        }
+    };
+    Vec<bf16> v[8];
+    auto fetch_rows = [&](int i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bf16* from = s.v + (long)rows[i + g * 8 + e] * s.ld_v + c;
+            v[e] = full ? load16(from) : load_part(from, left);
+        }
+    };
+    if (t.cnt > 0) fetch_low(0);
     for (int i = threadIdx.x; i < ((t.cnt + 31) & ~31); i += 256) rows[i] = p.perm[t.start + min(i, t.cnt - 1)];
     __syncthreads();
-    if (c0 >= s.w) return;
-    const bool full = c0 + 128 <= s.w;
-    const int c = c0 + l16 * 8, left = s.w - c;
+    if (active && t.cnt > 0) fetch_rows(0);
     f32x4 acc[NB][8];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const bf16* low[NB];
+    for (int i = 0; i < t.cnt; i += S) {
+        const int turn = i / S & 1;
+        stage_low(turn);
+        __syncthreads();  // one is enough: the other half is written again only after the next
+        if (i + S < t.cnt) fetch_low(i + S);
+        if (!active) continue;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) low[b] = s.low + (long)min(rank0 + b * 16 + l16, p.r - 1) * p.ld_t + t.start + g * 8;
-    const long to_lo = (long)p.r * p.ld_t;
-    struct Step {
-        Vec<bf16> v[8], hi[NB], lo[NB];
-    };
-    // The operands of rows i .. i + 31 (those past the chunk belong to other adapters: zeros).
-    auto fetch = [&](Step& f, int i) {
+        for (int h = 0; h < S / 32; ++h) {
+            const int k = i + h * 32;
+            if (k >= t.cnt) break;
+            if (k + 32 > t.cnt)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bf16* from = s.v + (long)rows[i + g * 8 + e] * s.ld_v + c;
-            f.v[e] = full ? load16(from) : load_part(from, left);
-        }
+                for (int e = 0; e < 8; ++e)
+                    if (k + g * 8 + e >= t.cnt) v[e] = Vec<bf16>{};
+            Vec<bf16> x[8];
+            transpose8(v, x);
+            if (k + 32 < t.cnt) fetch_rows(k + 32);  // on their way while these are multiplied
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            f.hi[b] = load16(low[b] + i);
-            f.lo[b] = load16(low[b] + to_lo + i);
-        }
-    };
-    auto use = [&](Step& f, int i) {
-        if (i + 32 > t.cnt) {
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (i + g * 8 + e >= t.cnt) {
-                    f.v[e] = Vec<bf16>{};
+                for (int half = 0; half < 2; ++half) {
+                    const Vec<bf16> f = *reinterpret_cast<const Vec<bf16>*>(&low[turn][half][b * 16 + l16][h * 32 + g * 8]);
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) f.hi[b][e] = f.lo[b][e] = (bf16)0.f;
+                    for (int j = 0; j < 8; ++j) acc[b][j] = mfma16(f, x[j], acc[b][j]);
                 }
         }
-        Vec<bf16> x[8];
-        transpose8(f.v, x);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[b][j] = mfma16(f.lo[b], x[j], mfma16(f.hi[b], x[j], acc[b][j]));
-    };
-    Step f0, f1;
-    if (t.cnt > 0) fetch(f0, 0);
-    for (int i = 0; i < t.cnt; i += 64) {  // the next 32 rows are on their way while 32 are multiplied
-        if (i + 32 < t.cnt) fetch(f1, i + 32);
-        use(f0, i);
-        if (i + 64 < t.cnt) fetch(f0, i + 64);
-        if (i + 32 < t.cnt) use(f1, i + 32);
     }
+    if (!active) return;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -985,7 +1001,7 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     L.rp = (r + 15) & ~15;
     L.chunk = chunk_rows(n, d < o ? d : o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
-    L.ld_t = ((n + 31) & ~31l) + 32;
+    L.ld_t = ((n + 63) & ~63l) + 96;  // 64 rows past the last; not a power of two apart
     const int zs = (r + 63) / 64;
     L.down_splits = split_count(L.full_tiles, d, type, zs);
     L.up_splits = split_count(L.full_tiles, o, type, zs);
