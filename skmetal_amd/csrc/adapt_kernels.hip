@@ -416,7 +416,7 @@ __device__ __forceinline__ void stage_rows(const ExpandArgs<T>& p, const Tile& t
     if (threadIdx.x < RT * 16) {
         const int row = row_at(p.rows, t.start + min((int)threadIdx.x, t.cnt - 1));
         R.row[threadIdx.x] = row;
-        R.f[threadIdx.x] = has ? (p.gates ? p.gates[row * p.gates_stride] : 1.f) * sc : 0.f;
+        R.f[threadIdx.x] = has ? (p.gates ? p.gates[(long)row * p.gates_stride] : 1.f) * sc : 0.f;
     }
 }
 
@@ -669,7 +669,9 @@ struct OuterSide {
 };
 template <typename T>
 struct OuterArgs {
-    const Tile* chunks; const int2* merge; const int* perm; int a, r;
+    const Tile* chunks;                      // nullable: chunk q is all of adapter q's rows, at most kMaxChunk, found here
+    const int2* merge; const int* perm; int a, r;
+    const int* ids; long ids_stride; int n;  // for finding them
     const float* gates; long gates_stride; const float* scales;
     OuterSide<T> side[2];                    // parts below `split`: side 0
     int split, parts;                        // parts: of both sides' columns
@@ -689,18 +691,36 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
     extern __shared__ char lds[];
     float* sum = reinterpret_cast<float*>(lds);  // [2][NB * 16][W]
     const Place at = place_spread(blockIdx.x, p.parts);
-    const Tile t = p.chunks[at.tile];
+    Tile t{at.tile, 0, 0, -1};
+    if (p.chunks != nullptr) t = p.chunks[at.tile];
     if (t.q < 0) return;
     const bool second = at.part >= p.split;
     const OuterSide<T>& s = p.side[second];
     const int c0 = (at.part - (second ? p.split : 0)) * W, rank0 = blockIdx.z * (NB * 16);
     const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const float sc = p.scales ? p.scales[t.q] : 1.f;
-    for (int i = threadIdx.x; i < t.cnt; i += 256) {
-        const int row = p.perm[t.start + i];
-        rows[i] = row;
-        fac[i] = (p.gates ? p.gates[row * p.gates_stride] : 1.f) * sc;
+    if (p.chunks != nullptr) {
+        for (int i = threadIdx.x; i < t.cnt; i += 256) rows[i] = p.perm[t.start + i];
+    } else {
+        __shared__ int found[kMaxChunk / 64];
+        unsigned long long m[kMaxChunk / 256];
+#pragma unroll
+        for (int u = 0; u < kMaxChunk / 256; ++u) {
+            const int i = u * 256 + threadIdx.x;
+            m[u] = __ballot(i < p.n && p.ids[(long)min(i, p.n - 1) * p.ids_stride] == t.q);
+            if (lane == 0) found[u * 4 + wave] = __popcll(m[u]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kMaxChunk / 256; ++u) {
+            int place = __popcll(m[u] & ((1ull << lane) - 1));
+            for (int w = 0; w < u * 4 + wave; ++w) place += found[w];
+            if (m[u] >> lane & 1) rows[place] = u * 256 + threadIdx.x;
+        }
+        for (int w = 0; w < kMaxChunk / 64; ++w) t.cnt += found[w];
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.cnt; i += 256) fac[i] = (p.gates ? p.gates[(long)rows[i] * p.gates_stride] : 1.f) * sc;
     __syncthreads();
     f32x4 acc[NB][V];
 #pragma unroll
@@ -925,9 +945,15 @@ __global__ __launch_bounds__(256) void k_outer_merge(OuterArgs<T> p)
 
 // ---- host ----
 
-// Rows up to which every row is its own tile (no sort): its adapter is then read once a
-// row instead of once a tile.
-constexpr long kDirectRows = 128;
+// Whether every row is its own tile, without a sort: the call then has a launch less and reads
+// an adapter once a row instead of once a tile.  us without and with the sort, bf16, d = o:
+//   d = 1,024, rank 16:  256 rows 9, 13;  512 rows 13, 14;  1,024 rows 17, 15
+//   d = 4,096, rank 16:   64 rows 10, 15;  128 rows 14, 15;    256 rows 17, 15
+//   d = 4,096, rank 64:   64 rows 15, 18;  128 rows 24, 19
+bool is_direct(long n, int d, int o, int rp)
+{
+    return n <= kMaxChunk && (size_t)n * rp * ((size_t)d + o) <= (n <= 64 ? size_t(1) << 25 : size_t(1) << 24);
+}
 
 size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 
@@ -991,14 +1017,14 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
 {
     Layout L{};
     L.n = n; L.a = a; L.r = r;
-    L.direct = n <= kDirectRows && !backward;
-    L.split = type == kBF16;
+    L.rp = (r + 15) & ~15;
+    L.direct = is_direct(n, d, o, L.rp);
+    L.split = type == kBF16 && !L.direct;
     L.tile = L.direct ? 1 : tile_rows(n, d < o ? d : o, type);
     L.full_tiles = (n + L.tile - 1) / L.tile;
     L.ntiles = L.direct ? (int)n : (int)(n / L.tile + a + 1);
     L.segments = (int)((n + kPlanRows - 1) / kPlanRows);
     if (L.segments < 1) L.segments = 1;
-    L.rp = (r + 15) & ~15;
     L.chunk = chunk_rows(n, d < o ? d : o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
     L.ld_t = ((n + 63) & ~63l) + 96;  // 64 rows past the last; not a power of two apart
@@ -1013,7 +1039,8 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
         take(L.tiles, (size_t)L.ntiles * sizeof(Tile));
     }
     take(L.part, (size_t)(backward ? L.up_splits : L.down_splits) * n * L.rp * 4);
-    if (backward) {
+    if (backward && L.direct) take(L.low, (size_t)n * r * 4);
+    if (backward && !L.direct) {
         take(L.chunks, (size_t)L.nchunks * sizeof(Tile));
         take(L.merge, (size_t)a * sizeof(int2));
         take(L.low, L.split ? 0 : (size_t)n * r * 4);
@@ -1095,10 +1122,12 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
 {
     const Layout L = layout(a.type, a.n, a.d, a.o, a.r, a.a, true);
     if (a.n == 0 && a.a == 0) return hipSuccess;
-    const hipError_t planned = launch_plan(L, a.ids, a.ids_stride, a.ws, true, s);
-    if (planned != hipSuccess) return planned;
-    const Rows rows{reinterpret_cast<const Tile*>(a.ws + L.tiles), reinterpret_cast<const int*>(a.ws + L.perm), a.ids, a.ids_stride, a.a};
-    const Tile* chunks = reinterpret_cast<const Tile*>(a.ws + L.chunks);
+    if (!L.direct) {
+        const hipError_t e = launch_plan(L, a.ids, a.ids_stride, a.ws, true, s);
+        if (e != hipSuccess) return e;
+    }
+    const Rows rows{L.direct ? nullptr : reinterpret_cast<const Tile*>(a.ws + L.tiles), reinterpret_cast<const int*>(a.ws + L.perm), a.ids, a.ids_stride, a.a};
+    const Tile* chunks = L.direct ? nullptr : reinterpret_cast<const Tile*>(a.ws + L.chunks);
     float* part = reinterpret_cast<float*>(a.ws + L.part);
     float* u = L.split ? nullptr : reinterpret_cast<float*>(a.ws + L.low);
     bf16* u_t = L.split ? reinterpret_cast<bf16*>(a.ws + L.low_t) : nullptr;
@@ -1109,8 +1138,9 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
         using T = decltype(tag);
         if (a.n > 0) {
             const ShrinkArgs<T> sh{rows, (const T*)a.dy, a.ld_dy, (const T*)a.up, a.up_sa, a.up_ld, a.o, a.r, a.n, L.ntiles, L.up_splits, part, L.rp};
-            const ExpandArgs<T> ex{rows, L.ntiles, part_count(L.full_tiles, a.d, a.type), part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld, a.gates, a.gates_stride, a.scales,
-                                   (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t, L.ld_t};
+            const ExpandArgs<T> ex{rows, L.ntiles, part_count(L.full_tiles, a.d, a.type), part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld,
+                                   a.gates, a.gates_stride, a.scales, (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t,
+                                   L.ld_t};
             const hipError_t e = with_tile(L.tile, [&](auto rt) {
                 const hipError_t e = a.a > 0 ? launch_shrink<T, rt.value>(sh, s) : hipSuccess;
                 return e != hipSuccess ? e : launch_expand<T, rt.value, true>(ex, s);
@@ -1119,29 +1149,32 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
         }
         if (a.a == 0) return hipSuccess;
         constexpr int W = 16 * kVec<T>;
-        const OuterArgs<T> ou{chunks, reinterpret_cast<const int2*>(a.ws + L.merge), rows.perm, a.a, a.r, a.gates, a.gates_stride, a.scales,
+        const OuterArgs<T> ou{chunks, reinterpret_cast<const int2*>(a.ws + L.merge), rows.perm, a.a, a.r, a.ids, a.ids_stride, (int)a.n,
+                              a.gates, a.gates_stride, a.scales,
                               {{u, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {a.low, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
                               (a.d + W - 1) / W, (a.d + W - 1) / W + (a.o + W - 1) / W};
-        if constexpr (std::is_same_v<T, bf16>) {
-            const OuterSplitArgs os{chunks, rows.perm, a.r, L.ld_t,
-                                    {{u_t, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {t_t, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
-                                    (a.d + 511) / 512, (a.d + 511) / 512 + (a.o + 511) / 512};
-            const unsigned grid = (unsigned)(L.nchunks * os.parts);
-            if (a.r <= 16)
-                SKM_TRY_LAUNCH(k_outer_split<1>, dim3(grid), 256, 0, s, os);
-            else if (a.r <= 32)
-                SKM_TRY_LAUNCH(k_outer_split<2>, dim3(grid), 256, 0, s, os);
-            else
-                SKM_TRY_LAUNCH(k_outer_split<4>, dim3(grid, 1, (a.r + 63) / 64), 256, 0, s, os);
+        if (L.split) {
+            if constexpr (std::is_same_v<T, bf16>) {
+                const OuterSplitArgs os{chunks, rows.perm, a.r, L.ld_t,
+                                        {{u_t, (const T*)a.x, a.ld_x, a.d, (T*)a.ddown, dpart}, {t_t, (const T*)a.dy, a.ld_dy, a.o, (T*)a.dup, upart}},
+                                        (a.d + 511) / 512, (a.d + 511) / 512 + (a.o + 511) / 512};
+                const unsigned grid = (unsigned)(L.nchunks * os.parts);
+                if (a.r <= 16)
+                    SKM_TRY_LAUNCH(k_outer_split<1>, dim3(grid), 256, 0, s, os);
+                else if (a.r <= 32)
+                    SKM_TRY_LAUNCH(k_outer_split<2>, dim3(grid), 256, 0, s, os);
+                else
+                    SKM_TRY_LAUNCH(k_outer_split<4>, dim3(grid, 1, (a.r + 63) / 64), 256, 0, s, os);
+            }
         } else {
-            const unsigned grid = (unsigned)(L.nchunks * ou.parts);
+            const unsigned grid = (unsigned)((L.direct ? a.a : L.nchunks) * ou.parts);
             if (a.r <= 16)
                 SKM_TRY_LAUNCH((k_outer<T, 1>), dim3(grid), 256, 2 * 16 * W * 4, s, ou);
             else
                 SKM_TRY_LAUNCH((k_outer<T, 2>), dim3(grid, 1, (a.r + 31) / 32), 256, 2 * 32 * W * 4, s, ou);
         }
+        if (L.direct || L.n <= L.chunk) return hipSuccess;  // one chunk an adapter
         const long most = (long)a.r * (a.d > a.o ? a.d : a.o);
-        if (L.n <= L.chunk) return hipSuccess;  // one chunk an adapter
         const bool vec = ((long)a.r * a.d % 4 == 0) && ((long)a.r * a.o % 4 == 0);
         const long blocks = (most / (vec ? 4 : 1) + 255) / 256;
         const dim3 grid((unsigned)(blocks < 256 ? blocks : 256), 2, a.a < 8 ? a.a : 8);

@@ -271,6 +271,15 @@ def test_adapt(experts, n, d, o, r, a, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,o,r,a", [(600, 200, 136, 128, 3), (1200, 1032, 520, 40, 6), (17000, 24, 16, 4, 9), (3000, 40, 48, 70, 2048), (33000, 16, 8, 16, 30),
+                                       (512, 64, 64, 16, 5), (900, 4096, 40, 64, 2), (5000, 72, 520, 33, 4)])
+def test_adapt_sorted_rows(experts, n, d, o, r, a, dtype):
+    """Calls that sort their rows: several segments, chunks of an adapter, every size of tile."""
+    print("adapt", n, d, o, r, a, dtype, flush=True)
+    check_adapt(experts, problem(n, d, o, r, a, dtype, n + d), dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("law", ["runs", "one", "none", "wild"])
 @pytest.mark.parametrize("n,d,o,r,a", [(40, 72, 48, 6, 4), (700, 160, 64, 16, 5), (1500, 65, 33, 9, 90)])
 def test_adapt_ids(experts, n, d, o, r, a, law, dtype):
