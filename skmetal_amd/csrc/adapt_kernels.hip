@@ -918,28 +918,44 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_outer_merge(OuterArgs<T> p)
 {
     constexpr int N = VEC ? 4 : 1;
+    __shared__ int4 some[256];  // adapter, first slot, chunks
+    __shared__ int found[4];
     const OuterSide<T>& s = p.side[blockIdx.y];
     const long size = (long)p.r * s.w;
-    int nth = 0;
-    for (int q = 0; q < p.a; ++q) {
-        const int2 m = p.merge[q];
-        if (m.y == 0 || nth++ % (int)gridDim.z != (int)blockIdx.z) continue;
-        const float* part = s.part + m.x * size;
-        for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * N; i < size; i += (long)gridDim.x * 256 * N) {
-            float v[N] = {};
-            for (int k = 0; k < m.y; k += 8) {
-                float x[8][N];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) __builtin_memcpy(x[u], part + min(k + u, m.y - 1) * size + i, 4 * N);
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) v[e] += k + u < m.y ? x[u][e] : 0.f;
-            }
-            T* o = s.dM + q * size + i;
-#pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = from_f<T>(v[e]);
+    const int lane = threadIdx.x & 63, wave = wave_index();
+    for (int q0 = 0; q0 < p.a; q0 += 256) {
+        const int q = q0 + threadIdx.x;
+        const int2 m = q < p.a ? p.merge[q] : make_int2(0, 0);
+        const unsigned long long several = __ballot(m.y != 0);
+        if (lane == 0) found[wave] = __popcll(several);
+        __syncthreads();
+        int at = __popcll(several & ((1ull << lane) - 1)), count = 0;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) at += found[w];
+            count += found[w];
         }
+        if (m.y != 0) some[at] = make_int4(q, m.x, m.y, 0);
+        __syncthreads();
+        for (int j = blockIdx.z; j < count; j += gridDim.z) {
+            const int4 m = some[j];
+            const float* part = s.part + m.y * size;
+            T* out = s.dM + m.x * size;
+            for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * N; i < size; i += (long)gridDim.x * 256 * N) {
+                float v[N] = {};
+                for (int k = 0; k < m.z; k += 8) {
+                    float x[8][N];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) __builtin_memcpy(x[u], part + min(k + u, m.z - 1) * size + i, 4 * N);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) v[e] += k + u < m.z ? x[u][e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) out[i + e] = from_f<T>(v[e]);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -1003,13 +1019,13 @@ int part_count(long tiles, int w, int type)
     return (int)(want < 1 ? 1 : want > most ? most : want);
 }
 
-// Rows a k_outer block sums up: as many as leave about two blocks a CU, for every cut
-// costs a partial matrix written and read.
+// Rows a k_outer block sums up: as many as leave a block a CU (k_outer_split) or two (k_outer,
+// whose waves share a chunk), for every cut costs a partial matrix written and read.
 int chunk_rows(long n, int w, int a, int type)
 {
-    const int cols = type == kBF16 ? 512 : 16 * (16 / (int)elem_size(type));
+    const int cols = type == kBF16 ? 512 : 16 * (16 / (int)elem_size(type)), blocks = type == kBF16 ? 256 : 512;
     int c = kMaxChunk;
-    while (c > 64 && (n / c + (a < n / c ? a : n / c)) * 2 * ((w + cols - 1) / cols) < 512) c /= 2;
+    while (c > 64 && (n / c + (a < n / c ? a : n / c)) * 2 * ((w + cols - 1) / cols) < blocks) c /= 2;
     return c;
 }
 
