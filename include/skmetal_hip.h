@@ -340,6 +340,9 @@ SKMETAL_API int skmetal_hip_lloyd_inertia(skmetal_hip_lloyd* h, double* out);
 #define SKMETAL_BF16 1
 #define SKMETAL_F16 2
 
+/* The device that skmetal_init set the library up on, -1 before. */
+SKMETAL_API int skmetal_hip_device(void);
+
 /* Top-k routing with the balance loss.  logits [n x E]; mask (nullable, one
  * byte a row, mask_stride bytes apart): rows that count.  E <= 2048, 1 <= k <=
  * min(E, 16), n < 2^31.  A score of -inf or NaN is excluded.

@@ -103,6 +103,7 @@ _REGISTRY = [
      ctypes.POINTER(ctypes.c_int)),
     ("skmetal_hip_kmeans_batch_fused_noalloc", ctypes.c_int, _vp, _vp, _vp, _c_size, _c_size, _c_size, _c_size,
      ctypes.c_float, ctypes.POINTER(ctypes.c_int32)),
+    ("skmetal_hip_device", _int),
     ("skmetal_hip_route_workspace", _c_size, _c_size, _c_size),
     ("skmetal_hip_route", _int, _int, _vp, _c_size, _vp, _c_size, _c_size, _c_size, _c_size, _int, _vp, _vp, _vp, _vp,
      _vp, _vp, _vp, _c_size, _vp),

@@ -1110,6 +1110,16 @@ hipError_t with_tile(int tile, F&& f)
 
 }  // namespace
 
+bool adapt_fits(int type, long n, int d, int o, int r, int a)
+{
+    const Layout L = layout(type, n, d, o, r, a, true);
+    const size_t tiles = ((size_t)L.full_tiles + a + 8) * (size_t)(L.down_splits > L.up_splits ? L.down_splits : L.up_splits);
+    const size_t wide = ((size_t)L.full_tiles + a + 8) * (size_t)(part_count(L.full_tiles, d, type) > part_count(L.full_tiles, o, type) ? part_count(L.full_tiles, d, type) : part_count(L.full_tiles, o, type));
+    const size_t cols = 16 * (16 / elem_size(type)), chunks = (L.direct ? (size_t)a : (size_t)n / L.chunk + a) * ((d + cols - 1) / cols + (o + cols - 1) / cols);
+    const size_t most = size_t(1) << 24;  // blocks of 256 threads in a grid that has less than 2^32 threads
+    return tiles < most && wide < most && chunks < most && L.segments < 65536;
+}
+
 size_t adapt_workspace(int type, long n, int d, int o, int r, int a, int backward) { return layout(type, n, d, o, r, a, backward != 0).bytes; }
 
 hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)

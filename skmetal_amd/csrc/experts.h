@@ -79,5 +79,7 @@ struct AdaptBackArgs {
 };
 hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s);
 size_t adapt_workspace(int type, long n, int d, int o, int r, int a, int backward);
+// Whether every launch of both directions has a grid that the device takes.
+bool adapt_fits(int type, long n, int d, int o, int r, int a);
 
 }  // namespace skm

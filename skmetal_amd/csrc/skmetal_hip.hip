@@ -2189,6 +2189,8 @@ int check_adapt(int dtype, const AdaptSizes& z, std::initializer_list<size_t> st
         return fail(SKMETAL_ERANGE, "n=%zu, a=%zu, d=%zu or o=%zu exceeds the supported range", z.n, z.a, z.d, z.o);
     for (const size_t s : strides)
         if (s > kMaxStride) return fail(SKMETAL_ERANGE, "a stride of %zu elements exceeds the supported range", s);
+    if (!adapt_fits(dtype, (long)z.n, (int)z.d, (int)z.o, (int)z.r, (int)z.a))
+        return fail(SKMETAL_ERANGE, "n=%zu, d=%zu, o=%zu: more blocks than a launch takes", z.n, z.d, z.o);
     return 0;
 }
 
@@ -2202,6 +2204,8 @@ int launched(hipError_t e, const char* what)
 }  // namespace
 
 extern "C" {
+
+int skmetal_hip_device(void) { return ctx().ready ? ctx().dev : -1; }
 
 size_t skmetal_hip_route_workspace(size_t n, size_t E)
 {

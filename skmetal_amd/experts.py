@@ -63,6 +63,11 @@ def _lib():
     return _bridge._lib
 
 
+@functools.lru_cache(maxsize=1)
+def _device_index():
+    return _lib().skmetal_hip_device()
+
+
 def _fail(name):
     raise RuntimeError(f"{name} failed: {_bridge.last_error()}")
 
@@ -109,7 +114,10 @@ def _first(t, name):
         raise ValueError(f"{name} is on {t.device}, expected the GPU")
     if t.dim() != 2:
         raise ValueError(f"{name} has {t.dim()} dimensions, expected 2")
-    return code, t.device
+    device = t.device
+    if device.index != _device_index():
+        raise ValueError(f"{name} is on {device}, the library was set up on device {_device_index()}")
+    return code, device
 
 
 def _mask(mask, n, device):
@@ -296,8 +304,8 @@ class _Routed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, mask, normalize):
         r = route(logits, top_k, mask=mask, normalize=normalize)
-        ctx.save_for_backward(logits, r.weights, r.experts, r.counts, r.prob_sums, r.rows)
-        ctx.mask, ctx.normalize = mask, normalize
+        ctx.save_for_backward(logits, mask, r.weights, r.experts, r.counts, r.prob_sums, r.rows)
+        ctx.normalize = normalize
         ctx.mark_non_differentiable(r.experts, r.counts, r.prob_sums, r.rows)
         ctx.set_materialize_grads(False)
         return tuple(r)
@@ -305,9 +313,9 @@ class _Routed(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_weights, _experts, _counts, _sums, _rows, grad_loss):
-        logits, *saved = ctx.saved_tensors
+        logits, mask, *saved = ctx.saved_tensors
         grad = route_backward(logits, Routing(*saved, None), grad_weights=None if grad_weights is None else grad_weights.contiguous(), grad_loss=grad_loss,
-                              mask=ctx.mask, normalize=ctx.normalize)
+                              mask=mask, normalize=ctx.normalize)
         return grad, None, None, None
 
 

@@ -89,7 +89,7 @@ def _route(lib, dtype=1, z=P, ld=64, mask=None, n=8, e=64, k=2, w=P, ex=P, c=P, 
     (dict(dtype=3), EINVAL, "dtype"), (dict(k=0), EINVAL, "k=0"), (dict(k=65), EINVAL, "k=65"), (dict(e=0, k=0), EINVAL, "E=0"),
     (dict(e=4096, k=2), ERANGE, "E=4096"), (dict(k=17), ERANGE, "k=17"), (dict(n=1 << 31), ERANGE, "n="), (dict(ld=1 << 50), ERANGE, "stride"),
     (dict(z=None), EINVAL, "null"), (dict(w=None), EINVAL, "null"), (dict(loss=None), EINVAL, "null"), (dict(z=P + 1), EINVAL, "aligned"),
-    (dict(size=16), EINVAL, "workspace"), (dict(ws=None), EINVAL, "workspace"), (dict(ws=P + 4), EINVAL, "aligned"),
+    (dict(n=100_000, size=16), EINVAL, "workspace"), (dict(n=100_000, ws=None), EINVAL, "workspace"), (dict(n=100_000, ws=P + 4), EINVAL, "aligned"),
 ])
 def test_route_refuses(lib, bad, code, says):
     assert _route(lib, **bad) == code
@@ -103,7 +103,7 @@ def _adapt(lib, dtype=1, x=P, down=P, up=P, ids=P, base=P, out=P, ld_out=64, n=8
 @pytest.mark.parametrize("bad,code,says", [
     (dict(dtype=-1), EINVAL, "dtype"), (dict(r=0), EINVAL, "r=0"), (dict(d=0), EINVAL, "d=0"), (dict(r=129), ERANGE, "r=129"), (dict(a=65536), ERANGE, "a=65536"),
     (dict(n=1 << 31), ERANGE, "n="), (dict(x=None), EINVAL, "null"), (dict(up=None), EINVAL, "null"), (dict(ids=None), EINVAL, "null"),
-    (dict(out=P + 1), EINVAL, "aligned"), (dict(ld_out=63), EINVAL, "overlap"),
+    (dict(out=P + 1), EINVAL, "aligned"), (dict(ld_out=63), EINVAL, "overlap"), (dict(n=1 << 29, d=1 << 20), ERANGE, "blocks"),
 ])
 def test_adapt_refuses(lib, bad, code, says):
     assert _adapt(lib, **bad) == code

@@ -493,3 +493,48 @@ def test_python_refusals(experts):
         experts.adapt(z, A, B, ids, out=torch.zeros(6, device="cuda").expand(4, 6))
     with pytest.raises(ValueError, match="low"):
         experts.adapt_backward(torch.zeros(4, 6, device="cuda"), z, A, B, ids, torch.zeros(4, 2, device="cuda"))
+
+
+def test_cluster_experts_example(experts):
+    """The whole path: a KMeans fit's centres as router, training steps, served rows.  The
+    fit brings the loss down, and a served row is the training pass's own (bf16: the same
+    products in another split of the sums, a few roundings of 2^-8)."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "cluster_experts.py"
+    spec = importlib.util.spec_from_file_location("cluster_experts", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, net, x = example.main(["--rows", "3000", "--width", "64", "--experts", "8", "--steps", "40"])
+    assert losses[-1] < 0.7 * losses[0]
+    with torch.no_grad():
+        y, _ = net(x)
+    for n in (1, 5, 200):
+        off = (net.serve(x[:n]).float() - y[:n].float()).abs()
+        assert float(off.max()) <= 4 * 2.0**-8 * float(y.float().abs().max())
+
+
+def test_labels_are_adapter_ids(experts):
+    """A cluster's rows through its adapter: KMeans labels as they come."""
+    from sklearn.cluster import KMeans
+
+    import skmetal_amd
+
+    s = problem(1500, 24, 32, 4, 5, "fp32", 4)
+    model = skmetal_amd.accelerate(KMeans(n_clusters=5, n_init=1, random_state=0)).fit(s["x"].cpu().numpy())
+    assert model.labels_.dtype == np.int32
+    s["ids"] = torch.from_numpy(model.labels_).cuda()
+    check_adapt(experts, s, "fp32")
+
+
+def test_sizes_around_the_kernels_choices(experts):
+    """Rows around the steps from one block to several (route) and from no sort to a sort."""
+    for n in (127, 128, 129, 1023, 1025):
+        check_route(experts, scores(n, 200, "normal", torch.bfloat16, n).cuda(), 4, None, True, torch.bfloat16, torch.ones(n, 4, device="cuda"), None)
+    for e in (8, 9, 32, 33, 64, 65, 256, 257, 512, 513, 1024):
+        check_route(experts, scores(40, e, "ties", torch.float16, e).cuda(), min(e, 8), None, False, torch.float16, None, torch.tensor(1.0, device="cuda"))
+    for n in (511, 512, 513):
+        check_adapt(experts, problem(n, 64, 64, 16, 5, "bf16", n), "bf16")
+    for n in (64, 65):  # 2^25 and 2^24 products
+        check_adapt(experts, problem(n, 4096, 4096, 64, 3, "bf16", n), "bf16")
