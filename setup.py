@@ -50,6 +50,7 @@ setup(
     package_data={"skmetal_amd": ["libskmetal_hip.so", "csrc/*.hip", "csrc/*.h"]},
     python_requires=">=3.10",
     install_requires=["numpy", "scikit-learn"],
+    extras_require={"experts": ["torch"]},  # a ROCm build
     cmdclass={"build_py": BuildWithHip},
     distclass=BinaryDistribution,
     zip_safe=False,

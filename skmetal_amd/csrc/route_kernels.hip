@@ -163,7 +163,13 @@ __device__ __forceinline__ void load_row(const void* z, long ld, const uint8_t* 
 // The blocks' sums and counts (or the only block's) become the results.
 __device__ __forceinline__ float balance_loss(double dot, int E, int k, int rows) { return rows > 0 ? (float)(dot * E / ((double)k * rows * rows)) : 0.f; }
 
-// ONE: a single block, a wave a group of rows.
+// The choice: every lane sorts its scores eight (or k) at a time by a bitonic network and merges
+// the lists, keeping the k largest; the row's lanes then merge theirs log2(L) times.  The
+// largest is the softmax's maximum, so the scores are decoded once, and their values stay in
+// registers for the exponentials and the column sums, which a wave keeps over all its rows.
+// At 131,072 x 256 bf16, k = 8, 40 us (67 MB: 13 us to read): some 900 vector instructions for
+// a wave's 8 rows bound it, about 400 of them the choice's.  ONE: a single block, a wave a
+// group of rows; 96 x 256, k = 8 takes 12 us, its instructions' first fetch most of it.
 template <typename T, int L, int NC, int KP, bool ONE>
 __global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArgs a, int nb, float* psum, int* pcnt, int* prow, unsigned* ticket)
 {
@@ -339,7 +345,8 @@ __global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArg
 }
 
 // The blocks' sums and counts added, 16 columns a block, always in the same order; the last
-// block to finish adds up the loss.
+// block to finish adds up the loss.  10 us for 768 blocks' 256 columns, 6 for 64: the chain of
+// loads, tree and counter.
 constexpr int kTotalThreads = 1024;
 __global__ __launch_bounds__(kTotalThreads) void k_route_total(RouteArgs a, int nb, const float* psum, const int* pcnt, const int* prow, double* dots,
                                                                unsigned* ticket)
@@ -404,7 +411,9 @@ __global__ __launch_bounds__(kTotalThreads) void k_route_total(RouteArgs a, int 
 
 // dz_ij = p_ij (G_j - sum_j p_ij G_j) + the chosen ones' gate part, with G_j = dloss E c_j / (k N^2).
 // The gate part of a chosen score is w (dw - sum w dw) for normalized weights; otherwise w dw,
-// and sum w dw joins the sum over the row.  It reaches its column through LDS.
+// and sum w dw joins the sum over the row.  It reaches its column through LDS.  Probabilities are
+// computed anew from the scores, which costs less than keeping them would.  At 131,072 x 256
+// bf16 37 us (134 MB, 3.7 TB/s).
 template <typename T, int L, int NC>
 __global__ __launch_bounds__(kThreads) void k_route_back(RouteBackArgs a, int nb)
 {
