@@ -1014,11 +1014,12 @@ int stretches(int w, int type)
     return (w + columns - 1) / columns;
 }
 
-// Rows a tile: as many as leave about three blocks a CU, for each reads its adapter anew.
-int tile_rows(long n, int w, int type)
+// Rows a tile: as many as leave about three blocks a CU on the average of both widths, for each
+// tile reads its adapter anew.
+int tile_rows(long n, int d, int o, int type)
 {
     int t = 64;
-    while (t > 16 && (n + t - 1) / t * stretches(w, type) < 768) t /= 2;
+    while (t > 16 && (n + t - 1) / t * (stretches(d, type) + stretches(o, type)) < 2 * 768) t /= 2;
     return t;
 }
 
@@ -1032,11 +1033,12 @@ int part_count(long tiles, int w, int type)
 
 // Rows a k_outer block sums up: as many as leave a block a CU (k_outer_split) or two (k_outer,
 // whose waves share a chunk), for every cut costs a partial matrix written and read.
-int chunk_rows(long n, int w, int a, int type)
+int chunk_rows(long n, int d, int o, int a, int type)
 {
     const int cols = type == kBF16 ? 512 : 16 * (16 / (int)elem_size(type)), blocks = type == kBF16 ? 256 : 512;
+    const long parts = (d + cols - 1) / cols + (o + cols - 1) / cols;
     int c = kMaxChunk;
-    while (c > 64 && (n / c + (a < n / c ? a : n / c)) * 2 * ((w + cols - 1) / cols) < blocks) c /= 2;
+    while (c > 64 && (n / c + (a < n / c ? a : n / c)) * parts < blocks) c /= 2;
     return c;
 }
 
@@ -1047,12 +1049,12 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     L.rp = (r + 15) & ~15;
     L.direct = is_direct(n, d, o, L.rp);
     L.split = type == kBF16 && !L.direct;
-    L.tile = L.direct ? 1 : tile_rows(n, d < o ? d : o, type);
+    L.tile = L.direct ? 1 : tile_rows(n, d, o, type);
     L.full_tiles = (n + L.tile - 1) / L.tile;
     L.ntiles = L.direct ? (int)n : (int)(n / L.tile + a + 1);
     L.segments = (int)((n + kPlanRows - 1) / kPlanRows);
     if (L.segments < 1) L.segments = 1;
-    L.chunk = chunk_rows(n, d < o ? d : o, a, type);
+    L.chunk = chunk_rows(n, d, o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
     L.ld_t = ((n + 63) & ~63l) + 96;  // 64 rows past the last; not a power of two apart
     const int zs = (r + 63) / 64;

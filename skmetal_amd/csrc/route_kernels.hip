@@ -9,7 +9,7 @@
 // A score of -inf or NaN is excluded: probability 0, never taken.  A row that is masked
 // or has no score left takes no expert (-1, weight 0) and counts nowhere.
 //
-// One pass over the scores each way.  A row lies on L lanes, NC times eight columns a
+// One pass over the scores each way.  A row lies on L lanes (1, 8, 16 or 64), NC times eight columns a
 // lane (column = (c L + lane) 8 + e), so a wave takes 64 / L rows at once and a row's sums
 // and its choice need log2(L) exchanges.
 #include "experts_common.h"
@@ -151,6 +151,8 @@ __device__ __forceinline__ void load_row(const void* z, long ld, const uint8_t* 
     for (int c = 0; c < NC; ++c) {
         const int col = c * L * 8;
         if (col + L * 8 <= E) {
+            __builtin_memcpy(raw[c], p + col, 8 * sizeof(T));
+        } else if (col + j + 8 <= E) {
             __builtin_memcpy(raw[c], p + col, 8 * sizeof(T));
         } else if (col < E) {  // the columns past the row as NaN (excluded)
 #pragma unroll
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(kThreads) void k_route_back(RouteBackArgs a, int nb
 #pragma unroll
             for (int e = 0; e < 8; ++e) out[e] = from_f<T>(x[c][e] * inv * (G[c][e] - g) + gt[e]);
             if (row < a.n) {
-                if ((c + 1) * L * 8 <= a.E)
+                if ((c + 1) * L * 8 <= a.E || col + 8 <= a.E)
                     __builtin_memcpy(dz + col, out, 8 * sizeof(T));
                 else
 #pragma unroll
@@ -525,9 +527,10 @@ __global__ __launch_bounds__(kThreads) void k_route_back(RouteBackArgs a, int nb
     }
 }
 
-// Lanes a row takes: one up to 32 experts (no exchanges at all), eight up to 256, a wave
-// beyond.
-int row_lanes(int E) { return E <= 32 ? 1 : E <= 256 ? 8 : 64; }
+// Lanes a row takes: as few as hold it in 32 scores each (one: no exchanges at all), for every
+// doubling costs an exchange of the k chosen.  65,536 x 500 fp32, k = 5 take 76 us on sixteen
+// lanes, 133 on a wave.
+int row_lanes(int E) { return E <= 32 ? 1 : E <= 256 ? 8 : E <= 512 ? 16 : 64; }
 
 int route_blocks(long n, int E)
 {
@@ -563,9 +566,8 @@ hipError_t with_shape(int E, F&& f)
     case 8:
         if (E <= 64) return f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
         return f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-    default:
-        if (E <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-        return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    case 16: return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    default: return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
     }
 }
 
