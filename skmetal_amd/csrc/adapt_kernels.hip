@@ -13,7 +13,8 @@
 // Three products in all: rows to ranks (k_shrink: t, u), ranks to rows (k_expand: out, dx)
 // and rows by rows (k_outer: dD, dU).  k_plan first puts the rows of each adapter side by
 // side (a stable counting sort) and cuts them into tiles of one adapter; with few rows
-// every row is its own tile and there is no sort.
+// every row is its own tile and there is no sort; where they are small besides, the first two
+// products are one launch (k_direct).
 #include "experts_common.h"
 
 namespace skm {
@@ -509,6 +510,49 @@ __device__ __forceinline__ void fetch_base(const ExpandArgs<T>& p, const Quad& q
     }
 }
 
+// A wave's M_q and first 16 rows' base of the 16 * kVec columns from c0 on.  A lane brings kVec
+// columns of eight ranks at a time: for bf16 g * 8 .. + 7 of every 32 (of the 16, where there
+// are no more), else g * 4 .. + 3 of every 16, two such.
+template <typename T, int KP>
+__device__ __forceinline__ void fetch_stretch(const ExpandArgs<T>& p, int q, bool has, const Quad& rows, int c0, Vec<T> (*m)[8], Vec<T>* y)
+{
+    constexpr int V = kVec<T>;
+    if (c0 >= p.w) return;
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = c0 + (lane & 15) * V;
+    const bool full = c0 + 16 * V <= p.w;
+    if (has) {
+#pragma unroll
+        for (int b = 0; b < (KP + 31) / 32; ++b) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int rank = std::is_same_v<T, bf16> ? (KP == 16 ? (g & 1) * 8 + e : b * 32 + g * 8 + e) : b * 32 + e / 4 * 16 + g * 4 + e % 4;
+                const T* from = p.M + q * p.sa + (long)min(rank, p.r - 1) * p.ld + c;
+                m[b][e] = full ? load16(from) : load_part(from, p.w - c);
+                if (rank >= p.r) m[b][e] = Vec<T>{};
+            }
+        }
+    }
+    if (full)
+        fetch_base<T, true>(p, rows, c, y);
+    else
+        fetch_base<T, false>(p, rows, c, y);
+}
+
+// M_q's ranks as the matrix cores want them.
+template <typename T, int KP>
+__device__ __forceinline__ void turn_ranks(Vec<T> (*m)[8])
+{
+    if constexpr (std::is_same_v<T, bf16>) {
+#pragma unroll
+        for (int b = 0; b < (KP + 31) / 32; ++b) {
+            Vec<T> x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = m[b][e];
+            transpose8(x, m[b]);
+        }
+    }
+}
+
 // The wave's rows and columns of a tile: out = base + L M, with the first 16 rows' base in
 // y[0].  A lane ends up with kVec columns (from c on) of four rows.
 //
@@ -608,56 +652,23 @@ __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand
     Quad row0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) row0.row[e] = row_at(p.rows, t.start + min(g * 4 + e, t.cnt - 1));
-    // eight ranks of kVec columns: bf16: g * 8 .. + 7 of every 32 (of 16, for half as many
-    // ranks); else g * 4 .. + 3 of every 16, two such
     constexpr int NM = (KP + 31) / 32;
     Vec<T> m[NM][8], y[2][4];
-    auto fetch = [&](int c0) {  // M and the first base of a stretch
-        if (c0 >= p.w) return;
-        const bool full = c0 + 16 * V <= p.w;
-        if (has) {
-            const int cm = c0 + l16 * V;
-#pragma unroll
-            for (int b = 0; b < NM; ++b) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int rank = Low::kSplit ? (KP == 16 ? (g & 1) * 8 + e : b * 32 + g * 8 + e) : b * 32 + e / 4 * 16 + g * 4 + e % 4;
-                    const T* from = p.M + t.q * p.sa + (long)min(rank, p.r - 1) * p.ld + cm;
-                    m[b][e] = full ? load16(from) : load_part(from, p.w - cm);
-                    if (rank >= p.r) m[b][e] = Vec<T>{};
-                }
-            }
-        }
-        if (full)
-            fetch_base<T, true>(p, row0, c0 + l16 * V, y[0]);
-        else
-            fetch_base<T, false>(p, row0, c0 + l16 * V, y[0]);
-    };
     int c0 = (at.part * 4 + wave) * 16 * V;
-    fetch(c0);
+    fetch_stretch<T, KP>(p, t.q, has, row0, c0, m, y[0]);
     const bool first = at.part == 0;
     stage_rows<T, RT>(p, t, has, sc, R);
     stage_low<T, RT, KP>(p, t, has, sc, L, R, first ? p.low : nullptr, BACK && first ? p.dgates : nullptr);
     __syncthreads();
     if (BACK && Low::kSplit && first && has && p.low_t != nullptr) store_by_rank<T, RT, KP>(p, t, L, p.low_t);
     while (c0 < p.w) {
-        if constexpr (Low::kSplit) {
-            if (has) {
-#pragma unroll
-                for (int b = 0; b < NM; ++b) {
-                    Vec<T> x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = m[b][e];
-                    transpose8(x, m[b]);
-                }
-            }
-        }
+        if (has) turn_ranks<T, KP>(m);
         if (c0 + 16 * V <= p.w)
             expand_columns<T, RT, KP, true>(p, t, m, L, R, y, c0 + l16 * V, has);
         else
             expand_columns<T, RT, KP, false>(p, t, m, L, R, y, c0 + l16 * V, has);
         c0 += p.parts * 64 * V;
-        fetch(c0);
+        fetch_stretch<T, KP>(p, t.q, has, row0, c0, m, y[0]);
     }
     if (BACK && Low::kSplit && has && p.dot_t != nullptr && at.part == p.parts - 1) {
         __syncthreads();
@@ -665,6 +676,105 @@ __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand
         __syncthreads();
         store_by_rank<T, RT, KP>(p, t, L, p.dot_t);
     }
+}
+
+// One row a block (and 128 * kVec of its columns): both products at once, low_row computed
+// anew by every block of the row.  Eight waves share its columns, several steps in flight.
+// One bf16 row of 1,024, rank 8, takes 6.4 us launch after launch (two kernels: 6.7), 64 of them
+// 6.7 (7.6): the launch and the three trips to memory, one after another, bound it.
+constexpr int kDirectThreads = 512;
+template <typename T, int KP, bool BACK>
+__global__ __launch_bounds__(kDirectThreads) void k_direct(ExpandArgs<T> p, const T* v, long ld_v, const T* D, long sa, long ld, int w)
+{
+    constexpr int V = kVec<T>, NB = KP / 16, KS = 128 / sizeof(T), W = kDirectThreads / 64, U = NB == 1 ? 4 : NB == 2 ? 2 : 1;
+    __shared__ __align__(16) LowTile<T, 1, KP> L;
+    __shared__ TileRows<1> R;
+    __shared__ __align__(16) float sum[W][KP];
+    const int i = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    const Tile t{adapter_of(p.rows.ids, p.rows.ids_stride, i, p.rows.a), i, 1, -1};
+    const bool has = t.q < p.rows.a;
+    const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
+    const float sc = has && p.scales ? p.scales[t.q] : 1.f;
+    if (threadIdx.x < 16) {
+        R.row[threadIdx.x] = i;
+        R.f[threadIdx.x] = has ? (p.gates ? p.gates[i * p.gates_stride] : 1.f) * sc : 0.f;
+    }
+    Vec<T> m[(KP + 31) / 32][8], y[2][4];
+    const int c0 = (part * W + wave) * 16 * V;
+    fetch_stretch<T, KP>(p, t.q, has, Quad{{i, i, i, i}}, c0, m, y[0]);
+    if (has) {
+        const T* x = v + i * ld_v + g * V;
+        const T* d[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) d[b] = D + t.q * sa + (long)min(b * 16 + l16, p.r - 1) * ld + g * V;
+        f32x4 acc[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int steps = (w + KS - 1) / KS, full = w / KS;
+        for (int k = wave; k < steps; k += W * U) {
+            Vec<T> a[U][2], b[U][NB][2];
+            if (k + (U - 1) * W < full) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int at = (k + u * W) * KS + h * (KS / 2);
+                        a[u][h] = load16(x + at);
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) b[u][n][h] = load16(d[n] + at);
+                    }
+            } else {  // the steps past the row, and the last one's columns past it, as 0
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int at = (k + u * W) * KS + h * (KS / 2), left = w - at - g * V;
+                        a[u][h] = load_part(x + at, left);
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) b[u][n][h] = load_part(d[n] + at, left);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) acc[n] = mfma16(a[u][h], b[u][n][h], acc[n]);
+        }
+        if (g == 0)  // all sixteen rows of the product are this row
+#pragma unroll
+            for (int b = 0; b < NB; ++b) sum[wave][b * 16 + l16] = acc[b][0];
+    }
+    __syncthreads();
+    if (threadIdx.x < KP / 4) {
+        const int k = threadIdx.x * 4;
+        f32x4 s{0.f, 0.f, 0.f, 0.f};
+        if (has)
+#pragma unroll
+            for (int u = 0; u < W; ++u) s += *reinterpret_cast<const f32x4*>(&sum[u][k]);
+        float dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (k + e >= p.r) s[e] = 0.f;
+            if (part == 0 && k + e < p.r) {
+                if (p.low != nullptr) p.low[(long)i * p.r + k + e] = s[e];
+                if (BACK && p.dgates != nullptr && has) dot += s[e] * p.dot[(long)i * p.r + k + e];
+            }
+        }
+        L.set(0, k, s * R.f[0]);
+        if (BACK && part == 0 && p.dgates != nullptr) {
+#pragma unroll
+            for (int off = 1; off < KP / 4; off <<= 1) dot += __shfl_xor(dot, off, 64);
+            if (threadIdx.x == 0) p.dgates[i] = has ? dot * sc : 0.f;
+        }
+    }
+    __syncthreads();
+    if (c0 >= p.w) return;
+    if (has) turn_ranks<T, KP>(m);
+    if (c0 + 16 * V <= p.w)
+        expand_columns<T, 1, KP, true>(p, t, m, L, R, y, c0 + l16 * V, has);
+    else
+        expand_columns<T, 1, KP, false>(p, t, m, L, R, y, c0 + l16 * V, has);
 }
 
 // ---- rows by rows ----
@@ -982,11 +1092,25 @@ bool is_direct(long n, int d, int o, int rp)
     return n <= kMaxChunk && (size_t)n * rp * ((size_t)d + o) <= (n <= 64 ? size_t(1) << 25 : size_t(1) << 24);
 }
 
+// Whether such a call's two products are one launch, every block of a row computing its
+// low-rank vector anew: where that reads little, 32 MiB of M in all and 128 KiB a block (64 KiB
+// in fp32, whose matrix instructions take four times as long for it).  Launch after launch, d = o,
+// two kernels and one, bf16: 1 row of 256, rank 64: 8.7 and 4.9 us; 64 of 1,024, rank 8: 7.6 and
+// 6.7; rank 64: 10.9 and 9.2; 64 of 4,096, rank 8: 9.4 and 7.5; fp32: 64 of 1,024, rank 8: 7.7 and
+// 6.3.  Beyond, bf16: 1 of 4,096, rank 64: 10.9 and 20.1; 128 of 4,096, rank 8: 12.9 and 14.4;
+// fp32: 1 of 1,024, rank 32: 8.1 and 8.9.
+bool is_fused(long n, int d, int o, int rp, int type)
+{
+    const size_t wide = d > o ? d : o, es = elem_size(type), cols = kDirectThreads / 4 * (16 / es);  // columns a block
+    const size_t row = rp * wide * es;
+    return rp <= 64 && row <= (size_t(type == kF32 ? 64 : 128) << 10) && n * ((wide + cols - 1) / cols) * row <= size_t(32) << 20;
+}
+
 size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 
 struct Layout {
     long n; int a, r;
-    bool direct, split;                   // split: k_outer_split
+    bool direct, fused, split;            // fused: k_direct; split: k_outer_split
     int tile, ntiles, nchunks, chunk, segments;
     long full_tiles;                      // of n rows, were they all of one adapter
     int rp;
@@ -1048,6 +1172,7 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     L.n = n; L.a = a; L.r = r;
     L.rp = (r + 15) & ~15;
     L.direct = is_direct(n, d, o, L.rp);
+    L.fused = L.direct && is_fused(n, d, o, L.rp, type);
     L.split = type == kBF16 && !L.direct;
     L.tile = L.direct ? 1 : tile_rows(n, d, o, type);
     L.full_tiles = (n + L.tile - 1) / L.tile;
@@ -1067,7 +1192,7 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
         take(L.perm, (size_t)n * 4);
         take(L.tiles, (size_t)L.ntiles * sizeof(Tile));
     }
-    take(L.part, (size_t)(backward ? L.up_splits : L.down_splits) * n * L.rp * 4);
+    if (!L.fused) take(L.part, (size_t)(backward ? L.up_splits : L.down_splits) * n * L.rp * 4);
     if (backward && L.direct) take(L.low, (size_t)n * r * 4);
     if (backward && !L.direct) {
         take(L.chunks, (size_t)L.nchunks * sizeof(Tile));
@@ -1112,6 +1237,17 @@ hipError_t launch_expand(const ExpandArgs<T>& p, hipStream_t s)
     return launch(k_expand<T, RT, 128, BACK>, grid, 256, 0, s, p);
 }
 
+// The row's own kernel, or both of a tile's.
+template <typename T, bool BACK>
+hipError_t launch_direct(const ShrinkArgs<T>& sh, ExpandArgs<T> ex, hipStream_t s)
+{
+    ex.parts = (ex.w + kDirectThreads / 4 * kVec<T> - 1) / (kDirectThreads / 4 * kVec<T>);
+    const dim3 grid((unsigned)(ex.n * ex.parts));
+    if (ex.r <= 16) return launch(k_direct<T, 16, BACK>, grid, kDirectThreads, 0, s, ex, sh.v, sh.ld_v, sh.M, sh.sa, sh.ld, sh.w);
+    if (ex.r <= 32) return launch(k_direct<T, 32, BACK>, grid, kDirectThreads, 0, s, ex, sh.v, sh.ld_v, sh.M, sh.sa, sh.ld, sh.w);
+    return launch(k_direct<T, 64, BACK>, grid, kDirectThreads, 0, s, ex, sh.v, sh.ld_v, sh.M, sh.sa, sh.ld, sh.w);
+}
+
 // f(row tiles of 16 a tile)
 template <typename F>
 hipError_t with_tile(int tile, F&& f)
@@ -1150,6 +1286,7 @@ hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
         const ShrinkArgs<T> sh{rows, (const T*)a.x, a.ld_x, (const T*)a.down, a.down_sa, a.down_ld, a.d, a.r, a.n, L.ntiles, L.down_splits, part, L.rp};
         const ExpandArgs<T> ex{rows, L.ntiles, part_count(L.full_tiles, a.o, a.type), part, L.down_splits, L.rp, a.n, (const T*)a.up, a.up_sa, a.up_ld, a.gates, a.gates_stride, a.scales,
                                (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, a.o, a.r, a.low, nullptr, nullptr, nullptr, nullptr, 0};
+        if (L.fused) return launch_direct<T, false>(sh, ex, s);
         return with_tile(L.tile, [&](auto rt) {
             const hipError_t e = a.a > 0 ? launch_shrink<T, rt.value>(sh, s) : hipSuccess;
             return e != hipSuccess ? e : launch_expand<T, rt.value, false>(ex, s);
@@ -1180,7 +1317,7 @@ hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
             const ExpandArgs<T> ex{rows, L.ntiles, part_count(L.full_tiles, a.d, a.type), part, L.up_splits, L.rp, a.n, (const T*)a.down, a.down_sa, a.down_ld,
                                    a.gates, a.gates_stride, a.scales, (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, a.d, a.r, u, a.low, a.dgates, u_t, t_t,
                                    L.ld_t};
-            const hipError_t e = with_tile(L.tile, [&](auto rt) {
+            const hipError_t e = L.fused ? launch_direct<T, true>(sh, ex, s) : with_tile(L.tile, [&](auto rt) {
                 const hipError_t e = a.a > 0 ? launch_shrink<T, rt.value>(sh, s) : hipSuccess;
                 return e != hipSuccess ? e : launch_expand<T, rt.value, true>(ex, s);
             });

@@ -280,6 +280,15 @@ def test_adapt_sorted_rows(experts, n, d, o, r, a, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,o,r,a", [(40, 1500, 2100, 9, 4), (3, 2048, 24, 32, 2), (3, 2049, 24, 32, 2), (200, 700, 1100, 17, 6), (20, 24, 300, 60, 3), (2, 12, 4096, 16, 1),
+                                       (12, 4100, 70, 16, 3), (300, 72, 513, 33, 7), (65, 1024, 1024, 16, 9), (70, 1024, 1000, 64, 4), (300, 1024, 8, 49, 3)])
+def test_adapt_few_rows(experts, n, d, o, r, a, dtype):
+    """Calls on either side of where both products become one launch."""
+    print("adapt", n, d, o, r, a, dtype, flush=True)
+    check_adapt(experts, problem(n, d, o, r, a, dtype, n + d), dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("law", ["runs", "one", "none", "wild"])
 @pytest.mark.parametrize("n,d,o,r,a", [(40, 72, 48, 6, 4), (700, 160, 64, 16, 5), (1500, 65, 33, 9, 90)])
 def test_adapt_ids(experts, n, d, o, r, a, law, dtype):
