@@ -66,13 +66,14 @@ __device__ __forceinline__ void plan_keys(const PlanArgs& p, int* key)
 {
     const long first = (long)blockIdx.y * kPlanRows + (threadIdx.x >> 6) * (64 * kPlanLoads) + (threadIdx.x & 63);
 #pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it) key[it] = p.a + 1;
+    if (p.n == 0) return;
+#pragma unroll
+    for (int it = 0; it < kPlanLoads; ++it) key[it] = p.ids[min(first + it * 64, (long)p.n - 1) * p.ids_stride];  // all in flight
+#pragma unroll
     for (int it = 0; it < kPlanLoads; ++it) {
-        const long i = first + it * 64;
-        key[it] = p.a + 1;
-        if (i < p.n) {
-            const int k = p.ids[i * p.ids_stride];
-            key[it] = k >= 0 && k < p.a ? k : p.a;
-        }
+        const int k = key[it] >= 0 && key[it] < p.a ? key[it] : p.a;
+        key[it] = first + it * 64 < p.n ? k : p.a + 1;
     }
 }
 
