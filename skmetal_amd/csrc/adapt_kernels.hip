@@ -110,8 +110,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_count(PlanArgs p)
 
 // The places of adapter blockIdx.x's rows (a: of the rows without one) among the rows of
 // segment blockIdx.y, in their order, and its tiles.  Every block reads the ids anew and counts
-// those below its own adapter: at 16,384 rows and 64 adapters 7 us against the 18 of one
-// block that sorts all the rows.
+// those below its own adapter: 16,384 rows and 64 adapters take 6.5 us, the launch and three
+// dependent trips to memory (11 with a wait after each of a lane's ids; one block that sorts all
+// the rows took 18).
 __global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs p)
 {
     __shared__ int below[kPlanThreads / 64], equal[kPlanThreads / 64], all[3];
@@ -1085,9 +1086,9 @@ __global__ __launch_bounds__(256) void k_outer_merge(OuterArgs<T> p)
 
 // Whether every row is its own tile, without a sort: the call then has a launch less and reads
 // an adapter once a row instead of once a tile.  us without and with the sort, bf16, d = o:
-//   d = 1,024, rank 16:  256 rows 9, 13;  512 rows 13, 14;  1,024 rows 17, 15
-//   d = 4,096, rank 16:   64 rows 10, 15;  128 rows 14, 15;    256 rows 17, 15
-//   d = 4,096, rank 64:   64 rows 15, 18;  128 rows 24, 19
+//   d = 1,024, rank 16:  256 rows 7, 15;  512 rows 12, 14
+//   d = 4,096, rank 16:   64 rows 9, 15;  128 rows 14, 16;  256 rows 17, 16
+//   d = 4,096, rank 64:   64 rows 15, 19;  128 rows 24, 20
 bool is_direct(long n, int d, int o, int rp)
 {
     return n <= kMaxChunk && (size_t)n * rp * ((size_t)d + o) <= (n <= 64 ? size_t(1) << 25 : size_t(1) << 24);
