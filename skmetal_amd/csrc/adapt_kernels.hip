@@ -346,13 +346,16 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
 
 // ---- ranks to rows ----
 
-// v = hi + lo + (at most 2^-17 |v|): a low-rank value enters products of bf16 matrix cores
-// as two bf16, so that its rounding stays far under that of a bf16 result.
-__device__ __forceinline__ void split2(float v, bf16& hi, bf16& lo)
+// v = hi + mid + lo, exactly down to bf16's smallest steps: 8 bits each of the 24 of an fp32.  A
+// low-rank value enters products of bf16 matrix cores as three bf16, so that these are
+// fp32's; with two, which leave out up to 2^-17 |v|, one bf16 result in 700 came out a step
+// off its nearest.
+__device__ __forceinline__ void split3(float v, bf16& hi, bf16& mid, bf16& lo)
 {
     hi = (bf16)v;
-    const float rest = v - (float)hi;
-    lo = (bf16)(__builtin_isfinite((float)hi) ? rest : 0.f);  // an infinity stays one
+    const float rest = __builtin_isfinite((float)hi) ? v - (float)hi : 0.f;  // an infinity stays one
+    mid = (bf16)rest;
+    lo = (bf16)(rest - (float)mid);
 }
 
 // b[j] = element j of the eight vectors a[0 .. 7]: an 8 x 8 transposition in registers.
@@ -382,10 +385,10 @@ struct ExpandArgs {
     float* low;                              // nullable: [n x r], the splits' sum (0 for a row without an adapter)
     // backward (else null): the forward call's low, and its products with the splits' sum
     const float* dot; float* dgates;         // dgates[i] = s_q <low_i, dot_i>, nullable
-    bf16* low_t; bf16* dot_t; long ld_t;     // f low and f dot for k_outer_split, nullable: [2][r][ld_t], by place
+    bf16* low_t; bf16* dot_t; long ld_t;     // f low and f dot for k_outer_split, nullable: [3][r][ld_t], by place
 };
 
-// What k_expand keeps of a tile's low-rank rows: f low as two bf16 (bf16 rows) or as it is.
+// What k_expand keeps of a tile's low-rank rows: f low as three bf16 (bf16 rows) or as it is.
 template <typename T, int RT, int KP>
 struct LowTile {
     static constexpr bool kSplit = false;
@@ -395,19 +398,21 @@ struct LowTile {
 template <int RT, int KP>
 struct LowTile<bf16, RT, KP> {
     static constexpr bool kSplit = true;
-    bf16 v[RT * 16][2 * KP + 8];
+    bf16 v[RT * 16][3 * KP + 8];
     __device__ void set(int i, int k, f32x4 x)
     {
-        bf16 __attribute__((ext_vector_type(4))) hi, lo;
+        bf16 __attribute__((ext_vector_type(4))) hi, mid, lo;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            bf16 a, b;
-            split2(x[u], a, b);
+            bf16 a, b, c;
+            split3(x[u], a, b, c);
             hi[u] = a;
-            lo[u] = b;
+            mid[u] = b;
+            lo[u] = c;
         }
         __builtin_memcpy(&v[i][k], &hi, 8);
-        __builtin_memcpy(&v[i][KP + k], &lo, 8);
+        __builtin_memcpy(&v[i][KP + k], &mid, 8);
+        __builtin_memcpy(&v[i][2 * KP + k], &lo, 8);
     }
 };
 
@@ -492,9 +497,9 @@ template <typename T, int RT, int KP>
 __device__ __forceinline__ void store_by_rank(const ExpandArgs<T>& p, const Tile& t, const LowTile<T, RT, KP>& L, bf16* out)
 {
     if constexpr (LowTile<T, RT, KP>::kSplit)
-        for (int idx = threadIdx.x; idx < 2 * p.r * RT * 16; idx += 256) {
-            const int i = idx % (RT * 16), k = idx / (RT * 16);  // k: a rank's hi, and from r on its lo
-            if (i < t.cnt) out[k * p.ld_t + t.start + i] = L.v[i][k < p.r ? k : KP + k - p.r];
+        for (int idx = threadIdx.x; idx < 3 * p.r * RT * 16; idx += 256) {
+            const int i = idx % (RT * 16), k = idx / (RT * 16), part = k / p.r;  // k: the ranks' hi, then their mid, then lo
+            if (i < t.cnt) out[k * p.ld_t + t.start + i] = L.v[i][part * KP + k - part * p.r];
         }
 }
 
@@ -559,8 +564,8 @@ __device__ __forceinline__ void turn_ranks(Vec<T> (*m)[8])
 // y[0].  A lane ends up with kVec columns (from c on) of four rows.
 //
 // bf16: lanes hold eight ranks of eight columns each, transposed in registers, so M goes
-// to the matrix cores without a detour; L enters as two bf16 (one product of 32 where the
-// ranks fill half of it: hi and lo side by side, M twice).  Other types: fp32 matrix
+// to the matrix cores without a detour; L enters as three bf16 (where the ranks fill half of
+// a product of 32: hi and mid side by side, M twice, then lo beside zeros).  Other types: fp32 matrix
 // cores, four ranks at a time, which need M by columns as it lies and L unrounded.
 // FULL: all the columns exist.
 //
@@ -590,16 +595,22 @@ __device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Til
             for (int e = 0; e < 4; ++e) acc[j][e] = kBaseFirst ? to_f(y[i & 1][e][j]) : 0.f;
         if (has) {
             if constexpr (LowTile<T, RT, KP>::kSplit) {
+                auto part = [&](int k) { return *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][k]); };
+                if constexpr (KP == 16) {
+                    const Vec<T> hi_mid = part(g * 8), lo = g < 2 ? part(32 + g * 8) : Vec<T>{};
 #pragma unroll
-                for (int b = 0; b < (KP + 31) / 32; ++b) {
-                    const Vec<T> hi = *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][b * 32 + g * 8]);
+                    for (int j = 0; j < V; ++j) acc[j] = mfma16(hi_mid, m[0][j], acc[j]);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) acc[j] = mfma16(hi, m[b][j], acc[j]);
-                    if constexpr (KP >= 32) {
-                        const Vec<T> lo = *reinterpret_cast<const Vec<T>*>(&L.v[i * 16 + l16][KP + b * 32 + g * 8]);
+                    for (int j = 0; j < V; ++j) acc[j] = mfma16(lo, m[0][j], acc[j]);
+                } else {
 #pragma unroll
-                        for (int j = 0; j < V; ++j) acc[j] = mfma16(lo, m[b][j], acc[j]);
-                    }
+                    for (int b = 0; b < KP / 32; ++b)
+#pragma unroll
+                        for (int of = 0; of < 3; ++of) {
+                            const Vec<T> some = part(of * KP + b * 32 + g * 8);
+#pragma unroll
+                            for (int j = 0; j < V; ++j) acc[j] = mfma16(some, m[b][j], acc[j]);
+                        }
                 }
             } else {
 #pragma unroll
@@ -908,12 +919,13 @@ __global__ __launch_bounds__(256) void k_outer(OuterArgs<T> p)
 }
 
 // The same for bf16 rows on the bf16 matrix cores, 32 rows at a time: a lane's eight rows of
-// eight columns are transposed in registers, and f low comes by rank as two bf16 (k_expand's
+// eight columns are transposed in registers, and f low comes by rank as three bf16 (k_expand's
 // low_t, dot_t) through LDS, 64 rows at a time, for the block's four waves.  A block takes a
-// chunk and 512 columns, a wave 128 of them.  (16,384 rows x 4,096 twice, rank 64: 82 us
-// so; 120 with each wave's own loads of f low, 16 lines of 64 bytes apiece.)
+// chunk and 512 columns, a wave 128 of them.  16,384 rows x 4,096 twice, rank 64: 104 us, of
+// which the third part takes 11; with each wave's own loads of f low, 16 lines of 64 bytes
+// apiece, it took half as long again.
 struct SplitSide {
-    const bf16* low;                         // [2][r][ld_t]: hi, lo
+    const bf16* low;                         // [3][r][ld_t]: hi, mid, lo
     const bf16* v; long ld_v; int w;
     bf16* dM; float* part;
 };
@@ -926,9 +938,9 @@ template <int NB>
 __global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
 {
     constexpr int R = NB * 16;
-    constexpr int S = NB == 4 ? 32 : 64, NM = 2 * R * S / 8 / 256;  // rows staged at once, a thread's 16 bytes of them
+    constexpr int S = 8 * 256 / R;  // rows staged at once: 16 bytes of each part a thread
     __shared__ __align__(16) int rows[kMaxChunk + 32];
-    __shared__ __align__(16) bf16 low[2][2][R][S + 8];  // twice: hi and lo of S rows by rank
+    __shared__ __align__(16) bf16 low[2][3][R][S + 8];  // twice: hi, mid and lo of S rows by rank
     const Place at = place_spread(blockIdx.x, p.parts);
     const Tile t = p.chunks[at.tile];
     if (t.q < 0) return;
@@ -938,24 +950,22 @@ __global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
     const int c0 = ((at.part - (second ? p.split : 0)) * 4 + wave) * 128, rank0 = blockIdx.z * R;
     const bool active = c0 < s.w, full = c0 + 128 <= s.w;
     const int c = c0 + l16 * 8, left = s.w - c;
-    Vec<bf16> mine[NM];
+    const int seg = threadIdx.x % (S / 8), line = threadIdx.x / (S / 8);
+    const bf16* from = s.low + min(rank0 + line, p.r - 1) * p.ld_t + t.start + seg * 8;
+    Vec<bf16> mine[3];
     auto fetch_low = [&](int i) {
 #pragma unroll
-        for (int u = 0; u < NM; ++u) {
-            const int idx = threadIdx.x + u * 256, seg = idx % (S / 8), rank = idx / (S / 8) % R, half = idx / (S / 8 * R);
-            mine[u] = load16(s.low + (half * p.r + min(rank0 + rank, p.r - 1)) * p.ld_t + t.start + i + seg * 8);
+        for (int of = 0; of < 3; ++of) {
+            mine[of] = load16(from + of * p.r * p.ld_t + i);
             if (i + S > t.cnt)  // the places past the chunk belong to other adapters
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (i + seg * 8 + e >= t.cnt) mine[u][e] = (bf16)0.f;
+                    if (i + seg * 8 + e >= t.cnt) mine[of][e] = (bf16)0.f;
         }
     };
     auto stage_low = [&](int turn) {
 #pragma unroll
-        for (int u = 0; u < NM; ++u) {
-            const int idx = threadIdx.x + u * 256, seg = idx % (S / 8), rank = idx / (S / 8) % R, half = idx / (S / 8 * R);
-            *reinterpret_cast<Vec<bf16>*>(&low[turn][half][rank][seg * 8]) = mine[u];
-        }
+        for (int of = 0; of < 3; ++of) *reinterpret_cast<Vec<bf16>*>(&low[turn][of][line][seg * 8]) = mine[of];
     };
     Vec<bf16> v[8];
     auto fetch_rows = [&](int i) {
@@ -994,8 +1004,8 @@ __global__ __launch_bounds__(256, 2) void k_outer_split(OuterSplitArgs p)
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const Vec<bf16> f = *reinterpret_cast<const Vec<bf16>*>(&low[turn][half][b * 16 + l16][h * 32 + g * 8]);
+                for (int of = 0; of < 3; ++of) {
+                    const Vec<bf16> f = *reinterpret_cast<const Vec<bf16>*>(&low[turn][of][b * 16 + l16][h * 32 + g * 8]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) acc[b][j] = mfma16(f, x[j], acc[b][j]);
                 }
@@ -1183,7 +1193,7 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
     if (L.segments < 1) L.segments = 1;
     L.chunk = chunk_rows(n, d, o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
-    L.ld_t = ((n + 63) & ~63l) + 96;  // 64 rows past the last; not a power of two apart
+    L.ld_t = ((n + 63) & ~63l) + 160;  // 128 rows past the last (k_outer_split's most at once); not a power of two apart
     const int zs = (r + 63) / 64;
     L.down_splits = split_count(L.full_tiles, d, type, zs);
     L.up_splits = split_count(L.full_tiles, o, type, zs);
@@ -1200,8 +1210,8 @@ Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
         take(L.chunks, (size_t)L.nchunks * sizeof(Tile));
         take(L.merge, (size_t)a * sizeof(int2));
         take(L.low, L.split ? 0 : (size_t)n * r * 4);
-        take(L.low_t, L.split ? (size_t)2 * r * L.ld_t * 2 : 0);
-        take(L.dot_t, L.split ? (size_t)2 * r * L.ld_t * 2 : 0);
+        take(L.low_t, L.split ? (size_t)3 * r * L.ld_t * 2 : 0);
+        take(L.dot_t, L.split ? (size_t)3 * r * L.ld_t * 2 : 0);
         take(L.dpart, (size_t)L.nchunks * r * d * 4);
         take(L.upart, (size_t)L.nchunks * r * o * 4);
     }
