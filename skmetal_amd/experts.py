@@ -258,6 +258,7 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
     if x.shape[1] != d:
         raise ValueError(f"x has {x.shape[1]} columns, down has {d}")
     dtype = x.dtype
+    x_ld = _rows(x, "x", dtype, (n, d), device)
     base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, o), device))
     lib = _lib()
     if out is None:
@@ -267,7 +268,7 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
     low = torch.empty((n, r), dtype=torch.float32, device=device) if return_low else None
     size = _adapt_workspace(code, n, d, o, r, a, 0)
     ws, ws_ptr = _workspace(size, device)
-    if lib.skmetal_hip_adapt(code, x.data_ptr(), x.stride(0), *shared, base_ptr, base_ld, out.data_ptr(), out_ld,
+    if lib.skmetal_hip_adapt(code, x.data_ptr(), x_ld, *shared, base_ptr, base_ld, out.data_ptr(), out_ld,
                              None if low is None else low.data_ptr(), n, d, o, r, a, ws_ptr, size, _stream(device)):
         _fail("adapt")
     return (out, low) if return_low else out
@@ -283,6 +284,7 @@ def adapt_backward(grad, x, down, up, ids, low, *, base=None, gates=None, scales
     if grad.shape[1] != o:
         raise ValueError(f"grad has {grad.shape[1]} columns, up has {o}")
     dtype = grad.dtype
+    grad_ld = _rows(grad, "grad", dtype, (n, o), device)
     x_ld = _rows(x, "x", dtype, (n, d), device)
     low_ptr = _dense(low, "low", torch.float32, (n, r), device)
     base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, d), device))
@@ -293,7 +295,7 @@ def adapt_backward(grad, x, down, up, ids, low, *, base=None, gates=None, scales
     grad_gates = None if gates is None else torch.empty(n, dtype=torch.float32, device=device)
     size = _adapt_workspace(code, n, d, o, r, a, 1)
     ws, ws_ptr = _workspace(size, device)
-    if lib.skmetal_hip_adapt_backward(code, grad.data_ptr(), grad.stride(0), x.data_ptr(), x_ld, *shared, low_ptr, base_ptr, base_ld, grad_x.data_ptr(), d,
+    if lib.skmetal_hip_adapt_backward(code, grad.data_ptr(), grad_ld, x.data_ptr(), x_ld, *shared, low_ptr, base_ptr, base_ld, grad_x.data_ptr(), d,
                                       grad_down.data_ptr(), grad_up.data_ptr(), None if grad_gates is None else grad_gates.data_ptr(), n, d, o, r, a,
                                       ws_ptr, size, _stream(device)):
         _fail("adapt_backward")
