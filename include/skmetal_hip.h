@@ -331,7 +331,8 @@ SKMETAL_API int skmetal_hip_lloyd_inertia(skmetal_hip_lloyd* h, double* out);
  * `workspace` holds at least the bytes that the *_workspace function gives for
  * the same sizes (16-byte aligned).  skmetal_init must have succeeded, and the
  * calling thread's current device must be the library's.  A bad argument
- * returns an error and enqueues nothing.
+ * returns an error and enqueues nothing.  An output shares no memory with an
+ * input or another output but where its call says so.
  *
  * dtype: the type of scores, rows and adapters.  Sums, softmax statistics and
  * the low-rank products are fp32, each result rounded once to its type.  Rows
@@ -365,7 +366,8 @@ SKMETAL_API int skmetal_hip_route(int dtype, const void* logits, size_t ld_logit
 /* grad_logits [n x E] from grad_weights [n x k] and grad_loss [1] (each
  * nullable: no gradient), with weights, experts, counts and rows as
  * skmetal_hip_route gave them (counts are held constant, as they have no
- * gradient).  Excluded scores and masked rows get 0. */
+ * gradient).  Excluded scores and masked rows get 0.  grad_logits may be logits
+ * itself (the same address and distance of rows). */
 SKMETAL_API int skmetal_hip_route_backward(int dtype, const void* logits, size_t ld_logits, const uint8_t* mask,
                                            size_t mask_stride, size_t n, size_t E, size_t k, int normalize,
                                            const float* weights, const int32_t* experts, const int32_t* counts,
@@ -374,13 +376,18 @@ SKMETAL_API int skmetal_hip_route_backward(int dtype, const void* logits, size_t
 
 /* Low-rank adapters beside a shared projection: with q = ids[i],
  *   out_i = base_i + gates_i scales_q up_q^T (down_q x_i)
- * x [n x d], base [n x o] (nullable: 0), out [n x o] (may be base itself);
+ * x [n x d], base [n x o] (nullable: 0), out [n x o] (may be base itself: the
+ * same address and distance of rows; may share any memory with x);
  * down [a][r][d] and up [a][r][o], adapters *_stride and ranks *_ld elements
  * apart; ids [n] int32 (ids_stride elements apart), outside [0, a): the row has
  * no adapter; gates [n] (nullable: 1, gates_stride elements apart) and scales
  * [a] (nullable: 1) fp32.  low (nullable): [n x r] fp32, receives down_q x_i,
- * which the backward call takes.  1 <= r <= 128, n < 2^30, a <= 2048. */
-SKMETAL_API size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int backward);
+ * which the backward call takes.  1 <= r <= 128, n < 2^30, a <= 2048.
+ * The workspace depends on the call: one of SKMETAL_ADAPT... */
+#define SKMETAL_ADAPT 0          /* skmetal_hip_adapt, out apart from x */
+#define SKMETAL_ADAPT_BACKWARD 1 /* skmetal_hip_adapt_backward */
+#define SKMETAL_ADAPT_IN_X 2     /* skmetal_hip_adapt, out shares memory with x */
+SKMETAL_API size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int call);
 SKMETAL_API int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const void* down, size_t down_stride,
                                   size_t down_ld, const void* up, size_t up_stride, size_t up_ld, const int32_t* ids,
                                   size_t ids_stride, const float* gates, size_t gates_stride, const float* scales,
@@ -388,7 +395,7 @@ SKMETAL_API int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const v
                                   size_t d, size_t o, size_t r, size_t a, void* workspace, size_t workspace_bytes,
                                   void* stream);
 /* Gradients from grad [n x o], that of out: grad_x_i = base_i + the adapters'
- * part (base [n x d] nullable: 0; may be grad_x itself), grad_down [a][r][d]
+ * part (base [n x d] nullable: 0; grad_x may be base itself), grad_down [a][r][d]
  * and grad_up [a][r][o] (dense; 0 for an adapter without rows), grad_gates [n]
  * fp32 (nullable).  base's own gradient is grad. */
 SKMETAL_API int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t ld_grad, const void* x, size_t ld_x,

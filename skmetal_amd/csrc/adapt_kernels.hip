@@ -1178,13 +1178,15 @@ int chunk_rows(long n, int d, int o, int a, int type)
     return c;
 }
 
-Layout layout(int type, long n, int d, int o, int r, int a, bool backward)
+Layout layout(int type, long n, int d, int o, int r, int a, AdaptCall call)
 {
+    const bool backward = call == kAdaptBackward;
     Layout L{};
     L.n = n; L.a = a; L.r = r;
     L.rp = (r + 15) & ~15;
     L.direct = is_direct(n, d, o, L.rp);
-    L.fused = L.direct && is_fused(n, d, o, L.rp, type);
+    // k_direct's blocks of a row each read all of x while others write out already
+    L.fused = L.direct && call != kAdaptInX && is_fused(n, d, o, L.rp, type);
     L.split = type == kBF16 && !L.direct;
     L.tile = L.direct ? 1 : tile_rows(n, d, o, type);
     L.full_tiles = (n + L.tile - 1) / L.tile;
@@ -1273,7 +1275,7 @@ hipError_t with_tile(int tile, F&& f)
 
 bool adapt_fits(int type, long n, int d, int o, int r, int a)
 {
-    const Layout L = layout(type, n, d, o, r, a, true);
+    const Layout L = layout(type, n, d, o, r, a, kAdaptBackward);
     const size_t tiles = ((size_t)L.full_tiles + a + 8) * (size_t)(L.down_splits > L.up_splits ? L.down_splits : L.up_splits);
     const size_t wide = ((size_t)L.full_tiles + a + 8) * (size_t)(part_count(L.full_tiles, d, type) > part_count(L.full_tiles, o, type) ? part_count(L.full_tiles, d, type) : part_count(L.full_tiles, o, type));
     const size_t cols = 16 * (16 / elem_size(type)), chunks = (L.direct ? (size_t)a : (size_t)n / L.chunk + a) * ((d + cols - 1) / cols + (o + cols - 1) / cols);
@@ -1281,12 +1283,12 @@ bool adapt_fits(int type, long n, int d, int o, int r, int a)
     return tiles < most && wide < most && chunks < most && L.segments < 65536;
 }
 
-size_t adapt_workspace(int type, long n, int d, int o, int r, int a, int backward) { return layout(type, n, d, o, r, a, backward != 0).bytes; }
+size_t adapt_workspace(int type, long n, int d, int o, int r, int a, AdaptCall call) { return layout(type, n, d, o, r, a, call).bytes; }
 
 hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
 {
     if (a.n == 0) return hipSuccess;
-    const Layout L = layout(a.type, a.n, a.d, a.o, a.r, a.a, false);
+    const Layout L = layout(a.type, a.n, a.d, a.o, a.r, a.a, a.in_x ? kAdaptInX : kAdapt);
     if (!L.direct) {
         const hipError_t e = launch_plan(L, a.ids, a.ids_stride, a.ws, false, s);
         if (e != hipSuccess) return e;
@@ -1308,7 +1310,7 @@ hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s)
 
 hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s)
 {
-    const Layout L = layout(a.type, a.n, a.d, a.o, a.r, a.a, true);
+    const Layout L = layout(a.type, a.n, a.d, a.o, a.r, a.a, kAdaptBackward);
     if (a.n == 0 && a.a == 0) return hipSuccess;
     if (!L.direct) {
         const hipError_t e = launch_plan(L, a.ids, a.ids_stride, a.ws, true, s);

@@ -56,7 +56,8 @@ struct AdaptArgs {
     const float* scales;                               // nullable, [a]
     const void* base; long ld_base;                    // nullable, [n x o]
     void* out; long ld_out;                            // [n x o]
-    float* low;                                        // nullable (then in ws), [n x r]
+    float* low;                                        // nullable, [n x r]
+    bool in_x;                                         // out shares memory with x
     char* ws;
 };
 hipError_t launch_adapt(const AdaptArgs& a, hipStream_t s);
@@ -78,7 +79,8 @@ struct AdaptBackArgs {
     char* ws;
 };
 hipError_t launch_adapt_back(const AdaptBackArgs& a, hipStream_t s);
-size_t adapt_workspace(int type, long n, int d, int o, int r, int a, int backward);
+enum AdaptCall : int { kAdapt = 0, kAdaptBackward = 1, kAdaptInX = 2 };
+size_t adapt_workspace(int type, long n, int d, int o, int r, int a, AdaptCall call);
 // Whether every launch of both directions has a grid that the device takes.
 bool adapt_fits(int type, long n, int d, int o, int r, int a);
 

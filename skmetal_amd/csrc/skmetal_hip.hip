@@ -2166,6 +2166,38 @@ int check_workspace(const void* ws, size_t have, size_t need)
     return check_aligned(ws, 16, "the workspace");
 }
 
+// A matrix's rows in memory, in bytes: `width` each, `apart` from one to the next.
+struct RowSpan {
+    uintptr_t at;
+    size_t apart, width, n;
+    RowSpan(const void* p, size_t ld, size_t w, size_t rows, size_t es) : at(reinterpret_cast<uintptr_t>(p)), apart(ld * es), width(w * es), n(rows)
+    {
+        if (n > 1 && apart >= width) return;
+        width = n == 0 ? 0 : (n - 1) * apart + width;  // rows that meet or cross are one stretch
+        apart = width;
+        n = n != 0;
+    }
+    bool same(const RowSpan& b) const { return at == b.at && apart == b.apart && n == b.n; }
+};
+
+// Whether an element of one lies in the other.
+bool share(const RowSpan& a, const RowSpan& b)
+{
+    if (a.n == 0 || b.n == 0 || a.at >= b.at + (b.n - 1) * b.apart + b.width || b.at >= a.at + (a.n - 1) * a.apart + a.width) return false;
+    if (a.apart == b.apart) {  // row i of a and row i + m of b: -b.width < b.at + m apart - a.at < a.width
+        const intptr_t off = static_cast<intptr_t>(b.at - a.at), w = static_cast<intptr_t>(a.apart), low = -off - static_cast<intptr_t>(b.width);
+        intptr_t m = (low >= 0 ? low / w : -((-low + w - 1) / w)) + 1;
+        m = std::max(m, -static_cast<intptr_t>(a.n - 1));
+        return m <= static_cast<intptr_t>(b.n - 1) && m * w + off < static_cast<intptr_t>(a.width);
+    }
+    for (size_t i = 0, j = 0; i < a.n && j < b.n;) {
+        const uintptr_t x = a.at + i * a.apart, y = b.at + j * b.apart;
+        if (x < y + b.width && y < x + a.width) return true;
+        (x + a.width <= y ? i : j) += 1;
+    }
+    return false;
+}
+
 int check_route(int dtype, size_t n, size_t E, size_t k, size_t ld, size_t mask_stride)
 {
     TRY(check_dtype(dtype));
@@ -2241,16 +2273,19 @@ int skmetal_hip_route_backward(int dtype, const void* logits, size_t ld_logits, 
         return fail(SKMETAL_EINVAL, "null pointer argument");
     TRY(check_aligned(logits, elem_size(dtype), "logits"));
     TRY(check_aligned(grad_logits, elem_size(dtype), "grad_logits"));
+    const RowSpan z(logits, ld_logits, E, n, elem_size(dtype)), dz(grad_logits, ld_grad, E, n, elem_size(dtype));
+    if (!dz.same(z) && share(dz, z)) return fail(SKMETAL_EINVAL, "grad_logits shares memory with logits without being it");
     TRY(on_device());
     RouteBackArgs a{logits, dtype, (long)n, (int)E, (long)ld_logits, mask, (long)mask_stride, (int)k, normalize, weights,
                     experts, counts, rows, grad_weights, grad_loss, grad_logits, (long)ld_grad};
     return launched(launch_route_back(a, static_cast<hipStream_t>(stream)), "route_backward");
 }
 
-size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int backward)
+size_t skmetal_hip_adapt_workspace(int dtype, size_t n, size_t d, size_t o, size_t r, size_t a, int call)
 {
     if (check_adapt(dtype, {n, d, o, r, a}, {}) != 0) return 0;
-    return adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, backward);
+    const AdaptCall which = call == SKMETAL_ADAPT ? kAdapt : call == SKMETAL_ADAPT_IN_X ? kAdaptInX : kAdaptBackward;
+    return adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, which);
 }
 
 int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const void* down, size_t down_stride, size_t down_ld,
@@ -2269,11 +2304,17 @@ int skmetal_hip_adapt(int dtype, const void* x, size_t ld_x, const void* down, s
     TRY(check_aligned(up, es, "up"));
     TRY(check_aligned(base, es, "base"));
     TRY(check_aligned(out, es, "out"));
-    TRY(check_workspace(workspace, workspace_bytes, adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, 0)));
+    const RowSpan result(out, ld_out, o, n, es);
+    if (base != nullptr) {
+        const RowSpan b(base, ld_base, o, n, es);
+        if (!result.same(b) && share(result, b)) return fail(SKMETAL_EINVAL, "out shares memory with base without being it");
+    }
+    const bool in_x = share(result, RowSpan(x, ld_x, d, n, es));
+    TRY(check_workspace(workspace, workspace_bytes, adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, in_x ? kAdaptInX : kAdapt)));
     TRY(on_device());
     AdaptArgs A{dtype, (long)n, (int)d, (int)o, (int)r, (int)a, x, (long)ld_x, down, (long)down_stride, (long)down_ld,
                 up, (long)up_stride, (long)up_ld, ids, (long)ids_stride, gates, (long)gates_stride, scales, base,
-                (long)ld_base, out, (long)ld_out, low, static_cast<char*>(workspace)};
+                (long)ld_base, out, (long)ld_out, low, in_x, static_cast<char*>(workspace)};
     return launched(launch_adapt(A, static_cast<hipStream_t>(stream)), "adapt");
 }
 
@@ -2299,7 +2340,14 @@ int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t ld_grad, cons
     TRY(check_aligned(grad_x, es, "grad_x"));
     TRY(check_aligned(grad_down, es, "grad_down"));
     TRY(check_aligned(grad_up, es, "grad_up"));
-    TRY(check_workspace(workspace, workspace_bytes, adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, 1)));
+    const RowSpan result(grad_x, ld_grad_x, d, n, es);
+    if (share(result, RowSpan(grad, ld_grad, o, n, es)) || share(result, RowSpan(x, ld_x, d, n, es)))
+        return fail(SKMETAL_EINVAL, "grad_x shares memory with grad or x");
+    if (base != nullptr) {
+        const RowSpan b(base, ld_base, d, n, es);
+        if (!result.same(b) && share(result, b)) return fail(SKMETAL_EINVAL, "grad_x shares memory with base without being it");
+    }
+    TRY(check_workspace(workspace, workspace_bytes, adapt_workspace(dtype, (long)n, (int)d, (int)o, (int)r, (int)a, kAdaptBackward)));
     TRY(on_device());
     AdaptBackArgs A{dtype, (long)n, (int)d, (int)o, (int)r, (int)a, grad, (long)ld_grad, x, (long)ld_x, down,
                     (long)down_stride, (long)down_ld, up, (long)up_stride, (long)up_ld, ids, (long)ids_stride, gates,

@@ -31,6 +31,7 @@ MAX_EXPERTS = 2048
 MAX_TOP_K = 16
 MAX_RANK = 128
 
+_ADAPT, _ADAPT_BACKWARD, _ADAPT_IN_X = 0, 1, 2
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -141,8 +142,8 @@ def _route_workspace(n, e):
 
 
 @functools.lru_cache(maxsize=4096)
-def _adapt_workspace(code, n, d, o, r, a, backward):
-    return _lib().skmetal_hip_adapt_workspace(code, n, d, o, r, a, backward)
+def _adapt_workspace(code, n, d, o, r, a, call):
+    return _lib().skmetal_hip_adapt_workspace(code, n, d, o, r, a, call)
 
 
 # the current stream's handle, without an object around it where torch offers that
@@ -252,7 +253,8 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
     up-projection), ids int32 [n] in any order, with any value outside [0, a) for a row
     without an adapter; base [n, o] is the shared projection's output (None: 0), gates
     [n] (a router's weights) and scales [a] are float32 (None: 1).  x, down, up, base
-    and out have one type.  `out` may be base.  With `return_low` also returns down_q
+    and out have one type.  `out` may be base and may share memory with x (a residual
+    stream in place: base=x, out=x); nothing else may share memory with it.  With `return_low` also returns down_q
     x_i, float32 [n, r], for ``adapt_backward``."""
     code, device, n, d, o, r, a, shared = _check_adapt(x, "x", down, up, ids, gates, scales)
     if x.shape[1] != d:
@@ -261,14 +263,19 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
     x_ld = _rows(x, "x", dtype, (n, d), device)
     base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, o), device))
     lib = _lib()
+    x_ptr, call = x.data_ptr(), _ADAPT
     if out is None:
         out, out_ld = torch.empty((n, o), dtype=dtype, device=device), o
+        out_ptr = out.data_ptr()
     else:
         out_ld = _rows(out, "out", dtype, (n, o), device)
+        out_ptr, es = out.data_ptr(), dtype.itemsize
+        if x_ptr < out_ptr + (n * out_ld + o) * es and out_ptr < x_ptr + (n * x_ld + d) * es:
+            call = _ADAPT_IN_X  # or between x's rows, which the library finds out
     low = torch.empty((n, r), dtype=torch.float32, device=device) if return_low else None
-    size = _adapt_workspace(code, n, d, o, r, a, 0)
+    size = _adapt_workspace(code, n, d, o, r, a, call)
     ws, ws_ptr = _workspace(size, device)
-    if lib.skmetal_hip_adapt(code, x.data_ptr(), x_ld, *shared, base_ptr, base_ld, out.data_ptr(), out_ld,
+    if lib.skmetal_hip_adapt(code, x_ptr, x_ld, *shared, base_ptr, base_ld, out_ptr, out_ld,
                              None if low is None else low.data_ptr(), n, d, o, r, a, ws_ptr, size, _stream(device)):
         _fail("adapt")
     return (out, low) if return_low else out
@@ -293,7 +300,7 @@ def adapt_backward(grad, x, down, up, ids, low, *, base=None, gates=None, scales
     grad_down = torch.empty((a, r, d), dtype=dtype, device=device)
     grad_up = torch.empty((a, r, o), dtype=dtype, device=device)
     grad_gates = None if gates is None else torch.empty(n, dtype=torch.float32, device=device)
-    size = _adapt_workspace(code, n, d, o, r, a, 1)
+    size = _adapt_workspace(code, n, d, o, r, a, _ADAPT_BACKWARD)
     ws, ws_ptr = _workspace(size, device)
     if lib.skmetal_hip_adapt_backward(code, grad.data_ptr(), grad_ld, x.data_ptr(), x_ld, *shared, low_ptr, base_ptr, base_ld, grad_x.data_ptr(), d,
                                       grad_down.data_ptr(), grad_up.data_ptr(), None if grad_gates is None else grad_gates.data_ptr(), n, d, o, r, a,

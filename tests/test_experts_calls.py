@@ -73,3 +73,96 @@ def test_rows_apart_keep_their_distance(calls):
     experts.adapt(torch.zeros(40, 7)[:, :1].T.T, one["down"], one["up"], one["ids"])
     experts.adapt_backward(torch.zeros(40, 60)[:, :24], s["x"], s["down"], s["up"], s["ids"], s["low"])
     assert [c[1][2] for c in calls] == [50, 7, 60]
+
+
+def test_an_out_in_x_asks_for_the_workspace_of_two_launches(calls, monkeypatch):
+    from skmetal_amd import experts
+
+    asked = []
+    monkeypatch.setattr(experts, "_adapt_workspace", lambda *sizes: asked.append(sizes[-1]) or 0)
+    s = problem(o=16)
+    wide = torch.zeros(40, 64)
+    for out, call in ((None, 0), (torch.zeros(40, 16), 0), (s["x"], 2), (wide[:, 8:24], 2), (wide[:, 16:32], 2)):
+        x = wide[:, :16] if out is not None and out.shape == (40, 16) and out.stride(0) == 64 else s["x"]
+        experts.adapt(x, s["down"], s["up"], s["ids"], base=out, out=out)
+        assert asked.pop() == call and calls.pop()[0] == "adapt"
+
+
+# ---- the entry points' own checks of places, on addresses that nothing reads ----
+
+P = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from skmetal_amd import _bridge
+
+    if _bridge._lib is None:
+        pytest.fail(f"library not loaded: {_bridge.last_error()}")
+    if _bridge.HIP_AVAILABLE:
+        pytest.skip("an accepted call would run on these addresses")
+    return _bridge._lib
+
+
+EINVAL, ENODEV = 1, 2
+
+
+def elements(at, ld, w, n):
+    return {at + i * ld + j for i in range(n) for j in range(w)}
+
+
+def test_out_and_base_share_all_or_nothing(lib):
+    """Against the sets of elements themselves: rows in step with each other, out of step,
+    crossing, single."""
+    import random
+
+    rng = random.Random(5)
+    seen = {EINVAL: 0, ENODEV: 0}
+    for _ in range(4000):
+        n, o = rng.choice([1, 2, 3, 7]), rng.randint(1, 9)
+        ld_out = o + rng.choice([0, 1, 5, 12])
+        ld_base = rng.choice([ld_out, ld_out, o, rng.randint(0, 25)])
+        out, base = rng.randint(0, 60), rng.randint(0, 60)
+        code = lib.skmetal_hip_adapt(0, P // 2, 4, P // 4, 8, 4, P // 4, 2 * o, o, P // 8, 1, None, 0, None, P + 4 * base, ld_base, P + 4 * out, ld_out, None, n, 4, o,
+                                     2, 1, 4096, 1 << 30, None)
+        shared = elements(out, ld_out, o, n) & elements(base, ld_base, o, n)
+        fine = not shared or (out == base and (ld_out == ld_base or n == 1))
+        assert code == (ENODEV if fine else EINVAL), (n, o, ld_out, ld_base, out, base, lib.skmetal_hip_last_error())
+        if not fine:
+            assert b"out shares memory with base" in lib.skmetal_hip_last_error()
+        seen[code] += 1
+    assert min(seen.values()) > 500
+
+
+def test_out_in_x_needs_the_larger_workspace(lib):
+    """64 rows of 4,096 at rank 16 are one launch without scratch, unless out lies in x."""
+    sizes = (1, 64, 4096, 4096, 16, 8)
+    apart, back, in_x = (lib.skmetal_hip_adapt_workspace(*sizes, call) for call in range(3))
+    assert apart == 0 and 0 < in_x and 0 < back
+
+    def adapt(x, out, ld, ws):
+        return lib.skmetal_hip_adapt(1, x, ld, P // 4, 16 * 4096, 4096, P // 4, 16 * 4096, 4096, P // 8, 1, None, 0, None, None, 0, out, ld, None, 64, 4096, 4096, 16, 8,
+                                     4096, ws, None)
+
+    assert adapt(P, 2 * P, 4096, 0) == ENODEV
+    assert adapt(P, P + 2 * 4096, 8192, 0) == ENODEV  # between x's rows
+    for x, out, ld in ((P, P, 4096), (P, P + 2, 4096), (P, P + 2 * 4095, 8192), (P + 2 * 63 * 4096 + 2, P, 4096)):
+        assert adapt(x, out, ld, in_x - 1) == EINVAL and b"workspace" in lib.skmetal_hip_last_error()
+        assert adapt(x, out, ld, in_x) == ENODEV
+
+
+def test_gradients_share_no_memory_with_what_they_are_made_of(lib):
+    def adapt_back(grad=P, x=2 * P, base=None, grad_x=3 * P, ld_base=8):
+        return lib.skmetal_hip_adapt_backward(0, grad, 8, x, 8, P // 4, 16, 8, P // 4, 16, 8, P // 8, 1, None, 0, None, P // 2, base, ld_base, grad_x, 8, P // 32, P // 16,
+                                              None, 5, 8, 8, 2, 1, 4096, 1 << 30, None)
+
+    assert adapt_back() == ENODEV and adapt_back(base=3 * P) == ENODEV and adapt_back(base=3 * P + 4 * 40) == ENODEV
+    for bad in (dict(grad_x=P), dict(grad_x=2 * P + 4 * 39), dict(base=3 * P + 4), dict(base=3 * P, ld_base=16), dict(base=3 * P, ld_base=0)):
+        assert adapt_back(**bad) == EINVAL and b"grad_x shares memory" in lib.skmetal_hip_last_error(), bad
+
+    def route_back(grad, ld=8):
+        return lib.skmetal_hip_route_backward(0, P, 8, None, 0, 5, 8, 2, 0, P // 2, P // 2, P // 2, P // 2, None, None, grad, ld, None)
+
+    assert route_back(2 * P) == ENODEV and route_back(P) == ENODEV
+    for bad in ((P + 4,), (P + 4 * 39,), (P, 9)):
+        assert route_back(*bad) == EINVAL and b"grad_logits shares memory" in lib.skmetal_hip_last_error(), bad

@@ -1,0 +1,54 @@
+"""Routing and adapters as callers use them: results in place, inside autograd, on tensors
+that other code changes.  Bounds are those of test_gpu_experts."""
+
+from __future__ import annotations
+
+import experts_reference as ref
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_experts import HALF, STEP, TYPES, U, experts, f64, near, part, problem  # noqa: E402, F401 -- a fixture
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,r", [(1, 1024, 8), (64, 4096, 16), (20, 1200, 5), (300, 640, 33), (700, 520, 12)])
+def test_out_in_place_of_x(experts, n, d, r, dtype):  # noqa: F811
+    """A residual stream in place, where one launch, two and three take the rows: the same
+    bits every time, and no column formed from another's result."""
+    print("out in x", n, d, r, dtype, flush=True)
+    s = problem(n, d, d, r, 5, dtype, n + d)
+    opt = dict(gates=s["gates"], scales=s["scales"])
+    want, _, mag = ref.adapt(f64(s["x"]), f64(s["down"]), f64(s["up"]), s["ids"].cpu().numpy(), f64(s["x"]), f64(s["gates"]), f64(s["scales"]))
+    bound = ((d + r + 16) * U + part(dtype)) * mag + 2 * U * abs(want) + HALF[dtype] * abs(want) + STEP[dtype]
+    first = None
+    for _ in range(4):
+        x = s["x"].clone()
+        out = experts.adapt(x, s["down"], s["up"], s["ids"], base=x, out=x, **opt)
+        assert out.data_ptr() == x.data_ptr()
+        first = out.clone() if first is None else first
+        assert torch.equal(out, first)
+    near(first, want, bound, "out")
+    # rows that lie in x's, one column on: x is read before any of them is written
+    wide = torch.zeros(n, d + 8, dtype=TYPES[dtype], device="cuda")
+    wide[:, :d] = s["x"]
+    out = experts.adapt(wide[:, :d], s["down"], s["up"], s["ids"], base=s["x"], out=wide[:, 1 : d + 1], **opt)
+    assert torch.equal(out, first)
+    # between x's rows
+    both = torch.zeros(n, 2 * d, dtype=TYPES[dtype], device="cuda")
+    both[:, :d] = s["x"]
+    out = experts.adapt(both[:, :d], s["down"], s["up"], s["ids"], base=s["x"], out=both[:, d:], **opt)
+    near(out, want, bound, "out")
+    assert torch.equal(both[:, :d], s["x"])
+
+
+def test_out_partly_in_base_is_refused(experts):  # noqa: F811
+    s = problem(9, 32, 24, 4, 3, "bf16", 1)
+    wide = torch.zeros(9, 40, dtype=torch.bfloat16, device="cuda")
+    for base, out in ((wide[:, :24], wide[:, 1:25]), (wide[:1, :24].expand(9, 24), wide[:, :24]), (wide[1:, :24], wide[:-1, :24])):
+        n = out.shape[0]
+        with pytest.raises(RuntimeError, match="out shares memory with base"):
+            experts.adapt(s["x"][:n], s["down"], s["up"], s["ids"][:n], base=base, out=out)
+    experts.adapt(s["x"], s["down"], s["up"], s["ids"], base=wide[:, :12].repeat(1, 2), out=wide[:, 16:])
