@@ -168,16 +168,8 @@ def _check_route(logits, top_k):
     return code, device, n, e, top_k, ld
 
 
-def route(logits, top_k, *, mask=None, normalize=False) -> Routing:
-    """The `top_k` largest scores of every row of logits [n, e], equal ones by the lowest
-    index, with their softmax probabilities as weights (over the row's e scores;
-    `normalize` divides them by their sum over the chosen ones).  A score of -inf or NaN
-    is excluded; a row that `mask` (bool [n]) leaves out, or whose scores are all
-    excluded, takes no expert (-1, weight 0) and counts nowhere.
-
-    ``loss`` = e / (top_k N^2) sum_j counts_j prob_sums_j over the N rows that count: 1
-    where rows and probabilities are spread evenly, more where the same experts get
-    both.  The same inputs give the same bits on every call."""
+def _run_route(logits, top_k, mask, normalize, loss=None):
+    """weights, experts and one tensor that holds counts, prob_sums, rows and, unless `loss` takes it, the loss."""
     code, device, n, e, k, ld = _check_route(logits, top_k)
     mask_ptr, mask_stride = _mask(mask, n, device)
     lib = _lib()
@@ -188,10 +180,31 @@ def route(logits, top_k, *, mask=None, normalize=False) -> Routing:
     ws, ws_ptr = _workspace(size, device)
     at = whole.data_ptr()
     if lib.skmetal_hip_route(code, logits.data_ptr(), ld, mask_ptr, mask_stride, n, e, k, 1 if normalize else 0, weights.data_ptr(), experts.data_ptr(),
-                             at, at + 4 * e, at + 8 * e, at + 8 * e + 4, ws_ptr, size, _stream(device)):
+                             at, at + 4 * e, at + 8 * e, at + 8 * e + 4 if loss is None else loss.data_ptr(), ws_ptr, size, _stream(device)):
         _fail("route")
+    return weights, experts, whole
+
+
+def _statistics(whole):
+    """The parts of _run_route's last tensor."""
+    e = whole.shape[0] // 2 - 1
     counts, sums, rows, loss = whole.split_with_sizes((e, e, 1, 1))
-    return Routing(weights, experts, counts, sums.view(torch.float32), rows, loss.view(torch.float32)[0])
+    return counts, sums.view(torch.float32), rows, loss
+
+
+def route(logits, top_k, *, mask=None, normalize=False) -> Routing:
+    """The `top_k` largest scores of every row of logits [n, e], equal ones by the lowest
+    index, with their softmax probabilities as weights (over the row's e scores;
+    `normalize` divides them by their sum over the chosen ones).  A score of -inf or NaN
+    is excluded; a row that `mask` (bool [n]) leaves out, or whose scores are all
+    excluded, takes no expert (-1, weight 0) and counts nowhere.
+
+    ``loss`` = e / (top_k N^2) sum_j counts_j prob_sums_j over the N rows that count: 1
+    where rows and probabilities are spread evenly, more where the same experts get
+    both.  The same inputs give the same bits on every call."""
+    weights, experts, whole = _run_route(logits, top_k, mask, normalize)
+    counts, sums, rows, loss = _statistics(whole)
+    return Routing(weights, experts, counts, sums, rows, loss.view(torch.float32)[0])
 
 
 def route_backward(logits, routing: Routing, *, grad_weights=None, grad_loss=None, mask=None, normalize=False):
@@ -312,19 +325,24 @@ def adapt_backward(grad, x, down, up, ids, low, *, base=None, gates=None, scales
 class _Routed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, mask, normalize):
-        r = route(logits, top_k, mask=mask, normalize=normalize)
-        ctx.save_for_backward(logits, mask, r.weights, r.experts, r.counts, r.prob_sums, r.rows)
+        # the loss in memory of its own, the statistics whole and only cut apart outside: views that a
+        # Function returns cannot be changed in place
+        loss = torch.empty((), dtype=torch.float32, device=logits.device)
+        weights, experts, whole = _run_route(logits, top_k, mask, normalize, loss)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, mask, weights, experts, whole.clone())  # the caller may add up its own
         ctx.normalize = normalize
-        ctx.mark_non_differentiable(r.experts, r.counts, r.prob_sums, r.rows)
+        ctx.mark_non_differentiable(experts, whole)
         ctx.set_materialize_grads(False)
-        return tuple(r)
+        return weights, experts, whole, loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_weights, _experts, _counts, _sums, _rows, grad_loss):
-        logits, mask, *saved = ctx.saved_tensors
-        grad = route_backward(logits, Routing(*saved, None), grad_weights=None if grad_weights is None else grad_weights.contiguous(), grad_loss=grad_loss,
-                              mask=mask, normalize=ctx.normalize)
+    def backward(ctx, grad_weights, _experts, _whole, grad_loss):
+        logits, mask, weights, experts, whole = ctx.saved_tensors
+        counts, sums, rows, _ = _statistics(whole)
+        grad = route_backward(logits, Routing(weights, experts, counts, sums, rows, None), grad_weights=None if grad_weights is None else grad_weights.contiguous(),
+                              grad_loss=grad_loss, mask=mask, normalize=ctx.normalize)
         return grad, None, None, None
 
 
@@ -346,8 +364,12 @@ class _Adapted(torch.autograd.Function):
 
 
 def routed(logits, top_k, *, mask=None, normalize=False) -> Routing:
-    """``route`` inside autograd: weights and loss pass their gradients to logits."""
-    return Routing(*_Routed.apply(logits, top_k, mask, normalize))
+    """``route`` inside autograd: weights and loss pass their gradients to logits.  loss,
+    counts, prob_sums and rows may be changed in place (weighted, summed over processes);
+    the gradient stays that of this call's own."""
+    weights, experts, whole, loss = _Routed.apply(logits, top_k, mask, normalize)
+    counts, sums, rows, _ = _statistics(whole)
+    return Routing(weights, experts, counts, sums, rows, loss)
 
 
 def adapted(x, down, up, ids, *, base=None, gates=None, scales=None):

@@ -88,6 +88,22 @@ def test_an_out_in_x_asks_for_the_workspace_of_two_launches(calls, monkeypatch):
         assert asked.pop() == call and calls.pop()[0] == "adapt"
 
 
+def test_routed_results_may_be_changed_in_place(calls):
+    from skmetal_amd import experts
+
+    z = torch.zeros(40, 8, requires_grad=True)
+    q = experts.routed(z, 2)
+    loss = q.loss
+    loss.mul_(0.5)
+    loss += q.weights.sum()
+    for statistic in (q.counts, q.prob_sums, q.rows):
+        statistic.add_(1)
+    loss.backward()
+    assert [c[0] for c in calls] == ["route", "route_backward"] and z.grad.shape == z.shape
+    assert q.counts.shape == q.prob_sums.shape == (8,) and q.rows.shape == (1,) and q.loss.shape == ()
+    assert q.counts.dtype == q.rows.dtype == torch.int32 and q.prob_sums.dtype == torch.float32
+
+
 # ---- the entry points' own checks of places, on addresses that nothing reads ----
 
 P = 1 << 20

@@ -52,3 +52,55 @@ def test_out_partly_in_base_is_refused(experts):  # noqa: F811
         with pytest.raises(RuntimeError, match="out shares memory with base"):
             experts.adapt(s["x"][:n], s["down"], s["up"], s["ids"][:n], base=base, out=out)
     experts.adapt(s["x"], s["down"], s["up"], s["ids"], base=wide[:, :12].repeat(1, 2), out=wide[:, 16:])
+
+
+@pytest.mark.parametrize("normalize", [False, True])
+def test_routed_results_changed_in_place(experts, normalize):  # noqa: F811
+    """Statistics summed up and a loss weighted in place leave the gradient as it is."""
+    g = torch.Generator().manual_seed(1)
+    z, dw = torch.randn(300, 24, generator=g).cuda(), torch.randn(300, 3, generator=g).cuda()
+    mask = (torch.rand(300, generator=g) < 0.8).cuda()
+    plain = experts.route(z, 3, mask=mask, normalize=normalize)
+    want = experts.route_backward(z, plain, grad_weights=dw, grad_loss=torch.tensor(0.25, device="cuda"), mask=mask, normalize=normalize)
+    z.requires_grad_()
+    q = experts.routed(z, 3, mask=mask, normalize=normalize)
+    for got, same in zip(q, plain):
+        assert torch.equal(got, same) and got.shape == same.shape and got.dtype == same.dtype
+    total, loss = (q.weights * dw).sum(), q.loss
+    loss.mul_(0.25)
+    loss += total
+    q.counts.add_(1000)
+    q.prob_sums.zero_()
+    q.rows.mul_(8)
+    loss.backward()
+    assert torch.equal(z.grad, want)
+    with torch.no_grad():
+        q = experts.routed(z, 3, mask=mask, normalize=normalize)
+    assert not q.loss.requires_grad and torch.equal(q.counts, plain.counts)
+
+
+def test_routed_in_a_graph(experts):  # noqa: F811
+    """Forward and gradient captured; each replay on new scores, beside eager work."""
+    z = torch.randn(700, 40, device="cuda").bfloat16().requires_grad_()
+    dw, dl = torch.randn(700, 2, device="cuda"), torch.ones((), device="cuda")
+
+    def work():
+        q = experts.routed(z, 2, normalize=True)
+        return [*q, *torch.autograd.grad([q.weights, q.loss], [z], [dw, dl])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for i in range(4):
+        with torch.no_grad():
+            z.copy_(torch.randn(700, 40, device="cuda"))
+        want = work()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, want):
+            assert torch.equal(a, b), i
