@@ -38,7 +38,7 @@ struct PlanArgs {
     Tile* tiles; int ntiles, tile;    // `tile` rows each
     Tile* chunks; int nchunks;  // nullable; `chunk` rows each, one at least per adapter
     int2* merge;         // [a] first slot and number of an adapter's chunks where there are several
-    int chunk;
+    int chunk; bool slot_by_entry;
 };
 
 __device__ __forceinline__ int adapter_of(const int* ids, long stride, long i, int a)
@@ -50,15 +50,15 @@ __device__ __forceinline__ int adapter_of(const int* ids, long stride, long i, i
 // The tiles of adapter q, of `len` rows each (`whole`: one at least, and none for the rows
 // without an adapter).  Tile j of q has the entry start_q / len + q + j: start_(q+1) / len + q + 1
 // is at least that many entries on, so q's block needs no other's count; the entries
-// between stay unused.
-__device__ void write_tiles(int q, int a, int start, int cnt, int len, bool whole, Tile* out, int bound, int2* merge)
+// between stay unused.  `slot` is the first of the slots that the tiles take where they are several.
+__device__ void write_tiles(int q, int a, int start, int cnt, int len, bool whole, Tile* out, int bound, int slot, int2* merge)
 {
     const int first = start / len + q;
     const int tiles = !whole ? (cnt + len - 1) / len : q == a ? 0 : max(1, (cnt + len - 1) / len);
     const int next = q == a ? bound : (start + cnt) / len + q + 1;
     for (int j = threadIdx.x; first + j < next; j += kPlanThreads)
-        out[first + j] = j < tiles ? Tile{q, start + j * len, min(len, cnt - j * len), whole && tiles > 1 ? first + j : -1} : Tile{-1, 0, 0, -1};
-    if (merge != nullptr && q < a && threadIdx.x == 0) merge[q] = make_int2(first, tiles > 1 ? tiles : 0);
+        out[first + j] = j < tiles ? Tile{q, start + j * len, min(len, cnt - j * len), whole && tiles > 1 ? slot + j : -1} : Tile{-1, 0, 0, -1};
+    if (merge != nullptr && q < a && threadIdx.x == 0) merge[q] = make_int2(slot, tiles > 1 ? tiles : 0);
 }
 
 // The keys of a segment of kPlanRows rows, a wave's side by side (a + 1: no row).
@@ -149,8 +149,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs p)
         place += __popcll(m);
     }
     if (blockIdx.y != 0) return;
-    write_tiles(q, p.a, start, cnt, p.tile, false, p.tiles, p.ntiles, nullptr);
-    if (p.chunks != nullptr) write_tiles(q, p.a, start, cnt, p.chunk, true, p.chunks, p.nchunks, p.merge);
+    write_tiles(q, p.a, start, cnt, p.tile, false, p.tiles, p.ntiles, 0, nullptr);
+    // Slots by the chunks' entries, or, where that takes fewer, from 2 start / chunk on: an adapter of several
+    // chunks has more than `chunk` rows, of which floor(2 cnt / chunk) is no less than ceil(cnt / chunk).
+    if (p.chunks != nullptr) write_tiles(q, p.a, start, cnt, p.chunk, true, p.chunks, p.nchunks, p.slot_by_entry ? start / p.chunk + q : 2 * start / p.chunk, p.merge);
 }
 
 // ---- loads of 16 bytes of a row, the elements past `left` as 0 ----
@@ -1124,6 +1126,7 @@ struct Layout {
     long n; int a, r;
     bool direct, fused, split;            // fused: k_direct; split: k_outer_split
     int tile, ntiles, nchunks, chunk, segments;
+    int slots; bool slot_by_entry;        // partial sums of chunks
     long full_tiles;                      // of n rows, were they all of one adapter
     int rp;
     int down_splits, up_splits;           // of d (t = D x) and of o (u = U dy)
@@ -1195,6 +1198,8 @@ Layout layout(int type, long n, int d, int o, int r, int a, AdaptCall call)
     if (L.segments < 1) L.segments = 1;
     L.chunk = chunk_rows(n, d, o, a, type);
     L.nchunks = (int)(n / L.chunk) + a;
+    L.slot_by_entry = L.nchunks <= 2 * n / L.chunk;
+    L.slots = n <= L.chunk ? 0 : L.slot_by_entry ? L.nchunks : (int)(2 * n / L.chunk);
     L.ld_t = ((n + 63) & ~63l) + 160;  // 128 rows past the last (k_outer_split's most at once); not a power of two apart
     const int zs = (r + 63) / 64;
     L.down_splits = split_count(L.full_tiles, d, type, zs);
@@ -1214,8 +1219,8 @@ Layout layout(int type, long n, int d, int o, int r, int a, AdaptCall call)
         take(L.low, L.split ? 0 : (size_t)n * r * 4);
         take(L.low_t, L.split ? (size_t)3 * r * L.ld_t * 2 : 0);
         take(L.dot_t, L.split ? (size_t)3 * r * L.ld_t * 2 : 0);
-        take(L.dpart, (size_t)L.nchunks * r * d * 4);
-        take(L.upart, (size_t)L.nchunks * r * o * 4);
+        take(L.dpart, (size_t)L.slots * r * d * 4);
+        take(L.upart, (size_t)L.slots * r * o * 4);
     }
     L.bytes = at;
     return L;
@@ -1226,7 +1231,7 @@ hipError_t launch_plan(const Layout& L, const int* ids, long ids_stride, char* w
     const PlanArgs p{ids, ids_stride, (int)L.n, L.a, reinterpret_cast<int2*>(ws + L.seen), reinterpret_cast<int*>(ws + L.perm),
                      reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles, L.tile,
                      backward ? reinterpret_cast<Tile*>(ws + L.chunks) : nullptr, L.nchunks,
-                     backward ? reinterpret_cast<int2*>(ws + L.merge) : nullptr, L.chunk};
+                     backward ? reinterpret_cast<int2*>(ws + L.merge) : nullptr, L.chunk, L.slot_by_entry};
     const dim3 grid(L.a + 1, L.segments);
     if (L.segments > 1) SKM_TRY_LAUNCH(k_plan_count, grid, kPlanThreads, 0, s, p);
     return launch(k_plan, grid, kPlanThreads, 0, s, p);

@@ -182,3 +182,19 @@ def test_gradients_share_no_memory_with_what_they_are_made_of(lib):
     assert route_back(2 * P) == ENODEV and route_back(P) == ENODEV
     for bad in ((P + 4,), (P + 4 * 39,), (P, 9)):
         assert route_back(*bad) == EINVAL and b"grad_logits shares memory" in lib.skmetal_hip_last_error(), bad
+
+
+@pytest.mark.parametrize("n,d,o,r,a", [(600, 4096, 4096, 16, 2048), (2048, 4096, 4096, 128, 2048), (16_384, 4096, 4096, 64, 2048), (513, 64, 64, 8, 2000),
+                                       (100_000, 256, 512, 16, 1000), (16_384, 4096, 4096, 64, 64), (8192, 2048, 2048, 32, 8), (5000, 777, 1001, 5, 1)])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_backward_workspace_follows_the_rows(n, d, o, r, a, dtype):
+    """Not the adapters, however many: partial sums are those of adapters with more rows than
+    a chunk's 64 or more, at most 2 n / 64 of them; beside them the low-rank rows (up to 8
+    parts of a sum in fp32, and two sets of three bf16 a rank and up to 256 places more), and a
+    few numbers a row and an adapter."""
+    from skmetal_amd import _bridge
+
+    rp = -(-r // 16) * 16
+    most = 2 * n // 64 * r * (d + o) * 4 + 8 * n * rp * 4 + 12 * r * (n + 256) + 16 * n + 64 * (a + 1) + 8 * (n // 16384 + 1) * (a + 1) + 1024
+    size = _bridge._lib.skmetal_hip_adapt_workspace(dtype, n, d, o, r, a, 1)
+    assert 0 < size <= most
