@@ -282,6 +282,9 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
         out_ptr = out.data_ptr()
     else:
         out_ld = _rows(out, "out", dtype, (n, o), device)
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out requires a gradient, which this call does not record: use adapted, or torch.no_grad")
+        torch.autograd.graph.increment_version(out)
         out_ptr, es = out.data_ptr(), dtype.itemsize
         if x_ptr < out_ptr + (n * out_ld + o) * es and out_ptr < x_ptr + (n * x_ld + d) * es:
             call = _ADAPT_IN_X  # or between x's rows, which the library finds out

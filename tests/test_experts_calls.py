@@ -104,6 +104,31 @@ def test_routed_results_may_be_changed_in_place(calls):
     assert q.counts.dtype == q.rows.dtype == torch.int32 and q.prob_sums.dtype == torch.float32
 
 
+def test_out_is_known_to_autograd(calls):
+    """A result in place counts as a change of it: a gradient that needs its old values says
+    so, and a tensor on the way of a gradient is refused, since the call records none."""
+    from skmetal_amd import experts
+
+    s = problem()
+    w = torch.ones(24, requires_grad=True)
+    y = torch.zeros(40, 24)
+    z = y * w  # keeps y for w's gradient
+    experts.adapt(s["x"], s["down"], s["up"], s["ids"], base=y, out=y)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        z.sum().backward()
+    z = torch.zeros(40, 24) * w
+    assert len(calls) == 1
+    with pytest.raises(ValueError, match="out requires a gradient"):
+        experts.adapt(s["x"], s["down"], s["up"], s["ids"], base=z, out=z)
+    assert len(calls) == 1
+    with torch.no_grad():
+        experts.adapt(s["x"], s["down"], s["up"], s["ids"], base=z, out=z)
+    with torch.inference_mode():
+        t = torch.zeros(40, 24)
+        experts.adapt(s["x"], s["down"], s["up"], s["ids"], out=t)
+    assert len(calls) == 3
+
+
 # ---- the entry points' own checks of places, on addresses that nothing reads ----
 
 P = 1 << 20
