@@ -33,10 +33,16 @@ def _find_library() -> str:
     raise RuntimeError(f"{LIB_NAME} not found; build it with `python -m skmetal_amd._build`")
 
 
+_torch_runtime_error = None  # why torch's runtime could not be loaded
+
+
 def _share_torch_runtime() -> None:
     """A process has one HIP runtime that its tensors and streams belong to.  A ROCm build
     of PyTorch brings its own libamdhip64; loading that one first (torch itself is not
-    imported) makes this library bind to it whichever of the two is imported first."""
+    imported) makes this library bind to it whichever of the two is imported first.  Where
+    that fails the library uses ROCm's own: KMeans needs no torch, and
+    require_torch_runtime says what became of it."""
+    global _torch_runtime_error
     if "torch" in sys.modules:
         return
     try:
@@ -44,8 +50,8 @@ def _share_torch_runtime() -> None:
         path = Path(spec.origin).parent / "lib" / "libamdhip64.so" if spec is not None and spec.origin else None
         if path is not None and path.exists():
             ctypes.CDLL(str(path))
-    except Exception:  # noqa: BLE001 -- the library then uses ROCm's own runtime
-        pass
+    except (ImportError, ValueError, OSError) as e:
+        _torch_runtime_error = str(e)
 
 
 def require_torch_runtime() -> None:
@@ -53,7 +59,8 @@ def require_torch_runtime() -> None:
     with open("/proc/self/maps") as f:
         runtimes = sorted({line.split()[-1] for line in f if "/libamdhip64.so" in line})
     if len(runtimes) > 1:
-        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(runtimes)}): import torch before skmetal_amd")
+        why = f"; torch's did not load before this library: {_torch_runtime_error}" if _torch_runtime_error else ""
+        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(runtimes)}): import torch before skmetal_amd, and use a torch of this library's ROCm version{why}")
 
 
 _c_size = ctypes.c_size_t

@@ -223,3 +223,24 @@ def test_backward_workspace_follows_the_rows(n, d, o, r, a, dtype):
     most = 2 * n // 64 * r * (d + o) * 4 + 8 * n * rp * 4 + 12 * r * (n + 256) + 16 * n + 64 * (a + 1) + 8 * (n // 16384 + 1) * (a + 1) + 1024
     size = _bridge._lib.skmetal_hip_adapt_workspace(dtype, n, d, o, r, a, 1)
     assert 0 < size <= most
+
+
+def test_a_torch_runtime_that_does_not_load_is_named(monkeypatch, tmp_path):
+    """KMeans does without it; the operators on torch's tensors say why they cannot run."""
+    import importlib.machinery
+    import importlib.util
+    import io
+    import sys
+
+    from skmetal_amd import _bridge
+
+    (tmp_path / "lib").mkdir()
+    (tmp_path / "lib" / "libamdhip64.so").write_text("not a library")
+    monkeypatch.delitem(sys.modules, "torch", raising=False)
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name: importlib.machinery.ModuleSpec(name, None, origin=str(tmp_path / "__init__.py")))
+    monkeypatch.setattr(_bridge, "_torch_runtime_error", None)
+    _bridge._share_torch_runtime()
+    maps = "7f00-7f01 r-xp 00000000 00:00 0    /a/libamdhip64.so.7\n7f02-7f03 r-xp 00000000 00:00 0    /b/libamdhip64.so\n"
+    monkeypatch.setattr("builtins.open", lambda *a, **k: io.StringIO(maps))
+    with pytest.raises(RuntimeError, match="two HIP runtimes .*libamdhip64.so: (invalid|file too short)"):
+        _bridge.require_torch_runtime()
