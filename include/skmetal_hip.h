@@ -346,7 +346,9 @@ SKMETAL_API int skmetal_hip_device(void);
 
 /* Top-k routing with the balance loss.  logits [n x E]; mask (nullable, one
  * byte a row, mask_stride bytes apart): rows that count.  E <= 2048, 1 <= k <=
- * min(E, 16), n < 2^31.  A score of -inf or NaN is excluded.
+ * min(E, 16), n < 2^31.  A score of -inf or NaN is excluded; one of +inf is
+ * the largest and makes its row's probabilities NaN, and with them prob_sums
+ * and loss.
  *   weights, experts [n x k]: per row the experts of the k largest scores,
  *     largest first, equal scores by the lowest index, and their softmax
  *     probabilities (normalize != 0: divided by their sum).  A row that is

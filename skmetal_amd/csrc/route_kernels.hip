@@ -7,7 +7,8 @@
 //   c_j = rows that take j,  S_j = sum_i p_ij,  N = rows that count
 //   loss = E / (k N^2) sum_j c_j S_j
 // A score of -inf or NaN is excluded: probability 0, never taken.  A row that is masked
-// or has no score left takes no expert (-1, weight 0) and counts nowhere.
+// or has no score left takes no expert (-1, weight 0) and counts nowhere.  +inf is a score:
+// the largest, and its row's probabilities are NaN, as inf - inf is.
 //
 // One pass over the scores each way.  A row lies on L lanes (1, 8, 16 or 64), NC times eight columns a
 // lane (column = (c L + lane) 8 + e), so a wave takes 64 / L rows at once and a row's sums
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArg
             for (int i = 0; i < SL; ++i) {
                 const int t = i * L + j;
                 if (t >= a.k) continue;
-                a.w[row * a.k + t] = w[i] * scale;
+                a.w[row * a.k + t] = ex[i] >= 0 ? w[i] * scale : 0.f;  // 0 beside a score of +inf too, whose row's scale is NaN
                 a.ex[row * a.k + t] = ex[i];
                 if (ex[i] >= 0) atomicAdd(&counts[ex[i]], 1);
             }

@@ -197,7 +197,8 @@ def route(logits, top_k, *, mask=None, normalize=False) -> Routing:
     index, with their softmax probabilities as weights (over the row's e scores;
     `normalize` divides them by their sum over the chosen ones).  A score of -inf or NaN
     is excluded; a row that `mask` (bool [n]) leaves out, or whose scores are all
-    excluded, takes no expert (-1, weight 0) and counts nowhere.
+    excluded, takes no expert (-1, weight 0) and counts nowhere.  A score of +inf is the
+    largest, and its row's weights are NaN like a softmax's, prob_sums and loss with them.
 
     ``loss`` = e / (top_k N^2) sum_j counts_j prob_sums_j over the N rows that count: 1
     where rows and probabilities are spread evenly, more where the same experts get

@@ -104,3 +104,33 @@ def test_routed_in_a_graph(experts):  # noqa: F811
         torch.cuda.synchronize()
         for a, b in zip(held, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("e", [24, 200, 600])
+def test_route_infinite_score(experts, e, normalize, dtype):  # noqa: F811
+    """+inf is a score: the largest, and its row's probabilities are NaN as a softmax's are.
+    Which experts a row takes, the places that hold none, masked rows and the other rows
+    stay what they are."""
+    g = torch.Generator().manual_seed(e)
+    z = torch.randn(60, e, generator=g).to(TYPES[dtype])
+    z[3, 7] = z[9, 5] = z[9, 2] = z[20, 1] = float("inf")
+    z[9, :2] = -float("inf")
+    z[9, 6:] = float("nan")  # leaves 2, 3, 4 and 5
+    mask = torch.arange(60) != 20
+    clean = z.clone()
+    clean[3, 7], clean[9, 5], clean[9, 2] = 100.0, 100.0, 100.0
+    clean[20] = 0.0
+    z, clean, mask = z.cuda(), clean.cuda(), mask.cuda()
+    r, c = (experts.route(t, 6, mask=mask, normalize=normalize) for t in (z, clean))
+    assert torch.equal(r.experts, c.experts) and torch.equal(r.counts, c.counts) and torch.equal(r.rows, c.rows)
+    assert r.experts[9].tolist()[:2] == [2, 5] and r.experts[9].tolist()[4:] == [-1, -1]
+    rest = torch.ones(60, dtype=torch.bool)
+    rest[[3, 9]] = False
+    assert torch.equal(r.weights[rest], c.weights[rest])
+    assert r.weights[3].isnan().all() and r.weights[9, :4].isnan().all() and (r.weights[9, 4:] == 0).all()
+    assert r.prob_sums.isnan().any() and r.loss.isnan()
+    dw, dl = torch.randn(60, 6, generator=g).cuda(), torch.ones((), device="cuda")
+    a, b = (experts.route_backward(t, q, grad_weights=dw, grad_loss=dl, mask=mask, normalize=normalize) for t, q in ((z, r), (clean, c)))
+    assert torch.equal(a[rest], b[rest]) and a[3].isnan().any() and (a[20] == 0).all()
