@@ -204,8 +204,9 @@ def route(logits, top_k, *, mask=None, normalize=False) -> Routing:
     where rows and probabilities are spread evenly, more where the same experts get
     both.  The same inputs give the same bits on every call."""
     weights, experts, whole = _run_route(logits, top_k, mask, normalize)
-    counts, sums, rows, loss = _statistics(whole)
-    return Routing(weights, experts, counts, sums, rows, loss.view(torch.float32)[0])
+    e = logits.shape[1]
+    counts, sums, rows, loss = whole.split_with_sizes((e, e, 1, 1))
+    return Routing(weights, experts, counts, sums.view(torch.float32), rows, loss.view(torch.float32)[0])
 
 
 def route_backward(logits, routing: Routing, *, grad_weights=None, grad_loss=None, mask=None, normalize=False):
