@@ -244,7 +244,10 @@ def _adapters(t, name, dtype, device):
 
 def _check_adapt(x, first, down, up, ids, gates, scales):
     code, device = _first(x, first)
-    n = x.shape[0]
+    n, width = x.shape
+    ld, one = x.stride()
+    if one != 1 and width > 1:
+        raise ValueError(f"{first}'s rows must have their elements side by side (stride(1) is {one})")
     dtype = x.dtype
     a, r, d, down_sa, down_ld = _adapters(down, "down", dtype, device)
     a2, r2, o, up_sa, up_ld = _adapters(up, "up", dtype, device)
@@ -256,7 +259,7 @@ def _check_adapt(x, first, down, up, ids, gates, scales):
     gate_ptr, gate_stride = (None, 0) if gates is None else (gates.data_ptr(), _vector(gates, "gates", torch.float32, n, device))
     scale_ptr = None if scales is None else _dense(scales, "scales", torch.float32, (a,), device)
     shared = (down.data_ptr(), down_sa, down_ld, up.data_ptr(), up_sa, up_ld, ids.data_ptr(), ids_stride, gate_ptr, gate_stride, scale_ptr)
-    return code, device, n, d, o, r, a, shared
+    return code, device, n, d, o, r, a, width, ld, shared
 
 
 def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, return_low=False):
@@ -271,11 +274,10 @@ def adapt(x, down, up, ids, *, base=None, gates=None, scales=None, out=None, ret
     and out have one type.  `out` may be base and may share memory with x (a residual
     stream in place: base=x, out=x); nothing else may share memory with it.  With `return_low` also returns down_q
     x_i, float32 [n, r], for ``adapt_backward``."""
-    code, device, n, d, o, r, a, shared = _check_adapt(x, "x", down, up, ids, gates, scales)
-    if x.shape[1] != d:
-        raise ValueError(f"x has {x.shape[1]} columns, down has {d}")
+    code, device, n, d, o, r, a, width, x_ld, shared = _check_adapt(x, "x", down, up, ids, gates, scales)
+    if width != d:
+        raise ValueError(f"x has {width} columns, down has {d}")
     dtype = x.dtype
-    x_ld = _rows(x, "x", dtype, (n, d), device)
     base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, o), device))
     lib = _lib()
     x_ptr, call = x.data_ptr(), _ADAPT
@@ -305,11 +307,10 @@ def adapt_backward(grad, x, down, up, ids, low, *, base=None, gates=None, scales
     projection's part; None: 0); the gradient of the forward call's base is grad
     itself.  Those of down and up have their shapes and type, 0 for an adapter without
     rows; that of gates is None where there are none."""
-    code, device, n, d, o, r, a, shared = _check_adapt(grad, "grad", down, up, ids, gates, scales)
-    if grad.shape[1] != o:
-        raise ValueError(f"grad has {grad.shape[1]} columns, up has {o}")
+    code, device, n, d, o, r, a, width, grad_ld, shared = _check_adapt(grad, "grad", down, up, ids, gates, scales)
+    if width != o:
+        raise ValueError(f"grad has {width} columns, up has {o}")
     dtype = grad.dtype
-    grad_ld = _rows(grad, "grad", dtype, (n, o), device)
     x_ld = _rows(x, "x", dtype, (n, d), device)
     low_ptr = _dense(low, "low", torch.float32, (n, r), device)
     base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, d), device))
