@@ -1108,11 +1108,23 @@ bool is_direct(long n, int d, int o, int rp)
 
 // Whether such a call's two products are one launch, every block of a row computing its
 // low-rank vector anew: where that reads little, 32 MiB of M in all and 128 KiB a block (64 KiB
-// in fp32, whose matrix instructions take four times as long for it).  Launch after launch, d = o,
-// two kernels and one, bf16: 1 row of 256, rank 64: 8.7 and 4.9 us; 64 of 1,024, rank 8: 7.6 and
-// 6.7; rank 64: 10.9 and 9.2; 64 of 4,096, rank 8: 9.4 and 7.5; fp32: 64 of 1,024, rank 8: 7.7 and
-// 6.3.  Beyond, bf16: 1 of 4,096, rank 64: 10.9 and 20.1; 128 of 4,096, rank 8: 12.9 and 14.4;
-// fp32: 1 of 1,024, rank 32: 8.1 and 8.9.
+// in fp32, whose matrix instructions take four times as long for it).  A second launch and its
+// workspace also cost the caller 4 us on the host (300 fp32 rows of 768, rank 16, forward and
+// backward from Python: 31.6 us with one, 36.2 with two).  Launch after launch, d = o, two kernels
+// and one:
+//   bf16:  1 row of 256, rank 64: 8.7, 4.9;   64 of 1,024, rank 8: 7.6, 6.8;   256 of 1,024, rank 8: 8.7, 6.7
+//         64 of 1,024, rank 64: 10.9, 9.4;    64 of 4,096, rank 8: 9.5, 7.5;   512 of 512, rank 32: 10.2, 6.9
+//         96 of 2,048, rank 32: 10.5, 9.0;   128 of 2,048, rank 32: 11.0, 10.0
+//   fp16: 512 of 1,024, rank 8: 11.2, 9.1;   256 of 2,048, rank 8: 11.3, 8.4
+//   fp32: 256 of 1,024, rank 8: 10.1, 9.1;   512 of 512, rank 32: 15.8, 12.2
+// Within the limits and slower on the device, for the host's sake, where more than 256 blocks
+// (one a CU) take a second turn:
+//   bf16: 288 of 1,024, rank 8: 9.7, 11.7;   320 of 1,536, rank 8: 10.7, 15.4; 160 of 1,536, rank 32: 11.0, 12.8
+//   fp32: 288 of 768, rank 8: 10.4, 11.9
+// Beyond the limits:
+//   bf16:  72 of 4,096, rank 8: 11.1, 13.3;   96: 10.6, 13.5;   1 of 4,096, rank 64: 10.9, 20.3;   64 of 2,048, rank 64: 11.7, 14.5
+//   fp16:  96 of 4,096, rank 8: 11.0, 11.5
+//   fp32:   1 of 1,024, rank 32: 8.1, 8.9;    48 of 4,096, rank 8: 10.3, 22.4
 bool is_fused(long n, int d, int o, int rp, int type)
 {
     const size_t wide = d > o ? d : o, es = elem_size(type), cols = kDirectThreads / 4 * (16 / es);  // columns a block

@@ -111,3 +111,11 @@ def test_adapt_long_runs_in_large_tiles(experts, dtype):  # noqa: F811
     at = torch.arange(40_003)
     s["ids"] = torch.where(at % 11 == 0, -1, torch.where(at < 39_000, 7, at % 300)).int().cuda()
     check_adapt(experts, s, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,r", [(256, 1024, 8), (257, 1024, 8), (128, 1536, 32), (129, 1536, 32), (512, 512, 20), (340, 768, 3), (64, 4096, 9), (65, 4096, 9), (511, 256, 60)])
+def test_adapt_few_rows_in_one_turn_and_two(experts, n, d, r, dtype):  # noqa: F811
+    """Calls of 256 blocks of one launch, one a CU, and of more."""
+    print("adapt one launch", n, d, r, dtype, flush=True)
+    check_adapt(experts, problem(n, d, d, r, 7, dtype, n + d), dtype)
