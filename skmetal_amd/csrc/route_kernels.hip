@@ -172,7 +172,8 @@ __device__ __forceinline__ float balance_loss(double dot, int E, int k, int rows
 // registers for the exponentials and the column sums, which a wave keeps over all its rows.
 // At 131,072 x 256 bf16, k = 8, 40 us (67 MB: 13 us to read): some 900 vector instructions for
 // a wave's 8 rows bound it, about 400 of them the choice's.  ONE: a single block, a wave a
-// group of rows; 96 x 256, k = 8 takes 12 us, its instructions' first fetch most of it.
+// group of rows; 96 x 256, k = 8 takes 12 us on one CU, of which its 12 waves' instructions
+// are some 4.5 by their count; the launch and each instruction's first fetch are among the rest.
 template <typename T, int L, int NC, int KP, bool ONE>
 __global__ __launch_bounds__(ONE ? kOneThreads : kThreads) void k_route(RouteArgs a, int nb, float* psum, int* pcnt, int* prow, unsigned* ticket)
 {
@@ -613,6 +614,9 @@ hipError_t launch_route_back(const RouteBackArgs& a, hipStream_t s)
 {
     if (a.n == 0) return hipSuccess;
     const long rw = 64 / row_lanes(a.E), b = ((a.n + rw - 1) / rw + kThreads / 64 - 1) / (kThreads / 64);
+    // A row of one step of columns a lane leaves registers for six blocks a CU.  us with three and with
+    // six: bf16, 131,072 x 37 12.8, 11.7; x 64 13.5, 12.7; 50,003 x 37 7.5, 7.2; x 64 7.4, 8.2 (27 blocks
+    // past the six); fp32, 131,072 x 37 16.2, 14.7.  Four steps: 131,072 x 256 34.0, 42.7.
     const long most = a.E <= 64 && a.E > 32 ? 2 * kMaxBlocks : kMaxBlocks;
     const int nb = (int)(b < most ? b : most);
     return with_type(a.type, [&](auto t) {
