@@ -257,7 +257,7 @@ struct ShrinkArgs {
 // are split over blocks where there are too few tiles to keep the memory busy.
 //
 // Bound by the reading: 8,192 bf16 rows of 4,096, rank 16, take 18 us (3.6 TB/s).  At rank 64
-// (16,384 rows, 64 adapters: 56 us) an adapter is as long as its tile's rows, first read
+// (16,384 rows, 64 adapters: 58 us) an adapter is as long as its tile's rows, first read
 // from memory, and the waves' sums take 7 us to meet.
 template <typename T, int RT, int NB>
 __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs<T> p)
@@ -648,9 +648,9 @@ __device__ __forceinline__ void expand_columns(const ExpandArgs<T>& p, const Til
 // every parts-th stretch of 64 * kVec columns, 16 * kVec a wave, which keeps M_q for them in
 // registers.  KP: the ranks, rounded up.
 //
-// Bound by the base read and the result written: 8,192 bf16 rows of 4,096, rank 16, take 28 us
-// (4.8 TB/s), 16,384 at rank 64 75 us (3.6 TB/s: the adapters' reads and the low-rank rows
-// staged in every block come on top).
+// Bound by the base read and the result written: 8,192 bf16 rows of 4,096, rank 16, take 27 us
+// (5.0 TB/s), 16,384 at rank 64 82 us (3.3 TB/s: the adapters' reads and the low-rank rows
+// staged in every block come on top), 105 backward with those written by rank.
 template <typename T, int RT, int KP, bool BACK>
 __global__ __launch_bounds__(256, KP <= 32 ? 3 : KP <= 64 ? 2 : 1) void k_expand(ExpandArgs<T> p)
 {
