@@ -134,3 +134,36 @@ def test_route_infinite_score(experts, e, normalize, dtype):  # noqa: F811
     dw, dl = torch.randn(60, 6, generator=g).cuda(), torch.ones((), device="cuda")
     a, b = (experts.route_backward(t, q, grad_weights=dw, grad_loss=dl, mask=mask, normalize=normalize) for t, q in ((z, r), (clean, c)))
     assert torch.equal(a[rest], b[rest]) and a[3].isnan().any() and (a[20] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,e,k", [(70, 40, 3), (30_001, 200, 4)])
+def test_gradient_of_the_scores_in_their_place(experts, n, e, k, dtype):  # noqa: F811
+    """The C entry's grad_logits over logits, from one group of rows a wave and from several."""
+    g = torch.Generator().manual_seed(n)
+    z = torch.randn(n, e, generator=g).to(TYPES[dtype]).cuda()
+    dw, dl = torch.randn(n, k, generator=g).cuda(), torch.ones((), device="cuda")
+    r = experts.route(z, k)
+    want = experts.route_backward(z, r, grad_weights=dw, grad_loss=dl)
+    code = experts._lib().skmetal_hip_route_backward(experts._CODE[z.dtype], z.data_ptr(), e, None, 0, n, e, k, 0, r.weights.data_ptr(), r.experts.data_ptr(), r.counts.data_ptr(),
+                                                     r.rows.data_ptr(), dw.data_ptr(), dl.data_ptr(), z.data_ptr(), e, experts._stream(z.device))
+    assert code == 0 and torch.equal(z, want)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [20, 150, 700])
+def test_gradient_of_the_rows_in_place_of_its_base(experts, n, dtype):  # noqa: F811
+    """The C entry's grad_x over its base."""
+    d, o, r, a = 1100, 96, 20, 4
+    s = problem(n, d, o, r, a, dtype, n)
+    _, low = experts.adapt(s["x"], s["down"], s["up"], s["ids"], return_low=True)
+    want = experts.adapt_backward(s["grad"], s["x"], s["down"], s["up"], s["ids"], low, base=s["grad_base"])
+    place, down, up = s["grad_base"].clone(), torch.empty_like(s["down"]), torch.empty_like(s["up"])
+    code, stream = experts._CODE[TYPES[dtype]], experts._stream(place.device)
+    size = experts._adapt_workspace(code, n, d, o, r, a, 1)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    at = place.data_ptr()
+    done = experts._lib().skmetal_hip_adapt_backward(code, s["grad"].data_ptr(), o, s["x"].data_ptr(), d, s["down"].data_ptr(), r * d, d, s["up"].data_ptr(), r * o, o, s["ids"].data_ptr(),
+                                                     1, None, 0, None, low.data_ptr(), at, d, at, d, down.data_ptr(), up.data_ptr(), None, n, d, o, r, a, ws.data_ptr(), size, stream)
+    assert done == 0
+    assert torch.equal(place, want.x) and torch.equal(down, want.down) and torch.equal(up, want.up)
