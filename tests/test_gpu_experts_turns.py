@@ -32,10 +32,10 @@ def test_adapters_of_several_chunks_among_many(experts, n, a, dtype):  # noqa: F
     check_adapt(experts, s, dtype)
 
 
-# ---- route: 768 blocks of four waves take 3,072 groups of rows at once (twice that backward for 33 to 64
+# ---- route: 768 blocks of four waves take a group of rows each at once (twice that backward for 33 to 64
 # experts); a group has 64 rows up to 32 experts, 8 up to 256, 4 up to 512, one beyond ----
 
-WAVES = 3072
+WAVES = 768 * 4
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
