@@ -408,6 +408,45 @@ SKMETAL_API int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t l
                                            void* grad_down, void* grad_up, float* grad_gates, size_t n, size_t d, size_t o,
                                            size_t r, size_t a, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- dropout and log probabilities: device pointers and streams as above ----
+ *
+ * out_ij = base_ij + (word(i d + j) >= p 2^32 ? x_ij / (1 - p) : 0)   for x, base
+ * (nullable: 0) and out [n x d], 0 <= p < 1.  word(e) is number e mod 4 of the
+ * four 32-bit words of Philox4x32-10 with the counter (e / 4: 64 bits, site, low
+ * 32 bits of key[1]) and the 64-bit seed key[0]; key [2] is in device memory, so
+ * that a captured graph may change it between replays.  A dropped x does not
+ * reach out, not even a NaN.  The gradient of x is the same call on that of out
+ * (base NULL), the gradient of base is that of out.  out may be x or base (the
+ * same address and distance of rows).  n, d < 2^31. */
+SKMETAL_API int skmetal_hip_drop(int dtype, const void* x, size_t ld_x, const void* base, size_t ld_base, void* out,
+                                 size_t ld_out, size_t n, size_t d, double p, const int64_t* key, uint32_t site,
+                                 void* stream);
+
+/* Of every row of scores [n x v], all fp32: log_probs [n], the log probability of
+ * its target (targets int32, targets_stride elements apart; outside [0, v): none,
+ * log_probs 0); entropy [n] of its softmax; lse [n], the log of its sum of exp,
+ * and lse_rest [n], what fp32 leaves out of that; top, top_log_probs [n x k]
+ * (k <= 16, 0: not written): the places of the k largest scores, largest first,
+ * equal ones by the lowest place, and their log probabilities.  A score of -inf
+ * or NaN is excluded: log probability -inf, never among the largest (-1 in the
+ * places that remain).  A row without a score left has lse -inf and entropy 0;
+ * one with a score of +inf has NaN for its log probabilities and entropy.
+ * v <= 2^22.  The same inputs give the same bits on every call. */
+SKMETAL_API size_t skmetal_hip_rate_workspace(int dtype, size_t n, size_t v, size_t k);
+SKMETAL_API int skmetal_hip_rate(int dtype, const void* logits, size_t ld_logits, const int32_t* targets,
+                                 size_t targets_stride, size_t n, size_t v, size_t k, float* log_probs, float* entropy,
+                                 float* lse, float* lse_rest, int32_t* top, float* top_log_probs, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+/* grad_logits [n x v] from the gradients of log_probs, entropy and lse [n] (each
+ * nullable: no gradient), with lse, lse_rest and entropy as skmetal_hip_rate gave
+ * them.  Excluded scores get 0.  grad_logits may be logits (the same address and
+ * distance of rows). */
+SKMETAL_API int skmetal_hip_rate_backward(int dtype, const void* logits, size_t ld_logits, const int32_t* targets,
+                                          size_t targets_stride, size_t n, size_t v, const float* lse,
+                                          const float* lse_rest, const float* entropy, const float* grad_log_probs,
+                                          const float* grad_entropy, const float* grad_lse, void* grad_logits,
+                                          size_t ld_grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -43,6 +43,8 @@ SOURCES = [
     ("sample_kernels.hip", []),
     ("route_kernels.hip", []),
     ("adapt_kernels.hip", []),
+    ("drop_kernels.hip", []),
+    ("rate_kernels.hip", []),
     ("skmetal_hip.hip", VGPR_FORM),
 ]
 

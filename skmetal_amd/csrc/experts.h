@@ -1,5 +1,5 @@
 // experts.h -- the operators of skmetal_amd.experts: argument blocks and launchers
-// (route_kernels.hip, adapt_kernels.hip).  Everything is in device memory and every
+// (route_kernels.hip, adapt_kernels.hip, feed_kernels.hip, drop_kernels.hip, rate_kernels.hip).  Everything is in device memory and every
 // launch goes to the caller's stream; nothing here allocates or waits.
 #pragma once
 
@@ -83,5 +83,46 @@ enum AdaptCall : int { kAdapt = 0, kAdaptBackward = 1, kAdaptInX = 2 };
 size_t adapt_workspace(int type, long n, int d, int o, int r, int a, AdaptCall call);
 // Whether every launch of both directions has a grid that the device takes.
 bool adapt_fits(int type, long n, int d, int o, int r, int a);
+
+// ---- drop_kernels.hip ----
+
+struct DropCall {
+    int type; long n, d;
+    const void* x; long ld_x;                          // [n x d]
+    const void* base; long ld_base;                    // nullable, [n x d]
+    void* out; long ld_out;                            // [n x d]; may be x or base
+    const long long* key; unsigned site;               // key: seed, step
+    unsigned limit; float scale;                       // p 2^32, 1 / (1 - p)
+};
+hipError_t launch_drop(const DropCall& a, hipStream_t s);
+
+// ---- rate_kernels.hip ----
+
+constexpr int kRateMaxK = 16;       // largest scores a row names
+constexpr int kRateMaxV = 1 << 22;  // scores a row
+constexpr int kRateSplits = 64;     // parts a row
+constexpr int kRateList = 4096;     // scores that a part's choice looks at twice, at most
+
+struct RateCall {
+    const void* z; int type; long n; int v; long ld;   // scores [n x v]
+    const int* targets; long target_stride;            // [n]; outside [0, v): none
+    int k;
+    float* log_probs; float* entropy; float* lse; float* rest;  // [n]
+    int* top; float* top_log_probs;                    // [n x k]
+    char* ws;                                          // rate_workspace() bytes
+};
+hipError_t launch_rate(const RateCall& a, hipStream_t s);
+size_t rate_workspace(long n, int v, int type, int k);
+// Whether every launch of both directions has a grid that the device takes.
+bool rate_fits(long n, int v, int type, int k);
+
+struct RateBackCall {
+    const void* z; int type; long n; int v; long ld;
+    const int* targets; long target_stride;
+    const float* lse; const float* rest; const float* entropy;   // launch_rate's
+    const float* dlog; const float* dent; const float* dlse;     // nullable, [n]
+    void* dz; long ld_dz;                              // [n x v]; may be z
+};
+hipError_t launch_rate_back(const RateBackCall& a, hipStream_t s);
 
 }  // namespace skm

@@ -1,0 +1,383 @@
+// rate_kernels.hip -- log probabilities of given targets under rows of scores, with the rows'
+// entropy and their largest scores, and the gradient of the scores.
+//
+//   m = max_j z_j,  S = sum_j exp(z_j - m),  T = sum_j exp(z_j - m) (z_j - m)
+//   lse = m + ln S        log p_j = z_j - lse        H = -sum_j p_j log p_j = ln S - T / S
+//   dz_j = p_j (g_lse - g_t - g_H (log p_j + H)) + [j = t] g_t
+// with g_t the gradient of the target's log p.  A score of -inf or NaN is excluded (p = 0); +inf makes its
+// row's results NaN, as inf - inf is.
+//
+// One pass over the scores each way.  A row's scores are split over blocks where there are few
+// rows; a part leaves (m, S, T) and its k largest scores, which a second launch joins.
+#include "experts_common.h"
+
+namespace skm {
+namespace {
+
+constexpr int kMaxTop = kRateMaxK;
+constexpr float kLowest = -3.402823466e38f;
+// exp(-200) is 0 in fp32: as a lower bound it also turns the differences of excluded scores (-inf, and NaN, which
+// fmaxf leaves for the other operand) into probability 0 without a comparison.
+constexpr float kZero = -200.f;
+
+// A score and its place as a whole number, ordered by (score, lowest place first); -0 as 0, 0 for an excluded one.
+__device__ __forceinline__ unsigned long long key_of(float z, unsigned j)
+{
+    if (!(z > -__builtin_inff())) return 0;
+    const unsigned u = __float_as_uint(z + 0.f);
+    return (unsigned long long)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - j);
+}
+__device__ __forceinline__ float score_of(unsigned long long key)
+{
+    const unsigned o = (unsigned)(key >> 32);
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ int place_of(unsigned long long key) { return (int)(0xffffffffu - (unsigned)key); }
+
+// The softmax's sums relative to a maximum.
+struct Sums {
+    float m, s, t;  // the largest score (kLowest: none yet), sum e, sum e (z - m), e = exp(z - m)
+    __device__ __forceinline__ void raise(float to)
+    {
+        const float by = fminf(to - m, -kZero), c = exp_of(-by);
+        t = c * (t - by * s);
+        s *= c;
+        m = to;
+    }
+    __device__ __forceinline__ void add(float z)
+    {
+        const float d = fmaxf(z - m, kZero), e = exp_of(d);
+        s += e;
+        t = fmaf(e, d, t);
+    }
+    __device__ __forceinline__ void join(const Sums& o)
+    {
+        const float to = fmaxf(m, o.m), a = fminf(to - m, -kZero), b = fminf(to - o.m, -kZero), ca = exp_of(-a), cb = exp_of(-b);
+        t = ca * (t - a * s) + cb * (o.t - b * o.s);
+        s = ca * s + cb * o.s;
+        m = to;
+    }
+};
+
+__device__ __forceinline__ Sums joined(Sums v, int lanes_apart)
+{
+    v.join(Sums{__shfl_xor(v.m, lanes_apart), __shfl_xor(v.s, lanes_apart), __shfl_xor(v.t, lanes_apart)});
+    return v;
+}
+
+struct RateOut {
+    const int* targets; long target_stride; int v;
+    float* log_probs; float* entropy; float* lse; float* rest;  // [n]
+    int k; int* top; float* top_log_probs;                      // [n x k]
+};
+
+// A row's results from its sums, by one lane.
+template <typename T>
+__device__ __forceinline__ void finish(const RateOut& o, long row, const Sums& v, const T* z)
+{
+    const float log_s = logf(v.s);
+    const int t = o.targets[row * o.target_stride];
+    const bool inf = v.m == __builtin_inff(), none = v.s == 0.f;
+    const float lse = none && !inf ? -__builtin_inff() : v.m + log_s;
+    // lse to twice fp32's bits, for the gradient: what the sum's rounding left out
+    const float part = lse - v.m, rest = (v.m - (lse - part)) + (log_s - part);
+    o.lse[row] = inf ? v.m : lse;
+    o.rest[row] = none || inf ? 0.f : rest;
+    o.entropy[row] = inf ? __builtin_nanf("") : none ? 0.f : fmaxf(log_s - v.t / v.s, 0.f);
+    float lp = 0.f;
+    if (t >= 0 && t < o.v) {
+        const float zt = to_f(z[t]);
+        lp = inf ? __builtin_nanf("") : zt > -__builtin_inff() ? (zt - v.m) - log_s : -__builtin_inff();
+    }
+    o.log_probs[row] = lp;
+}
+
+// Place `at` of a row's largest scores.
+__device__ __forceinline__ void put_top(const RateOut& o, long row, int at, unsigned long long key, const Sums& v)
+{
+    o.top[row * o.k + at] = key ? place_of(key) : -1;
+    o.top_log_probs[row * o.k + at] = v.m == __builtin_inff() ? __builtin_nanf("") : key ? (score_of(key) - v.m) - logf(v.s) : -__builtin_inff();
+}
+
+template <typename T>
+struct RateArgs {
+    const T* z; long ld;
+    long n; int splits;         // parts of a row
+    int part;                   // scores a part, a multiple of a block's step
+    RateOut out;
+    Sums* sums;                 // [n][splits], several parts only
+    unsigned long long* keys;   // [n][splits][k]
+};
+
+// One part of a row on NT lanes: 16 bytes a lane, UN at once.
+//
+// The k largest: every lane knows the first place of its own largest score, at no cost but a comparison every 16 bytes.
+// The k-th largest of those is a lower bound for the k-th largest of all, and only the k lanes whose
+// largest reach it hold scores that do, so a second look at the part (from the caches) finds at most
+// k of a lane's share and hardly more than k as a rule; these are ranked by counting.
+template <typename T, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
+{
+    constexpr int V = kVec<T>, UN = 4, STEP = NT * V;
+    const long row = blockIdx.x / p.splits;
+    const int split = (int)(blockIdx.x % p.splits);
+    const T* z = p.z + row * p.ld;
+    const int lo = split * p.part, hi = min(p.out.v, lo + p.part), tid = threadIdx.x;
+    Sums s{kLowest, 0.f, 0.f};
+    int first = -1;  // where a vector held the lane's largest score first
+    auto take = [&](const float* x, int at) {
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) top = fmaxf(top, x[j]);
+        if (top > s.m || (first < 0 && top == kLowest)) {
+            s.raise(top);
+            first = at;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) s.add(x[j]);
+    };
+    int at = lo + tid * V;
+    for (; at + (UN - 1) * STEP + V <= hi; at += UN * STEP) {
+        Vec<T> raw[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) raw[u] = load16(z + at + u * STEP);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            float x[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = to_f(raw[u][j]);
+            take(x, at + u * STEP);
+        }
+    }
+    for (; at < hi; at += STEP) {
+        float x[V];
+        if (at + V <= hi) {
+            const Vec<T> raw = load16(z + at);
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = to_f(raw[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = at + j < hi ? to_f(z[at + j]) : -__builtin_inff();
+        }
+        take(x, at);
+    }
+
+    __shared__ Sums wave_sums[NT / 64];
+    __shared__ unsigned long long lane_keys[TOP ? NT : 1];
+    __shared__ unsigned long long list[TOP ? kRateList : 1];
+    __shared__ unsigned long long bound;
+    __shared__ int count;
+    Sums all = s;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) all = joined(all, x);
+    if (NT > 64) {
+        if ((tid & 63) == 0) wave_sums[tid >> 6] = all;
+    }
+    if constexpr (TOP) {
+        unsigned long long mine = 0;
+        if (first >= 0)
+            for (int j = 0; j < V; ++j) {
+                const unsigned long long key = first + j < hi ? key_of(to_f(z[first + j]), first + j) : 0;
+                mine = key > mine ? key : mine;
+            }
+        lane_keys[tid] = mine;
+        if (tid == 0) {
+            bound = 1;  // above the excluded scores
+            count = 0;
+        }
+        __syncthreads();
+        int above = 0;
+        for (int j = 0; j < NT; ++j) above += lane_keys[j] > mine;
+        if (mine && above == p.out.k - 1) bound = mine;
+        __syncthreads();
+        const unsigned long long least = bound;
+        for (at = lo + tid * V; mine >= least && at < hi; at += STEP)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const unsigned long long key = at + j < hi ? key_of(to_f(z[at + j]), at + j) : 0;
+                if (key >= least) list[atomicAdd(&count, 1)] = key;
+            }
+    }
+    if (NT > 64 || TOP) __syncthreads();
+    if (NT > 64) {
+        all = wave_sums[0];
+#pragma unroll
+        for (int w = 1; w < NT / 64; ++w) all.join(wave_sums[w]);
+    }
+    const bool whole = p.splits == 1;
+    if (tid == 0) {
+        if (whole)
+            finish(p.out, row, all, z);
+        else
+            p.sums[row * p.splits + split] = all;
+    }
+    if constexpr (TOP) {
+        const int k = p.out.k, found = count;
+        unsigned long long* keys = p.keys + (row * p.splits + split) * k;
+        for (int i = tid; i < max(found, k); i += NT) {
+            const unsigned long long key = i < found ? list[i] : 0;
+            int place = i;
+            if (i < found) {
+                place = 0;
+                for (int j = 0; j < found; ++j) place += list[j] > key;
+            }
+            if (place >= k) continue;
+            if (whole)
+                put_top(p.out, row, place, key, all);
+            else
+                keys[place] = key;
+        }
+    }
+}
+
+// The parts of a row joined, in their order.
+template <typename T>
+__global__ __launch_bounds__(64) void k_rate_join(RateArgs<T> p)
+{
+    __shared__ unsigned long long list[kRateSplits * kMaxTop];
+    const long row = blockIdx.x;
+    const int lane = threadIdx.x, k = p.out.k;
+    Sums all = lane < p.splits ? p.sums[row * p.splits + lane] : Sums{kLowest, 0.f, 0.f};
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) all = joined(all, x);
+    if (lane == 0) finish(p.out, row, all, p.z + row * p.ld);
+    if (k == 0) return;
+    const int found = p.splits * k;
+    for (int i = lane; i < found; i += 64) list[i] = p.keys[row * found + i];
+    __syncthreads();
+    for (int i = lane; i < found; i += 64) {
+        const unsigned long long key = list[i];
+        int place = 0;
+        for (int j = 0; j < found; ++j) place += list[j] > key || (list[j] == key && j < i);  // empty places are alike
+        if (place < k) put_top(p.out, row, place, key, all);
+    }
+}
+
+template <typename T>
+struct RateBackArgs {
+    const T* z; long ld;
+    const int* targets; long target_stride;
+    const float* lse; const float* rest; const float* entropy;
+    const float* dlog; const float* dent; const float* dlse;  // nullable
+    T* dz; long ld_dz;
+    int v, splits, part;
+};
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_rate_back(RateBackArgs<T> p)
+{
+    constexpr int V = kVec<T>, UN = 4, STEP = NT * V;
+    const long row = blockIdx.x / p.splits;
+    const int lo = (int)(blockIdx.x % p.splits) * p.part, hi = min(p.v, lo + p.part);
+    const T* z = p.z + row * p.ld;
+    T* dz = p.dz + row * p.ld_dz;
+    int t = p.targets[row * p.target_stride];
+    if (t < 0 || t >= p.v) t = -1;
+    const float lse = p.lse[row], rest = p.rest[row], ent = p.entropy[row];
+    const float gt = p.dlog != nullptr && t >= 0 ? p.dlog[row] : 0.f;
+    const float gh = p.dent != nullptr ? p.dent[row] : 0.f, gl = (p.dlse != nullptr ? p.dlse[row] : 0.f) - gt;
+    const bool inf = lse == __builtin_inff();
+    const float a = gl - gh * ent;  // dz = p (a - gh log p)
+    auto one = [&](float x, int j) {
+        const float lp = fmaxf((x - lse) - rest, kZero), e = exp_of(lp);
+        float g = e > 0.f ? e * fmaf(-gh, lp, a) : 0.f;
+        if (j == t && x > -__builtin_inff()) g += gt;
+        return inf && x > -__builtin_inff() ? __builtin_nanf("") : g;
+    };
+    int at = lo + (int)threadIdx.x * V;
+    for (; at + (UN - 1) * STEP + V <= hi; at += UN * STEP) {
+        Vec<T> raw[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) raw[u] = load16(z + at + u * STEP);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            Vec<T> g;
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[j] = from_f<T>(one(to_f(raw[u][j]), at + u * STEP + j));
+            stream16(dz + at + u * STEP, g);
+        }
+    }
+    for (; at < hi; at += STEP) {
+        if (at + V <= hi) {
+            const Vec<T> raw = load16(z + at);
+            Vec<T> g;
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[j] = from_f<T>(one(to_f(raw[j]), at + j));
+            stream16(dz + at, g);
+        } else {
+            for (int j = 0; at + j < hi; ++j) dz[at + j] = from_f<T>(one(to_f(z[at + j]), at + j));
+        }
+    }
+}
+
+// Rows of at most this many scores take one wave each.
+constexpr int kShort = 2048;
+
+struct Parts {
+    int threads, splits, part;
+};
+
+// How a row is cut: parts of at least 4,096 scores, as many as leave about four blocks a CU, at most
+// kRateSplits; with the k largest none of more scores than a lane's share of the list allows.
+Parts parts_of(long n, int v, int type, int k)
+{
+    const int vec = 16 / (int)elem_size(type);
+    if (v <= kShort) return {64, 1, v};
+    long splits = n > 0 ? (1024 + n - 1) / n : 1;
+    const long most = (v + 4095) / 4096;
+    if (splits > most) splits = most;
+    if (splits > kRateSplits) splits = kRateSplits;
+    const int longest = k > 0 ? kRateList / k / vec * vec * 256 : v;
+    const long least = ((long)v + longest - 1) / longest;
+    if (splits < least) splits = least;
+    const int step = 256 * vec;
+    const int part = (int)((((v + splits - 1) / splits + step - 1) / step) * step);
+    return {256, (v + part - 1) / part, part};
+}
+
+size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
+
+}  // namespace
+
+bool rate_fits(long n, int v, int type, int k)
+{
+    const Parts c = parts_of(n, v, type, k);
+    return c.splits <= kRateSplits && (unsigned long long)n * c.splits * c.threads < 1ull << 32;
+}
+
+size_t rate_workspace(long n, int v, int type, int k)
+{
+    const Parts c = parts_of(n, v, type, k);
+    return c.splits == 1 ? 0 : up16((size_t)n * c.splits * sizeof(Sums)) + (size_t)n * c.splits * k * 8;
+}
+
+hipError_t launch_rate(const RateCall& a, hipStream_t s)
+{
+    if (a.n == 0) return hipSuccess;
+    const Parts c = parts_of(a.n, a.v, a.type, a.k);
+    return with_type(a.type, [&](auto tag) {
+        using T = decltype(tag);
+        RateArgs<T> p{(const T*)a.z, a.ld, a.n, c.splits, c.part,
+                      {a.targets, a.target_stride, a.v, a.log_probs, a.entropy, a.lse, a.rest, a.k, a.top, a.top_log_probs},
+                      reinterpret_cast<Sums*>(a.ws), reinterpret_cast<unsigned long long*>(a.ws + up16((size_t)a.n * c.splits * sizeof(Sums)))};
+        const dim3 grid((unsigned)(a.n * c.splits));
+        const hipError_t e = c.threads == 64 ? (a.k > 0 ? launch(k_rate<T, 64, true>, grid, 64, 0, s, p) : launch(k_rate<T, 64, false>, grid, 64, 0, s, p))
+                                             : (a.k > 0 ? launch(k_rate<T, 256, true>, grid, 256, 0, s, p) : launch(k_rate<T, 256, false>, grid, 256, 0, s, p));
+        if (e != hipSuccess || c.splits == 1) return e;
+        return launch(k_rate_join<T>, dim3((unsigned)a.n), 64, 0, s, p);
+    });
+}
+
+hipError_t launch_rate_back(const RateBackCall& a, hipStream_t s)
+{
+    if (a.n == 0) return hipSuccess;
+    const Parts c = parts_of(a.n, a.v, a.type, 0);
+    return with_type(a.type, [&](auto tag) {
+        using T = decltype(tag);
+        const RateBackArgs<T> p{(const T*)a.z, a.ld, a.targets, a.target_stride, a.lse, a.rest, a.entropy, a.dlog, a.dent, a.dlse, (T*)a.dz, a.ld_dz, a.v, c.splits, c.part};
+        const dim3 grid((unsigned)(a.n * c.splits));
+        return c.threads == 64 ? launch(k_rate_back<T, 64>, grid, 64, 0, s, p) : launch(k_rate_back<T, 256>, grid, 256, 0, s, p);
+    });
+}
+
+}  // namespace skm

@@ -2124,7 +2124,7 @@ int skmetal_hip_lloyd_inertia(skmetal_hip_lloyd* h, double* out)
     return h->L.inertia(out);
 }
 
-// ---- routing and low-rank adapters: device pointers, the caller's stream, no lock ----
+// ---- the operators of skmetal_amd.experts: device pointers, the caller's stream, no lock ----
 
 }  // extern "C"
 
@@ -2223,6 +2223,18 @@ int check_adapt(int dtype, const AdaptSizes& z, std::initializer_list<size_t> st
         if (s > kMaxStride) return fail(SKMETAL_ERANGE, "a stride of %zu elements exceeds the supported range", s);
     if (!adapt_fits(dtype, (long)z.n, (int)z.d, (int)z.o, (int)z.r, (int)z.a))
         return fail(SKMETAL_ERANGE, "n=%zu, d=%zu, o=%zu: more blocks than a launch takes", z.n, z.d, z.o);
+    return 0;
+}
+
+int check_rate(int dtype, size_t n, size_t v, size_t k, std::initializer_list<size_t> strides)
+{
+    TRY(check_dtype(dtype));
+    if (v == 0 || k > v) return fail(SKMETAL_EINVAL, "v=%zu must be positive and at least k=%zu", v, k);
+    if (v > size_t(kRateMaxV) || k > size_t(kRateMaxK))
+        return fail(SKMETAL_ERANGE, "v=%zu, k=%zu: at most %d scores a row, of which at most %d are named", v, k, kRateMaxV, kRateMaxK);
+    for (const size_t s : strides)
+        if (s > kMaxStride) return fail(SKMETAL_ERANGE, "a stride of %zu elements exceeds the supported range", s);
+    if (n > kMaxRows || !rate_fits((long)n, (int)v, dtype, (int)k)) return fail(SKMETAL_ERANGE, "n=%zu, v=%zu: more blocks than a launch takes", n, v);
     return 0;
 }
 
@@ -2354,6 +2366,76 @@ int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t ld_grad, cons
                     (long)gates_stride, scales, low, base, (long)ld_base, grad_x, (long)ld_grad_x, grad_down, grad_up,
                     grad_gates, static_cast<char*>(workspace)};
     return launched(launch_adapt_back(A, static_cast<hipStream_t>(stream)), "adapt_backward");
+}
+
+int skmetal_hip_drop(int dtype, const void* x, size_t ld_x, const void* base, size_t ld_base, void* out, size_t ld_out,
+                     size_t n, size_t d, double p, const int64_t* key, uint32_t site, void* stream)
+{
+    g_err.clear();
+    TRY(check_dtype(dtype));
+    if (!(p >= 0.0 && p < 1.0)) return fail(SKMETAL_EINVAL, "p=%g is not in [0, 1)", p);
+    if (d == 0) return fail(SKMETAL_EINVAL, "d must be positive");
+    if (n > kMaxRows || d > kMaxRows || ld_x > kMaxStride || ld_base > kMaxStride || ld_out > kMaxStride)
+        return fail(SKMETAL_ERANGE, "n=%zu, d=%zu or a stride exceeds the supported range", n, d);
+    if (!key || (n > 0 && (!x || !out))) return fail(SKMETAL_EINVAL, "null pointer argument");
+    if (ld_out < d && n > 1) return fail(SKMETAL_EINVAL, "ld_out=%zu: the rows of out overlap", ld_out);
+    const size_t es = elem_size(dtype);
+    TRY(check_aligned(x, es, "x"));
+    TRY(check_aligned(base, es, "base"));
+    TRY(check_aligned(out, es, "out"));
+    TRY(check_aligned(key, 8, "key"));
+    const RowSpan result(out, ld_out, d, n, es), rows(x, ld_x, d, n, es);
+    if (!result.same(rows) && share(result, rows)) return fail(SKMETAL_EINVAL, "out shares memory with x without being it");
+    if (base != nullptr) {
+        const RowSpan b(base, ld_base, d, n, es);
+        if (!result.same(b) && share(result, b)) return fail(SKMETAL_EINVAL, "out shares memory with base without being it");
+    }
+    if (share(result, RowSpan(key, 2, 2, 1, 8))) return fail(SKMETAL_EINVAL, "out shares memory with key");
+    TRY(on_device());
+    const double limit = std::nearbyint(p * 4294967296.0);  // a p under 1 leaves the largest word, if nothing else
+    DropCall a{dtype, (long)n, (long)d, x, (long)ld_x, base, (long)ld_base, out, (long)ld_out, reinterpret_cast<const long long*>(key), site,
+               limit < 4294967295.0 ? (unsigned)limit : 4294967295u, (float)(1.0 / (1.0 - p))};
+    return launched(launch_drop(a, static_cast<hipStream_t>(stream)), "drop");
+}
+
+size_t skmetal_hip_rate_workspace(int dtype, size_t n, size_t v, size_t k)
+{
+    return check_rate(dtype, n, v, k, {}) != 0 ? 0 : rate_workspace((long)n, (int)v, dtype, (int)k);
+}
+
+int skmetal_hip_rate(int dtype, const void* logits, size_t ld_logits, const int32_t* targets, size_t targets_stride, size_t n,
+                     size_t v, size_t k, float* log_probs, float* entropy, float* lse, float* lse_rest, int32_t* top,
+                     float* top_log_probs, void* workspace, size_t workspace_bytes, void* stream)
+{
+    g_err.clear();
+    TRY(check_rate(dtype, n, v, k, {ld_logits, targets_stride}));
+    if (n > 0 && (!logits || !targets || !log_probs || !entropy || !lse || !lse_rest || (k > 0 && (!top || !top_log_probs))))
+        return fail(SKMETAL_EINVAL, "null pointer argument");
+    TRY(check_aligned(logits, elem_size(dtype), "logits"));
+    TRY(check_workspace(workspace, workspace_bytes, rate_workspace((long)n, (int)v, dtype, (int)k)));
+    TRY(on_device());
+    RateCall a{logits, dtype, (long)n, (int)v, (long)ld_logits, targets, (long)targets_stride, (int)k, log_probs, entropy, lse, lse_rest,
+               top, top_log_probs, static_cast<char*>(workspace)};
+    return launched(launch_rate(a, static_cast<hipStream_t>(stream)), "rate");
+}
+
+int skmetal_hip_rate_backward(int dtype, const void* logits, size_t ld_logits, const int32_t* targets, size_t targets_stride,
+                              size_t n, size_t v, const float* lse, const float* lse_rest, const float* entropy,
+                              const float* grad_log_probs, const float* grad_entropy, const float* grad_lse,
+                              void* grad_logits, size_t ld_grad, void* stream)
+{
+    g_err.clear();
+    TRY(check_rate(dtype, n, v, 0, {ld_logits, targets_stride, ld_grad}));
+    if (ld_grad < v && n > 1) return fail(SKMETAL_EINVAL, "ld_grad=%zu: the rows of grad_logits overlap", ld_grad);
+    if (n > 0 && (!logits || !targets || !lse || !lse_rest || !entropy || !grad_logits)) return fail(SKMETAL_EINVAL, "null pointer argument");
+    TRY(check_aligned(logits, elem_size(dtype), "logits"));
+    TRY(check_aligned(grad_logits, elem_size(dtype), "grad_logits"));
+    const RowSpan z(logits, ld_logits, v, n, elem_size(dtype)), dz(grad_logits, ld_grad, v, n, elem_size(dtype));
+    if (!dz.same(z) && share(dz, z)) return fail(SKMETAL_EINVAL, "grad_logits shares memory with logits without being it");
+    TRY(on_device());
+    RateBackCall a{logits, dtype, (long)n, (int)v, (long)ld_logits, targets, (long)targets_stride, lse, lse_rest, entropy,
+                   grad_log_probs, grad_entropy, grad_lse, grad_logits, (long)ld_grad};
+    return launched(launch_rate_back(a, static_cast<hipStream_t>(stream)), "rate_backward");
 }
 
 }  // extern "C"

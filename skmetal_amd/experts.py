@@ -30,6 +30,7 @@ from . import _bridge
 MAX_EXPERTS = 2048
 MAX_TOP_K = 16
 MAX_RANK = 128
+MAX_SCORES = 1 << 22
 
 _ADAPT, _ADAPT_BACKWARD, _ADAPT_IN_X = 0, 1, 2
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -44,6 +45,17 @@ class Routing(NamedTuple):
     prob_sums: torch.Tensor  # [e] float32: its probabilities' sum over the rows
     rows: torch.Tensor       # [1] int32: rows that count
     loss: torch.Tensor       # [] float32
+
+
+class Rating(NamedTuple):
+    """``rate``'s results."""
+
+    log_probs: torch.Tensor             # [n] float32: of the row's target, 0 where it has none
+    entropy: torch.Tensor               # [n] float32
+    lse: torch.Tensor                   # [n] float32: the log of the sum of exp
+    lse_rest: torch.Tensor              # [n] float32: what float32 leaves out of that
+    top: torch.Tensor | None            # [n, top_k] int32, largest first, -1: none
+    top_log_probs: torch.Tensor | None  # [n, top_k] float32
 
 
 class AdaptGrads(NamedTuple):
@@ -381,3 +393,151 @@ def routed(logits, top_k, *, mask=None, normalize=False) -> Routing:
 def adapted(x, down, up, ids, *, base=None, gates=None, scales=None):
     """``adapt`` inside autograd: gradients go to x, down, up, base and gates."""
     return _Adapted.apply(x, down, up, ids, base, gates, scales)
+
+
+# ---- dropout ----
+
+
+def _check_key(key, device):
+    return _dense(key, "key", torch.int64, (2,), device)
+
+
+def drop(x, p, key, *, site=0, base=None, out=None):
+    """base + dropout of x [n, d]: every element is 0 with probability `p`, else divided by
+    1 - p.  Which ones is a function of their places (row times d plus column), of `key`
+    (int64 [2] on the device: a seed and a step, of which the low 32 bits count) and of `site`, a
+    number below 2^32 that tells a program's dropouts apart: nothing is stored, and the same call
+    on out's gradient is x's.  A program changes key[1] from step to step, in place where a
+    graph was captured.  `out` may be x or base, and shares no memory with them otherwise."""
+    code, device = _first(x, "x")
+    n, d = x.shape
+    if d == 0:
+        raise ValueError("x has rows of no elements")
+    dtype = x.dtype
+    p, site = float(p), int(site)
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"p={p} is not in [0, 1)")
+    if not 0 <= site < 1 << 32:
+        raise ValueError(f"site={site} is not in [0, 2**32)")
+    x_ld = _rows(x, "x", dtype, (n, d), device)
+    key_ptr = _check_key(key, device)
+    base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, d), device))
+    lib = _lib()
+    if out is None:
+        out, out_ld = torch.empty((n, d), dtype=dtype, device=device), d
+    else:
+        out_ld = _rows(out, "out", dtype, (n, d), device)
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out requires a gradient, which this call does not record: use dropped, or torch.no_grad")
+        torch.autograd.graph.increment_version(out)
+    if lib.skmetal_hip_drop(code, x.data_ptr(), x_ld, base_ptr, base_ld, out.data_ptr(), out_ld, n, d, p, key_ptr, site, _stream(device)):
+        _fail("drop")
+    return out
+
+
+class _Dropped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, key, site, base):
+        ctx.save_for_backward(key)
+        ctx.p, ctx.site = p, site
+        return drop(x, p, key, site=site, base=base)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (key,) = ctx.saved_tensors
+        rows = grad if grad.stride(1) == 1 or grad.shape[1] == 1 else grad.contiguous()
+        return drop(rows, ctx.p, key, site=ctx.site) if ctx.needs_input_grad[0] else None, None, None, None, grad if ctx.needs_input_grad[4] else None
+
+
+def dropped(x, p, key, *, site=0, base=None):
+    """``drop`` inside autograd: gradients go to x and base.  `key` may be changed once the
+    gradient has been taken; autograd refuses one that was changed before."""
+    return _Dropped.apply(x, p, key, site, base)
+
+
+# ---- log probabilities ----
+
+
+@functools.lru_cache(maxsize=4096)
+def _rate_workspace(code, n, v, k):
+    return _lib().skmetal_hip_rate_workspace(code, n, v, k)
+
+
+def _check_rate(logits, targets):
+    code, device = _first(logits, "logits")
+    n, v = logits.shape
+    if not 1 <= v <= MAX_SCORES:
+        raise ValueError(f"logits has rows of {v} scores, expected 1 to {MAX_SCORES}")
+    ld, one = logits.stride()
+    if one != 1 and v > 1:
+        raise ValueError(f"logits' rows must have their elements side by side (stride(1) is {one})")
+    return code, device, n, v, ld, targets.data_ptr(), _vector(targets, "targets", torch.int32, n, device)
+
+
+def rate(logits, targets, *, top_k=0) -> Rating:
+    """How likely the scores logits [n, v] make each row's target (int32 [n]; a value outside
+    [0, v) is a row without one, whose log probability is 0), with the entropy of the
+    row's softmax and, for `top_k` of 1 to 16, the places of its largest scores, equal
+    ones by the lowest, and their log probabilities.
+
+    A score of -inf or NaN is excluded: its log probability is -inf and it is never among the largest (-1 in
+    the places that remain).  A row without a score left has an entropy of 0 and a ``lse`` of -inf; with a
+    score of +inf its log probabilities and entropy are NaN.  The same inputs give the same bits on every call."""
+    code, device, n, v, ld, target_ptr, target_stride = _check_rate(logits, targets)
+    k = int(top_k)
+    if not 0 <= k <= min(v, MAX_TOP_K):
+        raise ValueError(f"top_k={k} is not in [0, {min(v, MAX_TOP_K)}]")
+    lib = _lib()
+    whole = torch.empty((4, n), dtype=torch.float32, device=device)
+    at = whole.data_ptr()
+    top = torch.empty((n, k), dtype=torch.int32, device=device) if k else None
+    top_log_probs = torch.empty((n, k), dtype=torch.float32, device=device) if k else None
+    size = _rate_workspace(code, n, v, k)
+    ws, ws_ptr = _workspace(size, device)
+    if lib.skmetal_hip_rate(code, logits.data_ptr(), ld, target_ptr, target_stride, n, v, k, at, at + 4 * n, at + 8 * n, at + 12 * n,
+                            top.data_ptr() if k else None, top_log_probs.data_ptr() if k else None, ws_ptr, size, _stream(device)):
+        _fail("rate")
+    return Rating(*whole.unbind(0), top, top_log_probs)
+
+
+def rate_backward(logits, targets, rating: Rating, *, grad_log_probs=None, grad_entropy=None, grad_lse=None):
+    """The gradient of ``rate``'s logits from those of its log_probs, entropy and lse
+    (float32 [n] each; None: no gradient).  `rating` is the forward call's."""
+    code, device, n, v, ld, target_ptr, target_stride = _check_rate(logits, targets)
+    lib = _lib()
+    lse = _dense(rating.lse, "rating.lse", torch.float32, (n,), device)
+    rest = _dense(rating.lse_rest, "rating.lse_rest", torch.float32, (n,), device)
+    entropy = _dense(rating.entropy, "rating.entropy", torch.float32, (n,), device)
+    given = [None if g is None else _dense(g, name, torch.float32, (n,), device)
+             for g, name in ((grad_log_probs, "grad_log_probs"), (grad_entropy, "grad_entropy"), (grad_lse, "grad_lse"))]
+    grad = torch.empty((n, v), dtype=logits.dtype, device=device)
+    if lib.skmetal_hip_rate_backward(code, logits.data_ptr(), ld, target_ptr, target_stride, n, v, lse, rest, entropy, *given, grad.data_ptr(), v,
+                                     _stream(device)):
+        _fail("rate_backward")
+    return grad
+
+
+class _Rated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k):
+        r = rate(logits, targets, top_k=top_k)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, targets, r.lse.clone(), r.lse_rest, r.entropy.clone())
+        ctx.mark_non_differentiable(*(t for t in (r.lse_rest, r.top, r.top_log_probs) if t is not None))
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_log_probs, grad_entropy, grad_lse, _rest, _top, _top_log_probs):
+        logits, targets, lse, rest, entropy = ctx.saved_tensors
+        dense = [None if g is None else g.contiguous() for g in (grad_log_probs, grad_entropy, grad_lse)]
+        return rate_backward(logits, targets, Rating(None, entropy, lse, rest, None, None), grad_log_probs=dense[0], grad_entropy=dense[1],
+                             grad_lse=dense[2]), None, None
+
+
+def rated(logits, targets, *, top_k=0) -> Rating:
+    """``rate`` inside autograd: log_probs, entropy and lse pass their gradients to logits (the
+    mean of -log_probs over the rows with a target is their cross entropy)."""
+    return Rating(*_Rated.apply(logits, targets, top_k))
