@@ -408,6 +408,42 @@ SKMETAL_API int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t l
                                            void* grad_down, void* grad_up, float* grad_gates, size_t n, size_t d, size_t o,
                                            size_t r, size_t a, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The gated feed-forward block of every row's experts: with q = chosen[i][j],
+ *   out_i = base_i + sum_j weights_ij down_q (act(gate_q x_i) * (up_q x_i))
+ * x [n x d], base [n x o] (nullable: 0), out [n x o] (may be base itself: the same
+ * address and distance of rows); gate and up [a][f][d], down [a][o][f], experts
+ * *_stride and rows *_ld elements apart; chosen [n x k] int32, outside [0, a): no
+ * expert (null, with k = a = 1: every row takes the one there is); weights [n x k]
+ * fp32 (nullable: 1).  pre (nullable): [n x k][2][f] fp32, receives gate_q x_i and
+ * up_q x_i (0 without an expert), which the backward call takes.  act: silu g / (1
+ * + exp(-g)), gelu g Phi(g), relu.  The hidden vector, weighted, and its gradients
+ * enter the second products in dtype, each rounded once; with fp16 they share its
+ * range.  k <= 16, a <= 2048, n k < 2^30. */
+#define SKMETAL_SILU 0
+#define SKMETAL_GELU 1
+#define SKMETAL_RELU 2
+SKMETAL_API size_t skmetal_hip_feed_workspace(int dtype, size_t n, size_t d, size_t f, size_t o, size_t k, size_t a,
+                                              int backward);
+SKMETAL_API int skmetal_hip_feed(int dtype, const void* x, size_t ld_x, const void* gate, size_t gate_stride,
+                                 size_t gate_ld, const void* up, size_t up_stride, size_t up_ld, const void* down,
+                                 size_t down_stride, size_t down_ld, const int32_t* chosen, const float* weights, int act,
+                                 const void* base, size_t ld_base, void* out, size_t ld_out, float* pre, size_t n,
+                                 size_t d, size_t f, size_t o, size_t k, size_t a, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+/* Gradients from grad [n x o], that of out: grad_x_i = base_i + the experts' part
+ * (base [n x d] nullable: 0; grad_x nullable: not wanted; it may be base itself),
+ * grad_gate, grad_up [a][f][d] and grad_down [a][o][f] (dense, 0 for an expert without
+ * rows; nullable together) and grad_weights [n x k] fp32 (nullable; 0 without an
+ * expert).  The gradient of the forward call's base is grad. */
+SKMETAL_API int skmetal_hip_feed_backward(int dtype, const void* grad, size_t ld_grad, const void* x, size_t ld_x,
+                                          const void* gate, size_t gate_stride, size_t gate_ld, const void* up,
+                                          size_t up_stride, size_t up_ld, const void* down, size_t down_stride,
+                                          size_t down_ld, const int32_t* chosen, const float* weights, int act,
+                                          const float* pre, const void* base, size_t ld_base, void* grad_x,
+                                          size_t ld_grad_x, void* grad_gate, void* grad_up, void* grad_down,
+                                          float* grad_weights, size_t n, size_t d, size_t f, size_t o, size_t k, size_t a,
+                                          void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- dropout and log probabilities: device pointers and streams as above ----
  *
  * out_ij = base_ij + (word(i d + j) >= p 2^32 ? x_ij / (1 - p) : 0)   for x, base

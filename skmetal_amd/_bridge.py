@@ -122,6 +122,12 @@ _REGISTRY = [
     ("skmetal_hip_adapt_backward", _int, _int, _vp, _c_size, _vp, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _c_size,
      _vp, _c_size, _vp, _c_size, _vp, _vp, _vp, _c_size, _vp, _c_size, _vp, _vp, _vp, _c_size, _c_size, _c_size, _c_size,
      _c_size, _vp, _c_size, _vp),
+    ("skmetal_hip_feed_workspace", _c_size, _int, _c_size, _c_size, _c_size, _c_size, _c_size, _c_size, _int),
+    ("skmetal_hip_feed", _int, _int, _vp, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _c_size, _vp, _vp,
+     _int, _vp, _c_size, _vp, _c_size, _vp, _c_size, _c_size, _c_size, _c_size, _c_size, _c_size, _vp, _c_size, _vp),
+    ("skmetal_hip_feed_backward", _int, _int, _vp, _c_size, _vp, _c_size, _vp, _c_size, _c_size, _vp, _c_size, _c_size, _vp,
+     _c_size, _c_size, _vp, _vp, _int, _vp, _vp, _c_size, _vp, _c_size, _vp, _vp, _vp, _vp, _c_size, _c_size, _c_size, _c_size,
+     _c_size, _c_size, _vp, _c_size, _vp),
     ("skmetal_hip_drop", _int, _int, _vp, _c_size, _vp, _c_size, _vp, _c_size, _c_size, _c_size, ctypes.c_double, _vp,
      ctypes.c_uint32, _vp),
     ("skmetal_hip_rate_workspace", _c_size, _int, _c_size, _c_size, _c_size),

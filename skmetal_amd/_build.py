@@ -43,6 +43,7 @@ SOURCES = [
     ("sample_kernels.hip", []),
     ("route_kernels.hip", []),
     ("adapt_kernels.hip", []),
+    ("feed_kernels.hip", []),
     ("drop_kernels.hip", []),
     ("rate_kernels.hip", []),
     ("skmetal_hip.hip", VGPR_FORM),

@@ -84,6 +84,53 @@ size_t adapt_workspace(int type, long n, int d, int o, int r, int a, AdaptCall c
 // Whether every launch of both directions has a grid that the device takes.
 bool adapt_fits(int type, long n, int d, int o, int r, int a);
 
+// ---- feed_kernels.hip ----
+
+constexpr int kFeedMaxK = 16;    // experts of a row
+constexpr int kFeedMaxA = 2048;  // experts
+enum Activation : int { kSilu = 0, kGelu = 1, kRelu = 2 };
+
+struct FeedSizes {
+    int type; long n; int d, f, o, k, a;
+    bool sorted;                                       // false: one expert takes every row
+    bool aligned;                                      // rows and matrices in whole 16 bytes
+};
+struct FeedCall {
+    FeedSizes z;
+    const void* x; long ld_x;                          // [n x d]
+    const void* gate; long gate_sa, gate_ld;           // [a][f][d]
+    const void* up; long up_sa, up_ld;                 // [a][f][d]
+    const void* down; long down_sa, down_ld;           // [a][o][f]
+    const int* chosen;                                 // [n x k]; outside [0, a): none; null where not sorted
+    const float* weights;                              // nullable, [n x k]
+    int act;
+    const void* base; long ld_base;                    // nullable, [n x o]
+    void* out; long ld_out;                            // [n x o]
+    float* pre;                                        // nullable, [n x k][2][f]
+    char* ws;
+};
+hipError_t launch_feed(const FeedCall& a, hipStream_t s);
+
+struct FeedBackCall {
+    FeedSizes z;
+    const void* dy; long ld_dy;                        // [n x o]
+    const void* x; long ld_x;
+    const void* gate; long gate_sa, gate_ld;
+    const void* up; long up_sa, up_ld;
+    const void* down; long down_sa, down_ld;
+    const int* chosen; const float* weights; int act;
+    const float* pre;                                  // launch_feed's
+    const void* base; long ld_base;                    // nullable, [n x d]: added to dx
+    void* dx; long ld_dx;                              // nullable, [n x d]
+    void *dgate, *dup, *ddown;                         // nullable together; dense
+    float* dweights;                                   // nullable, [n x k]
+    char* ws;
+};
+hipError_t launch_feed_back(const FeedBackCall& a, hipStream_t s);
+size_t feed_workspace(const FeedSizes& z, bool backward);
+// Whether every launch of both directions has a grid that the device takes.
+bool feed_fits(const FeedSizes& z);
+
 // ---- drop_kernels.hip ----
 
 struct DropCall {

@@ -1,0 +1,798 @@
+// feed_kernels.hip -- the gated feed-forward block of every row's experts.
+//
+// Row i goes to the experts q_ij = chosen[i][j], j < k (none outside [0, a)), with the
+// weights w_ij; a slot is one such pair.  With expert q's matrices P, Q [f x d] and R [o x f]:
+//   g = P x_i, u = Q x_i, h = w act(g) u        out_i = base_i + sum_j R h
+// and from dy_i, the gradient of out_i:
+//   e = R^T dy_i       dw_ij = <e, act(g) u>     dg = w e u act'(g), du = w e act(g)
+//   dx_i = base_i + sum_j P^T dg + Q^T du
+//   dP = sum dg x_i^T, dQ = sum du x_i^T, dR = sum dy_i h^T        over the slots of q
+//
+// k_plan first puts the slots of each expert side by side, cut into tiles of one expert.  Six
+// matrix products follow, all by one kernel, k_product: tiles of C = A B^T whose operands are rows in
+// memory, either along the sum (a row holds successive terms: "along") or across it (a row holds one term of
+// successive results: "across"), gathered through the sort where they are the caller's rows.  Each
+// differs in its operands and in what it does with a finished tile.
+//
+// Between the products h, dg and du are in the rows' type, each rounded once: the matrix cores
+// take 16-bit operands, and every result then has one rounding of its terms and one of its own, half
+// of what its variance would be with a second rounding.  What enters no product stays fp32: g and u
+// (kept from the forward pass for the backward one), e, dw, and the k parts of a row's sum.
+#include "plan_common.h"
+
+namespace skm {
+namespace {
+
+enum Kind : int { kGated, kDown, kHidden, kRows, kGates, kOuts };
+
+// 16 bytes of zeros for loads of what does not exist.
+__device__ __attribute__((aligned(16))) unsigned g_zeros[4];
+
+// slot / k for slots below 2^30 and k <= 16.
+struct ByK {
+    unsigned k, mul, shift;
+    __device__ __forceinline__ unsigned row(unsigned slot) const { return (unsigned)(((unsigned long long)slot * mul) >> shift); }
+};
+ByK by_k(int k)
+{
+    unsigned l = 0;
+    while ((1 << l) < k) ++l;
+    return ByK{(unsigned)k, (unsigned)(((1ull << (30 + l)) + k - 1) / k), 30 + l};
+}
+
+template <typename T>
+struct FeedArgs {
+    // tiles of slots (row products) or the slots of each expert (gradients of matrices)
+    const Tile* tiles; int ntiles; const int* perm; int slots, a;  // tiles null: one expert has all slots in their order
+    ByK byk;
+    // operands
+    const T *A, *A2; long lda;
+    const T *B, *B2; long sb, ldb, sb2, ldb2;  // expert and row strides
+    int M, N, K;                               // of the result and the sum; what the tiles give is 0
+    int nm, nn;                                // tiles of M (kGates, kOuts) and N
+    // results
+    T *h, *dg, *du; long ldh;                  // [slots][ldh], by place
+    float* pre;                                // [slots][2][f], by slot; nullable in kGated
+    const float* weights; int act;             // weights nullable
+    float* dots; int ndots;                    // [slots][ndots] parts of <e, act(g) u>, nullable
+    const T* base; long ld_base; T* out; long ld_out;  // k = 1
+    float* sums;                               // [slots][N] by slot: k > 1
+    T *dm, *dm2; float* part; int splits;      // [a][M][N]; partial sums [splits][a][2 where dm2][M][N] where splits > 1
+};
+
+__device__ __forceinline__ float gelu_cdf(float g) { return 0.5f * (1.f + erff(g * 0.70710678118654752f)); }
+
+// act(g) and its derivative
+__device__ __forceinline__ float2 activate(float g, int act)
+{
+    if (act == kSilu) {
+        const float t = 1.f / (1.f + expf(-g));
+        return make_float2(g * t, t * (1.f + g * (1.f - t)));
+    }
+    if (act == kGelu) {
+        const float c = gelu_cdf(g);
+        return make_float2(g * c, c + g * 0.39894228040143268f * expf(-0.5f * g * g));
+    }
+    return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);
+}
+
+template <typename T> using Quad = T __attribute__((ext_vector_type(4)));
+
+// Four neighbouring elements of a row, of which `left` exist.
+template <typename T>
+__device__ __forceinline__ void put4(T* p, f32x4 v, int left)
+{
+    Quad<T> r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = from_f<T>(v[e]);
+    if (left >= 4)
+        __builtin_memcpy(p, &r, sizeof r);
+    else
+        for (int e = 0; e < left; ++e) p[e] = r[e];
+}
+template <typename T>
+__device__ __forceinline__ f32x4 get4(const T* p, int left)
+{
+    Quad<T> r{};
+    if (left >= 4)
+        __builtin_memcpy(&r, p, sizeof r);
+    else
+        for (int e = 0; e < left; ++e) r[e] = p[e];
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = to_f(r[e]);
+    return v;
+}
+
+// ---- staging ----
+
+// 16 bytes a lane from memory to LDS, a wave's side by side from `to` on.  As assembly, for the compiler waits for
+// a load of its own builtin before every transposing read of LDS, and so leaves none in flight
+// under a step's products.  It writes no register but m0, which nothing else here uses; landed() waits for it.
+__device__ __forceinline__ void to_lds(const void* from, char* to)
+{
+    const unsigned at = (unsigned)(size_t)(__attribute__((address_space(3))) char*)to;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+}
+
+constexpr int kStepBytes = 128;  // of a row along the sum: terms a step
+template <typename T> constexpr int kStep = kStepBytes / (int)sizeof(T);
+
+// How far the 16-byte chunks of term k's row are displaced in an operand across the sum, so that the lanes of a
+// read, which take 16 terms at once, find them in different banks.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ int displaced(int k)
+{
+    if constexpr (sizeof(T) == 2) return (((k & 3) | ((k >> 3) & 1) << 2) << 1) & (CHUNKS - 1);
+    return (((k >> 2) & 3) << 2) & (CHUNKS - 1);
+}
+
+// A block's way to an operand's R rows (or columns) of a tile, a step of terms after another: from memory to
+// LDS, 16 bytes a lane.  Along the sum a row takes 128 bytes a step, its chunks exchanged by the row's number, so that
+// 16 rows' chunks of the same terms lie in different banks; across it a term's row takes
+// R elements.  FAST: every chunk is 16 bytes that exist or not, at addresses of 16 bytes; they go to LDS without
+// registers between, and those that do not exist come from g_zeros.
+template <typename T, bool ALONG, int R, int NT, bool FAST>
+struct Stager {
+    static constexpr int V = kVec<T>, C = R * 8 / NT, CHUNKS = ALONG ? 8 : R / V;
+    static_assert(C * NT == R * 8, "whole chunks a lane");
+    const T* p[C];       // ALONG: the row's chunk of the present step; else the column of the chunk in row 0
+    Vec<T> held[FAST ? 1 : C];
+
+    static __device__ __forceinline__ int index(int c) { return c * NT + (int)threadIdx.x; }
+    static __device__ __forceinline__ int line(int c) { return index(c) / CHUNKS; }  // row, or term of the step
+    static __device__ __forceinline__ int chunk(int c)
+    {
+        const int l = line(c), s = index(c) % CHUNKS;
+        return ALONG ? s ^ (l & 7) : s ^ displaced<T, CHUNKS>(l);
+    }
+
+    // along: row(i) is the address of row i of the tile (one that exists, also where the tile has no such row)
+    template <typename F>
+    __device__ __forceinline__ void rows(F&& row)
+    {
+#pragma unroll
+        for (int c = 0; c < C; ++c) p[c] = row(line(c)) + chunk(c) * V;
+    }
+
+    // across: the columns from `col` on, of which `left` exist
+    __device__ __forceinline__ int column(int c, int left) const { return FAST ? min(chunk(c) * V, left - V) : chunk(c) * V; }
+
+    __device__ __forceinline__ void fetch(int c, const T* from, bool there, int left, char* to)
+    {
+        if constexpr (FAST) {
+            to_lds(there ? (const void*)from : (const void*)g_zeros, to + (c * NT + wave_index() * 64) * 16);
+        } else {
+            held[c] = there && left > 0 ? load_part(from, left) : Vec<T>{};
+        }
+    }
+    __device__ __forceinline__ void settle(char* to)
+    {
+        if constexpr (!FAST)
+#pragma unroll
+            for (int c = 0; c < C; ++c) *reinterpret_cast<Vec<T>*>(to + index(c) * 16) = held[c];
+    }
+
+    // the step that begins at term k0 of `terms`
+    __device__ __forceinline__ void along(int k0, int terms, char* to)
+    {
+        if (k0 + kStep<T> <= terms) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) fetch(c, p[c], true, V, to);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) fetch(c, p[c], k0 + chunk(c) * V < terms, terms - k0 - chunk(c) * V, to);
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) p[c] += kStep<T>;
+    }
+    // row(k): the address of term k's row, at column 0 of the tile; `left` of its columns exist
+    template <typename F>
+    __device__ __forceinline__ void across(int k0, int terms, int left, F&& row, char* to)
+    {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k = k0 + line(c);
+            fetch(c, row(min(k, terms - 1)) + column(c, left), k < terms, left - chunk(c) * V, to);
+        }
+    }
+};
+
+// The chunks that this wave has asked for are in LDS: to be followed by a barrier.
+template <bool FAST>
+__device__ __forceinline__ void landed()
+{
+    if constexpr (FAST) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// ---- fragments: a lane's terms of one row (or column) for a 16 x 16 product ----
+
+template <typename T, bool ALONG, int R>
+struct Reader {
+    // `first`: the wave's first of R rows
+    int at[ALONG ? 2 : 1], lane_, first_;
+    __device__ __forceinline__ explicit Reader(int first)
+    {
+        const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+        lane_ = lane;
+        first_ = first;
+        if constexpr (ALONG) {
+            at[0] = (first + l16) * kStepBytes + ((g ^ (l16 & 7)) * 16);
+            at[1] = (first + l16) * kStepBytes + (((4 + g) ^ (l16 & 7)) * 16);
+        } else if constexpr (sizeof(T) == 2) {
+            at[0] = (g * 8 + (l16 >> 2)) * R * 2 + ((l16 & 3) >> 1) * 16 + (l16 & 1) * 8;
+        } else {
+            at[0] = g * 4 * R * 4 + (l16 >> 2) * 16 + (l16 & 3) * 4;
+        }
+    }
+    __device__ __forceinline__ Vec<T> read(const char* lds, int tile, int half) const
+    {
+        if constexpr (ALONG) {
+            return *reinterpret_cast<const Vec<T>*>(lds + at[half] + tile * 16 * kStepBytes);
+        } else if constexpr (sizeof(T) == 2) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s4* Lds4;
+            const int g = lane_ >> 4, l16 = lane_ & 15, s = ((((l16 >> 2) | (g & 1) << 2)) << 1) & (R / 8 - 1);
+            const char* p = lds + at[0] + half * 32 * R * 2 + ((((first_ >> 3) + tile * 2) ^ s) * 16);
+            union { s4 q[2]; Vec<T> v; } r;
+            r.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)p);
+            r.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(p + 4 * R * 2));
+            return r.v;
+        } else {
+            const int g = lane_ >> 4, s = (g << 2) & (R / 4 - 1);
+            const char* p = lds + at[0] + half * 16 * R * 4 + ((((first_ >> 2) + tile * 4) ^ s) * 16);
+            Vec<T> v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(p + j * R * 4);
+            return v;
+        }
+    }
+};
+
+// Which of `count` pieces of work a block takes: blocks go to the 8 XCDs in turn, and an XCD gets an eighth of the
+// pieces side by side, which share operands in its L2.
+__device__ __forceinline__ int piece_of(unsigned x, int count) { return (int)(x & 7) * ((count + 7) / 8) + (int)(x >> 3); }
+
+// ---- the product ----
+
+// A block's tile of WM TM 16 x WN TN 16 results; a wave's is TM 16 x TN 16.
+template <typename T, int KIND, int WM, int WN, int TM, int TN, bool FAST>
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
+{
+    constexpr int NT = WM * WN * 64, RA = WM * TM * 16, RB = WN * TN * 16, STAGE = (RA + RB) * kStepBytes;
+    constexpr bool MATRIX = KIND == kGates || KIND == kOuts;  // the sum runs over slots
+    constexpr bool A_ALONG = !MATRIX, B_ALONG = KIND == kGated || KIND == kDown;
+    constexpr int GROUP = 4;  // tiles of M that neighbouring blocks take together
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+
+    const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+    Tile t;
+    int n0, m0 = 0, split = 0;
+    const T *A = p.A, *B = p.B, *A2 = p.A2, *B2 = p.B2;
+    T* dm = p.dm;
+    int terms = p.K, from = 0, matrix = 0;
+    if constexpr (MATRIX) {
+        const int per = p.nm * p.nn, both = KIND == kGates ? 2 : 1;
+        const int piece = piece_of(blockIdx.x, p.a * p.splits * both * per);
+        if (piece >= p.a * p.splits * both * per) return;
+        const int i = piece % per, rest = piece / per;
+        const int group = i / (GROUP * p.nn), in = i - group * GROUP * p.nn, high = min(GROUP, p.nm - group * GROUP);
+        m0 = (group * GROUP + in % high) * RA;
+        n0 = in / high * RB;
+        split = rest % p.splits;
+        matrix = rest / p.splits % both;
+        const int q = rest / p.splits / both;
+        t = p.tiles != nullptr ? p.tiles[q] : Tile{0, 0, p.slots, -1};
+        t.q = q;
+        if (matrix) {
+            A = A2;
+            dm = p.dm2;
+        }
+        // this part's slots, whole steps
+        const int steps = (t.cnt + kStep<T> - 1) / kStep<T>;
+        from = (int)((long)steps * split / p.splits) * kStep<T>;
+        terms = min(t.cnt, (int)((long)steps * (split + 1) / p.splits) * kStep<T>) - from;
+        if (terms < 0) terms = 0;
+    } else {
+        const int all = p.ntiles * p.nn, piece = piece_of(blockIdx.x, all);
+        if (piece >= all) return;
+        const int group = piece / (GROUP * p.nn), in = piece - group * GROUP * p.nn, high = min(GROUP, p.ntiles - group * GROUP);
+        const int m = group * GROUP + in % high;
+        n0 = in / high * (KIND == kGated ? RB / 2 : RB);
+        t = p.tiles != nullptr ? p.tiles[m] : Tile{0, m * RA, min(RA, p.slots - m * RA), -1};
+        if (t.q < 0) return;
+        if (t.q >= p.a) {  // slots without an expert
+            if constexpr (KIND == kGated) {
+                if (p.pre == nullptr) return;
+                for (int i = threadIdx.x; i < t.cnt * (RB / 2); i += NT) {
+                    const int f = n0 + i % (RB / 2);
+                    float* to = p.pre + (long)p.perm[t.start + i / (RB / 2)] * 2 * p.N;
+                    if (f < p.N) to[f] = to[p.N + f] = 0.f;
+                }
+            }
+            if constexpr (KIND == kDown || KIND == kRows) {
+                if (p.out == nullptr) return;
+                for (int i = threadIdx.x; i < t.cnt * RB; i += NT) {
+                    const int n = n0 + i % RB;
+                    const long row = p.perm[t.start + i / RB];
+                    if (n < p.N) p.out[row * p.ld_out + n] = p.base != nullptr ? p.base[row * p.ld_base + n] : (T)0.f;
+                }
+            }
+            return;
+        }
+    }
+    auto slot_of = [&](int place) -> int { return p.perm != nullptr ? p.perm[place] : place; };
+    // the caller's row of the tile's i-th slot
+    auto row_of = [&](int i) -> long { return (long)p.byk.row((unsigned)slot_of(t.start + i)); };
+
+    Stager<T, A_ALONG, RA, NT, FAST> sa;
+    Stager<T, B_ALONG, RB, NT, FAST> sb;
+    if constexpr (!MATRIX) {
+        B += t.q * p.sb;
+        if constexpr (KIND == kGated || KIND == kRows) B2 += t.q * p.sb2;
+    }
+    auto begin_a = [&](const T* from_a) {
+        if constexpr (KIND == kGated || KIND == kHidden) sa.rows([&](int r) { return from_a + row_of(min(r, t.cnt - 1)) * p.lda; });
+        if constexpr (KIND == kDown || KIND == kRows) sa.rows([&](int r) { return from_a + (long)(t.start + min(r, t.cnt - 1)) * p.lda; });
+    };
+    begin_a(A);
+    if constexpr (KIND == kGated)  // 16 rows of one matrix beside 16 of the other
+        sb.rows([&](int r) {
+            const int f = min(n0 + (r >> 5) * 16 + (r & 15), p.N - 1);
+            return r & 16 ? B2 + f * p.ldb2 : B + f * p.ldb;
+        });
+    if constexpr (KIND == kDown) sb.rows([&](int r) { return B + (long)min(n0 + r, p.N - 1) * p.ldb; });
+
+    const int steps1 = (terms + kStep<T> - 1) / kStep<T>, steps = KIND == kRows ? 2 * steps1 : steps1;
+    auto fetch = [&](int step, char* to) {
+        int k0 = step * kStep<T>;
+        if constexpr (KIND == kRows)
+            if (step >= steps1) {
+                k0 -= steps1 * kStep<T>;
+                if (step == steps1) begin_a(A2);
+            }
+        if constexpr (A_ALONG)
+            sa.along(k0, terms, to);
+        else
+            sa.across(k0, terms, p.M - m0,
+                      [&](int k) { return A + m0 + (KIND == kOuts ? row_of(from + k) : (long)(t.start + from + k)) * p.lda; }, to);
+        if constexpr (B_ALONG)
+            sb.along(k0, terms, to + RA * kStepBytes);
+        else if constexpr (MATRIX)
+            sb.across(k0, terms, p.N - n0,
+                      [&](int k) { return B + n0 + (KIND == kGates ? row_of(from + k) : (long)(t.start + from + k)) * p.ldb; }, to + RA * kStepBytes);
+        else {
+            const bool second = KIND == kRows && step >= steps1;
+            const T* b = second ? B2 : B;
+            const long ld = second ? p.ldb2 : p.ldb;
+            sb.across(k0, terms, p.N - n0, [&](int k) { return b + n0 + k * ld; }, to + RA * kStepBytes);
+        }
+    };
+    auto settle = [&](char* to) {
+        sa.settle(to);
+        sb.settle(to + RA * kStepBytes);
+    };
+
+    const Reader<T, A_ALONG, RA> ra(wm * TM * 16);
+    const Reader<T, B_ALONG, RB> rb(wn * TN * 16);
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (steps > 0) {
+        fetch(0, lds);
+        settle(lds);
+    }
+    landed<FAST>();
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        char* now = lds + (s & 1) * STAGE;
+        char* next = lds + ((s + 1) & 1) * STAGE;
+        if (s + 1 < steps) fetch(s + 1, next);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            Vec<T> x[TM], y[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) y[j] = rb.read(now + RA * kStepBytes, j, half);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) x[i] = ra.read(now, i, half);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mfma16(y[j], x[i], acc[i][j]);
+        }
+        if (s + 1 < steps) settle(next);
+        landed<FAST>();
+        __syncthreads();
+    }
+
+    // Lane (l16, g) holds results m = i 16 + l16 and n = j 16 + 4 g + 0 .. 3 of the wave's.
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = (wm * TM + i) * 16 + l16;
+        if constexpr (MATRIX) {
+            if (m0 + m >= p.M) continue;
+            const long line = (long)(m0 + m) * p.N;
+            const long each = (long)p.M * p.N;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int n = n0 + (wn * TN + j) * 16 + g * 4;
+                if (p.splits == 1)
+                    put4(dm + t.q * each + line + n, acc[i][j], p.N - n);
+                else
+                    put4(p.part + (((long)split * p.a + t.q) * (KIND == kGates ? 2 : 1) + matrix) * each + line + n, acc[i][j], p.N - n);
+            }
+        } else {
+            const bool there = m < t.cnt;
+            const int place = t.start + min(m, t.cnt - 1), slot = slot_of(place);
+            if constexpr (KIND == kGated) {
+                if (!there) continue;
+                const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
+#pragma unroll
+                for (int j = 0; j < TN; j += 2) {
+                    const int f = n0 + (wn * TN + j) * 8 + g * 4;
+                    if (p.pre != nullptr) {
+                        float* to = p.pre + (long)slot * 2 * p.N + f;
+                        put4(to, acc[i][j], p.N - f);
+                        put4(to + p.N, acc[i][j + 1], p.N - f);
+                    }
+                    f32x4 h;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[e] = f + e < p.N ? w * (activate(acc[i][j][e], p.act).x * acc[i][j + 1][e]) : 0.f;
+                    if (f < p.ldh) put4(p.h + place * p.ldh + f, h, 4);
+                }
+            } else if constexpr (KIND == kHidden) {
+                const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
+                float dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int f = n0 + (wn * TN + j) * 16 + g * 4;
+                    if (f >= p.ldh) continue;
+                    const float* pre = p.pre + (long)slot * 2 * p.N + f;
+                    const f32x4 gate = get4(pre, p.N - f), up = get4(pre + p.N, p.N - f);
+                    f32x4 h, dg, du;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 act = activate(gate[e], p.act);
+                        const bool in = f + e < p.N;
+                        const float hidden = act.x * up[e], err = in ? acc[i][j][e] : 0.f;
+                        dot += in ? err * hidden : 0.f;
+                        h[e] = in ? w * hidden : 0.f;
+                        dg[e] = in ? w * err * up[e] * act.y : 0.f;
+                        du[e] = in ? w * err * act.x : 0.f;
+                    }
+                    if (there) {
+                        if (p.h != nullptr) put4(p.h + place * p.ldh + f, h, 4);
+                        put4(p.dg + place * p.ldh + f, dg, 4);
+                        put4(p.du + place * p.ldh + f, du, 4);
+                    }
+                }
+                if (p.dots != nullptr) {
+                    dot += __shfl_xor(dot, 16);
+                    dot += __shfl_xor(dot, 32);
+                    if (there && g == 0) p.dots[(long)slot * p.ndots + n0 / RB * WN + wn] = dot;
+                }
+            } else {
+                if (!there) continue;
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int n = n0 + (wn * TN + j) * 16 + g * 4;
+                    if (n >= p.N) continue;
+                    if (p.out != nullptr) {
+                        f32x4 v = acc[i][j];
+                        if (p.base != nullptr) v += get4(p.base + slot * p.ld_base + n, p.N - n);
+                        put4(p.out + slot * p.ld_out + n, v, p.N - n);
+                    } else {
+                        put4(p.sums + (long)slot * p.N + n, acc[i][j], p.N - n);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---- what joins parts ----
+
+template <typename T>
+struct JoinArgs {
+    const float* sums; const int* chosen; int n, k, a, w;  // [n k][w]
+    const T* base; long ld_base; T* out; long ld_out;
+};
+
+// out_i = base_i + the sum of row i's slots, in their order; a block a stretch of 1,024 columns of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_feed_join(JoinArgs<T> p)
+{
+    const long row = blockIdx.x;
+    const int n = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;
+    if (n >= p.w) return;
+    const int left = p.w - n;
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    if (p.base != nullptr) v = get4(p.base + row * p.ld_base + n, left);
+    for (int j = 0; j < p.k; ++j) {
+        const int q = p.chosen != nullptr ? p.chosen[row * p.k + j] : 0;
+        if (q >= 0 && q < p.a) v += get4(p.sums + (row * p.k + j) * p.w + n, left);
+    }
+    put4(p.out + row * p.ld_out + n, v, left);
+}
+
+// dw of every slot: the sum of its parts in their order, 0 for one without an expert.
+__global__ __launch_bounds__(256) void k_feed_dots(const float* dots, int ndots, const int* chosen, int slots, int a, float* dw)
+{
+    const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (i >= slots) return;
+    const int q = chosen != nullptr ? chosen[i] : 0;
+    float v = 0.f;
+    if (q >= 0 && q < a)
+        for (int j = 0; j < ndots; ++j) v += dots[(long)i * ndots + j];
+    dw[i] = v;
+}
+
+// The matrices' gradients from their parts, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_feed_merge(const float* part, int splits, long each, int both, int a, T* dm, T* dm2)
+{
+    const long all = each * both * a;
+    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (long)gridDim.x * 1024) {
+        f32x4 v{0.f, 0.f, 0.f, 0.f};
+        const int left = (int)(all - i < 4 ? all - i : 4);
+        for (int s = 0; s < splits; ++s) v += get4(part + s * all + i, left);
+        for (int e = 0; e < left; ++e) {
+            const long at = i + e, q = at / (each * both), in = at - q * each * both;
+            (in >= each ? dm2 : dm)[q * each + (in >= each ? in - each : in)] = from_f<T>(v[e]);
+        }
+    }
+}
+
+// ---- launches ----
+
+size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
+
+struct Layout {
+    int slots, tile, ntiles, segments;
+    bool fast, sorted;
+    int ldh, ndots, gsplits, osplits;
+    size_t seen, perm, tiles, groups, merge, h, dg, du, dots, sums, part, bytes;
+};
+
+// Rows of a block's tile, 128 or 256.
+constexpr int kBig = 256, kMid = 128;
+
+int tiles_of(long m, int r) { return (int)((m + r - 1) / r); }
+
+// Parts of the slots for the matrices' gradients: enough for two blocks a CU, each with 8 steps at least.
+int matrix_splits(long slots, int a, int m, int n, int both, int r, int step)
+{
+    const long blocks = (long)a * both * tiles_of(m, r) * tiles_of(n, r);
+    long s = 512 / (blocks > 0 ? blocks : 1);
+    const long most = slots / a / (8 * step);
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+
+Layout layout(const FeedSizes& z, bool backward)
+{
+    Layout L{};
+    const int vec = 16 / (int)elem_size(z.type), step = 128 / (int)elem_size(z.type);
+    L.slots = (int)(z.n * z.k);
+    L.sorted = z.sorted;
+    L.fast = z.aligned;
+    L.ldh = (z.f + vec - 1) / vec * vec;
+    L.tile = kMid;
+    if (z.aligned && (long)tiles_of(L.slots, kBig) * tiles_of(z.f, kBig) >= 256) L.tile = kBig;
+    L.ntiles = z.sorted ? L.slots / L.tile + z.a + 1 : tiles_of(L.slots, L.tile);
+    L.segments = (L.slots + kPlanRows - 1) / kPlanRows;
+    if (L.segments < 1) L.segments = 1;
+    L.ndots = tiles_of(z.f, L.tile) * (L.tile == kBig ? 4 : 2);
+    L.gsplits = matrix_splits(L.slots, z.a, z.f, z.d, 2, L.tile, step);
+    L.osplits = matrix_splits(L.slots, z.a, z.o, z.f, 1, L.tile, step);
+    size_t at = 0;
+    auto take = [&](size_t& where, size_t bytes) { where = at; at += up16(bytes); };
+    if (L.sorted) {
+        take(L.seen, L.segments > 1 ? (size_t)L.segments * (z.a + 1) * sizeof(int2) : 0);
+        take(L.perm, (size_t)L.slots * 4);
+        take(L.tiles, (size_t)L.ntiles * sizeof(Tile));
+        if (backward) {
+            take(L.groups, (size_t)z.a * sizeof(Tile));
+            take(L.merge, (size_t)z.a * sizeof(int2));
+        }
+    }
+    const size_t es = elem_size(z.type), hidden = (size_t)L.slots * L.ldh * es;
+    take(L.h, hidden);
+    const int w = backward ? z.d : z.o;
+    if (z.k > 1) take(L.sums, (size_t)L.slots * w * 4);
+    if (backward) {
+        take(L.dg, hidden);
+        take(L.du, hidden);
+        take(L.dots, (size_t)L.slots * L.ndots * 4);
+        const size_t g = L.gsplits > 1 ? (size_t)L.gsplits * z.a * 2 * z.f * z.d * 4 : 0, o = L.osplits > 1 ? (size_t)L.osplits * z.a * z.o * z.f * 4 : 0;
+        take(L.part, g > o ? g : o);
+    }
+    L.bytes = at;
+    return L;
+}
+
+hipError_t launch_plan(const Layout& L, const int* chosen, int a, char* ws, bool backward, hipStream_t s)
+{
+    // "chunks" of the plan: all slots of an expert
+    const PlanArgs p{chosen, 1, L.slots, a, reinterpret_cast<int2*>(ws + L.seen), reinterpret_cast<int*>(ws + L.perm),
+                     reinterpret_cast<Tile*>(ws + L.tiles), L.ntiles, L.tile,
+                     backward ? reinterpret_cast<Tile*>(ws + L.groups) : nullptr, a,
+                     backward ? reinterpret_cast<int2*>(ws + L.merge) : nullptr, 1 << 30, true};
+    const dim3 grid(a + 1, L.segments);
+    if (L.segments > 1) SKM_TRY_LAUNCH(k_plan_count, grid, kPlanThreads, 0, s, p);
+    return launch(k_plan, grid, kPlanThreads, 0, s, p);
+}
+
+template <typename T, int KIND>
+hipError_t launch_product(const Layout& L, FeedArgs<T> p, hipStream_t s)
+{
+    constexpr bool MATRIX = KIND == kGates || KIND == kOuts;
+    const int r = L.tile;
+    p.nn = tiles_of(KIND == kGated ? 2l * p.N : p.N, r);
+    p.nm = MATRIX ? tiles_of(p.M, r) : 0;
+    const long pieces = MATRIX ? (long)p.a * p.splits * (KIND == kGates ? 2 : 1) * p.nm * p.nn : (long)p.ntiles * p.nn;
+    if (pieces == 0) return hipSuccess;
+    const dim3 grid((unsigned)((pieces + 7) / 8 * 8));
+    if (r == kBig) return launch(k_product<T, KIND, 2, 4, 8, 4, true>, grid, 512, 0, s, p);
+    if (L.fast) return launch(k_product<T, KIND, 2, 2, 4, 4, true>, grid, 256, 0, s, p);
+    return launch(k_product<T, KIND, 2, 2, 4, 4, false>, grid, 256, 0, s, p);
+}
+
+template <typename T>
+hipError_t launch_join(const float* sums, const int* chosen, const FeedSizes& z, int w, const T* base, long ld_base, T* out, long ld_out, hipStream_t s)
+{
+    const JoinArgs<T> p{sums, chosen, (int)z.n, z.k, z.a, w, base, ld_base, out, ld_out};
+    return launch(k_feed_join<T>, dim3((unsigned)z.n, (unsigned)((w + 1023) / 1024)), 256, 0, s, p);
+}
+
+}  // namespace
+
+bool feed_fits(const FeedSizes& z)
+{
+    if (z.n * z.k >= 1l << 30) return false;
+    const size_t most = size_t(1) << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
+    const size_t wide = z.d > z.o ? z.d : z.o, rows = (size_t)z.n * z.k / kMid + z.a + 1;
+    const size_t columns = (2 * (size_t)z.f > wide ? 2 * (size_t)z.f : wide) / kMid + 2;
+    const size_t matrix = (size_t)z.a * 2 * ((size_t)z.f / kMid + 1) * (wide / kMid + 1) * 8;
+    return rows * columns < most && matrix < most && (size_t)z.n < most && (wide + 1023) / 1024 < 65536 && (z.n * z.k + kPlanRows - 1) / kPlanRows < 65536;
+}
+
+size_t feed_workspace(const FeedSizes& z, bool backward) { return layout(z, backward).bytes; }
+
+hipError_t launch_feed(const FeedCall& a, hipStream_t s)
+{
+    const FeedSizes& z = a.z;
+    if (z.n == 0) return hipSuccess;
+    const Layout L = layout(z, false);
+    if (L.sorted) {
+        const hipError_t e = launch_plan(L, a.chosen, z.a, a.ws, false, s);
+        if (e != hipSuccess) return e;
+    }
+    return with_type(z.type, [&](auto tag) {
+        using T = decltype(tag);
+        FeedArgs<T> p{};
+        p.tiles = L.sorted ? reinterpret_cast<const Tile*>(a.ws + L.tiles) : nullptr;
+        p.perm = L.sorted ? reinterpret_cast<const int*>(a.ws + L.perm) : nullptr;
+        p.ntiles = L.ntiles;
+        p.slots = L.slots;
+        p.a = z.a;
+        p.byk = by_k(z.k);
+        p.h = (T*)(a.ws + L.h);
+        p.ldh = L.ldh;
+        p.weights = a.weights;
+        p.act = a.act;
+        FeedArgs<T> q = p;
+        p.A = (const T*)a.x; p.lda = a.ld_x;
+        p.B = (const T*)a.gate; p.sb = a.gate_sa; p.ldb = a.gate_ld;
+        p.B2 = (const T*)a.up; p.sb2 = a.up_sa; p.ldb2 = a.up_ld;
+        p.N = z.f; p.K = z.d;
+        p.pre = a.pre;
+        hipError_t e = launch_product<T, kGated>(L, p, s);
+        if (e != hipSuccess) return e;
+        q.A = q.h; q.lda = L.ldh;
+        q.B = (const T*)a.down; q.sb = a.down_sa; q.ldb = a.down_ld;
+        q.N = z.o; q.K = z.f;
+        float* sums = reinterpret_cast<float*>(a.ws + L.sums);
+        if (z.k == 1) {
+            q.base = (const T*)a.base; q.ld_base = a.ld_base;
+            q.out = (T*)a.out; q.ld_out = a.ld_out;
+        } else {
+            q.sums = sums;
+        }
+        e = launch_product<T, kDown>(L, q, s);
+        if (e != hipSuccess || z.k == 1) return e;
+        return launch_join<T>(sums, a.chosen, z, z.o, (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, s);
+    });
+}
+
+hipError_t launch_feed_back(const FeedBackCall& a, hipStream_t s)
+{
+    const FeedSizes& z = a.z;
+    const Layout L = layout(z, true);
+    const bool matrices = a.dgate != nullptr;
+    if (z.n == 0 && !matrices) return hipSuccess;
+    if (L.sorted) {
+        const hipError_t e = launch_plan(L, a.chosen, z.a, a.ws, true, s);
+        if (e != hipSuccess) return e;
+    }
+    return with_type(z.type, [&](auto tag) {
+        using T = decltype(tag);
+        FeedArgs<T> p{};
+        p.tiles = L.sorted ? reinterpret_cast<const Tile*>(a.ws + L.tiles) : nullptr;
+        p.perm = L.sorted ? reinterpret_cast<const int*>(a.ws + L.perm) : nullptr;
+        p.ntiles = L.ntiles;
+        p.slots = L.slots;
+        p.a = z.a;
+        p.byk = by_k(z.k);
+        p.ldh = L.ldh;
+        p.splits = 1;
+        T *h = (T*)(a.ws + L.h), *dg = (T*)(a.ws + L.dg), *du = (T*)(a.ws + L.du);
+        float* part = reinterpret_cast<float*>(a.ws + L.part);
+        hipError_t e = hipSuccess;
+        if (z.n > 0) {
+            FeedArgs<T> q = p;
+            q.A = (const T*)a.dy; q.lda = a.ld_dy;
+            q.B = (const T*)a.down; q.sb = a.down_sa; q.ldb = a.down_ld;
+            q.N = z.f; q.K = z.o;
+            q.h = matrices ? h : nullptr;
+            q.dg = dg; q.du = du;
+            q.pre = const_cast<float*>(a.pre);
+            q.weights = a.weights;
+            q.act = a.act;
+            float* dots = reinterpret_cast<float*>(a.ws + L.dots);
+            q.dots = a.dweights != nullptr ? dots : nullptr;
+            q.ndots = L.ndots;
+            e = launch_product<T, kHidden>(L, q, s);
+            if (e != hipSuccess) return e;
+            if (a.dweights != nullptr) SKM_TRY_LAUNCH(k_feed_dots, dim3((L.slots + 255) / 256), 256, 0, s, dots, L.ndots, a.chosen, L.slots, z.a, a.dweights);
+            if (a.dx != nullptr) {
+                FeedArgs<T> r = p;
+                r.A = dg; r.A2 = du; r.lda = L.ldh;
+                r.B = (const T*)a.gate; r.sb = a.gate_sa; r.ldb = a.gate_ld;
+                r.B2 = (const T*)a.up; r.sb2 = a.up_sa; r.ldb2 = a.up_ld;
+                r.N = z.d; r.K = z.f;
+                float* sums = reinterpret_cast<float*>(a.ws + L.sums);
+                if (z.k == 1) {
+                    r.base = (const T*)a.base; r.ld_base = a.ld_base;
+                    r.out = (T*)a.dx; r.ld_out = a.ld_dx;
+                } else {
+                    r.sums = sums;
+                }
+                e = launch_product<T, kRows>(L, r, s);
+                if (e == hipSuccess && z.k > 1) e = launch_join<T>(sums, a.chosen, z, z.d, (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, s);
+                if (e != hipSuccess) return e;
+            }
+        }
+        if (!matrices) return e;
+        auto merge = [&](int splits, long each, int both, T* dm, T* dm2) {
+            const long blocks = (each * both * z.a + 1023) / 1024;
+            return launch(k_feed_merge<T>, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), 256, 0, s, part, splits, each, both, z.a, dm, dm2);
+        };
+        FeedArgs<T> u = p;
+        u.tiles = L.sorted ? reinterpret_cast<const Tile*>(a.ws + L.groups) : nullptr;
+        u.part = part;
+        FeedArgs<T> v = u;
+        u.A = dg; u.A2 = du; u.lda = L.ldh;
+        u.B = (const T*)a.x; u.ldb = a.ld_x;
+        u.M = z.f; u.N = z.d;
+        u.dm = (T*)a.dgate; u.dm2 = (T*)a.dup;
+        u.splits = L.gsplits;
+        e = launch_product<T, kGates>(L, u, s);
+        if (e == hipSuccess && L.gsplits > 1) e = merge(L.gsplits, (long)z.f * z.d, 2, u.dm, u.dm2);
+        if (e != hipSuccess) return e;
+        v.A = (const T*)a.dy; v.lda = a.ld_dy;
+        v.B = h; v.ldb = L.ldh;
+        v.M = z.o; v.N = z.f;
+        v.dm = (T*)a.ddown;
+        v.splits = L.osplits;
+        e = launch_product<T, kOuts>(L, v, s);
+        if (e == hipSuccess && L.osplits > 1) e = merge(L.osplits, (long)z.o * z.f, 1, v.dm, nullptr);
+        return e;
+    });
+}
+
+}  // namespace skm

@@ -2238,6 +2238,45 @@ int check_rate(int dtype, size_t n, size_t v, size_t k, std::initializer_list<si
     return 0;
 }
 
+struct FeedShape {
+    size_t n, d, f, o, k, a;
+};
+
+int check_feed(int dtype, const FeedShape& z, int act, std::initializer_list<size_t> strides)
+{
+    TRY(check_dtype(dtype));
+    if (z.d == 0 || z.f == 0 || z.o == 0 || z.k == 0 || z.a == 0)
+        return fail(SKMETAL_EINVAL, "d, f, o, k and a must be positive (d=%zu f=%zu o=%zu k=%zu a=%zu)", z.d, z.f, z.o, z.k, z.a);
+    if (act != SKMETAL_SILU && act != SKMETAL_GELU && act != SKMETAL_RELU)
+        return fail(SKMETAL_EINVAL, "act=%d is not SKMETAL_SILU, SKMETAL_GELU or SKMETAL_RELU", act);
+    if (z.k > size_t(kFeedMaxK) || z.a > size_t(kFeedMaxA))
+        return fail(SKMETAL_ERANGE, "k=%zu, a=%zu: at most %d experts, of which a row takes at most %d", z.k, z.a, kFeedMaxA, kFeedMaxK);
+    if (z.n > kMaxRows / 2 || z.d > kMaxDim || z.f > kMaxDim || z.o > kMaxDim)
+        return fail(SKMETAL_ERANGE, "n=%zu, d=%zu, f=%zu or o=%zu exceeds the supported range", z.n, z.d, z.f, z.o);
+    for (const size_t s : strides)
+        if (s > kMaxStride) return fail(SKMETAL_ERANGE, "a stride of %zu elements exceeds the supported range", s);
+    if (!feed_fits(FeedSizes{dtype, (long)z.n, (int)z.d, (int)z.f, (int)z.o, (int)z.k, (int)z.a, true, true}))
+        return fail(SKMETAL_ERANGE, "n=%zu, k=%zu, d=%zu, f=%zu, o=%zu, a=%zu: more blocks than a launch takes", z.n, z.k, z.d, z.f, z.o, z.a);
+    return 0;
+}
+
+// A matrix of a product as it lies in memory: whether each of its rows of `width` elements starts at 16 bytes.
+struct FeedMatrix {
+    const void* p;
+    size_t ld, sa, width;
+    bool aligned(size_t es) const
+    {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0 && sa * es % 16 == 0 && width * es % 16 == 0;
+    }
+};
+
+FeedSizes feed_sizes(int dtype, const FeedShape& z, bool sorted, std::initializer_list<FeedMatrix> all)
+{
+    bool aligned = true;
+    for (const FeedMatrix& m : all) aligned = aligned && m.aligned(elem_size(dtype));
+    return FeedSizes{dtype, (long)z.n, (int)z.d, (int)z.f, (int)z.o, (int)z.k, (int)z.a, sorted, aligned};
+}
+
 int launched(hipError_t e, const char* what)
 {
     if (e == hipSuccess) return 0;
@@ -2436,6 +2475,93 @@ int skmetal_hip_rate_backward(int dtype, const void* logits, size_t ld_logits, c
     RateBackCall a{logits, dtype, (long)n, (int)v, (long)ld_logits, targets, (long)targets_stride, lse, lse_rest, entropy,
                    grad_log_probs, grad_entropy, grad_lse, grad_logits, (long)ld_grad};
     return launched(launch_rate_back(a, static_cast<hipStream_t>(stream)), "rate_backward");
+}
+
+size_t skmetal_hip_feed_workspace(int dtype, size_t n, size_t d, size_t f, size_t o, size_t k, size_t a, int backward)
+{
+    if (check_feed(dtype, {n, d, f, o, k, a}, SKMETAL_SILU, {}) != 0) return 0;
+    size_t most = 0;  // whichever way the call takes its rows and matrices
+    for (int way = 0; way < 4; ++way)
+        most = std::max(most, feed_workspace(FeedSizes{dtype, (long)n, (int)d, (int)f, (int)o, (int)k, (int)a, (way & 1) != 0, (way & 2) != 0}, backward != 0));
+    return most;
+}
+
+int skmetal_hip_feed(int dtype, const void* x, size_t ld_x, const void* gate, size_t gate_stride, size_t gate_ld,
+                     const void* up, size_t up_stride, size_t up_ld, const void* down, size_t down_stride, size_t down_ld,
+                     const int32_t* chosen, const float* weights, int act, const void* base, size_t ld_base, void* out,
+                     size_t ld_out, float* pre, size_t n, size_t d, size_t f, size_t o, size_t k, size_t a,
+                     void* workspace, size_t workspace_bytes, void* stream)
+{
+    g_err.clear();
+    TRY(check_feed(dtype, {n, d, f, o, k, a}, act, {ld_x, gate_stride, gate_ld, up_stride, up_ld, down_stride, down_ld, ld_base, ld_out}));
+    if (!gate || !up || !down || (n > 0 && (!x || !out))) return fail(SKMETAL_EINVAL, "null pointer argument");
+    if (!chosen && (k != 1 || a != 1)) return fail(SKMETAL_EINVAL, "chosen is null: k=%zu and a=%zu must be 1", k, a);
+    if (ld_out < o && n > 1) return fail(SKMETAL_EINVAL, "ld_out=%zu: the rows of out overlap", ld_out);
+    const size_t es = elem_size(dtype);
+    TRY(check_aligned(x, es, "x"));
+    TRY(check_aligned(gate, es, "gate"));
+    TRY(check_aligned(up, es, "up"));
+    TRY(check_aligned(down, es, "down"));
+    TRY(check_aligned(base, es, "base"));
+    TRY(check_aligned(out, es, "out"));
+    const RowSpan result(out, ld_out, o, n, es);
+    if (base != nullptr) {
+        const RowSpan b(base, ld_base, o, n, es);
+        if (!result.same(b) && share(result, b)) return fail(SKMETAL_EINVAL, "out shares memory with base without being it");
+    }
+    const FeedSizes z = feed_sizes(dtype, {n, d, f, o, k, a}, chosen != nullptr,
+                                   {{x, ld_x, 0, d}, {gate, gate_ld, gate_stride, d}, {up, up_ld, up_stride, d}, {down, down_ld, down_stride, f}});
+    TRY(check_workspace(workspace, workspace_bytes, feed_workspace(z, false)));
+    TRY(on_device());
+    FeedCall A{z, x, (long)ld_x, gate, (long)gate_stride, (long)gate_ld, up, (long)up_stride, (long)up_ld, down, (long)down_stride,
+               (long)down_ld, chosen, weights, act, base, (long)ld_base, out, (long)ld_out, pre, static_cast<char*>(workspace)};
+    return launched(launch_feed(A, static_cast<hipStream_t>(stream)), "feed");
+}
+
+int skmetal_hip_feed_backward(int dtype, const void* grad, size_t ld_grad, const void* x, size_t ld_x, const void* gate,
+                              size_t gate_stride, size_t gate_ld, const void* up, size_t up_stride, size_t up_ld,
+                              const void* down, size_t down_stride, size_t down_ld, const int32_t* chosen,
+                              const float* weights, int act, const float* pre, const void* base, size_t ld_base,
+                              void* grad_x, size_t ld_grad_x, void* grad_gate, void* grad_up, void* grad_down,
+                              float* grad_weights, size_t n, size_t d, size_t f, size_t o, size_t k, size_t a,
+                              void* workspace, size_t workspace_bytes, void* stream)
+{
+    g_err.clear();
+    TRY(check_feed(dtype, {n, d, f, o, k, a}, act,
+                   {ld_grad, ld_x, gate_stride, gate_ld, up_stride, up_ld, down_stride, down_ld, ld_base, ld_grad_x}));
+    if (!gate || !up || !down || (n > 0 && (!grad || !x || !pre))) return fail(SKMETAL_EINVAL, "null pointer argument");
+    if ((grad_gate == nullptr) != (grad_up == nullptr) || (grad_gate == nullptr) != (grad_down == nullptr))
+        return fail(SKMETAL_EINVAL, "grad_gate, grad_up and grad_down must be given together or not at all");
+    if (!chosen && (k != 1 || a != 1)) return fail(SKMETAL_EINVAL, "chosen is null: k=%zu and a=%zu must be 1", k, a);
+    if (grad_x && ld_grad_x < d && n > 1) return fail(SKMETAL_EINVAL, "ld_grad_x=%zu: the rows of grad_x overlap", ld_grad_x);
+    const size_t es = elem_size(dtype);
+    TRY(check_aligned(grad, es, "grad"));
+    TRY(check_aligned(x, es, "x"));
+    TRY(check_aligned(gate, es, "gate"));
+    TRY(check_aligned(up, es, "up"));
+    TRY(check_aligned(down, es, "down"));
+    TRY(check_aligned(base, es, "base"));
+    TRY(check_aligned(grad_x, es, "grad_x"));
+    TRY(check_aligned(grad_gate, es, "grad_gate"));
+    TRY(check_aligned(grad_up, es, "grad_up"));
+    TRY(check_aligned(grad_down, es, "grad_down"));
+    if (grad_x != nullptr) {
+        const RowSpan result(grad_x, ld_grad_x, d, n, es);
+        if (share(result, RowSpan(grad, ld_grad, o, n, es)) || share(result, RowSpan(x, ld_x, d, n, es)))
+            return fail(SKMETAL_EINVAL, "grad_x shares memory with grad or x");
+        if (base != nullptr) {
+            const RowSpan b(base, ld_base, d, n, es);
+            if (!result.same(b) && share(result, b)) return fail(SKMETAL_EINVAL, "grad_x shares memory with base without being it");
+        }
+    }
+    const FeedSizes z = feed_sizes(dtype, {n, d, f, o, k, a}, chosen != nullptr,
+                                   {{grad, ld_grad, 0, o}, {x, ld_x, 0, d}, {gate, gate_ld, gate_stride, d}, {up, up_ld, up_stride, d}, {down, down_ld, down_stride, f}});
+    TRY(check_workspace(workspace, workspace_bytes, feed_workspace(z, true)));
+    TRY(on_device());
+    FeedBackCall A{z, grad, (long)ld_grad, x, (long)ld_x, gate, (long)gate_stride, (long)gate_ld, up, (long)up_stride, (long)up_ld, down,
+                   (long)down_stride, (long)down_ld, chosen, weights, act, pre, base, (long)ld_base, grad_x, (long)ld_grad_x, grad_gate,
+                   grad_up, grad_down, grad_weights, static_cast<char*>(workspace)};
+    return launched(launch_feed_back(A, static_cast<hipStream_t>(stream)), "feed_backward");
 }
 
 }  // extern "C"

@@ -33,6 +33,7 @@ MAX_RANK = 128
 MAX_SCORES = 1 << 22
 
 _ADAPT, _ADAPT_BACKWARD, _ADAPT_IN_X = 0, 1, 2
+_ACT = {"silu": 0, "gelu": 1, "relu": 2}
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -65,6 +66,16 @@ class AdaptGrads(NamedTuple):
     down: torch.Tensor
     up: torch.Tensor
     gates: torch.Tensor | None
+
+
+class FeedGrads(NamedTuple):
+    """``feed_backward``'s results; None for what was not asked for."""
+
+    x: torch.Tensor | None
+    gate: torch.Tensor | None
+    up: torch.Tensor | None
+    down: torch.Tensor | None
+    weights: torch.Tensor | None
 
 
 @functools.lru_cache(maxsize=1)
@@ -393,6 +404,140 @@ def routed(logits, top_k, *, mask=None, normalize=False) -> Routing:
 def adapted(x, down, up, ids, *, base=None, gates=None, scales=None):
     """``adapt`` inside autograd: gradients go to x, down, up, base and gates."""
     return _Adapted.apply(x, down, up, ids, base, gates, scales)
+
+
+# ---- gated feed-forward blocks ----
+
+
+@functools.lru_cache(maxsize=4096)
+def _feed_workspace(code, n, d, f, o, k, a, backward):
+    return _lib().skmetal_hip_feed_workspace(code, n, d, f, o, k, a, backward)
+
+
+def _matrices(t, name, dtype, shape, device):
+    """The expert and row strides of `t` [a, rows, columns]."""
+    if t.dtype != dtype or t.device != device or t.shape != shape:
+        _refuse(t, name, dtype, shape, device)
+    sa, ld, one = t.stride()
+    if one != 1 and shape[2] > 1:
+        raise ValueError(f"{name}'s rows must have their elements side by side (stride(2) is {one})")
+    return sa, ld
+
+
+def _check_feed(x, gate, up, down, chosen, weights, act):
+    code, device = _first(x, "x")
+    n, d = x.shape
+    dtype = x.dtype
+    ld = _rows(x, "x", dtype, (n, d), device)
+    if gate.dim() != 3:
+        raise ValueError(f"gate has shape {tuple(gate.shape)}, expected (experts, hidden, {d})")
+    a, f, _ = gate.shape
+    o = down.shape[1] if down.dim() == 3 else 0
+    if not (a >= 1 and f >= 1 and d >= 1 and (o >= 1 or down.dim() != 3)):
+        raise ValueError(f"gate has shape {tuple(gate.shape)} and down {tuple(down.shape)}: no size may be 0")
+    if a > MAX_EXPERTS:
+        raise ValueError(f"gate has {a} experts, expected at most {MAX_EXPERTS}")
+    strides = _matrices(gate, "gate", dtype, (a, f, d), device), _matrices(up, "up", dtype, (a, f, d), device)
+    strides += (_matrices(down, "down", dtype, (a, o or "out", f), device),)
+    if act not in _ACT:
+        raise ValueError(f"act={act!r} is not one of {', '.join(_ACT)}")
+    if chosen is None:
+        if a != 1:
+            raise ValueError(f"chosen is None, which takes one expert; gate has {a}")
+        k, chosen_ptr = 1, None
+    else:
+        k = chosen.shape[1] if chosen.dim() == 2 else 0
+        if not 1 <= k <= MAX_TOP_K:
+            raise ValueError(f"chosen has shape {tuple(chosen.shape)}, expected ({n}, 1 to {MAX_TOP_K})")
+        chosen_ptr = _dense(chosen, "chosen", torch.int32, (n, k), device)
+    weight_ptr = None if weights is None else _dense(weights, "weights", torch.float32, (n, k), device)
+    (gs, gl), (us, ul), (ds, dl) = strides
+    shared = (gate.data_ptr(), gs, gl, up.data_ptr(), us, ul, down.data_ptr(), ds, dl, chosen_ptr, weight_ptr, _ACT[act])
+    return code, device, n, d, f, o, k, a, ld, shared
+
+
+def feed(x, gate, up, down, chosen=None, *, weights=None, base=None, act="silu", out=None, return_pre=False):
+    """base + the gated feed-forward block of every row's experts: with q = chosen[i, j]
+
+        out_i = base_i + sum_j weights_ij down_q (act(gate_q x_i) * (up_q x_i))
+
+    x [n, d]; gate and up [a, f, d] and down [a, o, f], each expert's a projection's weight; chosen int32
+    [n, k], k up to 16, with any value outside [0, a) for no expert (a router's ``experts`` as
+    they come; None: all rows take the one expert that there is), and weights float32 [n, k] (None: 1); base [n, o]
+    is the residual stream (None: 0).  x, the matrices, base and out have one type; `act` is "silu", "gelu" (by
+    the normal distribution function) or "relu".  `out` may be base; it shares memory with nothing else.  With
+    `return_pre` also returns gate_q x_i and up_q x_i, float32 [n, k, 2, f], for ``feed_backward``.
+
+    Sums are float32.  The hidden vector, weighted, is rounded to the rows' type once before the second
+    product: float16 rows need it in that type's range."""
+    code, device, n, d, f, o, k, a, x_ld, shared = _check_feed(x, gate, up, down, chosen, weights, act)
+    dtype = x.dtype
+    base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, o), device))
+    lib = _lib()
+    if out is None:
+        out, out_ld = torch.empty((n, o), dtype=dtype, device=device), o
+    else:
+        out_ld = _rows(out, "out", dtype, (n, o), device)
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out requires a gradient, which this call does not record: use fed, or torch.no_grad")
+        torch.autograd.graph.increment_version(out)
+    pre = torch.empty((n, k, 2, f), dtype=torch.float32, device=device) if return_pre else None
+    size = _feed_workspace(code, n, d, f, o, k, a, 0)
+    ws, ws_ptr = _workspace(size, device)
+    if lib.skmetal_hip_feed(code, x.data_ptr(), x_ld, *shared, base_ptr, base_ld, out.data_ptr(), out_ld, None if pre is None else pre.data_ptr(),
+                            n, d, f, o, k, a, ws_ptr, size, _stream(device)):
+        _fail("feed")
+    return (out, pre) if return_pre else out
+
+
+def feed_backward(grad, x, gate, up, down, chosen, pre, *, weights=None, base=None, act="silu", rows=True, matrices=True) -> FeedGrads:
+    """The gradients of ``feed`` from grad [n, o], that of its output; `pre` is what the forward call
+    returned.  The gradient of x is added to `base` [n, d] (None: 0); those of the matrices have
+    their shapes and type, 0 for an expert without rows; that of weights is None where there are
+    none.  The gradient of the forward call's base is grad itself.  Without `rows` that of x is left
+    out, without `matrices` those of gate, up and down (frozen experts)."""
+    code, device, n, d, f, o, k, a, x_ld, shared = _check_feed(x, gate, up, down, chosen, weights, act)
+    dtype = x.dtype
+    grad_ld = _rows(grad, "grad", dtype, (n, o), device)
+    pre_ptr = _dense(pre, "pre", torch.float32, (n, k, 2, f), device)
+    base_ptr, base_ld = (None, 0) if base is None else (base.data_ptr(), _rows(base, "base", dtype, (n, d), device))
+    lib = _lib()
+    dx = torch.empty((n, d), dtype=dtype, device=device) if rows else None
+    dm = [torch.empty(s, dtype=dtype, device=device) for s in ((a, f, d), (a, f, d), (a, o, f))] if matrices else [None] * 3
+    dw = None if weights is None else torch.empty((n, k), dtype=torch.float32, device=device)
+    size = _feed_workspace(code, n, d, f, o, k, a, 1)
+    ws, ws_ptr = _workspace(size, device)
+    if lib.skmetal_hip_feed_backward(code, grad.data_ptr(), grad_ld, x.data_ptr(), x_ld, *shared, pre_ptr, base_ptr, base_ld,
+                                     *(None if t is None else t.data_ptr() for t in (dx,)), d, *(None if t is None else t.data_ptr() for t in (*dm, dw)),
+                                     n, d, f, o, k, a, ws_ptr, size, _stream(device)):
+        _fail("feed_backward")
+    return FeedGrads(dx, *dm, dw)
+
+
+class _Fed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, chosen, weights, base, act):
+        out, pre = feed(x, gate, up, down, chosen, weights=weights, base=base, act=act, return_pre=True)
+        ctx.save_for_backward(x, gate, up, down, chosen, pre, weights)
+        ctx.act = act
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, gate, up, down, chosen, pre, weights = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        rows = grad if grad.stride(1) == 1 or grad.shape[1] == 1 else grad.contiguous()
+        if any(need[:4]) or need[5]:
+            g = feed_backward(rows, x, gate, up, down, chosen, pre, weights=weights, act=ctx.act, rows=need[0], matrices=any(need[1:4]))
+        else:
+            g = FeedGrads(None, None, None, None, None)
+        return g.x, g.gate, g.up, g.down, None, g.weights, grad if need[6] else None, None
+
+
+def fed(x, gate, up, down, chosen=None, *, weights=None, base=None, act="silu"):
+    """``feed`` inside autograd: gradients go to x, the matrices, weights and base."""
+    return _Fed.apply(x, gate, up, down, chosen, weights, base, act)
 
 
 # ---- dropout ----
