@@ -60,8 +60,6 @@ struct FeedArgs {
     T *dm, *dm2; float* part; int splits;      // [a][M][N]; partial sums [splits][a][2 where dm2][M][N] where splits > 1
 };
 
-__device__ __forceinline__ float gelu_cdf(float g) { return 0.5f * (1.f + erff(g * 0.70710678118654752f)); }
-
 // act(g) and its derivative
 __device__ __forceinline__ float2 activate(float g, int act)
 {
@@ -70,7 +68,7 @@ __device__ __forceinline__ float2 activate(float g, int act)
         return make_float2(g * t, t * (1.f + g * (1.f - t)));
     }
     if (act == kGelu) {
-        const float c = gelu_cdf(g);
+        const float c = 0.5f * erfcf(g * -0.70710678118654752f);  // keeps its bits where 1 + erf would lose them
         return make_float2(g * c, c + g * 0.39894228040143268f * expf(-0.5f * g * g));
     }
     return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);

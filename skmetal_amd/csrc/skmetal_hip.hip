@@ -2495,7 +2495,7 @@ int skmetal_hip_feed(int dtype, const void* x, size_t ld_x, const void* gate, si
     g_err.clear();
     TRY(check_feed(dtype, {n, d, f, o, k, a}, act, {ld_x, gate_stride, gate_ld, up_stride, up_ld, down_stride, down_ld, ld_base, ld_out}));
     if (!gate || !up || !down || (n > 0 && (!x || !out))) return fail(SKMETAL_EINVAL, "null pointer argument");
-    if (!chosen && (k != 1 || a != 1)) return fail(SKMETAL_EINVAL, "chosen is null: k=%zu and a=%zu must be 1", k, a);
+    if (!chosen && n > 0 && (k != 1 || a != 1)) return fail(SKMETAL_EINVAL, "chosen is null: k=%zu and a=%zu must be 1", k, a);
     if (ld_out < o && n > 1) return fail(SKMETAL_EINVAL, "ld_out=%zu: the rows of out overlap", ld_out);
     const size_t es = elem_size(dtype);
     TRY(check_aligned(x, es, "x"));
@@ -2532,7 +2532,7 @@ int skmetal_hip_feed_backward(int dtype, const void* grad, size_t ld_grad, const
     if (!gate || !up || !down || (n > 0 && (!grad || !x || !pre))) return fail(SKMETAL_EINVAL, "null pointer argument");
     if ((grad_gate == nullptr) != (grad_up == nullptr) || (grad_gate == nullptr) != (grad_down == nullptr))
         return fail(SKMETAL_EINVAL, "grad_gate, grad_up and grad_down must be given together or not at all");
-    if (!chosen && (k != 1 || a != 1)) return fail(SKMETAL_EINVAL, "chosen is null: k=%zu and a=%zu must be 1", k, a);
+    if (!chosen && n > 0 && (k != 1 || a != 1)) return fail(SKMETAL_EINVAL, "chosen is null: k=%zu and a=%zu must be 1", k, a);
     if (grad_x && ld_grad_x < d && n > 1) return fail(SKMETAL_EINVAL, "ld_grad_x=%zu: the rows of grad_x overlap", ld_grad_x);
     const size_t es = elem_size(dtype);
     TRY(check_aligned(grad, es, "grad"));

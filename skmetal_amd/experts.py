@@ -620,6 +620,23 @@ def _check_rate(logits, targets):
     return code, device, n, v, ld, targets.data_ptr(), _vector(targets, "targets", torch.int32, n, device)
 
 
+def _run_rate(logits, targets, top_k, vectors):
+    code, device, n, v, ld, target_ptr, target_stride = _check_rate(logits, targets)
+    k = int(top_k)
+    if not 0 <= k <= min(v, MAX_TOP_K):
+        raise ValueError(f"top_k={k} is not in [0, {min(v, MAX_TOP_K)}]")
+    lib = _lib()
+    whole = vectors(n, device)
+    top = torch.empty((n, k), dtype=torch.int32, device=device) if k else None
+    top_log_probs = torch.empty((n, k), dtype=torch.float32, device=device) if k else None
+    size = _rate_workspace(code, n, v, k)
+    ws, ws_ptr = _workspace(size, device)
+    if lib.skmetal_hip_rate(code, logits.data_ptr(), ld, target_ptr, target_stride, n, v, k, *(t.data_ptr() for t in whole),
+                            top.data_ptr() if k else None, top_log_probs.data_ptr() if k else None, ws_ptr, size, _stream(device)):
+        _fail("rate")
+    return Rating(*whole, top, top_log_probs)
+
+
 def rate(logits, targets, *, top_k=0) -> Rating:
     """How likely the scores logits [n, v] make each row's target (int32 [n]; a value outside
     [0, v) is a row without one, whose log probability is 0), with the entropy of the
@@ -629,21 +646,8 @@ def rate(logits, targets, *, top_k=0) -> Rating:
     A score of -inf or NaN is excluded: its log probability is -inf and it is never among the largest (-1 in
     the places that remain).  A row without a score left has an entropy of 0 and a ``lse`` of -inf; with a
     score of +inf its log probabilities and entropy are NaN.  The same inputs give the same bits on every call."""
-    code, device, n, v, ld, target_ptr, target_stride = _check_rate(logits, targets)
-    k = int(top_k)
-    if not 0 <= k <= min(v, MAX_TOP_K):
-        raise ValueError(f"top_k={k} is not in [0, {min(v, MAX_TOP_K)}]")
-    lib = _lib()
-    whole = torch.empty((4, n), dtype=torch.float32, device=device)
-    at = whole.data_ptr()
-    top = torch.empty((n, k), dtype=torch.int32, device=device) if k else None
-    top_log_probs = torch.empty((n, k), dtype=torch.float32, device=device) if k else None
-    size = _rate_workspace(code, n, v, k)
-    ws, ws_ptr = _workspace(size, device)
-    if lib.skmetal_hip_rate(code, logits.data_ptr(), ld, target_ptr, target_stride, n, v, k, at, at + 4 * n, at + 8 * n, at + 12 * n,
-                            top.data_ptr() if k else None, top_log_probs.data_ptr() if k else None, ws_ptr, size, _stream(device)):
-        _fail("rate")
-    return Rating(*whole.unbind(0), top, top_log_probs)
+    # one tensor, cut apart
+    return _run_rate(logits, targets, top_k, lambda n, device: torch.empty((4, n), dtype=torch.float32, device=device).unbind(0))
 
 
 def rate_backward(logits, targets, rating: Rating, *, grad_log_probs=None, grad_entropy=None, grad_lse=None):
@@ -666,9 +670,10 @@ def rate_backward(logits, targets, rating: Rating, *, grad_log_probs=None, grad_
 class _Rated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k):
-        r = rate(logits, targets, top_k=top_k)
+        # vectors in memory of their own: views that a Function returns cannot be changed in place
+        r = _run_rate(logits, targets, top_k, lambda n, device: [torch.empty(n, dtype=torch.float32, device=device) for _ in range(4)])
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, targets, r.lse.clone(), r.lse_rest, r.entropy.clone())
+            ctx.save_for_backward(logits, targets, r.lse.clone(), r.lse_rest.clone(), r.entropy.clone())  # the caller may change its own
         ctx.mark_non_differentiable(*(t for t in (r.lse_rest, r.top, r.top_log_probs) if t is not None))
         ctx.set_materialize_grads(False)
         return tuple(r)
@@ -684,5 +689,6 @@ class _Rated(torch.autograd.Function):
 
 def rated(logits, targets, *, top_k=0) -> Rating:
     """``rate`` inside autograd: log_probs, entropy and lse pass their gradients to logits (the
-    mean of -log_probs over the rows with a target is their cross entropy)."""
+    mean of -log_probs over the rows with a target is their cross entropy).  The results may
+    be changed in place; the gradient stays that of this call's own."""
     return Rating(*_Rated.apply(logits, targets, top_k))
