@@ -134,7 +134,8 @@ template <typename T, bool ALONG, int R, int NT, bool FAST>
 struct Stager {
     static constexpr int V = kVec<T>, C = R * 8 / NT, CHUNKS = ALONG ? 8 : R / V;
     static_assert(C * NT == R * 8, "whole chunks a lane");
-    const T* p[C];       // ALONG: the row's chunk of the present step; else the column of the chunk in row 0
+    const T* p[C];  // the chunks of the next step
+    int slot[C];    // of their rows, where the rows are gathered
     Vec<T> held[FAST ? 1 : C];
 
     static __device__ __forceinline__ int index(int c) { return c * NT + (int)threadIdx.x; }
@@ -144,6 +145,9 @@ struct Stager {
         const int l = line(c), s = index(c) % CHUNKS;
         return ALONG ? s ^ (l & 7) : s ^ displaced<T, CHUNKS>(l);
     }
+    // across: where a chunk lies in its row, of which `left` elements are the tile's; FAST reads what exists instead of
+    // columns that do not, whose results nothing takes
+    static __device__ __forceinline__ int column(int c, int left) { return FAST ? min(chunk(c) * V, left - V) : chunk(c) * V; }
 
     // along: row(i) is the address of row i of the tile (one that exists, also where the tile has no such row)
     template <typename F>
@@ -152,17 +156,19 @@ struct Stager {
 #pragma unroll
         for (int c = 0; c < C; ++c) p[c] = row(line(c)) + chunk(c) * V;
     }
-
-    // across: the columns from `col` on, of which `left` exist
-    __device__ __forceinline__ int column(int c, int left) const { return FAST ? min(chunk(c) * V, left - V) : chunk(c) * V; }
+    // across: `first` is the address of the first term's row, at column 0 of the tile
+    __device__ __forceinline__ void terms(const T* first, long ld, int left)
+    {
+#pragma unroll
+        for (int c = 0; c < C; ++c) p[c] = first + line(c) * ld + column(c, left);
+    }
 
     __device__ __forceinline__ void fetch(int c, const T* from, bool there, int left, char* to)
     {
-        if constexpr (FAST) {
+        if constexpr (FAST)
             to_lds(there ? (const void*)from : (const void*)g_zeros, to + (c * NT + wave_index() * 64) * 16);
-        } else {
+        else
             held[c] = there && left > 0 ? load_part(from, left) : Vec<T>{};
-        }
     }
     __device__ __forceinline__ void settle(char* to)
     {
@@ -171,28 +177,45 @@ struct Stager {
             for (int c = 0; c < C; ++c) *reinterpret_cast<Vec<T>*>(to + index(c) * 16) = held[c];
     }
 
-    // the step that begins at term k0 of `terms`
-    __device__ __forceinline__ void along(int k0, int terms, char* to)
+    // The step that begins at term k0 of `count`, the first that was not taken yet.
+    __device__ __forceinline__ void along(int k0, int count, char* to)
     {
-        if (k0 + kStep<T> <= terms) {
+        if (k0 + kStep<T> <= count) {
 #pragma unroll
             for (int c = 0; c < C; ++c) fetch(c, p[c], true, V, to);
         } else {
 #pragma unroll
-            for (int c = 0; c < C; ++c) fetch(c, p[c], k0 + chunk(c) * V < terms, terms - k0 - chunk(c) * V, to);
+            for (int c = 0; c < C; ++c) fetch(c, p[c], k0 + chunk(c) * V < count, count - k0 - chunk(c) * V, to);
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) p[c] += kStep<T>;
     }
-    // row(k): the address of term k's row, at column 0 of the tile; `left` of its columns exist
-    template <typename F>
-    __device__ __forceinline__ void across(int k0, int terms, int left, F&& row, char* to)
+    __device__ __forceinline__ void across(int k0, int count, long ld, int left, char* to)
+    {
+        if (k0 + kStep<T> <= count) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) fetch(c, p[c], true, left - chunk(c) * V, to);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) fetch(c, p[c], k0 + line(c) < count, left - chunk(c) * V, to);
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) p[c] += kStep<T> * ld;
+    }
+    // The same for gathered rows: look() a step ahead, so that the slots are there when their rows are fetched.
+    __device__ __forceinline__ void look(int k0, int count, const int* perm, int start)
     {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int k = k0 + line(c);
-            fetch(c, row(min(k, terms - 1)) + column(c, left), k < terms, left - chunk(c) * V, to);
+            const int place = start + min(k0 + line(c), count - 1);
+            slot[c] = perm != nullptr ? perm[place] : place;
         }
+    }
+    __device__ __forceinline__ void gathered(int k0, int count, const ByK& byk, const T* first, long ld, int left, char* to)
+    {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            fetch(c, first + (long)byk.row((unsigned)slot[c]) * ld + column(c, left), k0 + line(c) < count, left - chunk(c) * V, to);
     }
 };
 
@@ -254,6 +277,11 @@ __device__ __forceinline__ int piece_of(unsigned x, int count) { return (int)(x 
 // ---- the product ----
 
 // A block's tile of WM TM 16 x WN TN 16 results; a wave's is TM 16 x TN 16.
+//
+// Two stages of LDS: while a step's products run from one, the next step's operands come into the other.  A step is 2 TM
+// groups of TN products (half of its terms, one row of fragments).  Fragments are read three groups ahead, across the
+// steps too: the barrier stands before the last three groups, when every wave has read what it needs of the
+// stage, so that the products of these hide it and the first reads of the next stage.
 template <typename T, int KIND, int WM, int WN, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
 {
@@ -267,14 +295,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
     const int wm = wave / WN, wn = wave % WN;
     Tile t;
     int n0, m0 = 0, split = 0;
-    const T *A = p.A, *B = p.B, *A2 = p.A2, *B2 = p.B2;
+    const T *A = p.A, *B = p.B, *B2 = p.B2;
     T* dm = p.dm;
     int terms = p.K, from = 0, matrix = 0;
     if constexpr (MATRIX) {
-        const int per = p.nm * p.nn, both = KIND == kGates ? 2 : 1;
-        const int piece = piece_of(blockIdx.x, p.a * p.splits * both * per);
-        if (piece >= p.a * p.splits * both * per) return;
-        const int i = piece % per, rest = piece / per;
+        // every XCD takes an eighth of each expert's tiles: experts differ in their slots
+        const int per = p.nm * p.nn, wide = (per + 7) / 8 * 8, both = KIND == kGates ? 2 : 1;
+        const int rest = blockIdx.x / wide, i = piece_of(blockIdx.x % wide, per);
+        if (i >= per) return;
         const int group = i / (GROUP * p.nn), in = i - group * GROUP * p.nn, high = min(GROUP, p.nm - group * GROUP);
         m0 = (group * GROUP + in % high) * RA;
         n0 = in / high * RB;
@@ -284,14 +312,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
         t = p.tiles != nullptr ? p.tiles[q] : Tile{0, 0, p.slots, -1};
         t.q = q;
         if (matrix) {
-            A = A2;
+            A = p.A2;
             dm = p.dm2;
         }
         // this part's slots, whole steps
         const int steps = (t.cnt + kStep<T> - 1) / kStep<T>;
         from = (int)((long)steps * split / p.splits) * kStep<T>;
-        terms = min(t.cnt, (int)((long)steps * (split + 1) / p.splits) * kStep<T>) - from;
-        if (terms < 0) terms = 0;
+        terms = max(0, min(t.cnt, (int)((long)steps * (split + 1) / p.splits) * kStep<T>) - from);
     } else {
         const int all = p.ntiles * p.nn, piece = piece_of(blockIdx.x, all);
         if (piece >= all) return;
@@ -319,53 +346,55 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
             }
             return;
         }
-    }
-    auto slot_of = [&](int place) -> int { return p.perm != nullptr ? p.perm[place] : place; };
-    // the caller's row of the tile's i-th slot
-    auto row_of = [&](int i) -> long { return (long)p.byk.row((unsigned)slot_of(t.start + i)); };
-
-    Stager<T, A_ALONG, RA, NT, FAST> sa;
-    Stager<T, B_ALONG, RB, NT, FAST> sb;
-    if constexpr (!MATRIX) {
         B += t.q * p.sb;
         if constexpr (KIND == kGated || KIND == kRows) B2 += t.q * p.sb2;
     }
-    auto begin_a = [&](const T* from_a) {
-        if constexpr (KIND == kGated || KIND == kHidden) sa.rows([&](int r) { return from_a + row_of(min(r, t.cnt - 1)) * p.lda; });
-        if constexpr (KIND == kDown || KIND == kRows) sa.rows([&](int r) { return from_a + (long)(t.start + min(r, t.cnt - 1)) * p.lda; });
+    auto slot_of = [&](int place) -> int { return p.perm != nullptr ? p.perm[place] : place; };
+
+    Stager<T, A_ALONG, RA, NT, FAST> sa;
+    Stager<T, B_ALONG, RB, NT, FAST> sb;
+    const int steps1 = (terms + kStep<T> - 1) / kStep<T>, steps = KIND == kRows ? 2 * steps1 : steps1;
+    const int left_a = p.M - m0, left_b = p.N - n0, start = t.start + from;
+    auto begin_a = [&](const T* a) {
+        if constexpr (KIND == kGated || KIND == kHidden)
+            sa.rows([&](int r) { return a + (long)p.byk.row((unsigned)slot_of(t.start + min(r, t.cnt - 1))) * p.lda; });
+        if constexpr (KIND == kDown || KIND == kRows) sa.rows([&](int r) { return a + (long)(t.start + min(r, t.cnt - 1)) * p.lda; });
     };
     begin_a(A);
+    if constexpr (KIND == kGates) sa.terms(A + m0 + start * p.lda, p.lda, left_a);
     if constexpr (KIND == kGated)  // 16 rows of one matrix beside 16 of the other
         sb.rows([&](int r) {
             const int f = min(n0 + (r >> 5) * 16 + (r & 15), p.N - 1);
             return r & 16 ? B2 + f * p.ldb2 : B + f * p.ldb;
         });
     if constexpr (KIND == kDown) sb.rows([&](int r) { return B + (long)min(n0 + r, p.N - 1) * p.ldb; });
+    if constexpr (KIND == kHidden || KIND == kRows) sb.terms(B + n0, p.ldb, left_b);
+    if constexpr (KIND == kOuts) sb.terms(B + n0 + start * p.ldb, p.ldb, left_b);
 
-    const int steps1 = (terms + kStep<T> - 1) / kStep<T>, steps = KIND == kRows ? 2 * steps1 : steps1;
+    auto look = [&](int step) {
+        if constexpr (KIND == kOuts) sa.look(step * kStep<T>, terms, p.perm, start);
+        if constexpr (KIND == kGates) sb.look(step * kStep<T>, terms, p.perm, start);
+    };
     auto fetch = [&](int step, char* to) {
+        char* to_b = to + RA * kStepBytes;
         int k0 = step * kStep<T>;
+        bool second = false;
         if constexpr (KIND == kRows)
             if (step >= steps1) {
+                second = true;
                 k0 -= steps1 * kStep<T>;
-                if (step == steps1) begin_a(A2);
+                if (step == steps1) {
+                    begin_a(p.A2);
+                    sb.terms(B2 + n0, p.ldb2, left_b);
+                }
             }
-        if constexpr (A_ALONG)
-            sa.along(k0, terms, to);
-        else
-            sa.across(k0, terms, p.M - m0,
-                      [&](int k) { return A + m0 + (KIND == kOuts ? row_of(from + k) : (long)(t.start + from + k)) * p.lda; }, to);
-        if constexpr (B_ALONG)
-            sb.along(k0, terms, to + RA * kStepBytes);
-        else if constexpr (MATRIX)
-            sb.across(k0, terms, p.N - n0,
-                      [&](int k) { return B + n0 + (KIND == kGates ? row_of(from + k) : (long)(t.start + from + k)) * p.ldb; }, to + RA * kStepBytes);
-        else {
-            const bool second = KIND == kRows && step >= steps1;
-            const T* b = second ? B2 : B;
-            const long ld = second ? p.ldb2 : p.ldb;
-            sb.across(k0, terms, p.N - n0, [&](int k) { return b + n0 + k * ld; }, to + RA * kStepBytes);
-        }
+        if constexpr (A_ALONG) sa.along(k0, terms, to);
+        if constexpr (KIND == kGates) sa.across(k0, terms, p.lda, left_a, to);
+        if constexpr (KIND == kOuts) sa.gathered(k0, terms, p.byk, A + m0, p.lda, left_a, to);
+        if constexpr (B_ALONG) sb.along(k0, terms, to_b);
+        if constexpr (KIND == kHidden || KIND == kRows || KIND == kOuts) sb.across(k0, terms, second ? p.ldb2 : p.ldb, left_b, to_b);
+        if constexpr (KIND == kGates) sb.gathered(k0, terms, p.byk, B + n0, p.ldb, left_b, to_b);
+        if (step + 1 < steps) look(step + 1);
     };
     auto settle = [&](char* to) {
         sa.settle(to);
@@ -381,114 +410,130 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     if (steps > 0) {
+        constexpr int GROUPS = 2 * TM, AHEAD = 3, RING = AHEAD + 1;
+        static_assert(GROUPS % RING == 0 && GROUPS - AHEAD >= TM, "a fragment's registers are free when the next step reads into them");
+        Vec<T> x[RING], y[2][TN];
+        look(0);
         fetch(0, lds);
         settle(lds);
-    }
-    landed<FAST>();
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        char* now = lds + (s & 1) * STAGE;
-        char* next = lds + ((s + 1) & 1) * STAGE;
-        if (s + 1 < steps) fetch(s + 1, next);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            Vec<T> x[TM], y[TN];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) y[j] = rb.read(now + RA * kStepBytes, j, half);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) x[i] = ra.read(now, i, half);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mfma16(y[j], x[i], acc[i][j]);
-        }
-        if (s + 1 < steps) settle(next);
         landed<FAST>();
         __syncthreads();
+        if (steps > 1) fetch(1, lds + STAGE);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) y[0][j] = rb.read(lds + RA * kStepBytes, j, 0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) x[i] = ra.read(lds, i, 0);
+        for (int s = 0; s < steps; ++s) {
+            char* now = lds + (s & 1) * STAGE;
+            char* next = lds + ((s + 1) & 1) * STAGE;
+#pragma unroll
+            for (int u = 0; u < GROUPS; ++u) {
+                if (u == GROUPS - AHEAD) {
+                    if (s + 1 < steps) settle(next);
+                    landed<FAST>();
+                    __syncthreads();
+                    if (s + 2 < steps) fetch(s + 2, now);
+                    // (after the last step these read what is left there, and nothing uses it)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) y[0][j] = rb.read(next + RA * kStepBytes, j, 0);
+                }
+                const int v = u + AHEAD;
+                x[v % RING] = v < GROUPS ? ra.read(now, v % TM, v / TM) : ra.read(next, v - GROUPS, 0);
+                if (v == TM)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) y[1][j] = rb.read(now + RA * kStepBytes, j, 1);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[u % TM][j] = mfma16(y[u / TM][j], x[u % RING], acc[u % TM][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
 
-    // Lane (l16, g) holds results m = i 16 + l16 and n = j 16 + 4 g + 0 .. 3 of the wave's.
+    // Results go through LDS, 64 rows of a wave at once in its own part of it, so that neighbouring lanes take neighbouring
+    // columns: lane (l16, g) holds m = i 16 + l16 and n = j 16 + 4 g + 0 .. 3.  Chunks of 16 bytes are exchanged by the row's number.
+    static_assert(2 * STAGE >= WM * WN * 64 * TN * 16 * 4 && TM % 4 == 0 && TN == 4, "64 rows of 64 results a wave");
+    char* mine = lds + wave * (64 * TN * 64);
+    auto result = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(mine + r * (TN * 64) + ((c ^ (r & 15)) * 16)); };
+    for (int part = 0; part < TM / 4; ++part) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int m = (wm * TM + i) * 16 + l16;
-        if constexpr (MATRIX) {
-            if (m0 + m >= p.M) continue;
-            const long line = (long)(m0 + m) * p.N;
-            const long each = (long)p.M * p.N;
+        for (int i = 0; i < TM; ++i)
+            if (i / 4 == part)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const int n = n0 + (wn * TN + j) * 16 + g * 4;
-                if (p.splits == 1)
-                    put4(dm + t.q * each + line + n, acc[i][j], p.N - n);
-                else
-                    put4(p.part + (((long)split * p.a + t.q) * (KIND == kGates ? 2 : 1) + matrix) * each + line + n, acc[i][j], p.N - n);
+                for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(mine + ((i & 3) * 16 + l16) * (TN * 64) + (((j * 4 + g) ^ l16) * 16)) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+        const int first = (wm * TM + part * 4) * 16;  // of the tile's rows
+        if constexpr (KIND == kGated) {
+#pragma unroll 2
+            for (int it = 0; it < 8; ++it) {
+                const int r = it * 8 + (lane >> 3), c = lane & 7, m = first + r;  // the c-th four columns of 32
+                const f32x4 gate = result(r, (c >> 2) * 8 + (c & 3)), up = result(r, (c >> 2) * 8 + 4 + (c & 3));
+                const int f = n0 + wn * (TN * 8) + c * 4;
+                if (m >= t.cnt || f >= p.ldh) continue;
+                const int place = t.start + m, slot = slot_of(place);
+                const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
+                if (p.pre != nullptr) {
+                    float* to = p.pre + (long)slot * 2 * p.N + f;
+                    put4(to, gate, p.N - f);
+                    put4(to + p.N, up, p.N - f);
+                }
+                f32x4 h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = f + e < p.N ? w * (activate(gate[e], p.act).x * up[e]) : 0.f;
+                put4(p.h + place * p.ldh + f, h, 4);
             }
         } else {
-            const bool there = m < t.cnt;
-            const int place = t.start + min(m, t.cnt - 1), slot = slot_of(place);
-            if constexpr (KIND == kGated) {
-                if (!there) continue;
-                const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
-#pragma unroll
-                for (int j = 0; j < TN; j += 2) {
-                    const int f = n0 + (wn * TN + j) * 8 + g * 4;
-                    if (p.pre != nullptr) {
-                        float* to = p.pre + (long)slot * 2 * p.N + f;
-                        put4(to, acc[i][j], p.N - f);
-                        put4(to + p.N, acc[i][j + 1], p.N - f);
-                    }
-                    f32x4 h;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) h[e] = f + e < p.N ? w * (activate(acc[i][j][e], p.act).x * acc[i][j + 1][e]) : 0.f;
-                    if (f < p.ldh) put4(p.h + place * p.ldh + f, h, 4);
-                }
-            } else if constexpr (KIND == kHidden) {
-                const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
-                float dot = 0.f;
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const int f = n0 + (wn * TN + j) * 16 + g * 4;
-                    if (f >= p.ldh) continue;
-                    const float* pre = p.pre + (long)slot * 2 * p.N + f;
-                    const f32x4 gate = get4(pre, p.N - f), up = get4(pre + p.N, p.N - f);
-                    f32x4 h, dg, du;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 act = activate(gate[e], p.act);
-                        const bool in = f + e < p.N;
-                        const float hidden = act.x * up[e], err = in ? acc[i][j][e] : 0.f;
-                        dot += in ? err * hidden : 0.f;
-                        h[e] = in ? w * hidden : 0.f;
-                        dg[e] = in ? w * err * up[e] * act.y : 0.f;
-                        du[e] = in ? w * err * act.x : 0.f;
-                    }
+#pragma unroll 2
+            for (int it = 0; it < 16; ++it) {
+                const int r = it * 4 + g, m = first + r, n = n0 + wn * (TN * 16) + l16 * 4;
+                f32x4 v = result(r, l16);
+                if constexpr (MATRIX) {
+                    if (m0 + m >= p.M || n >= p.N) continue;
+                    const long each = (long)p.M * p.N, at = (long)(m0 + m) * p.N + n;
+                    if (p.splits == 1)
+                        put4(dm + t.q * each + at, v, p.N - n);
+                    else
+                        put4(p.part + (((long)split * p.a + t.q) * (KIND == kGates ? 2 : 1) + matrix) * each + at, v, p.N - n);
+                } else if constexpr (KIND == kHidden) {
+                    const bool there = m < t.cnt && n < p.ldh;
+                    const int place = t.start + min(m, t.cnt - 1), slot = slot_of(place);
+                    float dot = 0.f;
                     if (there) {
-                        if (p.h != nullptr) put4(p.h + place * p.ldh + f, h, 4);
-                        put4(p.dg + place * p.ldh + f, dg, 4);
-                        put4(p.du + place * p.ldh + f, du, 4);
-                    }
-                }
-                if (p.dots != nullptr) {
-                    dot += __shfl_xor(dot, 16);
-                    dot += __shfl_xor(dot, 32);
-                    if (there && g == 0) p.dots[(long)slot * p.ndots + n0 / RB * WN + wn] = dot;
-                }
-            } else {
-                if (!there) continue;
+                        const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
+                        const float* pre = p.pre + (long)slot * 2 * p.N + n;
+                        const f32x4 gate = get4(pre, p.N - n), up = get4(pre + p.N, p.N - n);
+                        f32x4 h, dg, du;
 #pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const int n = n0 + (wn * TN + j) * 16 + g * 4;
-                    if (n >= p.N) continue;
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 act = activate(gate[e], p.act);
+                            const bool in = n + e < p.N;
+                            const float hidden = act.x * up[e], err = v[e];
+                            dot += in ? err * hidden : 0.f;
+                            h[e] = in ? w * hidden : 0.f;
+                            dg[e] = in ? w * err * up[e] * act.y : 0.f;
+                            du[e] = in ? w * err * act.x : 0.f;
+                        }
+                        if (p.h != nullptr) put4(p.h + place * p.ldh + n, h, 4);
+                        put4(p.dg + place * p.ldh + n, dg, 4);
+                        put4(p.du + place * p.ldh + n, du, 4);
+                    }
+                    if (p.dots != nullptr) {
+#pragma unroll
+                        for (int x = 1; x < 16; x <<= 1) dot += __shfl_xor(dot, x);
+                        if (m < t.cnt && l16 == 0) p.dots[(long)slot * p.ndots + n0 / (TN * 16) + wn] = dot;
+                    }
+                } else {
+                    if (m >= t.cnt || n >= p.N) continue;
+                    const long slot = slot_of(t.start + m);
                     if (p.out != nullptr) {
-                        f32x4 v = acc[i][j];
                         if (p.base != nullptr) v += get4(p.base + slot * p.ld_base + n, p.N - n);
                         put4(p.out + slot * p.ld_out + n, v, p.N - n);
                     } else {
-                        put4(p.sums + (long)slot * p.N + n, acc[i][j], p.N - n);
+                        put4(p.sums + slot * p.N + n, v, p.N - n);
                     }
                 }
             }
         }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -584,7 +629,7 @@ Layout layout(const FeedSizes& z, bool backward)
     L.ntiles = z.sorted ? L.slots / L.tile + z.a + 1 : tiles_of(L.slots, L.tile);
     L.segments = (L.slots + kPlanRows - 1) / kPlanRows;
     if (L.segments < 1) L.segments = 1;
-    L.ndots = tiles_of(z.f, L.tile) * (L.tile == kBig ? 4 : 2);
+    L.ndots = tiles_of(z.f, L.tile) * (L.tile / 64);
     L.gsplits = matrix_splits(L.slots, z.a, z.f, z.d, 2, L.tile, step);
     L.osplits = matrix_splits(L.slots, z.a, z.o, z.f, 1, L.tile, step);
     size_t at = 0;
@@ -632,9 +677,9 @@ hipError_t launch_product(const Layout& L, FeedArgs<T> p, hipStream_t s)
     const int r = L.tile;
     p.nn = tiles_of(KIND == kGated ? 2l * p.N : p.N, r);
     p.nm = MATRIX ? tiles_of(p.M, r) : 0;
-    const long pieces = MATRIX ? (long)p.a * p.splits * (KIND == kGates ? 2 : 1) * p.nm * p.nn : (long)p.ntiles * p.nn;
+    const long pieces = ((MATRIX ? (long)p.nm : p.ntiles) * p.nn + 7) / 8 * 8 * (MATRIX ? (long)p.a * p.splits * (KIND == kGates ? 2 : 1) : 1);
     if (pieces == 0) return hipSuccess;
-    const dim3 grid((unsigned)((pieces + 7) / 8 * 8));
+    const dim3 grid((unsigned)pieces);
     if (r == kBig) return launch(k_product<T, KIND, 2, 4, 8, 4, true>, grid, 512, 0, s, p);
     if (L.fast) return launch(k_product<T, KIND, 2, 2, 4, 4, true>, grid, 256, 0, s, p);
     return launch(k_product<T, KIND, 2, 2, 4, 4, false>, grid, 256, 0, s, p);
@@ -655,7 +700,7 @@ bool feed_fits(const FeedSizes& z)
     const size_t most = size_t(1) << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
     const size_t wide = z.d > z.o ? z.d : z.o, rows = (size_t)z.n * z.k / kMid + z.a + 1;
     const size_t columns = (2 * (size_t)z.f > wide ? 2 * (size_t)z.f : wide) / kMid + 2;
-    const size_t matrix = (size_t)z.a * 2 * ((size_t)z.f / kMid + 1) * (wide / kMid + 1) * 8;
+    const size_t matrix = (size_t)z.a * 2 * (((size_t)z.f / kMid + 1) * (wide / kMid + 1) + 8) * 8;
     return rows * columns < most && matrix < most && (size_t)z.n < most && (wide + 1023) / 1024 < 65536 && (z.n * z.k + kPlanRows - 1) / kPlanRows < 65536;
 }
 
