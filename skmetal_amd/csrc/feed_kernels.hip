@@ -60,16 +60,33 @@ struct FeedArgs {
     T *dm, *dm2; float* part; int splits;      // [a][M][N]; partial sums [splits][a][2 where dm2][M][N] where splits > 1
 };
 
-// act(g) and its derivative
+// exp(x) for |x| <= 88: the product with log2 e in two parts, so that its rounding does not grow with x.
+__device__ __forceinline__ float exp_near(float x)
+{
+    const float hi = x * 1.44269502162933349609f, lo = fmaf(x, 1.92596299112661746887e-8f, fmaf(x, 1.44269502162933349609f, -hi));
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return fmaf(e * 0.69314718055994530942f, lo, e);
+}
+
+// act(g) and its derivative.  Both products' tiles end in 64 of these a lane: silu takes 13 instructions so, gelu 30 (with the
+// library's expf, division and erfcf, which branch, the gated product of 4,096 x 2,048 by 8,192 took @GELU@).
 __device__ __forceinline__ float2 activate(float g, int act)
 {
     if (act == kSilu) {
-        const float t = 1.f / (1.f + expf(-g));
-        return make_float2(g * t, t * (1.f + g * (1.f - t)));
+        const float t = g < -88.f ? 0.f : __builtin_amdgcn_rcpf(1.f + exp_near(fminf(fmaxf(-g, -88.f), 88.f)));  // 88 e^-88: 5e-37
+        return make_float2(g * t, t * fmaf(g, 1.f - t, 1.f));
     }
     if (act == kGelu) {
-        const float c = 0.5f * erfcf(g * -0.70710678118654752f);  // keeps its bits where 1 + erf would lose them
-        return make_float2(g * c, c + g * 0.39894228040143268f * expf(-0.5f * g * g));
+        // The normal distribution function of -|g| is 0.5 erfc(x), x = |g| / sqrt(2); erfc(x) = t P(t) exp(-x^2) with t = 1 / (1 + x / 2) and P
+        // a polynomial fitted at Chebyshev points of t, relative error 1.5e-7 (so the lower tail keeps its bits).
+        const float x = fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.f));
+        const float e = g * g > 175.f ? 0.f : exp_near(-0.5f * fminf(g * g, 175.f));  // 13.2 times the tail there is 7e-39
+        constexpr float P[9] = {0.282087684f, 0.282353491f, 0.24326095f, 0.202070117f, -0.0251784418f, 0.2759794f, -0.485384911f, 0.283702582f, -0.0588909127f};
+        float q = P[8];
+#pragma unroll
+        for (int i = 7; i >= 0; --i) q = fmaf(q, t, P[i]);
+        const float tail = 0.5f * t * q * e, c = g > 0.f ? 1.f - tail : tail;
+        return make_float2(g * c, fmaf(g * 0.39894228040143268f, e, c));
     }
     return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);
 }
@@ -104,16 +121,16 @@ __device__ __forceinline__ f32x4 get4(const T* p, int left)
 
 // ---- staging ----
 
-// 16 bytes a lane from memory to LDS, a wave's side by side from `to` on.  As assembly, for the compiler waits for
+// 16 bytes a lane from memory to LDS, a wave's side by side from byte `to` on.  As assembly, for the compiler waits for
 // a load of its own builtin before every transposing read of LDS, and so leaves none in flight
 // under a step's products.  It writes no register but m0, which nothing else here uses; landed() waits for it.
-__device__ __forceinline__ void to_lds(const void* from, char* to)
+__device__ __forceinline__ void to_lds(const void* from, unsigned to)
 {
-    const unsigned at = (unsigned)(size_t)(__attribute__((address_space(3))) char*)to;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
 }
+__device__ __forceinline__ unsigned lds_offset(char* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) char*)p; }
 
-constexpr int kStepBytes = 128;  // of a row along the sum: terms a step
+constexpr int kStepBytes = 64;  // of a row along the sum: terms a step
 template <typename T> constexpr int kStep = kStepBytes / (int)sizeof(T);
 
 // How far the 16-byte chunks of term k's row are displaced in an operand across the sum, so that the lanes of a
@@ -126,16 +143,15 @@ __device__ __forceinline__ int displaced(int k)
 }
 
 // A block's way to an operand's R rows (or columns) of a tile, a step of terms after another: from memory to
-// LDS, 16 bytes a lane.  Along the sum a row takes 128 bytes a step, its chunks exchanged by the row's number, so that
+// LDS, 16 bytes a lane.  Along the sum a row takes 64 bytes a step, its chunks exchanged by the row's number, so that
 // 16 rows' chunks of the same terms lie in different banks; across it a term's row takes
 // R elements.  FAST: every chunk is 16 bytes that exist or not, at addresses of 16 bytes; they go to LDS without
 // registers between, and those that do not exist come from g_zeros.
 template <typename T, bool ALONG, int R, int NT, bool FAST>
 struct Stager {
-    static constexpr int V = kVec<T>, C = R * 8 / NT, CHUNKS = ALONG ? 8 : R / V;
-    static_assert(C * NT == R * 8, "whole chunks a lane");
+    static constexpr int V = kVec<T>, C = R * 4 / NT, CHUNKS = ALONG ? 4 : R / V;
+    static_assert(C * NT == R * 4, "whole chunks a lane");
     const T* p[C];  // the chunks of the next step
-    int slot[C];    // of their rows, where the rows are gathered
     Vec<T> held[FAST ? 1 : C];
 
     static __device__ __forceinline__ int index(int c) { return c * NT + (int)threadIdx.x; }
@@ -143,7 +159,7 @@ struct Stager {
     static __device__ __forceinline__ int chunk(int c)
     {
         const int l = line(c), s = index(c) % CHUNKS;
-        return ALONG ? s ^ (l & 7) : s ^ displaced<T, CHUNKS>(l);
+        return ALONG ? s ^ ((l >> 2) & 3) : s ^ displaced<T, CHUNKS>(l);
     }
     // across: where a chunk lies in its row, of which `left` elements are the tile's; FAST reads what exists instead of
     // columns that do not, whose results nothing takes
@@ -163,10 +179,11 @@ struct Stager {
         for (int c = 0; c < C; ++c) p[c] = first + line(c) * ld + column(c, left);
     }
 
-    __device__ __forceinline__ void fetch(int c, const T* from, bool there, int left, char* to)
+    // Chunk c of a step, from `from` where it is there; `to` is the byte of LDS where the wave's chunks of the step go.
+    __device__ __forceinline__ void fetch(int c, const T* from, bool there, int left, unsigned to)
     {
         if constexpr (FAST)
-            to_lds(there ? (const void*)from : (const void*)g_zeros, to + (c * NT + wave_index() * 64) * 16);
+            to_lds(there ? (const void*)from : (const void*)g_zeros, to + c * NT * 16);
         else
             held[c] = there && left > 0 ? load_part(from, left) : Vec<T>{};
     }
@@ -177,91 +194,67 @@ struct Stager {
             for (int c = 0; c < C; ++c) *reinterpret_cast<Vec<T>*>(to + index(c) * 16) = held[c];
     }
 
-    // The step that begins at term k0 of `count`, the first that was not taken yet.
-    __device__ __forceinline__ void along(int k0, int count, char* to)
+    // Chunk c of the step that begins at term k0 of `count`, the first that was not taken yet.
+    __device__ __forceinline__ void along(int c, int k0, int count, unsigned to)
     {
-        if (k0 + kStep<T> <= count) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) fetch(c, p[c], true, V, to);
-        } else {
-#pragma unroll
-            for (int c = 0; c < C; ++c) fetch(c, p[c], k0 + chunk(c) * V < count, count - k0 - chunk(c) * V, to);
-        }
-#pragma unroll
-        for (int c = 0; c < C; ++c) p[c] += kStep<T>;
+        fetch(c, p[c], chunk(c) * V < count - k0, count - k0 - chunk(c) * V, to);
+        p[c] += kStep<T>;
     }
-    __device__ __forceinline__ void across(int k0, int count, long ld, int left, char* to)
+    __device__ __forceinline__ void across(int c, int k0, int count, long ld, int left, unsigned to)
     {
-        if (k0 + kStep<T> <= count) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) fetch(c, p[c], true, left - chunk(c) * V, to);
-        } else {
-#pragma unroll
-            for (int c = 0; c < C; ++c) fetch(c, p[c], k0 + line(c) < count, left - chunk(c) * V, to);
-        }
-#pragma unroll
-        for (int c = 0; c < C; ++c) p[c] += kStep<T> * ld;
+        fetch(c, p[c], line(c) < count - k0, left - chunk(c) * V, to);
+        p[c] += kStep<T> * ld;
     }
-    // The same for gathered rows: look() a step ahead, so that the slots are there when their rows are fetched.
-    __device__ __forceinline__ void look(int k0, int count, const int* perm, int start)
+    // The same for gathered rows; `slots`: those of the step's terms, in LDS, or null where they are the places from `place` on.
+    __device__ __forceinline__ void gathered(int c, int k0, int count, const int* slots, int place, const ByK& byk, const T* first, long ld, int left, unsigned to)
     {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int place = start + min(k0 + line(c), count - 1);
-            slot[c] = perm != nullptr ? perm[place] : place;
-        }
-    }
-    __device__ __forceinline__ void gathered(int k0, int count, const ByK& byk, const T* first, long ld, int left, char* to)
-    {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            fetch(c, first + (long)byk.row((unsigned)slot[c]) * ld + column(c, left), k0 + line(c) < count, left - chunk(c) * V, to);
+        const bool there = line(c) < count - k0;
+        const int slot = slots != nullptr ? slots[line(c)] : place + line(c);
+        fetch(c, first + (long)byk.row((unsigned)slot) * ld + column(c, left), there, left - chunk(c) * V, to);
     }
 };
 
-// The chunks that this wave has asked for are in LDS: to be followed by a barrier.
-template <bool FAST>
+// All but the last LEFT of this wave's loads to LDS have landed (they do in their order): to be followed by a barrier.
+template <int LEFT>
 __device__ __forceinline__ void landed()
 {
-    if constexpr (FAST) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
 }
 
 // ---- fragments: a lane's terms of one row (or column) for a 16 x 16 product ----
 
 template <typename T, bool ALONG, int R>
 struct Reader {
-    // `first`: the wave's first of R rows
-    int at[ALONG ? 2 : 1], lane_, first_;
-    __device__ __forceinline__ explicit Reader(int first)
+    int at, displacement, first;  // `first`: the wave's first of R rows
+    __device__ __forceinline__ explicit Reader(int first_row) : first(first_row)
     {
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-        lane_ = lane;
-        first_ = first;
         if constexpr (ALONG) {
-            at[0] = (first + l16) * kStepBytes + ((g ^ (l16 & 7)) * 16);
-            at[1] = (first + l16) * kStepBytes + (((4 + g) ^ (l16 & 7)) * 16);
-        } else if constexpr (sizeof(T) == 2) {
-            at[0] = (g * 8 + (l16 >> 2)) * R * 2 + ((l16 & 3) >> 1) * 16 + (l16 & 1) * 8;
+            at = (first + l16) * kStepBytes + ((g ^ (l16 >> 2)) * 16);
+            displacement = 0;
+        } else if constexpr (sizeof(T) == 2) {  // a lane's terms are 8 g + 0 .. 7; it reads for others 8 bytes of term 8 g + l16 / 4 (+ 4)
+            at = (g * 8 + (l16 >> 2)) * R * 2 + ((l16 & 3) >> 1) * 16 + (l16 & 1) * 8;
+            displacement = displaced<T, R / 8>(g * 8 + (l16 >> 2));
         } else {
-            at[0] = g * 4 * R * 4 + (l16 >> 2) * 16 + (l16 & 3) * 4;
+            at = g * 4 * R * 4 + (l16 >> 2) * 16 + (l16 & 3) * 4;
+            displacement = displaced<T, R / 4>(g * 4);
         }
     }
-    __device__ __forceinline__ Vec<T> read(const char* lds, int tile, int half) const
+    __device__ __forceinline__ Vec<T> read(const char* lds, int tile) const
     {
         if constexpr (ALONG) {
-            return *reinterpret_cast<const Vec<T>*>(lds + at[half] + tile * 16 * kStepBytes);
+            return *reinterpret_cast<const Vec<T>*>(lds + at + tile * 16 * kStepBytes);
         } else if constexpr (sizeof(T) == 2) {
+            // a transposing read: lane i of 16 gets column i of the four rows that each four lanes point at
             typedef short s4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s4* Lds4;
-            const int g = lane_ >> 4, l16 = lane_ & 15, s = ((((l16 >> 2) | (g & 1) << 2)) << 1) & (R / 8 - 1);
-            const char* p = lds + at[0] + half * 32 * R * 2 + ((((first_ >> 3) + tile * 2) ^ s) * 16);
+            const char* p = lds + at + ((((first >> 3) + tile * 2) ^ displacement) * 16);
             union { s4 q[2]; Vec<T> v; } r;
             r.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)p);
             r.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(p + 4 * R * 2));
             return r.v;
         } else {
-            const int g = lane_ >> 4, s = (g << 2) & (R / 4 - 1);
-            const char* p = lds + at[0] + half * 16 * R * 4 + ((((first_ >> 2) + tile * 4) ^ s) * 16);
+            const char* p = lds + at + ((((first >> 2) + tile * 4) ^ displacement) * 16);
             Vec<T> v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(p + j * R * 4);
@@ -270,26 +263,69 @@ struct Reader {
     }
 };
 
-// Which of `count` pieces of work a block takes: blocks go to the 8 XCDs in turn, and an XCD gets an eighth of the
-// pieces side by side, which share operands in its L2.
-__device__ __forceinline__ int piece_of(unsigned x, int count) { return (int)(x & 7) * ((count + 7) / 8) + (int)(x >> 3); }
+// acc += a b^T in place.  With 64 accumulators a wave (256 registers, which only the accumulation registers have) the
+// compiler's own form of this instruction moves them about between steps; as assembly they stay where they
+// are.  It writes an instruction's result that the compiler does not know of: settled() stands before the first use.
+template <bool PLACED, typename T>
+__device__ __forceinline__ void mfma_into(f32x4& acc, Vec<T> a, Vec<T> b)
+{
+    if constexpr (!PLACED || sizeof(T) == 4)
+        acc = mfma16(a, b, acc);
+    else if constexpr (std::is_same_v<T, bf16>)
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+    else
+        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+// The last products' results are in their registers: 18 wait states after a 16 x 16 product, 32 are taken.
+template <bool PLACED, int TM, int TN>
+__device__ __forceinline__ void settled(f32x4 (&acc)[TM][TN])
+{
+    if constexpr (PLACED) {
+        asm volatile("s_nop 15\n\ts_nop 15" : : : "memory");
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
+    }
+}
+
+// The tile that a block takes, of `layers` times nm x nn.  Units of 4 x 4 tiles share operands in an XCD's L2 (blocks go to the
+// 8 XCDs in turn) and go to the XCDs in turn themselves, so that tiles which turn out to be empty are missing on all of
+// them alike: with an eighth of all tiles side by side on each XCD, the last of them had nothing to do at
+// 4,096 rows of one expert (an eighth more tiles than rows for, and 28 % of the time idle).
+constexpr int kUnit = 4;
+struct Place { int layer, m, n; };
+__device__ __forceinline__ Place place_of(unsigned block, int nm, int nn)
+{
+    const int i = block >> 3, unit = i / (kUnit * kUnit) * 8 + (int)(block & 7), in = i % (kUnit * kUnit);
+    const int across = (nn + kUnit - 1) / kUnit, per = (nm + kUnit - 1) / kUnit * across, u = unit % per;
+    return Place{unit / per, u / across * kUnit + in % kUnit, u % across * kUnit + in / kUnit};
+}
+long blocks_of(long layers, int nm, int nn)
+{
+    const long units = layers * ((nm + kUnit - 1) / kUnit) * ((nn + kUnit - 1) / kUnit);
+    return (units + 7) / 8 * 8 * kUnit * kUnit;
+}
 
 // ---- the product ----
 
 // A block's tile of WM TM 16 x WN TN 16 results; a wave's is TM 16 x TN 16.
 //
-// Two stages of LDS: while a step's products run from one, the next step's operands come into the other.  A step is 2 TM
-// groups of TN products (half of its terms, one row of fragments).  Fragments are read three groups ahead, across the
-// steps too: the barrier stands before the last three groups, when every wave has read what it needs of the
-// stage, so that the products of these hide it and the first reads of the next stage.
-template <typename T, int KIND, int WM, int WN, int TM, int TN, bool FAST>
-__global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
+// Four stages of LDS: while a step's products run from one, the operands of the three next steps come into the others
+// (with one step ahead, which is 64 KB a block every microsecond, every step waited for memory).  A step is TM groups of
+// TN products.  Fragments are read three groups ahead, across the steps too: the barrier stands before the last three
+// groups, when every wave has read what it needs of the stage, so that the products of these hide it and
+// the first reads of the next stage.
+template <typename T, int KIND, int WM, int WN, int TM, int TN, int STAGES, bool FAST>
+__global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(FeedArgs<T> p)
 {
     constexpr int NT = WM * WN * 64, RA = WM * TM * 16, RB = WN * TN * 16, STAGE = (RA + RB) * kStepBytes;
     constexpr bool MATRIX = KIND == kGates || KIND == kOuts;  // the sum runs over slots
     constexpr bool A_ALONG = !MATRIX, B_ALONG = KIND == kGated || KIND == kDown;
-    constexpr int GROUP = 4;  // tiles of M that neighbouring blocks take together
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    constexpr bool PLACED = TM * TN > 32 && sizeof(T) == 2;
+    constexpr bool GATHERED = MATRIX;
+    constexpr int ASLOTS = 8;  // slots of gathered rows: of 8 steps, a copy a wave
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE + (GATHERED ? NT / 64 * ASLOTS * 256 : 0)];
 
     const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
@@ -299,16 +335,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
     T* dm = p.dm;
     int terms = p.K, from = 0, matrix = 0;
     if constexpr (MATRIX) {
-        // every XCD takes an eighth of each expert's tiles: experts differ in their slots
-        const int per = p.nm * p.nn, wide = (per + 7) / 8 * 8, both = KIND == kGates ? 2 : 1;
-        const int rest = blockIdx.x / wide, i = piece_of(blockIdx.x % wide, per);
-        if (i >= per) return;
-        const int group = i / (GROUP * p.nn), in = i - group * GROUP * p.nn, high = min(GROUP, p.nm - group * GROUP);
-        m0 = (group * GROUP + in % high) * RA;
-        n0 = in / high * RB;
-        split = rest % p.splits;
-        matrix = rest / p.splits % both;
-        const int q = rest / p.splits / both;
+        const int both = KIND == kGates ? 2 : 1;
+        const Place at = place_of(blockIdx.x, p.nm, p.nn);
+        if (at.layer >= p.a * p.splits * both || at.m >= p.nm || at.n >= p.nn) return;
+        m0 = at.m * RA;
+        n0 = at.n * RB;
+        split = at.layer % p.splits;
+        matrix = at.layer / p.splits % both;
+        const int q = at.layer / p.splits / both;
         t = p.tiles != nullptr ? p.tiles[q] : Tile{0, 0, p.slots, -1};
         t.q = q;
         if (matrix) {
@@ -320,12 +354,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
         from = (int)((long)steps * split / p.splits) * kStep<T>;
         terms = max(0, min(t.cnt, (int)((long)steps * (split + 1) / p.splits) * kStep<T>) - from);
     } else {
-        const int all = p.ntiles * p.nn, piece = piece_of(blockIdx.x, all);
-        if (piece >= all) return;
-        const int group = piece / (GROUP * p.nn), in = piece - group * GROUP * p.nn, high = min(GROUP, p.ntiles - group * GROUP);
-        const int m = group * GROUP + in % high;
-        n0 = in / high * (KIND == kGated ? RB / 2 : RB);
-        t = p.tiles != nullptr ? p.tiles[m] : Tile{0, m * RA, min(RA, p.slots - m * RA), -1};
+        const Place at = place_of(blockIdx.x, p.ntiles, p.nn);
+        if (at.layer > 0 || at.m >= p.ntiles || at.n >= p.nn) return;
+        n0 = at.n * (KIND == kGated ? RB / 2 : RB);
+        t = p.tiles != nullptr ? p.tiles[at.m] : Tile{0, at.m * RA, min(RA, p.slots - at.m * RA), -1};
         if (t.q < 0) return;
         if (t.q >= p.a) {  // slots without an expert
             if constexpr (KIND == kGated) {
@@ -371,34 +403,52 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
     if constexpr (KIND == kHidden || KIND == kRows) sb.terms(B + n0, p.ldb, left_b);
     if constexpr (KIND == kOuts) sb.terms(B + n0 + start * p.ldb, p.ldb, left_b);
 
+    // The slots of step `step`'s gathered rows, which are fetched from step - ASLOTS / 2 on.
+    const unsigned lds_slots = lds_offset(lds) + STAGES * STAGE + wave * (ASLOTS * 256);
     auto look = [&](int step) {
-        if constexpr (KIND == kOuts) sa.look(step * kStep<T>, terms, p.perm, start);
-        if constexpr (KIND == kGates) sb.look(step * kStep<T>, terms, p.perm, start);
+        if constexpr (GATHERED) {
+            const int* from_perm = p.perm + start + min(step * kStep<T> + (lane & (kStep<T> - 1)), max(terms - 1, 0));
+            const void* src = p.perm != nullptr ? (const void*)from_perm : (const void*)g_zeros;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_slots + (step & (ASLOTS - 1)) * 256), "v"(src) : "memory");
+        }
     };
-    auto fetch = [&](int step, char* to) {
-        char* to_b = to + RA * kStepBytes;
+    // Part c of a step's operands, one chunk a lane: those of A, then those of B.  A step's are taken in their order; steps
+    // past the last are zeros.
+    constexpr int CHUNKS_A = decltype(sa)::C, CHUNKS = CHUNKS_A + decltype(sb)::C, LOADS = CHUNKS + (GATHERED ? 1 : 0);
+    const unsigned lds_wave = lds_offset(lds) + wave * 1024;
+    auto fetch = [&](int step, int stage, int c) {
+        unsigned to = lds_wave + stage;
         int k0 = step * kStep<T>;
         bool second = false;
         if constexpr (KIND == kRows)
             if (step >= steps1) {
                 second = true;
                 k0 -= steps1 * kStep<T>;
-                if (step == steps1) {
+                if (c == 0 && step == steps1) {
                     begin_a(p.A2);
                     sb.terms(B2 + n0, p.ldb2, left_b);
                 }
             }
-        if constexpr (A_ALONG) sa.along(k0, terms, to);
-        if constexpr (KIND == kGates) sa.across(k0, terms, p.lda, left_a, to);
-        if constexpr (KIND == kOuts) sa.gathered(k0, terms, p.byk, A + m0, p.lda, left_a, to);
-        if constexpr (B_ALONG) sb.along(k0, terms, to_b);
-        if constexpr (KIND == kHidden || KIND == kRows || KIND == kOuts) sb.across(k0, terms, second ? p.ldb2 : p.ldb, left_b, to_b);
-        if constexpr (KIND == kGates) sb.gathered(k0, terms, p.byk, B + n0, p.ldb, left_b, to_b);
-        if (step + 1 < steps) look(step + 1);
+        const int* slots = nullptr;
+        if constexpr (GATHERED) {
+            if (c == 0) look(step + ASLOTS / 2);  // landed three steps later at the latest, with that step's operands
+            if (p.perm != nullptr) slots = reinterpret_cast<const int*>(lds + STAGES * STAGE + wave * (ASLOTS * 256) + (step & (ASLOTS - 1)) * 256);
+        }
+        if (c < CHUNKS_A) {
+            if constexpr (A_ALONG) sa.along(c, k0, terms, to);
+            if constexpr (KIND == kGates) sa.across(c, k0, terms, p.lda, left_a, to);
+            if constexpr (KIND == kOuts) sa.gathered(c, k0, terms, slots, start + k0, p.byk, A + m0, p.lda, left_a, to);
+        } else {
+            c -= CHUNKS_A;
+            to += RA * kStepBytes;
+            if constexpr (B_ALONG) sb.along(c, k0, terms, to);
+            if constexpr (KIND == kHidden || KIND == kRows || KIND == kOuts) sb.across(c, k0, terms, second ? p.ldb2 : p.ldb, left_b, to);
+            if constexpr (KIND == kGates) sb.gathered(c, k0, terms, slots, start + k0, p.byk, B + n0, p.ldb, left_b, to);
+        }
     };
-    auto settle = [&](char* to) {
-        sa.settle(to);
-        sb.settle(to + RA * kStepBytes);
+    auto settle = [&](int stage) {
+        sa.settle(lds + stage);
+        sb.settle(lds + stage + RA * kStepBytes);
     };
 
     const Reader<T, A_ALONG, RA> ra(wm * TM * 16);
@@ -410,62 +460,87 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     if (steps > 0) {
-        constexpr int GROUPS = 2 * TM, AHEAD = 3, RING = AHEAD + 1;
-        static_assert(GROUPS % RING == 0 && GROUPS - AHEAD >= TM, "a fragment's registers are free when the next step reads into them");
+        constexpr int AHEAD = 3, RING = AHEAD + 1, EACH = (CHUNKS + TM - 1) / TM;
+        static_assert(TM % RING == 0, "a fragment's registers are free when the next step reads into them");
         Vec<T> x[RING], y[2][TN];
-        look(0);
-        fetch(0, lds);
-        settle(lds);
-        landed<FAST>();
+        if constexpr (GATHERED) {
+#pragma unroll
+            for (int i = 0; i < ASLOTS / 2; ++i) look(i);
+            landed<0>();
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) fetch(i, i * STAGE, c);
+            settle(i * STAGE);
+        }
+        landed<FAST ? (STAGES - 2) * LOADS : 0>();
         __syncthreads();
-        if (steps > 1) fetch(1, lds + STAGE);
+        auto take_y = [&](int stage, Vec<T>* to) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) y[0][j] = rb.read(lds + RA * kStepBytes, j, 0);
+            for (int j = 0; j < TN; ++j) to[j] = rb.read(lds + stage + RA * kStepBytes, j);
+        };
+        int before = (STAGES - 1) * STAGE, now = 0, next = STAGE;  // bytes: the stages of the last step, this one and the next
+        take_y(now, y[0]);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) x[i] = ra.read(lds, i, 0);
-        for (int s = 0; s < steps; ++s) {
-            char* now = lds + (s & 1) * STAGE;
-            char* next = lds + ((s + 1) & 1) * STAGE;
+        for (int i = 0; i < AHEAD; ++i) {
+            x[i] = ra.read(lds, i);
 #pragma unroll
-            for (int u = 0; u < GROUPS; ++u) {
-                if (u == GROUPS - AHEAD) {
-                    if (s + 1 < steps) settle(next);
-                    landed<FAST>();
-                    __syncthreads();
-                    if (s + 2 < steps) fetch(s + 2, now);
-                    // (after the last step these read what is left there, and nothing uses it)
+            for (int e = 0; e < EACH; ++e)
+                if (i * EACH + e < CHUNKS) fetch(STAGES - 1, before, i * EACH + e);
+        }
+        for (int s0 = 0; s0 < steps; s0 += 2) {
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) y[0][j] = rb.read(next + RA * kStepBytes, j, 0);
+            for (int h = 0; h < 2; ++h) {
+                const int s = s0 + h;
+#pragma unroll
+                for (int u = 0; u < TM; ++u) {
+                    const int v = u + AHEAD, v1 = v < TM ? v : v - TM;
+                    if (u == TM - AHEAD) {
+                        settle(before);
+                        landed<FAST ? (STAGES - 2) * LOADS : 0>();
+                        __syncthreads();
+                        take_y(next, y[h ^ 1]);
+                    }
+                    x[v % RING] = ra.read(lds + (v < TM ? now : next), v1);
+                    // a step's parts are fetched one by one, into the stage that the last barrier freed: all at once they
+                    // would fill the queue to memory, and the products behind them would wait
+#pragma unroll
+                    for (int e = 0; e < EACH; ++e)
+                        if (v1 * EACH + e < CHUNKS) fetch((v < TM ? s : s + 1) + STAGES - 1, v < TM ? before : now, v1 * EACH + e);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) mfma_into<PLACED, T>(acc[u][j], y[h][j], x[u % RING]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                const int v = u + AHEAD;
-                x[v % RING] = v < GROUPS ? ra.read(now, v % TM, v / TM) : ra.read(next, v - GROUPS, 0);
-                if (v == TM)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) y[1][j] = rb.read(now + RA * kStepBytes, j, 1);
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[u % TM][j] = mfma16(y[u / TM][j], x[u % RING], acc[u % TM][j]);
-                __builtin_amdgcn_sched_barrier(0);
+                before = now;
+                now = next;
+                next = next == (STAGES - 1) * STAGE ? 0 : next + STAGE;
             }
         }
+        settled<PLACED>(acc);
+        landed<0>();
+        __syncthreads();
     }
 
     // Results go through LDS, 64 rows of a wave at once in its own part of it, so that neighbouring lanes take neighbouring
     // columns: lane (l16, g) holds m = i 16 + l16 and n = j 16 + 4 g + 0 .. 3.  Chunks of 16 bytes are exchanged by the row's number.
-    static_assert(2 * STAGE >= WM * WN * 64 * TN * 16 * 4 && TM % 4 == 0 && TN == 4, "64 rows of 64 results a wave");
-    char* mine = lds + wave * (64 * TN * 64);
-    auto result = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(mine + r * (TN * 64) + ((c ^ (r & 15)) * 16)); };
+    constexpr int WIDE = TN * 16, QUADS = TN * 4;  // a row of the wave's results: columns, chunks
+    static_assert(STAGES * STAGE >= WM * WN * 64 * WIDE * 4 && TM % 4 == 0 && QUADS % 16 == 0, "64 rows a wave");
+    char* mine = lds + wave * (64 * WIDE * 4);
+    auto result = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(mine + r * (WIDE * 4) + ((c ^ (r & 15)) * 16)); };
     for (int part = 0; part < TM / 4; ++part) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
             if (i / 4 == part)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(mine + ((i & 3) * 16 + l16) * (TN * 64) + (((j * 4 + g) ^ l16) * 16)) = acc[i][j];
+                for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(mine + ((i & 3) * 16 + l16) * (WIDE * 4) + (((j * 4 + g) ^ l16) * 16)) = acc[i][j];
         __builtin_amdgcn_wave_barrier();
         const int first = (wm * TM + part * 4) * 16;  // of the tile's rows
         if constexpr (KIND == kGated) {
 #pragma unroll 2
-            for (int it = 0; it < 8; ++it) {
-                const int r = it * 8 + (lane >> 3), c = lane & 7, m = first + r;  // the c-th four columns of 32
+            for (int it = 0; it < QUADS / 2; ++it) {
+                const int r = it * (128 / QUADS) + lane / (QUADS / 2), c = lane % (QUADS / 2), m = first + r;  // the c-th four columns of f
                 const f32x4 gate = result(r, (c >> 2) * 8 + (c & 3)), up = result(r, (c >> 2) * 8 + 4 + (c & 3));
                 const int f = n0 + wn * (TN * 8) + c * 4;
                 if (m >= t.cnt || f >= p.ldh) continue;
@@ -483,9 +558,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
             }
         } else {
 #pragma unroll 2
-            for (int it = 0; it < 16; ++it) {
-                const int r = it * 4 + g, m = first + r, n = n0 + wn * (TN * 16) + l16 * 4;
-                f32x4 v = result(r, l16);
+            for (int it = 0; it < QUADS; ++it) {
+                const int r = it * (64 / QUADS) + lane / QUADS, c = lane % QUADS, m = first + r, n = n0 + wn * WIDE + c * 4;
+                f32x4 v = result(r, c);
                 if constexpr (MATRIX) {
                     if (m0 + m >= p.M || n >= p.N) continue;
                     const long each = (long)p.M * p.N, at = (long)(m0 + m) * p.N + n;
@@ -518,8 +593,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
                     }
                     if (p.dots != nullptr) {
 #pragma unroll
-                        for (int x = 1; x < 16; x <<= 1) dot += __shfl_xor(dot, x);
-                        if (m < t.cnt && l16 == 0) p.dots[(long)slot * p.ndots + n0 / (TN * 16) + wn] = dot;
+                        for (int x = 1; x < QUADS; x <<= 1) dot += __shfl_xor(dot, x);
+                        if (m < t.cnt && c == 0) p.dots[(long)slot * p.ndots + n0 / WIDE + wn] = dot;
                     }
                 } else {
                     if (m >= t.cnt || n >= p.N) continue;
@@ -629,7 +704,7 @@ Layout layout(const FeedSizes& z, bool backward)
     L.ntiles = z.sorted ? L.slots / L.tile + z.a + 1 : tiles_of(L.slots, L.tile);
     L.segments = (L.slots + kPlanRows - 1) / kPlanRows;
     if (L.segments < 1) L.segments = 1;
-    L.ndots = tiles_of(z.f, L.tile) * (L.tile / 64);
+    L.ndots = tiles_of(z.f, L.tile) * (L.tile / 64);  // one a wave's 64 columns
     L.gsplits = matrix_splits(L.slots, z.a, z.f, z.d, 2, L.tile, step);
     L.osplits = matrix_splits(L.slots, z.a, z.o, z.f, 1, L.tile, step);
     size_t at = 0;
@@ -677,12 +752,10 @@ hipError_t launch_product(const Layout& L, FeedArgs<T> p, hipStream_t s)
     const int r = L.tile;
     p.nn = tiles_of(KIND == kGated ? 2l * p.N : p.N, r);
     p.nm = MATRIX ? tiles_of(p.M, r) : 0;
-    const long pieces = ((MATRIX ? (long)p.nm : p.ntiles) * p.nn + 7) / 8 * 8 * (MATRIX ? (long)p.a * p.splits * (KIND == kGates ? 2 : 1) : 1);
-    if (pieces == 0) return hipSuccess;
-    const dim3 grid((unsigned)pieces);
-    if (r == kBig) return launch(k_product<T, KIND, 2, 4, 8, 4, true>, grid, 512, 0, s, p);
-    if (L.fast) return launch(k_product<T, KIND, 2, 2, 4, 4, true>, grid, 256, 0, s, p);
-    return launch(k_product<T, KIND, 2, 2, 4, 4, false>, grid, 256, 0, s, p);
+    const dim3 grid((unsigned)(MATRIX ? blocks_of((long)p.a * p.splits * (KIND == kGates ? 2 : 1), p.nm, p.nn) : blocks_of(1, p.ntiles, p.nn)));
+    if (L.tile == kBig) return launch(k_product<T, KIND, 2, 4, 8, 4, 4, true>, grid, 512, 0, s, p);
+    if (L.fast) return launch(k_product<T, KIND, 2, 2, 4, 4, 4, true>, grid, 256, 0, s, p);
+    return launch(k_product<T, KIND, 2, 2, 4, 4, 4, false>, grid, 256, 0, s, p);
 }
 
 template <typename T>
@@ -697,11 +770,11 @@ hipError_t launch_join(const float* sums, const int* chosen, const FeedSizes& z,
 bool feed_fits(const FeedSizes& z)
 {
     if (z.n * z.k >= 1l << 30) return false;
-    const size_t most = size_t(1) << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
-    const size_t wide = z.d > z.o ? z.d : z.o, rows = (size_t)z.n * z.k / kMid + z.a + 1;
-    const size_t columns = (2 * (size_t)z.f > wide ? 2 * (size_t)z.f : wide) / kMid + 2;
-    const size_t matrix = (size_t)z.a * 2 * (((size_t)z.f / kMid + 1) * (wide / kMid + 1) + 8) * 8;
-    return rows * columns < most && matrix < most && (size_t)z.n < most && (wide + 1023) / 1024 < 65536 && (z.n * z.k + kPlanRows - 1) / kPlanRows < 65536;
+    const long most = 1l << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
+    const long wide = z.d > z.o ? z.d : z.o, slots = (long)z.n * z.k;
+    const int rows = (int)(slots / kMid) + z.a + 1, hidden = tiles_of(2l * z.f, kMid), outer = tiles_of(wide, kMid);
+    return blocks_of(1, rows, hidden > outer ? hidden : outer) < most && blocks_of(16l * z.a, tiles_of(z.f, kMid), outer) < most && z.n < most &&
+           (wide + 1023) / 1024 < 65536 && (slots + kPlanRows - 1) / kPlanRows < 65536;
 }
 
 size_t feed_workspace(const FeedSizes& z, bool backward) { return layout(z, backward).bytes; }
