@@ -20,10 +20,12 @@
 // (kept from the forward pass for the backward one), e, dw, and the k parts of a row's sum.
 #include "plan_common.h"
 
+#include <algorithm>
+
 namespace skm {
 namespace {
 
-enum Kind : int { kGated, kDown, kHidden, kRows, kGates, kOuts };
+enum Kind : int { kGated, kDown, kHidden, kRows, kGates, kOuts, kKinds };
 
 // 16 bytes of zeros for loads of what does not exist.
 __device__ __attribute__((aligned(16))) unsigned g_zeros[4];
@@ -43,7 +45,7 @@ ByK by_k(int k)
 template <typename T>
 struct FeedArgs {
     // tiles of slots (row products) or the slots of each expert (gradients of matrices)
-    const Tile* tiles; int ntiles; const int* perm; int slots, a;  // tiles null: one expert has all slots in their order
+    const Tile* tiles; int ntiles, cut; const int* perm; int slots, a;  // each of the tiles cut in `cut`; tiles null: one expert has all slots in their order
     ByK byk;
     // operands
     const T *A, *A2; long lda;
@@ -357,7 +359,15 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         const Place at = place_of(blockIdx.x, p.ntiles, p.nn);
         if (at.layer > 0 || at.m >= p.ntiles || at.n >= p.nn) return;
         n0 = at.n * (KIND == kGated ? RB / 2 : RB);
-        t = p.tiles != nullptr ? p.tiles[at.m] : Tile{0, at.m * RA, min(RA, p.slots - at.m * RA), -1};
+        if (p.tiles != nullptr) {
+            t = p.tiles[at.m / p.cut];
+            const int skip = at.m % p.cut * RA;
+            t.start += skip;
+            t.cnt = min(RA, t.cnt - skip);
+            if (t.cnt <= 0) return;
+        } else {
+            t = Tile{0, at.m * RA, min(RA, p.slots - at.m * RA), -1};
+        }
         if (t.q < 0) return;
         if (t.q >= p.a) {  // slots without an expert
             if constexpr (KIND == kGated) {
@@ -460,7 +470,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     if (steps > 0) {
-        constexpr int AHEAD = 3, RING = AHEAD + 1, EACH = (CHUNKS + TM - 1) / TM;
+        constexpr int AHEAD = TM < 4 ? TM - 1 : 3, RING = AHEAD + 1, EACH = (CHUNKS + TM - 1) / TM;
         static_assert(TM % RING == 0, "a fragment's registers are free when the next step reads into them");
         Vec<T> x[RING], y[2][TN];
         if constexpr (GATHERED) {
@@ -523,23 +533,24 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         __syncthreads();
     }
 
-    // Results go through LDS, 64 rows of a wave at once in its own part of it, so that neighbouring lanes take neighbouring
+    // Results go through LDS, up to 64 rows of a wave at once in its own part of it, so that neighbouring lanes take neighbouring
     // columns: lane (l16, g) holds m = i 16 + l16 and n = j 16 + 4 g + 0 .. 3.  Chunks of 16 bytes are exchanged by the row's number.
-    constexpr int WIDE = TN * 16, QUADS = TN * 4;  // a row of the wave's results: columns, chunks
-    static_assert(STAGES * STAGE >= WM * WN * 64 * WIDE * 4 && TM % 4 == 0 && QUADS % 16 == 0, "64 rows a wave");
-    char* mine = lds + wave * (64 * WIDE * 4);
-    auto result = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(mine + r * (WIDE * 4) + ((c ^ (r & 15)) * 16)); };
-    for (int part = 0; part < TM / 4; ++part) {
+    constexpr int WIDE = TN * 16, QUADS = TN * 4, EX = QUADS < 16 ? QUADS - 1 : 15;  // a row of the wave's results: columns, chunks
+    constexpr int PART = TM < 4 ? TM : 4;                                          // tiles of 16 rows at once
+    static_assert(STAGES * STAGE >= WM * WN * PART * 16 * WIDE * 4 && TM % PART == 0, "the rows of all waves");
+    char* mine = lds + wave * (PART * 16 * WIDE * 4);
+    auto result = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(mine + r * (WIDE * 4) + ((c ^ (r & EX)) * 16)); };
+    for (int part = 0; part < TM / PART; ++part) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
-            if (i / 4 == part)
+            if (i / PART == part)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(mine + ((i & 3) * 16 + l16) * (WIDE * 4) + (((j * 4 + g) ^ l16) * 16)) = acc[i][j];
+                for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(mine + (i % PART * 16 + l16) * (WIDE * 4) + (((j * 4 + g) ^ (l16 & EX)) * 16)) = acc[i][j];
         __builtin_amdgcn_wave_barrier();
-        const int first = (wm * TM + part * 4) * 16;  // of the tile's rows
+        const int first = (wm * TM + part * PART) * 16;  // of the tile's rows
         if constexpr (KIND == kGated) {
 #pragma unroll 2
-            for (int it = 0; it < QUADS / 2; ++it) {
+            for (int it = 0; it < PART * QUADS / 8; ++it) {
                 const int r = it * (128 / QUADS) + lane / (QUADS / 2), c = lane % (QUADS / 2), m = first + r;  // the c-th four columns of f
                 const f32x4 gate = result(r, (c >> 2) * 8 + (c & 3)), up = result(r, (c >> 2) * 8 + 4 + (c & 3));
                 const int f = n0 + wn * (TN * 8) + c * 4;
@@ -558,7 +569,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
             }
         } else {
 #pragma unroll 2
-            for (int it = 0; it < QUADS; ++it) {
+            for (int it = 0; it < PART * QUADS / 4; ++it) {
                 const int r = it * (64 / QUADS) + lane / QUADS, c = lane % QUADS, m = first + r, n = n0 + wn * WIDE + c * 4;
                 f32x4 v = result(r, c);
                 if constexpr (MATRIX) {
@@ -610,6 +621,120 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+// ---- few slots: each with its expert's matrices as they come from memory ----
+
+constexpr int kFewThreads = 256, kFewRows = 2;  // rows of a matrix that a wave takes
+
+template <typename T>
+struct FewArgs {
+    const T* x; long ld_x;
+    const T* gate; long gate_sa, gate_ld;
+    const T* up; long up_sa, up_ld;
+    const T* down; long down_sa, down_ld;
+    const int* chosen; const float* weights; int act;
+    const T* base; long ld_base; T* out; long ld_out;
+    T* h; long ldh; float* pre;
+    int n, d, f, o, k, a;
+};
+
+// acc[i] += this lane's part of <m_i, v>, `terms` long.
+template <typename T, int ROWS>
+__device__ __forceinline__ void dots_with(const T* v, const T* const (&m)[ROWS], int terms, float (&acc)[ROWS])
+{
+    constexpr int V = kVec<T>, STEP = 64 * V;
+    int at = (int)(threadIdx.x & 63) * V;
+    auto add = [&](const Vec<T>& a, const Vec<T> (&b)[ROWS]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) acc[i] = fmaf(to_f(a[e]), to_f(b[i][e]), acc[i]);
+    };
+#pragma unroll 4
+    for (; at + V <= terms; at += STEP) {
+        const Vec<T> a = load16(v + at);
+        Vec<T> b[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) b[i] = load16(m[i] + at);
+        add(a, b);
+    }
+    if (at < terms) {
+        const Vec<T> a = load_part(v + at, terms - at);
+        Vec<T> b[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) b[i] = load_part(m[i] + at, terms - at);
+        add(a, b);
+    }
+}
+template <int ROWS>
+__device__ __forceinline__ void sum_lanes(float (&acc)[ROWS])
+{
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1)
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) acc[i] += __shfl_xor(acc[i], x);
+}
+
+// g, u and the weighted h of kFewRows hidden places of a slot, a wave each.
+template <typename T>
+__global__ __launch_bounds__(kFewThreads) void k_few_gated(FewArgs<T> p)
+{
+    const int per = (p.f + kFewRows - 1) / kFewRows, w = (int)blockIdx.x * (kFewThreads / 64) + wave_index();
+    const int slot = w / per, f0 = w % per * kFewRows, lane = threadIdx.x & 63;
+    if (slot >= p.n * p.k) return;
+    const int q = p.chosen != nullptr ? p.chosen[slot] : 0;
+    if (q < 0 || q >= p.a) {
+        if (p.pre != nullptr && lane < kFewRows && f0 + lane < p.f) {
+            float* to = p.pre + (long)slot * 2 * p.f + f0 + lane;
+            to[0] = to[p.f] = 0.f;
+        }
+        return;
+    }
+    const T* m[2 * kFewRows];
+#pragma unroll
+    for (int i = 0; i < kFewRows; ++i) {
+        const long f = min(f0 + i, p.f - 1);
+        m[i] = p.gate + q * p.gate_sa + f * p.gate_ld;
+        m[kFewRows + i] = p.up + q * p.up_sa + f * p.up_ld;
+    }
+    float acc[2 * kFewRows] = {};
+    dots_with<T, 2 * kFewRows>(p.x + slot / p.k * p.ld_x, m, p.d, acc);
+    sum_lanes(acc);
+#pragma unroll
+    for (int i = 0; i < kFewRows; ++i) {
+        if (lane != i || f0 + i >= p.f) continue;
+        const float g = acc[i], u = acc[kFewRows + i], wt = p.weights != nullptr ? p.weights[slot] : 1.f;
+        if (p.pre != nullptr) {
+            float* to = p.pre + (long)slot * 2 * p.f + f0 + i;
+            to[0] = g;
+            to[p.f] = u;
+        }
+        p.h[slot * p.ldh + f0 + i] = from_f<T>(wt * (activate(g, p.act).x * u));
+    }
+}
+
+// kFewRows results of a row, over all its slots.
+template <typename T>
+__global__ __launch_bounds__(kFewThreads) void k_few_down(FewArgs<T> p)
+{
+    const int per = (p.o + kFewRows - 1) / kFewRows, w = (int)blockIdx.x * (kFewThreads / 64) + wave_index();
+    const int row = w / per, o0 = w % per * kFewRows, lane = threadIdx.x & 63;
+    if (row >= p.n) return;
+    float acc[kFewRows] = {};
+    for (int j = 0; j < p.k; ++j) {
+        const int slot = row * p.k + j, q = p.chosen != nullptr ? p.chosen[slot] : 0;
+        if (q < 0 || q >= p.a) continue;
+        const T* m[kFewRows];
+#pragma unroll
+        for (int i = 0; i < kFewRows; ++i) m[i] = p.down + q * p.down_sa + (long)min(o0 + i, p.o - 1) * p.down_ld;
+        dots_with<T, kFewRows>(p.h + slot * p.ldh, m, p.f, acc);
+    }
+    sum_lanes(acc);
+#pragma unroll
+    for (int i = 0; i < kFewRows; ++i)
+        if (lane == i && o0 + i < p.o)
+            p.out[row * p.ld_out + o0 + i] = from_f<T>(p.base != nullptr ? to_f(p.base[row * p.ld_base + o0 + i]) + acc[i] : acc[i]);
 }
 
 // ---- what joins parts ----
@@ -669,17 +794,52 @@ __global__ __launch_bounds__(256) void k_feed_merge(const float* part, int split
 
 size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 
+// Forward calls of few slots take two launches that read every slot's matrices, instead of a sort and tiles of one expert, which are read
+// once, but slowly where there are few (and in fp32 the matrix cores bound them).  us, few and tiles:
+//   bf16, d = o = 4,096, f = 2,048, 16 experts, k = 2:  2 slots 21, 54;  16: 135, 150;  24: 181, 144
+//         d = o = 2,048, f = 1,024,  8 experts, k = 2:  2 slots 14, 35;  24:  32,  37;  32:  40,  38;  64: 72, 39
+//         d = o = 512, f = 512,     64 experts, k = 4: 16 slots 14, 28;  64:  19,  30
+//   fp32, d = o = 4,096, f = 2,048, 16 experts, k = 2:  2 slots 40, 399; 48: 715, 774;  64: 914, 779
+bool is_few(const FeedSizes& z)
+{
+    const size_t slots = (size_t)z.n * z.k;
+    return z.type == kF32 ? slots <= 48 : slots <= 16 || (slots <= 64 && slots * z.f * (2 * (size_t)z.d + z.o) * 2 <= size_t(384) << 20);
+}
+
 struct Layout {
-    int slots, tile, ntiles, segments;
-    bool fast, sorted;
+    int slots, ntiles, segments;
+    int tile, r[kKinds];                  // rows of the sort's tiles, and of each product's
+    bool few, fast, sorted;
     int ldh, ndots, gsplits, osplits;
     size_t seen, perm, tiles, groups, merge, h, dg, du, dots, sums, part, bytes;
 };
 
-// Rows of a block's tile, 128 or 256.
-constexpr int kBig = 256, kMid = 128;
-
 int tiles_of(long m, int r) { return (int)((m + r - 1) / r); }
+
+// Rows (and columns) of a block's tile: 256 (one block a CU, FAST only), 128 (two) or 64 (four).  What a tile costs is its
+// products over how well they keep the matrix cores busy, which the next block of the CU helps with; what a
+// launch costs is that of the CU with most tiles.
+
+int choose_tile(const FeedSizes& z, long rows, long columns, long layers, int parts)
+{
+    int best = 0;
+    double least = 0;
+    for (const int r : {256, 128, 64}) {
+        if (r == 256 && !z.aligned) continue;
+        const long tiles = layers * tiles_of(rows, r) + (parts > 1 ? parts / 2 : 0), busy = (tiles * tiles_of(columns, r) + 255) / 256;
+        const double waste = z.type == kF32 ? (r == 256 ? 1.0 : r == 128 ? (busy > 1 ? 1.0 : 1.1) : busy > 1 ? 1.15 : 1.3)
+                                            : (r == 256 ? 1.0 : r == 128 ? (busy > 1 ? 1.25 : 1.8) : busy > 3 ? 2.0 : busy > 1 ? 2.6 : 4.0);
+        const double cost = (double)busy * r * r * waste;
+        if (best == 0 || cost < least) {
+            best = r;
+            least = cost;
+        }
+    }
+#ifdef FEED_TILE
+    if (FEED_TILE < 256 || z.aligned) best = FEED_TILE;
+#endif
+    return best;
+}
 
 // Parts of the slots for the matrices' gradients: enough for two blocks a CU, each with 8 steps at least.
 int matrix_splits(long slots, int a, int m, int n, int both, int r, int step)
@@ -696,17 +856,29 @@ Layout layout(const FeedSizes& z, bool backward)
     Layout L{};
     const int vec = 16 / (int)elem_size(z.type), step = 128 / (int)elem_size(z.type);
     L.slots = (int)(z.n * z.k);
-    L.sorted = z.sorted;
+    L.few = !backward && is_few(z);
+    L.sorted = z.sorted && !L.few;
     L.fast = z.aligned;
     L.ldh = (z.f + vec - 1) / vec * vec;
-    L.tile = kMid;
-    if (z.aligned && (long)tiles_of(L.slots, kBig) * tiles_of(z.f, kBig) >= 256) L.tile = kBig;
-    L.ntiles = z.sorted ? L.slots / L.tile + z.a + 1 : tiles_of(L.slots, L.tile);
+    if (backward) {
+        L.r[kHidden] = choose_tile(z, L.slots, z.f, 1, z.a);
+        L.r[kRows] = choose_tile(z, L.slots, z.d, 1, z.a);
+        L.r[kGates] = choose_tile(z, z.f, z.d, 2 * z.a, 1);
+        L.r[kOuts] = choose_tile(z, z.o, z.f, z.a, 1);
+        L.tile = std::max(L.r[kHidden], L.r[kRows]);
+    } else {
+        L.r[kGated] = choose_tile(z, L.slots, 2l * z.f, 1, z.a);
+        L.r[kDown] = choose_tile(z, L.slots, z.o, 1, z.a);
+        L.tile = std::max(L.r[kGated], L.r[kDown]);
+    }
+    L.ntiles = L.slots / L.tile + z.a + 1;
     L.segments = (L.slots + kPlanRows - 1) / kPlanRows;
     if (L.segments < 1) L.segments = 1;
-    L.ndots = tiles_of(z.f, L.tile) * (L.tile / 64);  // one a wave's 64 columns
-    L.gsplits = matrix_splits(L.slots, z.a, z.f, z.d, 2, L.tile, step);
-    L.osplits = matrix_splits(L.slots, z.a, z.o, z.f, 1, L.tile, step);
+    if (backward) {
+        L.ndots = tiles_of(z.f, L.r[kHidden]) * (L.r[kHidden] == 256 ? 4 : 2);  // one for each wave's columns
+        L.gsplits = matrix_splits(L.slots, z.a, z.f, z.d, 2, L.r[kGates], step);
+        L.osplits = matrix_splits(L.slots, z.a, z.o, z.f, 1, L.r[kOuts], step);
+    }
     size_t at = 0;
     auto take = [&](size_t& where, size_t bytes) { where = at; at += up16(bytes); };
     if (L.sorted) {
@@ -721,7 +893,7 @@ Layout layout(const FeedSizes& z, bool backward)
     const size_t es = elem_size(z.type), hidden = (size_t)L.slots * L.ldh * es;
     take(L.h, hidden);
     const int w = backward ? z.d : z.o;
-    if (z.k > 1) take(L.sums, (size_t)L.slots * w * 4);
+    if (z.k > 1 && !L.few) take(L.sums, (size_t)L.slots * w * 4);
     if (backward) {
         take(L.dg, hidden);
         take(L.du, hidden);
@@ -749,13 +921,17 @@ template <typename T, int KIND>
 hipError_t launch_product(const Layout& L, FeedArgs<T> p, hipStream_t s)
 {
     constexpr bool MATRIX = KIND == kGates || KIND == kOuts;
-    const int r = L.tile;
+    const int r = L.r[KIND];
     p.nn = tiles_of(KIND == kGated ? 2l * p.N : p.N, r);
     p.nm = MATRIX ? tiles_of(p.M, r) : 0;
+    if (!MATRIX) {
+        p.cut = L.tile / r;
+        p.ntiles = p.tiles != nullptr ? L.ntiles * p.cut : tiles_of(L.slots, r);
+    }
     const dim3 grid((unsigned)(MATRIX ? blocks_of((long)p.a * p.splits * (KIND == kGates ? 2 : 1), p.nm, p.nn) : blocks_of(1, p.ntiles, p.nn)));
-    if (L.tile == kBig) return launch(k_product<T, KIND, 2, 4, 8, 4, 4, true>, grid, 512, 0, s, p);
-    if (L.fast) return launch(k_product<T, KIND, 2, 2, 4, 4, 4, true>, grid, 256, 0, s, p);
-    return launch(k_product<T, KIND, 2, 2, 4, 4, 4, false>, grid, 256, 0, s, p);
+    if (r == 256) return launch(k_product<T, KIND, 2, 4, 8, 4, 4, true>, grid, 512, 0, s, p);
+    if (r == 128) return L.fast ? launch(k_product<T, KIND, 2, 2, 4, 4, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 4, 4, 4, false>, grid, 256, 0, s, p);
+    return L.fast ? launch(k_product<T, KIND, 2, 2, 2, 2, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 2, 2, 4, false>, grid, 256, 0, s, p);
 }
 
 template <typename T>
@@ -772,8 +948,8 @@ bool feed_fits(const FeedSizes& z)
     if (z.n * z.k >= 1l << 30) return false;
     const long most = 1l << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
     const long wide = z.d > z.o ? z.d : z.o, slots = (long)z.n * z.k;
-    const int rows = (int)(slots / kMid) + z.a + 1, hidden = tiles_of(2l * z.f, kMid), outer = tiles_of(wide, kMid);
-    return blocks_of(1, rows, hidden > outer ? hidden : outer) < most && blocks_of(16l * z.a, tiles_of(z.f, kMid), outer) < most && z.n < most &&
+    const int rows = (int)(slots / 64) + 4 * (z.a + 1), hidden = tiles_of(2l * z.f, 64), outer = tiles_of(wide, 64);
+    return blocks_of(1, rows, hidden > outer ? hidden : outer) < most && blocks_of(16l * z.a, tiles_of(z.f, 64), outer) < most && z.n < most &&
            (wide + 1023) / 1024 < 65536 && (slots + kPlanRows - 1) / kPlanRows < 65536;
 }
 
@@ -790,10 +966,18 @@ hipError_t launch_feed(const FeedCall& a, hipStream_t s)
     }
     return with_type(z.type, [&](auto tag) {
         using T = decltype(tag);
+        if (L.few) {
+            const FewArgs<T> p{(const T*)a.x, a.ld_x, (const T*)a.gate, a.gate_sa, a.gate_ld, (const T*)a.up, a.up_sa, a.up_ld, (const T*)a.down, a.down_sa, a.down_ld,
+                               a.chosen, a.weights, a.act, (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, (T*)(a.ws + L.h), L.ldh, a.pre,
+                               (int)z.n, z.d, z.f, z.o, z.k, z.a};
+            constexpr int EACH = kFewRows * (kFewThreads / 64);
+            auto blocks = [&](long vectors, int rows) { return dim3((unsigned)((vectors * ((rows + kFewRows - 1) / kFewRows) * kFewRows + EACH - 1) / EACH)); };
+            SKM_TRY_LAUNCH(k_few_gated<T>, blocks(L.slots, z.f), kFewThreads, 0, s, p);
+            return launch(k_few_down<T>, blocks(z.n, z.o), kFewThreads, 0, s, p);
+        }
         FeedArgs<T> p{};
         p.tiles = L.sorted ? reinterpret_cast<const Tile*>(a.ws + L.tiles) : nullptr;
         p.perm = L.sorted ? reinterpret_cast<const int*>(a.ws + L.perm) : nullptr;
-        p.ntiles = L.ntiles;
         p.slots = L.slots;
         p.a = z.a;
         p.byk = by_k(z.k);
@@ -840,7 +1024,6 @@ hipError_t launch_feed_back(const FeedBackCall& a, hipStream_t s)
         FeedArgs<T> p{};
         p.tiles = L.sorted ? reinterpret_cast<const Tile*>(a.ws + L.tiles) : nullptr;
         p.perm = L.sorted ? reinterpret_cast<const int*>(a.ws + L.perm) : nullptr;
-        p.ntiles = L.ntiles;
         p.slots = L.slots;
         p.a = z.a;
         p.byk = by_k(z.k);
