@@ -147,7 +147,7 @@ hipError_t launch_drop(const DropCall& a, hipStream_t s);
 
 constexpr int kRateMaxK = 16;       // largest scores a row names
 constexpr int kRateMaxV = 1 << 22;  // scores a row
-constexpr int kRateSplits = 64;     // parts a row
+constexpr int kRateSplits = 256;    // parts a row
 constexpr int kRateList = 4096;     // scores that a part's choice looks at twice, at most
 
 struct RateCall {

@@ -817,10 +817,19 @@ struct Layout {
 int tiles_of(long m, int r) { return (int)((m + r - 1) / r); }
 
 // Rows (and columns) of a block's tile: 256 (one block a CU, FAST only), 128 (two) or 64 (four).  What a tile costs is its
-// products over how well they keep the matrix cores busy, which the next block of the CU helps with; what a
-// launch costs is that of the CU with most tiles.
-
-int choose_tile(const FeedSizes& z, long rows, long columns, long layers, int parts)
+// products over how well they keep the matrix cores busy, which the CU's other blocks help with; what a launch
+// costs is that of the CU with most tiles.  us, forward and gradients of rows and of matrices, all products with tiles of 64 / 128 / 256, and
+// by the rule:
+//   bf16   64 x 4,096 by 2,048, 16 experts, k = 2: 179 193 494 / 193 178 427 / 228 236 375, 181 194 379
+//         300 x 1,024 by 1,024,  4, 1:              25  43  50 /  39  69  65 /  72 118  97,  26  44  48
+//         512 x 2,048 by 2,048,  8, 2:             101 119 207 /  89 109 184 / 124 198 207,  88 109 167
+//       2,048 x 2,048 by 2,048,  8, 2:             268 350 383 / 211 281 331 / 204 256 299, 204 281 294
+//       4,096 x 2,048 by 8,192,  1, 1:             813 955 1,263 / 509 603 785 / 453 604 673, 461 577 674
+//       8,192 x 1,024 by 1,024,  8, 1:             140 157 199 / 117 153 170 / 130 150 256, 117 151 170
+//       1,024 x 1,001 by 777,    4, 2:              69  95 117 /  85 153 141 / -,             69  95 115
+//   fp32  256 x 512 by 1,024,    4, 1:              47  79  57 / 120 215 100 / 375 651 235,  47  78  58
+//       2,048 x 2,048 by 2,048,  4, 1:             538 572 714 / 655 834 779 / 980 1,538 1,068, 513 567 706
+int choose_tile(const FeedSizes& z, long rows, long columns, long layers, int parts, double tail = 1.0)
 {
     int best = 0;
     double least = 0;
@@ -828,16 +837,15 @@ int choose_tile(const FeedSizes& z, long rows, long columns, long layers, int pa
         if (r == 256 && !z.aligned) continue;
         const long tiles = layers * tiles_of(rows, r) + (parts > 1 ? parts / 2 : 0), busy = (tiles * tiles_of(columns, r) + 255) / 256;
         const double waste = z.type == kF32 ? (r == 256 ? 1.0 : r == 128 ? (busy > 1 ? 1.0 : 1.1) : busy > 1 ? 1.15 : 1.3)
-                                            : (r == 256 ? 1.0 : r == 128 ? (busy > 1 ? 1.25 : 1.8) : busy > 3 ? 2.0 : busy > 1 ? 2.6 : 4.0);
-        const double cost = (double)busy * r * r * waste;
+                           : r == 256       ? (busy == 1 && layers > 1 ? 1.4 : 1.0)  // matrices of unlike experts: a second turn evens them out
+                           : r == 128       ? (busy > 1 ? 1.35 : z.aligned ? 1.8 : 2.2)
+                                            : (busy > 3 ? 2.0 : busy > 1 ? 2.6 : 4.0);
+        const double cost = (double)busy * r * r * waste * (r == 256 ? tail : 1.0);
         if (best == 0 || cost < least) {
             best = r;
             least = cost;
         }
     }
-#ifdef FEED_TILE
-    if (FEED_TILE < 256 || z.aligned) best = FEED_TILE;
-#endif
     return best;
 }
 
@@ -861,7 +869,7 @@ Layout layout(const FeedSizes& z, bool backward)
     L.fast = z.aligned;
     L.ldh = (z.f + vec - 1) / vec * vec;
     if (backward) {
-        L.r[kHidden] = choose_tile(z, L.slots, z.f, 1, z.a);
+        L.r[kHidden] = choose_tile(z, L.slots, z.f, 1, z.a, 1.15);  // 22 bytes a result at its end, which nothing else hides there: 356 us with 256 rows, 333 with 128
         L.r[kRows] = choose_tile(z, L.slots, z.d, 1, z.a);
         L.r[kGates] = choose_tile(z, z.f, z.d, 2 * z.a, 1);
         L.r[kOuts] = choose_tile(z, z.o, z.f, z.a, 1);

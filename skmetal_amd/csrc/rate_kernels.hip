@@ -59,10 +59,42 @@ struct Sums {
     }
 };
 
-__device__ __forceinline__ Sums joined(Sums v, int lanes_apart)
+// The wave's sums joined, on every lane: relative to its maximum at once, so that a lane takes one exponential.
+__device__ __forceinline__ Sums joined(Sums v)
 {
-    v.join(Sums{__shfl_xor(v.m, lanes_apart), __shfl_xor(v.s, lanes_apart), __shfl_xor(v.t, lanes_apart)});
+    float m = v.m;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    v.raise(m);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        v.s += __shfl_xor(v.s, x);
+        v.t += __shfl_xor(v.t, x);
+    }
     return v;
+}
+
+// The wave's k-th largest key (1: fewer lanes hold one), on every lane; equal keys are 0.
+__device__ __forceinline__ unsigned long long kth_largest(unsigned long long key, int k)
+{
+    const unsigned lo = (unsigned)key, hi = (unsigned)(key >> 32);
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+        above += ((unsigned long long)__builtin_amdgcn_readlane(hi, j) << 32 | (unsigned)__builtin_amdgcn_readlane(lo, j)) > key;
+    const unsigned long long who = __ballot(key != 0 && above == k - 1);
+    if (who == 0) return 1;
+    const int lane = __ffsll(who) - 1;
+    return (unsigned long long)__builtin_amdgcn_readlane(hi, lane) << 32 | (unsigned)__builtin_amdgcn_readlane(lo, lane);
+}
+
+// How many of the list's `found` keys are larger.
+__device__ __forceinline__ int rank_of(const unsigned long long* list, int found, unsigned long long key)
+{
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < found; ++j) place += list[j] > key;
+    return place;
 }
 
 struct RateOut {
@@ -112,9 +144,10 @@ struct RateArgs {
 // One part of a row on NT lanes: 16 bytes a lane, UN at once.
 //
 // The k largest: every lane knows the first place of its own largest score, at no cost but a comparison every 16 bytes.
-// The k-th largest of those is a lower bound for the k-th largest of all, and only the k lanes whose
-// largest reach it hold scores that do, so a second look at the part (from the caches) finds at most
-// k of a lane's share and hardly more than k as a rule; these are ranked by counting.
+// The k-th largest of a wave's lanes is a lower bound for the k-th largest of all.  Of the wave that has the
+// largest of these bounds k lanes hold scores that reach it, of the others fewer, so a second look at the part
+// (from the caches) finds at most k of a lane's share in each wave, and hardly more than k in all as a rule; these
+// are ranked by counting.  (With a bound over all lanes through LDS a part of 4,096 scores took 11 us, not @PART@.)
 template <typename T, int NT, bool TOP>
 __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
 {
@@ -136,6 +169,16 @@ __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
 #pragma unroll
         for (int j = 0; j < V; ++j) s.add(x[j]);
     };
+    auto scores = [&](int at, float* x) {  // -inf past the part's end
+        if (at + V <= hi) {
+            const Vec<T> raw = load16(z + at);
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = to_f(raw[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = at + j < hi ? to_f(z[at + j]) : -__builtin_inff();
+        }
+    };
     int at = lo + tid * V;
     for (; at + (UN - 1) * STEP + V <= hi; at += UN * STEP) {
         Vec<T> raw[UN];
@@ -151,51 +194,43 @@ __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
     }
     for (; at < hi; at += STEP) {
         float x[V];
-        if (at + V <= hi) {
-            const Vec<T> raw = load16(z + at);
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = to_f(raw[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = at + j < hi ? to_f(z[at + j]) : -__builtin_inff();
-        }
+        scores(at, x);
         take(x, at);
     }
 
     __shared__ Sums wave_sums[NT / 64];
-    __shared__ unsigned long long lane_keys[TOP ? NT : 1];
     __shared__ unsigned long long list[TOP ? kRateList : 1];
-    __shared__ unsigned long long bound;
+    __shared__ unsigned long long bounds[NT / 64];
     __shared__ int count;
-    Sums all = s;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) all = joined(all, x);
-    if (NT > 64) {
-        if ((tid & 63) == 0) wave_sums[tid >> 6] = all;
-    }
+    Sums all = joined(s);
+    if (NT > 64 && (tid & 63) == 0) wave_sums[tid >> 6] = all;
     if constexpr (TOP) {
         unsigned long long mine = 0;
-        if (first >= 0)
-            for (int j = 0; j < V; ++j) {
-                const unsigned long long key = first + j < hi ? key_of(to_f(z[first + j]), first + j) : 0;
-                mine = key > mine ? key : mine;
-            }
-        lane_keys[tid] = mine;
-        if (tid == 0) {
-            bound = 1;  // above the excluded scores
-            count = 0;
-        }
-        __syncthreads();
-        int above = 0;
-        for (int j = 0; j < NT; ++j) above += lane_keys[j] > mine;
-        if (mine && above == p.out.k - 1) bound = mine;
-        __syncthreads();
-        const unsigned long long least = bound;
-        for (at = lo + tid * V; mine >= least && at < hi; at += STEP)
+        if (first >= 0) {
+            float x[V];
+            scores(first, x);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const unsigned long long key = at + j < hi ? key_of(to_f(z[at + j]), at + j) : 0;
-                if (key >= least) list[atomicAdd(&count, 1)] = key;
+                const unsigned long long key = key_of(x[j], first + j);
+                mine = key > mine ? key : mine;
+            }
+        }
+        unsigned long long least = kth_largest(mine, p.out.k);
+        if (NT > 64 && (tid & 63) == 0) bounds[tid >> 6] = least;
+        if (tid == 0) count = 0;
+        __syncthreads();
+        if (NT > 64)
+#pragma unroll
+            for (int w = 0; w < NT / 64; ++w) least = bounds[w] > least ? bounds[w] : least;
+        if (mine >= least)
+            for (at = lo + tid * V; at < hi; at += STEP) {
+                float x[V];
+                scores(at, x);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const unsigned long long key = key_of(x[j], at + j);
+                    if (key >= least) list[atomicAdd(&count, 1)] = key;
+                }
             }
     }
     if (NT > 64 || TOP) __syncthreads();
@@ -214,13 +249,9 @@ __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
     if constexpr (TOP) {
         const int k = p.out.k, found = count;
         unsigned long long* keys = p.keys + (row * p.splits + split) * k;
-        for (int i = tid; i < max(found, k); i += NT) {
+        for (int i = tid; i < max(found, k); i += NT) {  // places that no score takes: 0, behind the others
             const unsigned long long key = i < found ? list[i] : 0;
-            int place = i;
-            if (i < found) {
-                place = 0;
-                for (int j = 0; j < found; ++j) place += list[j] > key;
-            }
+            const int place = i < found ? rank_of(list, found, key) : i;
             if (place >= k) continue;
             if (whole)
                 put_top(p.out, row, place, key, all);
@@ -230,25 +261,43 @@ __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
     }
 }
 
-// The parts of a row joined, in their order.
+// The parts of a row joined, by a wave.  Of the parts' keys, each part's largest first, those count that reach the
+// largest of the parts' last ones: a lower bound for the k-th largest of all, which at most k - 1 keys of
+// every other part exceed.
 template <typename T>
 __global__ __launch_bounds__(64) void k_rate_join(RateArgs<T> p)
 {
     __shared__ unsigned long long list[kRateSplits * kMaxTop];
     const long row = blockIdx.x;
     const int lane = threadIdx.x, k = p.out.k;
-    Sums all = lane < p.splits ? p.sums[row * p.splits + lane] : Sums{kLowest, 0.f, 0.f};
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) all = joined(all, x);
+    Sums all{kLowest, 0.f, 0.f};
+    unsigned long long least = 1;
+    for (int i = lane; i < p.splits; i += 64) {
+        all.join(p.sums[row * p.splits + i]);
+        if (k > 0) {
+            const unsigned long long last = p.keys[(row * p.splits + i) * k + k - 1];
+            least = last > least ? last : least;
+        }
+    }
+    all = joined(all);
     if (lane == 0) finish(p.out, row, all, p.z + row * p.ld);
     if (k == 0) return;
-    const int found = p.splits * k;
-    for (int i = lane; i < found; i += 64) list[i] = p.keys[row * found + i];
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        const unsigned long long other = __shfl_xor(least, x);
+        least = other > least ? other : least;
+    }
+    int found = 0;
+    for (int i0 = 0; i0 < p.splits * k; i0 += 64) {
+        const unsigned long long key = i0 + lane < p.splits * k ? p.keys[row * p.splits * k + i0 + lane] : 0;
+        const unsigned long long who = __ballot(key >= least);
+        if (key >= least) list[found + __popcll(who & ((1ull << lane) - 1))] = key;
+        found += __popcll(who);
+    }
     __syncthreads();
-    for (int i = lane; i < found; i += 64) {
-        const unsigned long long key = list[i];
-        int place = 0;
-        for (int j = 0; j < found; ++j) place += list[j] > key || (list[j] == key && j < i);  // empty places are alike
+    for (int i = lane; i < max(found, k); i += 64) {
+        const unsigned long long key = i < found ? list[i] : 0;
+        const int place = i < found ? rank_of(list, found, key) : i;
         if (place < k) put_top(p.out, row, place, key, all);
     }
 }
@@ -327,7 +376,7 @@ Parts parts_of(long n, int v, int type, int k)
     const long most = (v + 4095) / 4096;
     if (splits > most) splits = most;
     if (splits > kRateSplits) splits = kRateSplits;
-    const int longest = k > 0 ? kRateList / k / vec * vec * 256 : v;
+    const int longest = k > 0 ? kRateList / (4 * k) / vec * vec * 256 : v;  // k lanes of each of four waves
     const long least = ((long)v + longest - 1) / longest;
     if (splits < least) splits = least;
     const int step = 256 * vec;
