@@ -58,8 +58,9 @@ struct FeedArgs {
     const float* weights; int act;             // weights nullable
     float* dots; int ndots;                    // [slots][ndots] parts of <e, act(g) u>, nullable
     const T* base; long ld_base; T* out; long ld_out;  // k = 1
-    float* sums;                               // [slots][N] by slot: k > 1
-    T *dm, *dm2; float* part; int splits;      // [a][M][N]; partial sums [splits][a][2 where dm2][M][N] where splits > 1
+    float* sums;                               // [splits][slots][N] by slot: k > 1 or several splits
+    T *dm, *dm2; float* part;                  // [a][M][N]; partial sums [splits][a][2 where dm2][M][N] where splits > 1
+    int splits;                                // of the sum, over blocks
 };
 
 // exp(x) for |x| <= 88: the product with log2 e in two parts, so that its rounding does not grow with x.
@@ -71,7 +72,7 @@ __device__ __forceinline__ float exp_near(float x)
 }
 
 // act(g) and its derivative.  Both products' tiles end in 64 of these a lane: silu takes 13 instructions so, gelu 30 (with the
-// library's expf, division and erfcf, which branch, the gated product of 4,096 x 2,048 by 8,192 took @GELU@).
+// library's expf, division and erfcf, which branch, the gated product of 4,096 x 2,048 by 8,192 took 341 us, not 319).
 __device__ __forceinline__ float2 activate(float g, int act)
 {
     if (act == kSilu) {
@@ -357,7 +358,8 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         terms = max(0, min(t.cnt, (int)((long)steps * (split + 1) / p.splits) * kStep<T>) - from);
     } else {
         const Place at = place_of(blockIdx.x, p.ntiles, p.nn);
-        if (at.layer > 0 || at.m >= p.ntiles || at.n >= p.nn) return;
+        if (at.layer >= p.splits || at.m >= p.ntiles || at.n >= p.nn) return;
+        split = at.layer;
         n0 = at.n * (KIND == kGated ? RB / 2 : RB);
         if (p.tiles != nullptr) {
             t = p.tiles[at.m / p.cut];
@@ -390,13 +392,29 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         }
         B += t.q * p.sb;
         if constexpr (KIND == kGated || KIND == kRows) B2 += t.q * p.sb2;
+        if constexpr (KIND == kDown) {
+            const int steps = (p.K + kStep<T> - 1) / kStep<T>;
+            from = (int)((long)steps * split / p.splits) * kStep<T>;
+            terms = min(p.K, (int)((long)steps * (split + 1) / p.splits) * kStep<T>) - from;
+            A += from;
+            B += from;
+        }
     }
+    // P^T dg + Q^T du: one sum after the other, or a block each
+    const bool both_sums = KIND == kRows && p.splits == 1;
+    long ldb = p.ldb;
+    if constexpr (KIND == kRows)
+        if (split > 0) {
+            A = p.A2;
+            B = B2;
+            ldb = p.ldb2;
+        }
     auto slot_of = [&](int place) -> int { return p.perm != nullptr ? p.perm[place] : place; };
 
     Stager<T, A_ALONG, RA, NT, FAST> sa;
     Stager<T, B_ALONG, RB, NT, FAST> sb;
-    const int steps1 = (terms + kStep<T> - 1) / kStep<T>, steps = KIND == kRows ? 2 * steps1 : steps1;
-    const int left_a = p.M - m0, left_b = p.N - n0, start = t.start + from;
+    const int steps1 = (terms + kStep<T> - 1) / kStep<T>, steps = both_sums ? 2 * steps1 : steps1;
+    const int left_a = p.M - m0, left_b = p.N - n0, start = t.start + (MATRIX ? from : 0);
     auto begin_a = [&](const T* a) {
         if constexpr (KIND == kGated || KIND == kHidden)
             sa.rows([&](int r) { return a + (long)p.byk.row((unsigned)slot_of(t.start + min(r, t.cnt - 1))) * p.lda; });
@@ -410,7 +428,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
             return r & 16 ? B2 + f * p.ldb2 : B + f * p.ldb;
         });
     if constexpr (KIND == kDown) sb.rows([&](int r) { return B + (long)min(n0 + r, p.N - 1) * p.ldb; });
-    if constexpr (KIND == kHidden || KIND == kRows) sb.terms(B + n0, p.ldb, left_b);
+    if constexpr (KIND == kHidden || KIND == kRows) sb.terms(B + n0, ldb, left_b);
     if constexpr (KIND == kOuts) sb.terms(B + n0 + start * p.ldb, p.ldb, left_b);
 
     // The slots of step `step`'s gathered rows, which are fetched from step - ASLOTS / 2 on.
@@ -431,7 +449,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
         int k0 = step * kStep<T>;
         bool second = false;
         if constexpr (KIND == kRows)
-            if (step >= steps1) {
+            if (both_sums && step >= steps1) {
                 second = true;
                 k0 -= steps1 * kStep<T>;
                 if (c == 0 && step == steps1) {
@@ -452,7 +470,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
             c -= CHUNKS_A;
             to += RA * kStepBytes;
             if constexpr (B_ALONG) sb.along(c, k0, terms, to);
-            if constexpr (KIND == kHidden || KIND == kRows || KIND == kOuts) sb.across(c, k0, terms, second ? p.ldb2 : p.ldb, left_b, to);
+            if constexpr (KIND == kHidden || KIND == kRows || KIND == kOuts) sb.across(c, k0, terms, second ? p.ldb2 : ldb, left_b, to);
             if constexpr (KIND == kGates) sb.gathered(c, k0, terms, slots, start + k0, p.byk, B + n0, p.ldb, left_b, to);
         }
     };
@@ -614,7 +632,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
                         if (p.base != nullptr) v += get4(p.base + slot * p.ld_base + n, p.N - n);
                         put4(p.out + slot * p.ld_out + n, v, p.N - n);
                     } else {
-                        put4(p.sums + slot * p.N + n, v, p.N - n);
+                        put4(p.sums + ((long)split * p.slots + slot) * p.N + n, v, p.N - n);
                     }
                 }
             }
@@ -741,7 +759,7 @@ __global__ __launch_bounds__(kFewThreads) void k_few_down(FewArgs<T> p)
 
 template <typename T>
 struct JoinArgs {
-    const float* sums; const int* chosen; int n, k, a, w;  // [n k][w]
+    const float* sums; const int* chosen; int n, k, a, w, splits;  // [splits][n k][w]
     const T* base; long ld_base; T* out; long ld_out;
 };
 
@@ -757,7 +775,8 @@ __global__ __launch_bounds__(256) void k_feed_join(JoinArgs<T> p)
     if (p.base != nullptr) v = get4(p.base + row * p.ld_base + n, left);
     for (int j = 0; j < p.k; ++j) {
         const int q = p.chosen != nullptr ? p.chosen[row * p.k + j] : 0;
-        if (q >= 0 && q < p.a) v += get4(p.sums + (row * p.k + j) * p.w + n, left);
+        if (q >= 0 && q < p.a)
+            for (int s = 0; s < p.splits; ++s) v += get4(p.sums + (((long)s * p.n + row) * p.k + j) * p.w + n, left);
     }
     put4(p.out + row * p.ld_out + n, v, left);
 }
@@ -809,8 +828,8 @@ bool is_few(const FeedSizes& z)
 struct Layout {
     int slots, ntiles, segments;
     int tile, r[kKinds];                  // rows of the sort's tiles, and of each product's
-    bool few, fast, sorted;
-    int ldh, ndots, gsplits, osplits;
+    bool few, fast, sorted, joined;       // joined: a launch adds up a row's parts
+    int ldh, ndots, rsplits, gsplits, osplits;
     size_t seen, perm, tiles, groups, merge, h, dg, du, dots, sums, part, bytes;
 };
 
@@ -859,6 +878,16 @@ int matrix_splits(long slots, int a, int m, int n, int both, int r, int step)
     return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
+// Parts of the sum of a product that goes back to the rows, where tiles of 256 leave half of the CUs without work: each part's results cost a
+// write and a read in fp32.  4,096 x 2,048 from 8,192 hidden: 197 us in one, 143 in two (tiles of 256 in one: 206).
+int row_splits(const FeedSizes& z, int r, long columns, long terms, int most)
+{
+    const long blocks = ((z.n * z.k + r - 1) / r + z.a / 2) * tiles_of(columns, r);
+    if (r != 256 || terms < 4096 || blocks > 128) return 1;
+    const int parts = std::min(most, (int)(256 / blocks));
+    return blocks * parts < 192 ? 1 : parts;  // fewer are left to smaller tiles
+}
+
 Layout layout(const FeedSizes& z, bool backward)
 {
     Layout L{};
@@ -873,10 +902,14 @@ Layout layout(const FeedSizes& z, bool backward)
         L.r[kRows] = choose_tile(z, L.slots, z.d, 1, z.a);
         L.r[kGates] = choose_tile(z, z.f, z.d, 2 * z.a, 1);
         L.r[kOuts] = choose_tile(z, z.o, z.f, z.a, 1);
+        if (z.type != kF32 && z.aligned && row_splits(z, 256, z.d, 2l * z.f, 2) == 2) L.r[kRows] = 256;
+        L.rsplits = row_splits(z, L.r[kRows], z.d, 2l * z.f, 2);
         L.tile = std::max(L.r[kHidden], L.r[kRows]);
     } else {
         L.r[kGated] = choose_tile(z, L.slots, 2l * z.f, 1, z.a);
         L.r[kDown] = choose_tile(z, L.slots, z.o, 1, z.a);
+        if (z.type != kF32 && z.aligned && row_splits(z, 256, z.o, z.f, 4) > 1) L.r[kDown] = 256;
+        L.rsplits = row_splits(z, L.r[kDown], z.o, z.f, 4);
         L.tile = std::max(L.r[kGated], L.r[kDown]);
     }
     L.ntiles = L.slots / L.tile + z.a + 1;
@@ -901,7 +934,8 @@ Layout layout(const FeedSizes& z, bool backward)
     const size_t es = elem_size(z.type), hidden = (size_t)L.slots * L.ldh * es;
     take(L.h, hidden);
     const int w = backward ? z.d : z.o;
-    if (z.k > 1 && !L.few) take(L.sums, (size_t)L.slots * w * 4);
+    L.joined = !L.few && (z.k > 1 || L.rsplits > 1);
+    if (L.joined) take(L.sums, (size_t)L.rsplits * L.slots * w * 4);
     if (backward) {
         take(L.dg, hidden);
         take(L.du, hidden);
@@ -936,16 +970,16 @@ hipError_t launch_product(const Layout& L, FeedArgs<T> p, hipStream_t s)
         p.cut = L.tile / r;
         p.ntiles = p.tiles != nullptr ? L.ntiles * p.cut : tiles_of(L.slots, r);
     }
-    const dim3 grid((unsigned)(MATRIX ? blocks_of((long)p.a * p.splits * (KIND == kGates ? 2 : 1), p.nm, p.nn) : blocks_of(1, p.ntiles, p.nn)));
+    const dim3 grid((unsigned)(MATRIX ? blocks_of((long)p.a * p.splits * (KIND == kGates ? 2 : 1), p.nm, p.nn) : blocks_of(p.splits, p.ntiles, p.nn)));
     if (r == 256) return launch(k_product<T, KIND, 2, 4, 8, 4, 4, true>, grid, 512, 0, s, p);
     if (r == 128) return L.fast ? launch(k_product<T, KIND, 2, 2, 4, 4, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 4, 4, 4, false>, grid, 256, 0, s, p);
     return L.fast ? launch(k_product<T, KIND, 2, 2, 2, 2, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 2, 2, 4, false>, grid, 256, 0, s, p);
 }
 
 template <typename T>
-hipError_t launch_join(const float* sums, const int* chosen, const FeedSizes& z, int w, const T* base, long ld_base, T* out, long ld_out, hipStream_t s)
+hipError_t launch_join(const float* sums, const int* chosen, const FeedSizes& z, int splits, int w, const T* base, long ld_base, T* out, long ld_out, hipStream_t s)
 {
-    const JoinArgs<T> p{sums, chosen, (int)z.n, z.k, z.a, w, base, ld_base, out, ld_out};
+    const JoinArgs<T> p{sums, chosen, (int)z.n, z.k, z.a, w, splits, base, ld_base, out, ld_out};
     return launch(k_feed_join<T>, dim3((unsigned)z.n, (unsigned)((w + 1023) / 1024)), 256, 0, s, p);
 }
 
@@ -957,7 +991,7 @@ bool feed_fits(const FeedSizes& z)
     const long most = 1l << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
     const long wide = z.d > z.o ? z.d : z.o, slots = (long)z.n * z.k;
     const int rows = (int)(slots / 64) + 4 * (z.a + 1), hidden = tiles_of(2l * z.f, 64), outer = tiles_of(wide, 64);
-    return blocks_of(1, rows, hidden > outer ? hidden : outer) < most && blocks_of(16l * z.a, tiles_of(z.f, 64), outer) < most && z.n < most &&
+    return blocks_of(1, rows, hidden > outer ? hidden : outer) < most / 4 && blocks_of(16l * z.a, tiles_of(z.f, 64), outer) < most && z.n < most &&
            (wide + 1023) / 1024 < 65536 && (slots + kPlanRows - 1) / kPlanRows < 65536;
 }
 
@@ -989,6 +1023,7 @@ hipError_t launch_feed(const FeedCall& a, hipStream_t s)
         p.slots = L.slots;
         p.a = z.a;
         p.byk = by_k(z.k);
+        p.splits = 1;
         p.h = (T*)(a.ws + L.h);
         p.ldh = L.ldh;
         p.weights = a.weights;
@@ -1005,15 +1040,16 @@ hipError_t launch_feed(const FeedCall& a, hipStream_t s)
         q.B = (const T*)a.down; q.sb = a.down_sa; q.ldb = a.down_ld;
         q.N = z.o; q.K = z.f;
         float* sums = reinterpret_cast<float*>(a.ws + L.sums);
-        if (z.k == 1) {
+        q.splits = L.rsplits;
+        if (!L.joined) {
             q.base = (const T*)a.base; q.ld_base = a.ld_base;
             q.out = (T*)a.out; q.ld_out = a.ld_out;
         } else {
             q.sums = sums;
         }
         e = launch_product<T, kDown>(L, q, s);
-        if (e != hipSuccess || z.k == 1) return e;
-        return launch_join<T>(sums, a.chosen, z, z.o, (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, s);
+        if (e != hipSuccess || !L.joined) return e;
+        return launch_join<T>(sums, a.chosen, z, L.rsplits, z.o, (const T*)a.base, a.ld_base, (T*)a.out, a.ld_out, s);
     });
 }
 
@@ -1063,14 +1099,15 @@ hipError_t launch_feed_back(const FeedBackCall& a, hipStream_t s)
                 r.B2 = (const T*)a.up; r.sb2 = a.up_sa; r.ldb2 = a.up_ld;
                 r.N = z.d; r.K = z.f;
                 float* sums = reinterpret_cast<float*>(a.ws + L.sums);
-                if (z.k == 1) {
+                r.splits = L.rsplits;
+                if (!L.joined) {
                     r.base = (const T*)a.base; r.ld_base = a.ld_base;
                     r.out = (T*)a.dx; r.ld_out = a.ld_dx;
                 } else {
                     r.sums = sums;
                 }
                 e = launch_product<T, kRows>(L, r, s);
-                if (e == hipSuccess && z.k > 1) e = launch_join<T>(sums, a.chosen, z, z.d, (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, s);
+                if (e == hipSuccess && L.joined) e = launch_join<T>(sums, a.chosen, z, L.rsplits, z.d, (const T*)a.base, a.ld_base, (T*)a.dx, a.ld_dx, s);
                 if (e != hipSuccess) return e;
             }
         }

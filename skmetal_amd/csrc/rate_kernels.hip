@@ -147,7 +147,7 @@ struct RateArgs {
 // The k-th largest of a wave's lanes is a lower bound for the k-th largest of all.  Of the wave that has the
 // largest of these bounds k lanes hold scores that reach it, of the others fewer, so a second look at the part
 // (from the caches) finds at most k of a lane's share in each wave, and hardly more than k in all as a rule; these
-// are ranked by counting.  (With a bound over all lanes through LDS a part of 4,096 scores took 11 us, not @PART@.)
+// are ranked by counting.  (With a bound over all lanes through LDS a part of 4,096 scores took 11 us, not 7.)
 template <typename T, int NT, bool TOP>
 __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
 {

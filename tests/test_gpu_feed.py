@@ -281,3 +281,12 @@ def test_feed_python_refusals(experts):  # noqa: F811
         experts.feed_backward(s["grad"], s["x"], *m, c, pre[:, :1])
     with pytest.raises(ValueError, match="grad has shape"):
         experts.feed_backward(s["grad"][:, :8], s["x"], *m, c, pre)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_feed_sums_in_parts(experts, dtype):  # noqa: F811
+    """Few rows and results, many hidden places: sums cut over blocks and joined, with and without a router."""
+    print("feed parts", dtype, flush=True)
+    check(experts, problem(600, 64, 4104, 72, 1, 1, dtype, 3), dtype, dense=True)
+    check(experts, problem(300, 72, 4232, 64, 2, 2, dtype, 4), dtype)
+    check(experts, problem(520, 64, 4360, 40, 2, 1, dtype, 5), dtype)
