@@ -266,32 +266,6 @@ struct Reader {
     }
 };
 
-// acc += a b^T in place.  With 64 accumulators a wave (256 registers, which only the accumulation registers have) the
-// compiler's own form of this instruction moves them about between steps; as assembly they stay where they
-// are.  It writes an instruction's result that the compiler does not know of: settled() stands before the first use.
-template <bool PLACED, typename T>
-__device__ __forceinline__ void mfma_into(f32x4& acc, Vec<T> a, Vec<T> b)
-{
-    if constexpr (!PLACED || sizeof(T) == 4)
-        acc = mfma16(a, b, acc);
-    else if constexpr (std::is_same_v<T, bf16>)
-        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-    else
-        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-}
-// The last products' results are in their registers: 18 wait states after a 16 x 16 product, 32 are taken.
-template <bool PLACED, int TM, int TN>
-__device__ __forceinline__ void settled(f32x4 (&acc)[TM][TN])
-{
-    if constexpr (PLACED) {
-        asm volatile("s_nop 15\n\ts_nop 15" : : : "memory");
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
-    }
-}
-
 // The tile that a block takes, of `layers` times nm x nn.  Units of 4 x 4 tiles share operands in an XCD's L2 (blocks go to the
 // 8 XCDs in turn) and go to the XCDs in turn themselves, so that tiles which turn out to be empty are missing on all of
 // them alike: with an eighth of all tiles side by side on each XCD, the last of them had nothing to do at
@@ -314,20 +288,28 @@ long blocks_of(long layers, int nm, int nn)
 
 // A block's tile of WM TM 16 x WN TN 16 results; a wave's is TM 16 x TN 16.
 //
-// Four stages of LDS: while a step's products run from one, the operands of the three next steps come into the others
-// (with one step ahead, which is 64 KB a block every microsecond, every step waited for memory).  A step is TM groups of
-// TN products.  Fragments are read three groups ahead, across the steps too: the barrier stands before the last three
-// groups, when every wave has read what it needs of the stage, so that the products of these hide it and
-// the first reads of the next stage.
-template <typename T, int KIND, int WM, int WN, int TM, int TN, int STAGES, bool FAST>
-__global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(FeedArgs<T> p)
+// Four stages of LDS: while a step's products run from one, the operands of the three next steps come into the others.  A
+// step is TM groups of TN products.  Fragments are read three groups ahead, across the steps too: the barrier stands
+// before the last three groups, when every wave has read what it needs of the stage, so that the products of these
+// hide it and the first reads of the next stage.
+//
+// Bound by how busy that keeps the matrix cores: at 8,192 x 2,048 by 4,096, one expert, both forward products run at 930 to
+// 1,080 TFLOP/s (rows a multiple of 4 KB apart, as all there are, cost a tenth: their chunks of the same terms lie in
+// few channels), where a large library product reaches 1,190.  Steps on the way, bf16, 8,192 x 2,048, 8 experts, k = 2, us:
+//   fragments read as they are used, results stored from the registers, one step ahead:  gated 390, gates 745, outs 347
+//   fragments three groups ahead, results by rows through LDS:                            377, 364, 199
+//   three steps ahead:                                                                    372, 268, 159
+// 4 waves of 128 x 128 (a quarter fewer bytes from LDS) were slower, 450 to 460 for the gated one; tiles of 256 x 128, two blocks a
+// CU, 400.  A tile's end is hidden by nothing where it has the CU alone: gated writes 8 bytes a result beside h
+// there, kHidden reads and writes 22.
+template <typename T, int KIND, int WM, int WN, int TM, int TN, bool FAST>
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
 {
     constexpr int NT = WM * WN * 64, RA = WM * TM * 16, RB = WN * TN * 16, STAGE = (RA + RB) * kStepBytes;
     constexpr bool MATRIX = KIND == kGates || KIND == kOuts;  // the sum runs over slots
     constexpr bool A_ALONG = !MATRIX, B_ALONG = KIND == kGated || KIND == kDown;
-    constexpr bool PLACED = TM * TN > 32 && sizeof(T) == 2;
     constexpr bool GATHERED = MATRIX;
-    constexpr int ASLOTS = 8;  // slots of gathered rows: of 8 steps, a copy a wave
+    constexpr int STAGES = 4, ASLOTS = 8;  // ASLOTS: the slots of gathered rows, of 8 steps, a copy a wave
     __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE + (GATHERED ? NT / 64 * ASLOTS * 256 : 0)];
 
     const int lane = threadIdx.x & 63, wave = wave_index(), l16 = lane & 15, g = lane >> 4;
@@ -538,7 +520,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
                     for (int e = 0; e < EACH; ++e)
                         if (v1 * EACH + e < CHUNKS) fetch((v < TM ? s : s + 1) + STAGES - 1, v < TM ? before : now, v1 * EACH + e);
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) mfma_into<PLACED, T>(acc[u][j], y[h][j], x[u % RING]);
+                    for (int j = 0; j < TN; ++j) acc[u][j] = mfma16(y[h][j], x[u % RING], acc[u][j]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 before = now;
@@ -546,7 +528,6 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN > 32 ? 1 : 2) void k_product(F
                 next = next == (STAGES - 1) * STAGE ? 0 : next + STAGE;
             }
         }
-        settled<PLACED>(acc);
         landed<0>();
         __syncthreads();
     }
@@ -971,9 +952,9 @@ hipError_t launch_product(const Layout& L, FeedArgs<T> p, hipStream_t s)
         p.ntiles = p.tiles != nullptr ? L.ntiles * p.cut : tiles_of(L.slots, r);
     }
     const dim3 grid((unsigned)(MATRIX ? blocks_of((long)p.a * p.splits * (KIND == kGates ? 2 : 1), p.nm, p.nn) : blocks_of(p.splits, p.ntiles, p.nn)));
-    if (r == 256) return launch(k_product<T, KIND, 2, 4, 8, 4, 4, true>, grid, 512, 0, s, p);
-    if (r == 128) return L.fast ? launch(k_product<T, KIND, 2, 2, 4, 4, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 4, 4, 4, false>, grid, 256, 0, s, p);
-    return L.fast ? launch(k_product<T, KIND, 2, 2, 2, 2, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 2, 2, 4, false>, grid, 256, 0, s, p);
+    if (r == 256) return launch(k_product<T, KIND, 2, 4, 8, 4, true>, grid, 512, 0, s, p);
+    if (r == 128) return L.fast ? launch(k_product<T, KIND, 2, 2, 4, 4, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 4, 4, false>, grid, 256, 0, s, p);
+    return L.fast ? launch(k_product<T, KIND, 2, 2, 2, 2, true>, grid, 256, 0, s, p) : launch(k_product<T, KIND, 2, 2, 2, 2, false>, grid, 256, 0, s, p);
 }
 
 template <typename T>
