@@ -162,7 +162,7 @@ struct Stager {
     static __device__ __forceinline__ int chunk(int c)
     {
         const int l = line(c), s = index(c) % CHUNKS;
-        return ALONG ? s ^ ((l >> 2) & 3) : s ^ displaced<T, CHUNKS>(l);
+        return ALONG ? s ^ ((l >> 1) & 3) : s ^ displaced<T, CHUNKS>(l);
     }
     // across: where a chunk lies in its row, of which `left` elements are the tile's; FAST reads what exists instead of
     // columns that do not, whose results nothing takes
@@ -233,7 +233,7 @@ struct Reader {
     {
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
         if constexpr (ALONG) {
-            at = (first + l16) * kStepBytes + ((g ^ (l16 >> 2)) * 16);
+            at = (first + l16) * kStepBytes + ((g ^ ((l16 >> 1) & 3)) * 16);
             displacement = 0;
         } else if constexpr (sizeof(T) == 2) {  // a lane's terms are 8 g + 0 .. 7; it reads for others 8 bytes of term 8 g + l16 / 4 (+ 4)
             at = (g * 8 + (l16 >> 2)) * R * 2 + ((l16 & 3) >> 1) * 16 + (l16 & 1) * 8;
