@@ -293,15 +293,18 @@ long blocks_of(long layers, int nm, int nn)
 // before the last three groups, when every wave has read what it needs of the stage, so that the products of these
 // hide it and the first reads of the next stage.
 //
-// Bound by how busy that keeps the matrix cores: at 8,192 x 2,048 by 4,096, one expert, both forward products run at 930 to
-// 1,080 TFLOP/s (rows a multiple of 4 KB apart, as all there are, cost a tenth: their chunks of the same terms lie in
-// few channels), where a large library product reaches 1,190.  Steps on the way, bf16, 8,192 x 2,048, 8 experts, k = 2, us:
-//   fragments read as they are used, results stored from the registers, one step ahead:  gated 390, gates 745, outs 347
+// Bound by the way from L2 to LDS and by what nothing hides: at 8,192 x 2,048, 8 experts, k = 2, bf16, both forward products and
+// their sums take 617 us; without the fetches in the loop 457, without the reads of fragments 625, without either 435, of which
+// 250 are the products (with 4.25 and 2.1 tiles a CU that take 5 and 3 turns) and 140 the tiles' ends: all CUs write then,
+// 8 bytes a result beside h in the gated product, which is the rate of the memory (kHidden reads and writes 22).  One expert, 8,192 x
+// 2,048 by 4,096, runs at 930 to 1,080 TFLOP/s where a large library product reaches 1,410; rows a multiple of 4 KB apart, as all
+// there are, cost a tenth, for their chunks of the same terms lie in few channels.
+// Steps on the way, us (gated, gates, outs):
+//   fragments read as they are used, results stored from the registers, one step ahead:  390, 745, 347
 //   fragments three groups ahead, results by rows through LDS:                            377, 364, 199
 //   three steps ahead:                                                                    372, 268, 159
-// 4 waves of 128 x 128 (a quarter fewer bytes from LDS) were slower, 450 to 460 for the gated one; tiles of 256 x 128, two blocks a
-// CU, 400.  A tile's end is hidden by nothing where it has the CU alone: gated writes 8 bytes a result beside h
-// there, kHidden reads and writes 22.
+// 4 waves of 128 x 128 were slower (450 to 460 for the gated one), tiles of 256 x 128, two blocks a CU, too (400): they read
+// more from L2.
 template <typename T, int KIND, int WM, int WN, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
 {
@@ -521,7 +524,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
                         if (v1 * EACH + e < CHUNKS) fetch((v < TM ? s : s + 1) + STAGES - 1, v < TM ? before : now, v1 * EACH + e);
 #pragma unroll
                     for (int j = 0; j < TN; ++j) acc[u][j] = mfma16(y[h][j], x[u % RING], acc[u][j]);
-                    __builtin_amdgcn_sched_barrier(0);
                 }
                 before = now;
                 now = next;
