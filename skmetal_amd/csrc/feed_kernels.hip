@@ -108,6 +108,16 @@ __device__ __forceinline__ void put4(T* p, f32x4 v, int left)
     else
         for (int e = 0; e < left; ++e) p[e] = r[e];
 }
+// The same past the caches, for what only a later launch or the backward pass reads: the gated and down products with their sums at
+// 8,192 x 2,048, 8 experts, k = 2, take 580 us so, 626 with plain stores (and h, which the next launch reads, past the caches: 592).
+__device__ __forceinline__ void stream4(float* p, f32x4 v, int left)
+{
+    typedef f32x4 Loose __attribute__((aligned(4)));
+    if (left >= 4)
+        __builtin_nontemporal_store(v, reinterpret_cast<Loose*>(p));
+    else
+        for (int e = 0; e < left; ++e) p[e] = v[e];
+}
 template <typename T>
 __device__ __forceinline__ f32x4 get4(const T* p, int left)
 {
@@ -294,7 +304,7 @@ long blocks_of(long layers, int nm, int nn)
 // hide it and the first reads of the next stage.
 //
 // Bound by the way from L2 to LDS and by what nothing hides: at 8,192 x 2,048, 8 experts, k = 2, bf16, both forward products and
-// their sums take 617 us; without the fetches in the loop 457, without the reads of fragments 625, without either 435, of which
+// their sums took 617 us (580 since stream4); without the fetches in the loop 457, without the reads of fragments 625, without either 435, of which
 // 250 are the products (with 4.25 and 2.1 tiles a CU that take 5 and 3 turns) and 140 the tiles' ends: all CUs write then,
 // 8 bytes a result beside h in the gated product, which is the rate of the memory (kHidden reads and writes 22).  One expert, 8,192 x
 // 2,048 by 4,096, runs at 930 to 1,080 TFLOP/s where a large library product reaches 1,410; rows a multiple of 4 KB apart, as all
@@ -560,8 +570,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
                 const float w = p.weights != nullptr ? p.weights[slot] : 1.f;
                 if (p.pre != nullptr) {
                     float* to = p.pre + (long)slot * 2 * p.N + f;
-                    put4(to, gate, p.N - f);
-                    put4(to + p.N, up, p.N - f);
+                    stream4(to, gate, p.N - f);
+                    stream4(to + p.N, up, p.N - f);
                 }
                 f32x4 h;
 #pragma unroll
@@ -579,7 +589,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
                     if (p.splits == 1)
                         put4(dm + t.q * each + at, v, p.N - n);
                     else
-                        put4(p.part + (((long)split * p.a + t.q) * (KIND == kGates ? 2 : 1) + matrix) * each + at, v, p.N - n);
+                        stream4(p.part + (((long)split * p.a + t.q) * (KIND == kGates ? 2 : 1) + matrix) * each + at, v, p.N - n);
                 } else if constexpr (KIND == kHidden) {
                     const bool there = m < t.cnt && n < p.ldh;
                     const int place = t.start + min(m, t.cnt - 1), slot = slot_of(place);
@@ -615,7 +625,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
                         if (p.base != nullptr) v += get4(p.base + slot * p.ld_base + n, p.N - n);
                         put4(p.out + slot * p.ld_out + n, v, p.N - n);
                     } else {
-                        put4(p.sums + ((long)split * p.slots + slot) * p.N + n, v, p.N - n);
+                        stream4(p.sums + ((long)split * p.slots + slot) * p.N + n, v, p.N - n);
                     }
                 }
             }
