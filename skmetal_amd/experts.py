@@ -1,21 +1,24 @@
-"""Routing and low-rank adapters on tensors in HBM: what a model whose rows go to
-clusters needs next to the clustering itself.
+"""Experts on tensors in HBM: what a model whose rows go to clusters needs next to the
+clustering itself, from the router to the loss.
 
 A router scores every row against the experts (for experts placed at the centres of a
 ``KMeans`` fit, a product with the centres) and ``route`` takes the best ones, with their
-weights, counts and the balance loss that keeps all experts in use; ``adapt`` puts each
-row through its expert, a low-rank adapter beside a projection that all rows share.  The
-adapter of a row may as well be its request's, or its cluster's: ``HipKMeans.predict``
-labels are valid ``ids``.
+weights, counts and the balance loss that keeps all experts in use.  ``feed`` puts each row
+through its experts, gated feed-forward blocks whose results the weights join; ``adapt`` through
+a low-rank adapter beside a projection that all rows share.  ``drop`` is dropout on the
+way to the residual stream, and ``rate`` says how likely the scores at the end make a row's
+target, with their entropy and the best alternatives: a training loss, or a served answer.  The
+expert or adapter of a row may as well be its request's, or its cluster's: ``HipKMeans.predict`` labels
+are valid ``ids`` and, one a row, a valid ``chosen``.
 
 The tensors are PyTorch's (a ROCm build), on the device that the library was set up on.
 The kernels run on the current stream like any torch operator: asynchronous, ordered
 with the other work of that stream; a tensor made on another stream is the caller's to
 wait for.  Rows may lie apart (``stride(0)``), their elements lie side by side.
 
-``route`` and ``adapt`` record no autograd graph: their gradients are ``route_backward``
-and ``adapt_backward``.  ``routed`` and ``adapted`` are the same operators inside
-autograd.
+``route``, ``feed``, ``adapt``, ``drop`` and ``rate`` record no autograd graph: their gradients are ``route_backward``,
+``feed_backward``, ``adapt_backward``, ``drop`` itself and ``rate_backward``.  ``routed``, ``fed``, ``adapted``,
+``dropped`` and ``rated`` are the same operators inside autograd.
 """
 
 from __future__ import annotations
@@ -517,18 +520,22 @@ def feed_backward(grad, x, gate, up, down, chosen, pre, *, weights=None, base=No
 class _Fed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, chosen, weights, base, act):
-        out, pre = feed(x, gate, up, down, chosen, weights=weights, base=base, act=act, return_pre=True)
-        ctx.save_for_backward(x, gate, up, down, chosen, pre, weights)
+        need = ctx.needs_input_grad
+        if any(need[:4]) or need[5]:
+            out, pre = feed(x, gate, up, down, chosen, weights=weights, base=base, act=act, return_pre=True)
+            ctx.save_for_backward(x, gate, up, down, chosen, pre, weights)
+        else:
+            out = feed(x, gate, up, down, chosen, weights=weights, base=base, act=act)
         ctx.act = act
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, gate, up, down, chosen, pre, weights = ctx.saved_tensors
         need = ctx.needs_input_grad
-        rows = grad if grad.stride(1) == 1 or grad.shape[1] == 1 else grad.contiguous()
         if any(need[:4]) or need[5]:
+            x, gate, up, down, chosen, pre, weights = ctx.saved_tensors
+            rows = grad if grad.stride(1) == 1 or grad.shape[1] == 1 else grad.contiguous()
             g = feed_backward(rows, x, gate, up, down, chosen, pre, weights=weights, act=ctx.act, rows=need[0], matrices=any(need[1:4]))
         else:
             g = FeedGrads(None, None, None, None, None)
