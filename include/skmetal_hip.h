@@ -411,7 +411,7 @@ SKMETAL_API int skmetal_hip_adapt_backward(int dtype, const void* grad, size_t l
 /* The gated feed-forward block of every row's experts: with q = chosen[i][j],
  *   out_i = base_i + sum_j weights_ij down_q (act(gate_q x_i) * (up_q x_i))
  * x [n x d], base [n x o] (nullable: 0), out [n x o] (may be base itself: the same
- * address and distance of rows); gate and up [a][f][d], down [a][o][f], experts
+ * address and distance of rows; may share any memory with x); gate and up [a][f][d], down [a][o][f], experts
  * *_stride and rows *_ld elements apart; chosen [n x k] int32, outside [0, a): no
  * expert (null, with k = a = 1: every row takes the one there is); weights [n x k]
  * fp32 (nullable: 1).  pre (nullable): [n x k][2][f] fp32, receives gate_q x_i and

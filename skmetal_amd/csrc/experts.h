@@ -129,7 +129,7 @@ struct FeedBackCall {
 hipError_t launch_feed_back(const FeedBackCall& a, hipStream_t s);
 size_t feed_workspace(const FeedSizes& z, bool backward);
 // Whether every launch of both directions has a grid that the device takes.
-bool feed_fits(const FeedSizes& z);
+bool feed_fits(FeedSizes z);
 
 // ---- drop_kernels.hip ----
 

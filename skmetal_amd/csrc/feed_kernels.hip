@@ -854,7 +854,7 @@ int choose_tile(const FeedSizes& z, long rows, long columns, long layers, int pa
     double least = 0;
     for (const int r : {256, 128, 64}) {
         if (r == 256 && !z.aligned) continue;
-        const long tiles = layers * tiles_of(rows, r) + (parts > 1 ? parts / 2 : 0), busy = (tiles * tiles_of(columns, r) + 255) / 256;
+        const long tiles = layers * tiles_of(rows, r) + (parts > 1 ? std::min<long>(parts, rows) / 2 : 0), busy = (tiles * tiles_of(columns, r) + 255) / 256;
         const double waste = z.type == kF32 ? (r == 256 ? 1.0 : r == 128 ? (busy > 1 ? 1.0 : 1.1) : busy > 1 ? 1.15 : 1.3)
                            : r == 256       ? (busy == 1 && layers > 1 ? 1.4 : 1.0)  // matrices of unlike experts: a second turn evens them out
                            : r == 128       ? (busy > 1 ? 1.35 : z.aligned ? 1.8 : 2.2)
@@ -985,14 +985,30 @@ hipError_t launch_join(const float* sums, const int* chosen, const FeedSizes& z,
 
 }  // namespace
 
-bool feed_fits(const FeedSizes& z)
+// Whether the rows and matrices of a call lie in whole 16 bytes is not known here: both ways have to fit.
+bool feed_fits(FeedSizes z)
 {
     if (z.n * z.k >= 1l << 30) return false;
-    const long most = 1l << 23;  // blocks of at most 512 threads in a grid that has less than 2^32
-    const long wide = z.d > z.o ? z.d : z.o, slots = (long)z.n * z.k;
-    const int rows = (int)(slots / 64) + 4 * (z.a + 1), hidden = tiles_of(2l * z.f, 64), outer = tiles_of(wide, 64);
-    return blocks_of(1, rows, hidden > outer ? hidden : outer) < most / 4 && blocks_of(16l * z.a, tiles_of(z.f, 64), outer) < most && z.n < most &&
-           (wide + 1023) / 1024 < 65536 && (slots + kPlanRows - 1) / kPlanRows < 65536;
+    const long most = 1l << 32, wide = z.d > z.o ? z.d : z.o;  // threads a launch has fewer than
+    if (z.n * 256 >= most || (wide + 1023) / 1024 >= 65536 || (z.n * z.k + kPlanRows - 1) / kPlanRows >= 65536) return false;
+    const int outer = tiles_of(wide, 64);  // small calls at once: tiles of 64, the most parts
+    if (blocks_of(4, (int)(z.n * z.k / 64) + 4 * (z.a + 1), std::max(tiles_of(2l * z.f, 64), outer)) * 512 < most && blocks_of(16l * z.a, tiles_of(z.f, 64), outer) * 512 < most) return true;
+    for (int way = 0; way < 4; ++way) {
+        z.aligned = (way & 1) != 0;
+        const Layout L = layout(z, (way & 2) != 0);
+        if (L.few) continue;
+        auto fits = [&](int kind, long layers, long m, long n) {
+            const long threads = L.r[kind] == 256 ? 512 : 256;
+            return blocks_of(layers, (int)m, tiles_of(n, L.r[kind])) * threads < most;
+        };
+        auto rows = [&](int kind) { return (long)L.ntiles * (L.tile / L.r[kind]); };
+        const bool fine = way & 2 ? fits(kHidden, 1, rows(kHidden), z.f) && fits(kRows, L.rsplits, rows(kRows), z.d) &&
+                                        fits(kGates, 2l * z.a * L.gsplits, tiles_of(z.f, L.r[kGates]), z.d) &&
+                                        fits(kOuts, (long)z.a * L.osplits, tiles_of(z.o, L.r[kOuts]), z.f)
+                                  : fits(kGated, 1, rows(kGated), 2l * z.f) && fits(kDown, L.rsplits, rows(kDown), z.o);
+        if (!fine) return false;
+    }
+    return true;
 }
 
 size_t feed_workspace(const FeedSizes& z, bool backward) { return layout(z, backward).bytes; }

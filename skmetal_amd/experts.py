@@ -468,7 +468,8 @@ def feed(x, gate, up, down, chosen=None, *, weights=None, base=None, act="silu",
     [n, k], k up to 16, with any value outside [0, a) for no expert (a router's ``experts`` as
     they come; None: all rows take the one expert that there is), and weights float32 [n, k] (None: 1); base [n, o]
     is the residual stream (None: 0).  x, the matrices, base and out have one type; `act` is "silu", "gelu" (by
-    the normal distribution function) or "relu".  `out` may be base; it shares memory with nothing else.  With
+    the normal distribution function) or "relu".  `out` may be base and may share memory with x (a residual
+    stream in place: base=x, out=x); nothing else may share memory with it.  With
     `return_pre` also returns gate_q x_i and up_q x_i, float32 [n, k, 2, f], for ``feed_backward``.
 
     Sums are float32.  The hidden vector, weighted, is rounded to the rows' type once before the second

@@ -42,6 +42,16 @@ def test_feed_refuses(lib, bad, code, says):
     assert says in lib.skmetal_hip_last_error().decode()
 
 
+def test_feed_accepts_large_models(lib):
+    """Many experts of wide blocks, and many rows: the launches of both directions have room."""
+    for z in (dict(n=4096, d=7168, f=2048, o=7168, k=8, a=256), dict(n=1 << 16, d=4096, f=14_336, o=4096, k=2, a=8), dict(n=1 << 20, d=2048, f=1024, o=2048, k=8, a=128),
+              dict(n=1, d=16_384, f=53_248, o=16_384, k=1, a=1), dict(n=512, d=4096, f=4096, o=4096, k=4, a=2048)):
+        for dtype in (0, 1, 2):
+            assert all(lib.skmetal_hip_feed_workspace(dtype, *z.values(), b) > 0 for b in (0, 1)), (z, lib.skmetal_hip_last_error())
+        big = dict(x=1 << 44, out=1 << 45, base=None, ld_x=z["d"], ld_gate=z["d"], ld_out=z["o"], size=1 << 50, **z)
+        assert _feed(lib, **big) == ENODEV, lib.skmetal_hip_last_error()
+
+
 def test_feed_accepts(lib):
     """Up to the missing device: in place, without a router, weights or base, no rows, x anywhere."""
     for good in (dict(), dict(base=8 * P), dict(base=None), dict(weights=None), dict(chosen=None, k=1, a=1), dict(n=0, x=None, out=None, chosen=None), dict(x=8 * P), dict(x=P + 2),

@@ -283,10 +283,61 @@ def test_feed_python_refusals(experts):  # noqa: F811
         experts.feed_backward(s["grad"][:, :8], s["x"], *m, c, pre)
 
 
+def check_parts(experts, s, dtype, act="silu"):  # noqa: F811
+    """A large problem by some of its rows (out, pre, the gradients of rows and weights are theirs alone) and
+    some of its hidden places (the matrices' gradients there are)."""
+    x, m, chosen = s["x"], (s["gate"], s["up"], s["down"]), s["chosen"]
+    n, f = x.shape[0], m[0].shape[1]
+    opt = dict(weights=s["weights"], act=act)
+    out, pre = experts.feed(x, *m, chosen, base=s["base"], return_pre=True, **opt)
+    assert torch.equal(out, experts.feed(x, *m, chosen, base=s["base"], **opt))
+    g = experts.feed_backward(s["grad"], x, *m, chosen, pre, base=s["grad_base"], **opt)
+    rows = sorted({*range(0, n, max(1, n // 13)), 15, 16, 63, 64, 127, 128, 255, 256, n - 1} & set(range(n)))
+    I, M = chosen.cpu().numpy(), [f64(v) for v in m]
+    want = ref.feed(f64(x[rows]), *M, I[rows], f64(s["weights"][rows]), f64(s["base"][rows]), act, dtype, f64(s["grad"][rows]), f64(s["grad_base"][rows]))
+    for name, got in (("out", out), ("pre", pre), ("x", g.x), ("weights", g.weights)):
+        near(got[rows], *want[name], name)
+    places = sorted({*range(0, f, max(1, f // 7)), 31, 32, 127, 128, 255, 256, f - 1} & set(range(f)))
+    some = M[0][:, places], M[1][:, places], M[2][:, :, places]
+    want = ref.feed(f64(x), *some, I, f64(s["weights"]), None, act, dtype, f64(s["grad"]))
+    for name, got in (("gate", g.gate[:, places]), ("up", g.up[:, places]), ("down", g.down[:, :, places])):
+        near(got, *want[name], f"grad_{name}")
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-def test_feed_sums_in_parts(experts, dtype):  # noqa: F811
-    """Few rows and results, many hidden places: sums cut over blocks and joined, with and without a router."""
-    print("feed parts", dtype, flush=True)
-    check(experts, problem(600, 64, 4104, 72, 1, 1, dtype, 3), dtype, dense=True)
-    check(experts, problem(300, 72, 4232, 64, 2, 2, dtype, 4), dtype)
-    check(experts, problem(520, 64, 4360, 40, 2, 1, dtype, 5), dtype)
+@pytest.mark.parametrize("n,d,f,o,a,k", [(4090, 4088, 4088, 4088, 1, 1), (6000, 2040, 3000, 2040, 3, 1), (2100, 2056, 4104, 2000, 2, 2)])
+def test_feed_large(experts, n, d, f, o, a, k, dtype):  # noqa: F811
+    """The largest tiles of every product, cut on all sides."""
+    print("feed large", n, d, f, o, a, k, dtype, flush=True)
+    s = problem(n, d, f, o, a, k, dtype, n)
+    if a == 1:
+        s["chosen"].clamp_(min=0, max=0)
+    check_parts(experts, s, dtype, act="gelu" if a == 1 else "silu")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,d,f,o,a,k", [(2500, 64, 4104, 2544, 1, 1), (1800, 72, 4200, 1800, 1, 1), (2500, 2544, 2064, 64, 1, 1), (1200, 2544, 2072, 2536, 1, 2), (2300, 2544, 4104, 2536, 3, 1), (2500, 2540, 2060, 2540, 1, 1)])
+def test_feed_sums_in_parts(experts, n, d, f, o, a, k, dtype):  # noqa: F811
+    """Sums that are cut over blocks, in two and in four, and joined: where tiles of 256 leave half of the CUs idle."""
+    print("feed parts", n, d, f, o, a, k, dtype, flush=True)
+    check_parts(experts, problem(n, d, f, o, a, k, dtype, n + d), dtype)
+
+
+def test_feed_fp32_large(experts):  # noqa: F811
+    check_parts(experts, problem(5000, 1000, 2052, 1004, 2, 1, "fp32", 3), "fp32")
+
+
+def test_feed_out_in_x(experts):  # noqa: F811
+    """out one column on in x's rows, and between them: the rows are read before any is written."""
+    for n, k in ((2, 2), (300, 1), (300, 2)):
+        s = problem(n, 64, 72, 64, 3, k, "bf16", 8)
+        m = s["gate"], s["up"], s["down"]
+        want = experts.feed(s["x"], *m, s["chosen"], weights=s["weights"], base=s["base"])
+        wide = torch.zeros(n, 72, dtype=torch.bfloat16, device="cuda")
+        wide[:, :64] = s["x"]
+        aligned = experts.feed(wide[:, :64], *m, s["chosen"], weights=s["weights"], base=s["base"])
+        assert torch.equal(aligned, want)
+        assert torch.equal(experts.feed(wide[:, :64], *m, s["chosen"], weights=s["weights"], base=s["base"], out=wide[:, 1:65]), want)
+        both = torch.zeros(n, 128, dtype=torch.bfloat16, device="cuda")
+        both[:, :64] = s["x"]
+        assert torch.equal(experts.feed(both[:, :64], *m, s["chosen"], weights=s["weights"], base=s["base"], out=both[:, 64:]), want) and torch.equal(both[:, :64], s["x"])
