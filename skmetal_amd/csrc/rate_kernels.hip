@@ -199,7 +199,7 @@ __global__ __launch_bounds__(NT) void k_rate(RateArgs<T> p)
     }
 
     __shared__ Sums wave_sums[NT / 64];
-    __shared__ unsigned long long list[TOP ? kRateList : 1];
+    extern __shared__ unsigned long long list[];  // TOP: list_of() keys
     __shared__ unsigned long long bounds[NT / 64];
     __shared__ int count;
     Sums all = joined(s);
@@ -366,6 +366,14 @@ struct Parts {
     int threads, splits, part;
 };
 
+// Keys that a part's second look collects at most: k lanes' shares in each wave.  Its LDS follows the shape, so that many
+// short rows run at once: 131,072 x 256 bf16 with the 4 largest 139 us, with room for kRateList keys in every block 533.
+int list_of(const Parts& c, int type, int k)
+{
+    const int vec = 16 / (int)elem_size(type), step = c.threads * vec;
+    return c.threads / 64 * k * ((c.part + step - 1) / step) * vec;
+}
+
 // How a row is cut: parts of at least 4,096 scores, as many as leave about four blocks a CU, at most
 // kRateSplits; with the k largest none of more scores than a lane's share of the list allows.
 Parts parts_of(long n, int v, int type, int k)
@@ -410,8 +418,9 @@ hipError_t launch_rate(const RateCall& a, hipStream_t s)
                       {a.targets, a.target_stride, a.v, a.log_probs, a.entropy, a.lse, a.rest, a.k, a.top, a.top_log_probs},
                       reinterpret_cast<Sums*>(a.ws), reinterpret_cast<unsigned long long*>(a.ws + up16((size_t)a.n * c.splits * sizeof(Sums)))};
         const dim3 grid((unsigned)(a.n * c.splits));
-        const hipError_t e = c.threads == 64 ? (a.k > 0 ? launch(k_rate<T, 64, true>, grid, 64, 0, s, p) : launch(k_rate<T, 64, false>, grid, 64, 0, s, p))
-                                             : (a.k > 0 ? launch(k_rate<T, 256, true>, grid, 256, 0, s, p) : launch(k_rate<T, 256, false>, grid, 256, 0, s, p));
+        const size_t lds = (size_t)list_of(c, a.type, a.k) * 8;  // at most kRateList keys
+        const hipError_t e = c.threads == 64 ? (a.k > 0 ? launch(k_rate<T, 64, true>, grid, 64, lds, s, p) : launch(k_rate<T, 64, false>, grid, 64, 0, s, p))
+                                             : (a.k > 0 ? launch(k_rate<T, 256, true>, grid, 256, lds, s, p) : launch(k_rate<T, 256, false>, grid, 256, 0, s, p));
         if (e != hipSuccess || c.splits == 1) return e;
         return launch(k_rate_join<T>, dim3((unsigned)a.n), 64, 0, s, p);
     });
