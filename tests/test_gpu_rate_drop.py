@@ -122,6 +122,33 @@ def test_rate_orders(experts, v, dtype):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("v,k", [(70, 16), (2000, 1), (2000, 16), (4100, 3), (70_000, 16)])
+def test_rate_few_distinct_scores(experts, v, k, sign, dtype):  # noqa: F811
+    """Which of the same scores are named: those of the lowest places, below 0 too."""
+    print("rate few distinct", v, k, sign, dtype, flush=True)
+    g = torch.Generator().manual_seed(v + k)
+    z = sign * torch.tensor([1.0, 1.5, 2.0, 0.0])[torch.randint(0, 3, (5, v), generator=g)]
+    z[1] = sign * 2.0
+    z[2] = sign * (2.0 + sign)
+    z[2, -5:] = sign * 2.0 + 1.0  # five at the end before all others
+    z[3, : v // 2] = -math.inf
+    z[4, 64:] = -math.inf
+    check(experts, z.to(TYPES[dtype]).cuda(), torch.tensor([0, v - 1, 3, v // 2, 1]).int().cuda(), k, dtype)
+
+
+def test_rate_longest_row(experts):  # noqa: F811
+    """The largest row: places up to the last, the same scores at both ends."""
+    v = 1 << 22
+    z = torch.zeros(1, v)
+    z[0, : 1 << 20] = -1.0
+    z[0, -3:] = torch.tensor([2.0, 3.0, 3.0])
+    z[0, 5] = 3.0
+    print("rate longest", flush=True)
+    check(experts, z.bfloat16().cuda(), torch.tensor([v - 1]).int().cuda(), 16, "bf16", backward=False)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_rate_infinite_scores(experts, dtype):  # noqa: F811
     z = scores(8, 300, "normal", TYPES[dtype], 2)
     z[1, 7] = math.inf
