@@ -883,7 +883,7 @@ int matrix_splits(long slots, int a, int m, int n, int both, int r, int step)
 int row_splits(const FeedSizes& z, int r, long columns, long terms, int most)
 {
     const long blocks = ((z.n * z.k + r - 1) / r + z.a / 2) * tiles_of(columns, r);
-    if (r != 256 || terms < 4096 || blocks > 128) return 1;
+    if (r != 256 || terms < 4096 || blocks > 128 || blocks == 0) return 1;  // 0: no rows
     const int parts = std::min(most, (int)(256 / blocks));
     return blocks * parts < 192 ? 1 : parts;  // fewer are left to smaller tiles
 }
