@@ -109,11 +109,12 @@ def _refuse(t, name, dtype, shape, device):
 
 
 def _rows(t, name, dtype, shape, device):
-    """The row stride of the matrix `t`, whose rows' elements lie side by side."""
+    """The row stride of the matrix `t`, whose rows' elements lie side by side (where it has rows: a
+    broadcast gradient of none keeps its strides of 0 through ``contiguous``)."""
     if t.dtype != dtype or t.shape != shape or t.device != device:
         _refuse(t, name, dtype, shape, device)
     ld, one = t.stride()
-    if one != 1 and shape[1] > 1:
+    if one != 1 and shape[1] > 1 and shape[0] > 0:
         raise ValueError(f"{name}'s rows must have their elements side by side (stride(1) is {one})")
     return ld
 
@@ -189,7 +190,7 @@ def _check_route(logits, top_k):
     if not 1 <= top_k <= min(e, MAX_TOP_K):
         raise ValueError(f"top_k={top_k} is not in [1, {min(e, MAX_TOP_K)}]")
     ld, one = logits.stride()
-    if one != 1 and e > 1:
+    if one != 1 and e > 1 and n > 0:
         raise ValueError(f"logits' rows must have their elements side by side (stride(1) is {one})")
     return code, device, n, e, top_k, ld
 
@@ -272,7 +273,7 @@ def _check_adapt(x, first, down, up, ids, gates, scales):
     code, device = _first(x, first)
     n, width = x.shape
     ld, one = x.stride()
-    if one != 1 and width > 1:
+    if one != 1 and width > 1 and n > 0:
         raise ValueError(f"{first}'s rows must have their elements side by side (stride(1) is {one})")
     dtype = x.dtype
     a, r, d, down_sa, down_ld = _adapters(down, "down", dtype, device)
@@ -623,7 +624,7 @@ def _check_rate(logits, targets):
     if not 1 <= v <= MAX_SCORES:
         raise ValueError(f"logits has rows of {v} scores, expected 1 to {MAX_SCORES}")
     ld, one = logits.stride()
-    if one != 1 and v > 1:
+    if one != 1 and v > 1 and n > 0:
         raise ValueError(f"logits' rows must have their elements side by side (stride(1) is {one})")
     return code, device, n, v, ld, targets.data_ptr(), _vector(targets, "targets", torch.int32, n, device)
 
