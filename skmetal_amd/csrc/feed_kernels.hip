@@ -143,10 +143,11 @@ __device__ __forceinline__ f32x4 once4(const float* p, int left)
 
 // 16 bytes a lane from memory to LDS, a wave's side by side from byte `to` on.  As assembly, for the compiler waits for
 // a load of its own builtin before every transposing read of LDS, and so leaves none in flight
-// under a step's products.  It writes no register but m0, which nothing else here uses; landed() waits for it.
+// under a step's products.  m0 is as before after it (a reserved register, which no clobber list covers); landed() waits for the load.
 __device__ __forceinline__ void to_lds(const void* from, unsigned to)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
+    unsigned kept;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0" : "=&s"(kept) : "s"(to), "v"(from) : "memory");
 }
 __device__ __forceinline__ unsigned lds_offset(char* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) char*)p; }
 
@@ -439,7 +440,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(FeedArgs<T> p)
         if constexpr (GATHERED) {
             const int* from_perm = p.perm + start + min(step * kStep<T> + (lane & (kStep<T> - 1)), max(terms - 1, 0));
             const void* src = p.perm != nullptr ? (const void*)from_perm : (const void*)g_zeros;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_slots + (step & (ASLOTS - 1)) * 256), "v"(src) : "memory");
+            unsigned kept;
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+                         : "=&s"(kept) : "s"(lds_slots + (step & (ASLOTS - 1)) * 256), "v"(src) : "memory");
         }
     };
     // Part c of a step's operands, one chunk a lane: those of A, then those of B.  A step's are taken in their order; steps
