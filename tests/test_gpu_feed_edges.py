@@ -39,3 +39,31 @@ def test_gradients_of_no_rows(experts):  # noqa: F811
     r = experts.rated(z, s["chosen"][:, 0])
     (r.log_probs.sum() + r.entropy.sum() + experts.routed(z, 2).weights.sum()).backward()
     assert z.grad.shape == (0, 64)
+
+
+@pytest.mark.parametrize("n", [16, 300])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activation_keeps_its_bits(experts, act, n):  # noqa: F811
+    """One product a sum, so that out is the activation and grad_gate its derivative, in fp32, each relative to itself.
+
+    In u = 2^-24.  gelu: x and its constant 1.5, t = rcp 3, t P(t) follows t at most in proportion, P's sum 3 and its fit 2.5, the
+    exponential 5 (exp2 2, three roundings), three products 3, the last 1: 20.  silu: the exponential 5, a sum 1, rcp 2, the last 1: 9, so 12.
+    Derivatives: as much of c + |g phi| or t (1 + |g|), with two roundings.  Below 2^-126 nothing is relative."""
+    gen = torch.Generator().manual_seed(n)
+    g = (torch.rand(n, n, generator=gen) * 21.2 - 13.2) if act == "gelu" else torch.rand(n, n, generator=gen) * 107.0 - 87.0
+    one = torch.eye(n, device="cuda")
+    out, pre = experts.feed(one, g.T.contiguous().cuda()[None], torch.ones(1, n, n, device="cuda"), one[None], act=act, return_pre=True)
+    assert torch.equal(pre[:, 0, 0].cpu(), g) and (pre[:, 0, 1] == 1).all()
+    grads = experts.feed_backward(torch.ones(n, n, device="cuda"), one, g.T.contiguous().cuda()[None], torch.ones(1, n, n, device="cuda"), one[None], None, pre, act=act)
+    z, u = g.double(), 2.0**-24
+    if act == "gelu":
+        c, slope = 0.5 * torch.special.erfc(-z / 2**0.5), z * torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5
+        want, derivative, size, bound = z * c, c + slope, c + slope.abs(), 20 * u
+    else:
+        c = torch.sigmoid(z)
+        want, derivative, size, bound = z * c, c * (1 + z * torch.sigmoid(-z)), c * (1 + z.abs()), 12 * u
+    least = 16 * 2.0**-126
+    off = (out.double().cpu() - want).abs() - least
+    assert (off <= bound * want.abs()).all(), (off / want.abs()).max() / u
+    off = (grads.gate[0].T.double().cpu() - derivative).abs() - least
+    assert (off <= (bound + 2 * u) * size).all(), (off / size).max() / u
