@@ -818,16 +818,33 @@ __global__ __launch_bounds__(256) void k_feed_merge(const float* part, int split
 
 size_t up16(size_t b) { return (b + 15) & ~size_t(15); }
 
-// Forward calls of few slots take two launches that read every slot's matrices, instead of a sort and tiles of one expert, which are read
-// once, but slowly where there are few (and in fp32 the matrix cores bound them).  us, few and tiles:
-//   bf16, d = o = 4,096, f = 2,048, 16 experts, k = 2:  2 slots 21, 54;  16: 135, 150;  24: 181, 144
-//         d = o = 2,048, f = 1,024,  8 experts, k = 2:  2 slots 14, 35;  24:  32,  37;  32:  40,  38;  64: 72, 39
-//         d = o = 512, f = 512,     64 experts, k = 4: 16 slots 14, 28;  64:  19,  30
-//   fp32, d = o = 4,096, f = 2,048, 16 experts, k = 2:  2 slots 40, 399; 48: 715, 774;  64: 914, 779
+// Forward calls of few slots may take two launches that read a slot's matrices as they come from memory, an expert's anew for each of
+// its slots (from the caches where they hold it), instead of tiles of one expert, which read them once, but by few blocks in
+// long chains of steps, behind a sort.  The rule compares estimates of both, us: the slots' reads at 16 TB/s where all matrices
+// fit the L2s, down to 7.6 where they do not (16-bit rows off 16 bytes: 9 to 6); the steps' chains, one expert's matrices by the blocks that
+// it has, all matrices, the sort.  us, few and tiles, with the matrices from memory at every call, and the slots from which on the rule takes tiles:
+//   bf16, d = o = 4,096, f = 11,008,  1 expert:         4 slots 147, 178;  8:  274, 182;  16:   554, 191;  64: 2,279, 257  (from 5 on)
+//                       f = 2,048,    1:                8 slots  36,  44; 12:   46,  45;  16:    58,  45;  64:   221,  51  (11)
+//                                     4, k = 2:         8 slots  53,  58; 12:   80,  61;  16:   108,  62;  64:   391,  63  (12)
+//                                    16, k = 2:         2 slots  24,  43; 16:  125, 133;  24:   175, 142;  64:   448, 173  (20)
+//         d = o = 2,048, f = 1,024,   1:                8 slots  15,  26; 16:   21,  26;  24:    26,  27;  64:    53,  30  (20)
+//                                     8, k = 2:         2 slots  14,  35; 16:   30,  39;  24:    39,  40;  64:    74,  40  (30)
+//         d = o = 512, f = 512,      64, k = 4:         4 slots  10,  22; 16:   13,  30;  64:    23,  33
+//         d = o = 4,095, f = 2,047,   1:                8 slots  67, 136; 16:  106, 136;  24:   150, 137;  64:   366, 137  (21)
+//   fp32, d = o = 4,096, f = 11,008,  1:                4 slots 312, 619;  8:  611, 624;  16: 1,220, 622;  48: 3,598, 622  (7)
+//                       f = 2,048,    1:                8 slots  68, 130; 16:  132, 131;  24:   198, 132;  48:   397, 132  (17)
+//                                     8, k = 2:         8 slots 125, 240; 16:  229, 235;  24:   319, 245;  48:   641, 251  (20)
+//         d = o = 1,024, f = 1,024,   1:                8 slots  14,  48; 48:   35,  50;  64:    43,  50  (54)
+//         d = o = 4,095, f = 2,047,   1:                8 slots  72, 346; 24:  214, 351;  48:   441, 352  (39)
 bool is_few(const FeedSizes& z)
 {
-    const size_t slots = (size_t)z.n * z.k;
-    return z.type == kF32 ? slots <= 48 : slots <= 16 || (slots <= 64 && slots * z.f * (2 * (size_t)z.d + z.o) * 2 <= size_t(384) << 20);
+    const double slots = (double)z.n * z.k;
+    if (slots > 64) return false;
+    const bool wide = z.type == kF32;
+    const double matrix = (double)z.f * (2.0 * z.d + z.o) * elem_size(z.type), all = std::min((double)z.a, slots) * matrix;
+    const double few = slots * matrix * (wide || z.aligned ? (1 + 1.1 * std::min(1.0, all / 2e8)) / 16e6 : (1 + 0.5 * std::min(1.0, all / 2e8)) / 9e6);
+    const double tiles = (z.sorted ? 10 : 0) + ((double)z.d + z.f) * (wide ? (z.aligned ? 0.02 : 0.056) : z.aligned ? 0.004 : 0.018) + matrix / 4e6 + all / 1e7;
+    return few <= tiles;
 }
 
 struct Layout {

@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from test_gpu_experts import TYPES, experts  # noqa: E402, F401 -- a fixture
-from test_gpu_feed import problem  # noqa: E402
+from test_gpu_feed import check, problem  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,12 @@ def test_activation_keeps_its_bits(experts, act, n):  # noqa: F811
     assert (off <= bound * want.abs()).all(), (off / want.abs()).max() / u
     off = (grads.gate[0].T.double().cpu() - derivative).abs() - least
     assert (off <= (bound + 2 * u) * size).all(), (off / size).max() / u
+
+
+@pytest.mark.parametrize("n,d,f,a,k,dtype", [(12, 4096, 2048, 1, 1, "bf16"), (24, 2048, 1024, 2, 2, "fp16"), (24, 4096, 2048, 1, 1, "fp32"), (60, 2047, 1023, 2, 1, "bf16"), (8, 4096, 2048, 4, 2, "fp32")])
+def test_few_slots_that_share_experts(experts, n, d, f, a, k, dtype):  # noqa: F811
+    """Up to 64 slots by tiles, which read an expert's matrices once, and the first rows by themselves, slot by slot."""
+    print("shared", n, d, f, a, k, dtype, flush=True)
+    s = problem(n, d, f, d, a, k, dtype, n)
+    check(experts, s, dtype, dense=a == 1, backward=False)
+    check(experts, {name: t if name in ("gate", "up", "down") else t[:2] for name, t in s.items()}, dtype, dense=a == 1, backward=False)
