@@ -500,7 +500,10 @@ def feed_backward(grad, x, gate, up, down, chosen, pre, *, weights=None, base=No
     returned.  The gradient of x is added to `base` [n, d] (None: 0); those of the matrices have
     their shapes and type, 0 for an expert without rows; that of weights is None where there are
     none.  The gradient of the forward call's base is grad itself.  Without `rows` that of x is left
-    out, without `matrices` those of gate, up and down (frozen experts)."""
+    out, without `matrices` those of gate, up and down (frozen experts).
+
+    The gradients of the gate and up products are rounded to the rows' type once before the second products: in
+    float16 what lies under 2^-24 is lost and what lies under 2^-14 loses bits, so its loss is scaled."""
     code, device, n, d, f, o, k, a, x_ld, shared = _check_feed(x, gate, up, down, chosen, weights, act)
     dtype = x.dtype
     grad_ld = _rows(grad, "grad", dtype, (n, o), device)

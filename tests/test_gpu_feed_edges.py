@@ -76,3 +76,64 @@ def test_few_slots_that_share_experts(experts, n, d, f, a, k, dtype):  # noqa: F
     s = problem(n, d, f, d, a, k, dtype, n)
     check(experts, s, dtype, dense=a == 1, backward=False)
     check(experts, {name: t if name in ("gate", "up", "down") else t[:2] for name, t in s.items()}, dtype, dense=a == 1, backward=False)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,f", [(9, 64, 48), (500, 128, 320), (300, 65, 33), (2600, 64, 4104)])
+def test_one_block_with_and_without_a_choice(experts, n, d, f, dtype):  # noqa: F811
+    """chosen None is every row's choice of the one expert: the same places in the same tiles, bit for bit in both directions."""
+    print("one block", n, d, f, dtype, flush=True)
+    s = problem(n, d, f, d, 1, 1, dtype, n)
+    m, zeros = (s["gate"], s["up"], s["down"]), torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    results = []
+    for chosen in (None, zeros):
+        out, pre = experts.feed(s["x"], *m, chosen, weights=s["weights"], base=s["base"], return_pre=True)
+        results.append([out, pre, *experts.feed_backward(s["grad"], s["x"], *m, chosen, pre, weights=s["weights"], base=s["grad_base"])])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n", [8, 300])
+def test_fp16_range(experts, n):  # noqa: F811
+    """A weighted hidden value past 65,504 is infinite, in its row alone; the weight comes first; gradients keep fp16's smallest
+    step (which the reference's bounds count)."""
+    s = problem(n, 64, 96, 64, 3, 1, "fp16", 4)
+    s["chosen"][:, 0] = torch.arange(n, device="cuda").int() % 3
+    m = s["gate"], s["up"], s["down"]
+    plain = experts.feed(s["x"], *m, s["chosen"], base=s["base"])
+    s["x"][5] *= 400
+    rest = torch.arange(n, device="cuda") != 5
+    out = experts.feed(s["x"], *m, s["chosen"], base=s["base"])
+    assert not torch.isfinite(out[5]).all() and torch.equal(out[rest], plain[rest])
+    s["weights"][5] = 2.0**-10
+    s["grad"] *= 2.0**-12
+    assert torch.isfinite(check(experts, s, "fp16")).all()
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_places_past_32_bits(experts, n):  # noqa: F811
+    """Rows and experts that lie more than 2^31 and 2^32 elements apart, in one allocation that is read only where they are."""
+    print("far", n, flush=True)
+    a, d, f, far = 3, 64, 40, 2**31 + 64
+    s = problem(n, d, f, d, a, 2, "bf16", 5)
+    room = torch.empty(3 * far, dtype=torch.bfloat16, device="cuda")
+    step = 2 * far // n // 64 * 64
+    place, views = 0, {}
+    for name in ("x", "base", "grad", "grad_base"):
+        views[name] = room.as_strided(s[name].shape, (step, 1), place)
+        place += d
+    for name in ("gate", "up", "down"):
+        views[name] = room.as_strided(s[name].shape, (far, s[name].shape[2], 1), place)
+        place += s[name][0].numel()
+    assert (n - 1) * step > 2**31 and place < step
+    for name, view in views.items():
+        view.copy_(s[name])
+    want = check(experts, s, "bf16")
+    assert torch.equal(check(experts, {**s, **views}, "bf16"), want)
+    got = experts.feed(views["x"], views["gate"], views["up"], views["down"], s["chosen"], weights=s["weights"], base=views["base"], out=views["base"])
+    assert torch.equal(got, want)
+    z, t = room.as_strided((n, 3000), (step, 1), place), torch.arange(n, device="cuda").int()
+    z.copy_(torch.randn(n, 3000, device="cuda"))
+    near, far_away = (experts.rate(v, t, top_k=3) for v in (z.contiguous(), z))
+    assert all(torch.equal(p, q) for p, q in zip(near, far_away))
+    assert torch.equal(*(experts.rate_backward(v, t, near, grad_log_probs=torch.ones(n, device="cuda")) for v in (z, z.contiguous())))
